@@ -460,6 +460,84 @@ MUI_API mui_status_t mui_parallel_moe_mlp_forward(mui_comm_t* comm, void* stream
 MUI_API mui_status_t mui_embedding_forward(void* stream, mui_dtype_t dtype, int num_tokens, int H, int vocab,
                                            const void* table, const int64_t* token_ids, void* out, unsigned flags);
 
+/* ---- paged KV cache: append with rotation, attention, e4m3 pages, windows with sink tokens ---------------
+ * For serving several sequences out of one pool of pages. Page p of a pool holds page_size consecutive cache rows of
+ * one sequence for every KV head: k_pages / v_pages are [num_pages, kv_heads, page_size, head_dim], so the rows of one
+ * head in one page are contiguous. block_table[b * table_stride + i] is the page of rows i * page_size ... of sequence
+ * b; context_lens[b] is the number of tokens that sequence b had in the cache BEFORE the new tokens of the call. The
+ * new tokens of all sequences are packed: sequence b owns rows cu_tokens[b] .. cu_tokens[b + 1] - 1 of q, k, v and of
+ * the output (cu_tokens[0] == 0), row i of them standing at cache position context_lens[b] + i; cu_tokens == NULL means
+ * one new token per sequence. Rows from cu_tokens[batch] on (padding) are neither read nor written. The same description
+ * serves the append and the attention of one layer; everything it points to lives on the device and may change between
+ * replays of a captured graph.
+ *
+ * MUI_KV_E4M3: elements are e4m3 bytes (4 exponent, 3 mantissa bits, +-448) with one fp32 scale per (page, KV head),
+ * k_scales / v_scales [num_pages, kv_heads]; the value is byte * scale. Scales are powers of two: the smallest one that
+ * fits every row written to the page so far. When a row needs a larger one, the rows before it are rescaled by an exact
+ * power of two (only e4m3 subnormals round again). A page whose row 0 is among the new rows starts afresh, so pages need
+ * no clearing between owners. Infinities saturate and do not count towards the scale; NaN stays NaN.
+ *
+ * Two sequences may share full pages; the page that a sequence appends to must be its own. A block-table entry outside
+ * [0, num_pages), a position beyond the table or beyond the rotary table, or more new tokens than max_new_tokens are
+ * recorded in the device status word and skipped (nothing is read or written out of bounds). No counterpart in the
+ * reference, whose caches are static, dynamic or sliding tensors (muillm/modules/kvcache/cache_utils.py:206-270). */
+typedef enum { MUI_KV_16BIT = 0, MUI_KV_E4M3 = 1 } mui_kv_format_t;
+typedef struct mui_strides2 { int64_t tok, head; } mui_strides2_t; /* in elements; innermost stride 1 */
+typedef struct mui_paged_kv {
+  mui_kv_format_t format;
+  int num_pages, page_size /* 16, 32, 64, 128 */, kv_heads, head_dim /* 64, 128 */;
+  int batch, table_stride, total_tokens;
+  void *k_pages, *v_pages;            /* 16-byte aligned */
+  float *k_scales, *v_scales;         /* MUI_KV_E4M3 only */
+  const int32_t* block_table;         /* [batch, table_stride] */
+  const int32_t* context_lens;        /* [batch] */
+  const int32_t* cu_tokens;           /* [batch + 1] or NULL */
+} mui_paged_kv_t;
+
+/* q_out[t, h, :] = rotate(q[t, h, :]) (q_out contiguous [total_tokens, num_q_heads, head_dim]; num_q_heads may be 0) and
+ * the cache rows of the new tokens receive rotate(k) and v. rotate turns the first rotary_dim elements of a head (even,
+ * <= head_dim) by freqs[position] ([max_positions, rotary_dim / 2, 2] fp32 (cos, sin) pairs, so that any scaling for
+ * long contexts is a matter of the table) in the half layout (pairs (i, i + rotary_dim / 2)) or, interleaved != 0,
+ * pairs (2i, 2i + 1); the rest passes through; freqs == NULL rotates nothing. position is position_ids[t] (int64) or,
+ * NULL, the cache position. Evaluated in fp32 and rounded once, to the 16-bit type or to e4m3. One launch. */
+MUI_API mui_status_t mui_paged_kv_append(void* stream, mui_dtype_t dtype, const mui_paged_kv_t* cache, int num_q_heads,
+                                         const float* freqs, int max_positions, int rotary_dim, int interleaved,
+                                         const int64_t* position_ids, const void* q, mui_strides2_t q_strides,
+                                         const void* k, mui_strides2_t k_strides, const void* v,
+                                         mui_strides2_t v_strides, void* q_out, unsigned flags);
+
+/* out[t, h, :] = softmax_j( q[t, h, :] . K[j, h / G, :] * scale ) V over the cache rows j of the token's sequence (G =
+ * num_q_heads / kv_heads, at most 32): a token at cache position p sees j <= p, its own row (appended before) included, and
+ * with window > 0 of those only j > p - window or j < sinks. out is contiguous [total_tokens, num_q_heads, head_dim].
+ * max_new_tokens bounds the new tokens of every sequence. max_context (> 0) is a hint for the work split, the longest
+ * sequence expected (any value gives right results). Rows of K and V that none of a sequence's new tokens sees are not
+ * looked at. Softmax statistics, sums and outputs are held in fp32 and rounded once. workspace:
+ * mui_paged_attention_workspace_bytes() bytes of scratch for the same sizes, 16-byte aligned, any contents; it may be
+ * used by one call at a time. */
+MUI_API size_t mui_paged_attention_workspace_bytes(int total_tokens, int batch, int num_q_heads, int kv_heads,
+                                                   int head_dim, int max_new_tokens, int max_context, int window,
+                                                   int sinks);
+MUI_API mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_paged_kv_t* cache, int num_q_heads,
+                                         int max_new_tokens, int max_context, int window, int sinks, float scale,
+                                         const void* q, mui_strides2_t q_strides, void* out, void* workspace,
+                                         size_t workspace_bytes, unsigned flags);
+
+/* ---- drawing tokens from logits -----------------------------------------------------------------------------
+ * For each row of logits [rows, vocab] (row_stride in elements; dtype MUI_F16, MUI_BF16 or MUI_COMM_F32): with z =
+ * (logit - largest logit) / temperature and weights w = exp(z), tokens are ranked by logit, equal ones by index; kept are
+ * the first top_k of them, of those the shortest run from the front whose weights reach top_p of the top_k's weight (one
+ * token at least), and of those the ones with w >= min_p. The drawn token is the first one, in index order, at which the
+ * running weight of the kept ones exceeds uniform * their weight. temperature, top_k, top_p, min_p and uniforms ([rows];
+ * fp32, top_k int32) live on the device; NULL means 1, off, off, off; top_k <= 0, top_p >= 1 and min_p <= 0 are off too;
+ * a temperature that is not above 0 takes the largest logit (lowest index). Logits of -infinity or NaN are never drawn
+ * (a row of nothing else gives token 0). logprobs (may be NULL): log of the drawn token's share of the kept weight.
+ * Weights are evaluated in fp64 and summed in integers, so a result depends neither on the order of summation nor on
+ * the launch. The reference samples through Hugging Face's logits processors (examples/llama3_8b.py:51-58). */
+MUI_API mui_status_t mui_sample_tokens(void* stream, int dtype, int rows, int vocab, const void* logits,
+                                       int64_t row_stride, const float* temperature, const int32_t* top_k,
+                                       const float* top_p, const float* min_p, const float* uniforms, int64_t* tokens,
+                                       float* logprobs, unsigned flags);
+
 /* ---- decode stack ----------------------------------------------------------------------------------
  * One call launches every kernel of a decode step of a Llama-architecture model for `batch` sequences:
  * embedding, per layer {fused-norm QKV GEMV, RoPE + static-cache write, flash decoding, o_proj + residual,

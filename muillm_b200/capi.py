@@ -30,6 +30,9 @@ MUI_ACT_SILU = 1
 MUI_W8_SYM_ROW = 0
 MUI_W8_GROUP_MIN = 1
 
+MUI_KV_16BIT = 0
+MUI_KV_E4M3 = 1
+
 MUI_FLAG_PDL = 1
 MUI_FLAG_FORCE_GENERIC = 2
 MUI_FLAG_FORCE_PIPELINE = 4
@@ -39,6 +42,21 @@ MUI_FLAG_SPLIT_CONTEXT = 32
 
 class Strides3(Structure):
     _fields_ = [("batch", c_int64), ("head", c_int64), ("tok", c_int64)]
+
+
+class Strides2(Structure):
+    _fields_ = [("tok", c_int64), ("head", c_int64)]
+
+
+class PagedKV(Structure):
+    _fields_ = [
+        ("format", c_int),
+        ("num_pages", c_int), ("page_size", c_int), ("kv_heads", c_int), ("head_dim", c_int),
+        ("batch", c_int), ("table_stride", c_int), ("total_tokens", c_int),
+        ("k_pages", c_void_p), ("v_pages", c_void_p),
+        ("k_scales", c_void_p), ("v_scales", c_void_p),
+        ("block_table", c_void_p), ("context_lens", c_void_p), ("cu_tokens", c_void_p),
+    ]
 
 
 class DeviceProps(Structure):
@@ -245,6 +263,23 @@ PROTOTYPES = {
          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_uint],
     ),
     "mui_embedding_forward": (c_int, [c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_uint]),
+    "mui_paged_kv_append": (
+        c_int,
+        [c_void_p, c_int, POINTER(PagedKV), c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, Strides2, c_void_p,
+         Strides2, c_void_p, Strides2, c_void_p, c_uint],
+    ),
+    "mui_paged_attention_workspace_bytes": (
+        c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "mui_paged_attention": (
+        c_int,
+        [c_void_p, c_int, POINTER(PagedKV), c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, Strides2, c_void_p,
+         c_void_p, c_size_t, c_uint],
+    ),
+    "mui_sample_tokens": (
+        c_int,
+        [c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+         c_void_p, c_uint],
+    ),
     "mui_llama_stack_scratch_bytes": (c_size_t, [POINTER(LlamaConfig)]),
     "mui_llama_stack_create": (
         c_int, [POINTER(LlamaConfig), POINTER(LlamaWeights), c_void_p, c_size_t, POINTER(c_void_p)]),

@@ -1,0 +1,427 @@
+// Append of the new tokens' keys and values to a paged cache, the rotary position embedding of q and k applied on the
+// way:  (y_a, y_b) = (x_a cos - x_b sin, x_b cos + x_a sin)  for the pairs (a, b) of the first rotary_dim elements of a
+// head, evaluated in fp32 and rounded once.
+//
+// Traffic: (Hq + 2 Hkv) * D * 2 bytes in per token, Hq * D * 2 bytes (q) and 2 * Hkv * D * (2 or 1) bytes out, one
+// (cos, sin) row per position: bound by memory for prompts, by the launch and two dependent round trips (lengths, then
+// block table and rows) for single tokens.
+//
+//  * 16-bit pages: every (token, head) row is independent.
+//  * e4m3 pages: all new rows of one (page, head) share a scale, so they are one unit of work: its rows are rotated in
+//    registers, their largest magnitude gives the scale 2^e, rows that were in the page before are rescaled when it grew,
+//    the new rows are rounded. No atomics, and K and V are units of their own. The q rows of an e4m3 call are rows as above, in
+//    further CTAs of the same launch.
+// Eight consecutive elements of a row sit in one lane (16 bytes). In the half layout the partner of an element is
+// rotary_dim / 2 elements away: in another lane, fetched with a shuffle, when that distance is a multiple of eight.
+#include "paged_common.cuh"
+
+MUI_STATUS_ACCESSOR(paged_cache)
+
+namespace {
+
+constexpr int PC_THREADS = 256;
+constexpr int PC_WARPS = PC_THREADS / 32;
+
+struct AppendArgs {
+  PagedView kv;
+  const void *q, *k, *v;
+  mui_strides2_t qs, ks, vs;
+  void* q_out;
+  const float* freqs;
+  const int64_t* position_ids;
+  int Hq, max_positions, rotary, interleaved;
+  int head_blocks;  // row part: blocks of heads per token
+  int unit_blocks;  // CTAs of the e4m3 unit part
+  int units;        // (sequence, page) candidates of the e4m3 unit part
+};
+
+// (cos, sin) of the eight elements from d0 on of a head; identity outside the rotated part
+struct Turn {
+  float c[8], s[8];
+};
+__device__ __forceinline__ void load_turn(const AppendArgs& a, long long pos, int d0, Turn& t) {
+  const int half = a.rotary >> 1;
+  const float* row = a.freqs + (a.freqs ? pos * a.rotary : 0);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int d = d0 + i;
+    t.c[i] = 1.f;
+    t.s[i] = 0.f;
+    if (a.freqs != nullptr && d < a.rotary) {
+      const int pair = a.interleaved ? d >> 1 : (d < half ? d : d - half);
+      t.c[i] = row[2 * pair];
+      t.s[i] = row[2 * pair + 1];
+      if (a.interleaved ? !(d & 1) : d < half) t.s[i] = -t.s[i];  // first of the pair: minus sine
+    }
+  }
+}
+
+// The lane's eight elements of a row as fp32, rotated when `turn`. ALIGNED: rows are 16-byte aligned and, in the half
+// layout, rotary / 2 is a multiple of eight. Whole warp (shuffles); lanes of rows that do not exist pass row = nullptr.
+template <typename T, int D, bool ALIGNED>
+__device__ __forceinline__ void load_row8(const AppendArgs& a, const T* row, int d0, bool turn, const Turn& t,
+                                          float (&y)[8]) {
+  float x[8], p[8];
+  if (ALIGNED) {
+    const uint4 raw = row ? ld_act16(row + d0) : make_uint4(0, 0, 0, 0);
+    unpack8<T>(raw, x);
+    if (a.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = x[i ^ 1];
+    } else {
+      const int step = a.rotary >> 4;  // lanes from an element to its partner
+      const int l = d0 >> 3;
+      const int other = (threadIdx.x & 31) + (l < step ? step : -step);
+      const int src = l < 2 * step ? other : (threadIdx.x & 31);
+      uint4 q;
+      q.x = __shfl_sync(MUI_FULL_MASK, raw.x, src);
+      q.y = __shfl_sync(MUI_FULL_MASK, raw.y, src);
+      q.z = __shfl_sync(MUI_FULL_MASK, raw.z, src);
+      q.w = __shfl_sync(MUI_FULL_MASK, raw.w, src);
+      unpack8<T>(q, p);
+    }
+  } else {
+    const int half = a.rotary >> 1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = d0 + i;
+      int o = d;
+      if (d < a.rotary) o = a.interleaved ? (d ^ 1) : (d < half ? d + half : d - half);
+      x[i] = row ? ld_act_f32<T>(row + d) : 0.f;
+      p[i] = row ? ld_act_f32<T>(row + o) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (turn && d0 + i < a.rotary) ? fmaf(x[i], t.c[i], p[i] * t.s[i]) : x[i];
+}
+
+// sequence, place and rotary position of new token t; false for a token behind the last sequence. Whole warp.
+__device__ __forceinline__ bool find_token(const AppendArgs& a, int t, int& b, int& ctx, int& i) {
+  const int32_t* cu = a.kv.cu;
+  if (cu == nullptr) {
+    b = t;
+    i = 0;
+  } else {
+    b = warp_count_le(a.kv.batch, t, [&](int k) { return __ldcg(cu + 1 + k); });
+    if (b >= a.kv.batch) return false;
+    i = t - __ldcg(cu + b);
+  }
+  ctx = __ldcg(a.kv.context_lens + b);
+  if (ctx < 0) mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx));
+  return i >= 0 && ctx >= 0;
+}
+
+// rotary position of a token; false (and recorded) when the table does not hold it
+__device__ __forceinline__ bool find_position(const AppendArgs& a, int t, int ctx, int i, long long& pos) {
+  pos = a.position_ids ? __ldcg(a.position_ids + t) : static_cast<long long>(ctx) + i;
+  if (a.freqs == nullptr) return true;
+  if (pos >= 0 && pos < a.max_positions) return true;
+  mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(pos));
+  return false;
+}
+
+// page of cache position p of sequence b; -1 (and recorded) when there is none
+__device__ __forceinline__ int find_page(const PagedView& kv, int b, long long p) {
+  const long long idx = p >> kv.page_shift;
+  if (p < 0 || idx >= kv.table_stride) {
+    mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(p));
+    return -1;
+  }
+  const int page = __ldcg(kv.block_table + static_cast<size_t>(b) * kv.table_stride + idx);
+  if (page < 0 || page >= kv.num_pages) {
+    mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(b));
+    return -1;
+  }
+  return page;
+}
+
+// Rows of token t and the heads [block * STEPS * rows per step, ...) of the concatenation q | k | v (q only with QONLY).
+// A warp loads the (cos, sin) row once for all its heads.
+template <typename T, int D, bool ALIGNED, int STEPS, bool QONLY>
+__device__ __forceinline__ void append_rows(const AppendArgs& a, long long unit) {
+  constexpr int LPR = D / 8, RPS = 32 / LPR;
+  const int lane = threadIdx.x & 31;
+  const int t = static_cast<int>(unit / a.head_blocks);
+  const int h0 = static_cast<int>(unit % a.head_blocks) * (STEPS * RPS) + lane / LPR;
+  const int d0 = (lane % LPR) * 8;
+  if (t >= a.kv.total) return;
+  int b, ctx, i;
+  if (!find_token(a, t, b, ctx, i)) return;
+  long long pos;
+  if (!find_position(a, t, ctx, i, pos)) return;
+  const int heads = QONLY ? a.Hq : a.Hq + 2 * a.kv.kv_heads;
+  T* krow = nullptr;
+  T* vrow = nullptr;
+  if (!QONLY) {
+    const long long p = static_cast<long long>(ctx) + i;
+    const int page = find_page(a.kv, b, p);
+    if (page >= 0) {
+      const size_t off = ((static_cast<size_t>(page) * a.kv.kv_heads << a.kv.page_shift) +
+                          static_cast<size_t>(p & ((1 << a.kv.page_shift) - 1))) * D + d0;
+      krow = reinterpret_cast<T*>(a.kv.k_pages) + off;
+      vrow = reinterpret_cast<T*>(a.kv.v_pages) + off;
+    }
+  }
+  Turn turn;
+  load_turn(a, pos, d0, turn);
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st) {
+    int h = h0 + st * RPS;
+    const T* in = nullptr;
+    T* out = nullptr;
+    bool rot = true;
+    if (h < a.Hq) {
+      in = reinterpret_cast<const T*>(a.q) + t * a.qs.tok + h * a.qs.head;
+      out = reinterpret_cast<T*>(a.q_out) + (static_cast<size_t>(t) * a.Hq + h) * D + d0;
+    } else if (h < heads) {
+      h -= a.Hq;
+      rot = h < a.kv.kv_heads;
+      if (!rot) h -= a.kv.kv_heads;
+      in = rot ? reinterpret_cast<const T*>(a.k) + t * a.ks.tok + h * a.ks.head
+               : reinterpret_cast<const T*>(a.v) + t * a.vs.tok + h * a.vs.head;
+      out = rot ? krow : vrow;
+      if (out != nullptr) out += (static_cast<size_t>(h) << a.kv.page_shift) * D;
+    }
+    float y[8];
+    load_row8<T, D, ALIGNED>(a, in, d0, rot && a.freqs != nullptr, turn, y);
+    if (out != nullptr) *reinterpret_cast<uint4*>(out) = pack8<T>(y);
+  }
+}
+
+template <typename T, int D, bool ALIGNED, int STEPS>
+__global__ void __launch_bounds__(PC_THREADS) append_rows_kernel(const AppendArgs a) {
+  pdl_wait_prior_grid();
+  pdl_launch_dependents();
+  append_rows<T, D, ALIGNED, STEPS, false>(a, static_cast<long long>(blockIdx.x) * PC_WARPS + (threadIdx.x >> 5));
+}
+
+// One unit: the new rows of K (which == 0) or V of one head in one page, by `GROUPS` groups of D / 8 lanes (group index
+// `group`), at most ROWS rows per group. BLOCK: the groups span the CTA, else one warp.
+template <typename T, int D, bool ALIGNED, int ROWS, bool BLOCK>
+__device__ __forceinline__ void append_unit(const AppendArgs& a, int b, int first_row, int count, int ctx, int page_idx,
+                                            int head, int which, float* s_max) {
+  constexpr int LPR = D / 8;
+  constexpr int GROUPS = (BLOCK ? PC_THREADS : 32) / LPR;
+  const int tid = BLOCK ? threadIdx.x : (threadIdx.x & 31);
+  const int group = tid / LPR, d0 = (tid % LPR) * 8;
+  const int ps = 1 << a.kv.page_shift;
+  const long long p0 = static_cast<long long>(page_idx) << a.kv.page_shift;  // first position of the page
+  const int lo = p0 < ctx ? static_cast<int>(ctx - p0) : 0;                   // slots [lo, hi) are new
+  const int hi = static_cast<int>(min(static_cast<long long>(ps), static_cast<long long>(ctx) + count - p0));
+  const int page = find_page(a.kv, b, p0);
+  if (page < 0) return;
+  const T* in = which == 0 ? reinterpret_cast<const T*>(a.k) + head * a.ks.head
+                           : reinterpret_cast<const T*>(a.v) + head * a.vs.head;
+  const int64_t tok_stride = which == 0 ? a.ks.tok : a.vs.tok;
+  float* scale_p = (which == 0 ? a.kv.k_scales : a.kv.v_scales) + static_cast<size_t>(page) * a.kv.kv_heads + head;
+  uint8_t* out = reinterpret_cast<uint8_t*>(which == 0 ? a.kv.k_pages : a.kv.v_pages) +
+                 ((static_cast<size_t>(page) * a.kv.kv_heads + head) << a.kv.page_shift) * D + d0;
+  const float old_scale = lo > 0 ? __ldcg(scale_p) : 0.f;
+
+  float y[ROWS][8];
+  bool have[ROWS];
+  float amax = 0.f;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int slot = lo + r * GROUPS + group;
+    const int i = static_cast<int>(p0 - ctx) + slot;  // place among the sequence's new tokens
+    have[r] = slot < hi;
+    long long pos = 0;
+    if (have[r]) have[r] = find_position(a, first_row + i, ctx, i, pos);
+    Turn turn;
+    const bool rot = which == 0 && a.freqs != nullptr;
+    if (rot) load_turn(a, have[r] ? pos : 0, d0, turn);
+    load_row8<T, D, ALIGNED>(a, have[r] ? in + (first_row + i) * tok_stride : nullptr, d0, rot, turn, y[r]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float m = fabsf(y[r][e]);
+      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);  // false for infinities and NaN
+    }
+  }
+  amax = warp_max(amax);
+  if (BLOCK) {
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+    __syncthreads();  // also: every thread has read the old scale
+#pragma unroll
+    for (int w = 0; w < PC_WARPS; ++w) amax = fmaxf(amax, s_max[w]);
+  }
+  float scale = exp2_int(e4m3_scale_exp(amax));
+  float inv = exp2_int(-e4m3_scale_exp(amax));
+  if (lo > 0 && !(old_scale < scale)) {
+    scale = old_scale;
+    inv = 1.f / old_scale;
+  } else if (lo > 0) {
+    // the page's earlier rows move to the larger scale
+    const float ratio = old_scale * inv;
+    for (int slot = group; slot < lo; slot += GROUPS) {
+      uint2* p = reinterpret_cast<uint2*>(out + static_cast<size_t>(slot) * D);
+      const uint2 w = __ldcg(p);
+      uint32_t n[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t u = h == 0 ? w.x : w.y;
+        const float2 f0 = Elt<__half>::unpack2(e4m3_to_half2(static_cast<uint16_t>(u)));
+        const float2 f1 = Elt<__half>::unpack2(e4m3_to_half2(static_cast<uint16_t>(u >> 16)));
+        n[h] = e4m3_pack2(f0.x * ratio, f0.y * ratio) | (e4m3_pack2(f1.x * ratio, f1.y * ratio) << 16);
+      }
+      *p = make_uint2(n[0], n[1]);
+    }
+  }
+  if (!BLOCK) __syncwarp();
+  if (tid == 0) *scale_p = scale;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (!have[r]) continue;
+    const int slot = lo + r * GROUPS + group;
+    uint2 w;
+    w.x = e4m3_pack2(y[r][0] * inv, y[r][1] * inv) | (e4m3_pack2(y[r][2] * inv, y[r][3] * inv) << 16);
+    w.y = e4m3_pack2(y[r][4] * inv, y[r][5] * inv) | (e4m3_pack2(y[r][6] * inv, y[r][7] * inv) << 16);
+    *reinterpret_cast<uint2*>(out + static_cast<size_t>(slot) * D) = w;
+  }
+}
+
+// e4m3 pages, one new token per sequence: a warp per (sequence, head, K or V), then the q rows.
+template <typename T, int D, bool ALIGNED>
+__global__ void __launch_bounds__(PC_THREADS) append_e4m3_token_kernel(const AppendArgs a) {
+  pdl_wait_prior_grid();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5;
+  if (static_cast<int>(blockIdx.x) >= a.unit_blocks) {
+    append_rows<T, D, ALIGNED, 1, true>(a, static_cast<long long>(blockIdx.x - a.unit_blocks) * PC_WARPS + warp);
+    return;
+  }
+  const long long u = static_cast<long long>(blockIdx.x) * PC_WARPS + warp;
+  const int per_seq = 2 * a.kv.kv_heads;
+  const int b = static_cast<int>(u / per_seq), r = static_cast<int>(u % per_seq);
+  if (b >= a.kv.batch) return;
+  const int ctx = __ldcg(a.kv.context_lens + b);
+  if (ctx < 0) {
+    mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx));
+    return;
+  }
+  append_unit<T, D, ALIGNED, 1, false>(a, b, b, 1, ctx, ctx >> a.kv.page_shift, r >> 1, r & 1, nullptr);
+}
+
+// e4m3 pages, any number of new tokens: a CTA per (sequence, page, head, K or V), then the q rows. Units are numbered
+// through: sequence b's start at cu[b] / page_size + 2 b, which leaves room for every page that its tokens can touch.
+template <typename T, int D, bool ALIGNED, int ROWS>
+__global__ void __launch_bounds__(PC_THREADS) append_e4m3_kernel(const AppendArgs a) {
+  __shared__ float s_max[PC_WARPS];
+  pdl_wait_prior_grid();
+  pdl_launch_dependents();
+  if (static_cast<int>(blockIdx.x) >= a.unit_blocks) {
+    append_rows<T, D, ALIGNED, 4, true>(
+        a, static_cast<long long>(blockIdx.x - a.unit_blocks) * PC_WARPS + (threadIdx.x >> 5));
+    return;
+  }
+  const int per_page = 2 * a.kv.kv_heads;
+  const int u = blockIdx.x / per_page, r = blockIdx.x % per_page;
+  const int32_t* cu = a.kv.cu;
+  const int sh = a.kv.page_shift;
+  const int b = warp_count_le(a.kv.batch, u, [&](int k) { return (__ldcg(cu + 1 + k) >> sh) + 2 * (k + 1); });
+  if (b >= a.kv.batch) return;
+  int first, count;
+  paged_new_tokens(a.kv, b, first, count);
+  const int ctx = __ldcg(a.kv.context_lens + b);
+  if (ctx < 0) {
+    if (threadIdx.x == 0) mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx));
+    return;
+  }
+  const int page_idx = (ctx >> sh) + u - ((first >> sh) + 2 * b);
+  if (count == 0 || (static_cast<long long>(page_idx) << sh) >= static_cast<long long>(ctx) + count) return;
+  append_unit<T, D, ALIGNED, ROWS, true>(a, b, first, count, ctx, page_idx, r >> 1, r & 1, s_max);
+}
+
+template <typename T, int D, bool ALIGNED>
+mui_status_t launch_append(cudaStream_t stream, AppendArgs a, bool e4m3, int page_size, unsigned flags) {
+  constexpr int RPS = 32 / (D / 8);
+  const int pdl = (flags & MUI_FLAG_PDL) ? 1 : 0;
+  const dim3 block(PC_THREADS);
+  const long long limit = 0x7fffffff;
+  auto blocks = [](long long units) { return (units + PC_WARPS - 1) / PC_WARPS; };
+  if (!e4m3) {
+    // one step of rows per warp while that leaves the GPU unfilled, four (loads in flight, shared table row) above
+    const int heads = a.Hq + 2 * a.kv.kv_heads;
+    const long long one = static_cast<long long>(a.kv.total) * ((heads + RPS - 1) / RPS);
+    const bool wide = one > 148 * 64;
+    a.head_blocks = wide ? (heads + 4 * RPS - 1) / (4 * RPS) : (heads + RPS - 1) / RPS;
+    const long long n = blocks(static_cast<long long>(a.kv.total) * a.head_blocks);
+    MUI_REQUIRE(n <= limit, MUI_ERR_UNSUPPORTED, "too many rows");
+    if (wide)
+      MUI_CUDA_CHECK(mui_launch(append_rows_kernel<T, D, ALIGNED, 4>, dim3((unsigned)n), block, 0, stream, pdl, a));
+    else
+      MUI_CUDA_CHECK(mui_launch(append_rows_kernel<T, D, ALIGNED, 1>, dim3((unsigned)n), block, 0, stream, pdl, a));
+    return MUI_OK;
+  }
+  if (a.kv.cu == nullptr) {
+    a.head_blocks = (a.Hq + RPS - 1) / RPS;
+    a.unit_blocks = static_cast<int>(blocks(static_cast<long long>(a.kv.batch) * 2 * a.kv.kv_heads));
+    const long long n = a.unit_blocks + blocks(static_cast<long long>(a.kv.total) * a.head_blocks);
+    MUI_REQUIRE(n <= limit, MUI_ERR_UNSUPPORTED, "too many rows");
+    MUI_CUDA_CHECK(mui_launch(append_e4m3_token_kernel<T, D, ALIGNED>, dim3((unsigned)n), block, 0, stream, pdl, a));
+    return MUI_OK;
+  }
+  a.head_blocks = (a.Hq + 4 * RPS - 1) / (4 * RPS);
+  const long long units = static_cast<long long>(a.kv.total / page_size + 2 * a.kv.batch) * 2 * a.kv.kv_heads;
+  const long long n = units + blocks(static_cast<long long>(a.kv.total) * a.head_blocks);
+  MUI_REQUIRE(n <= limit, MUI_ERR_UNSUPPORTED, "too many rows");
+  a.unit_blocks = static_cast<int>(units);
+  constexpr int GROUPS = PC_THREADS / (D / 8);  // 16 rows at a time for head dim 128, 32 for 64
+  const int rows = (page_size + GROUPS - 1) / GROUPS;
+  if (rows <= 1)
+    MUI_CUDA_CHECK(mui_launch(append_e4m3_kernel<T, D, ALIGNED, 1>, dim3((unsigned)n), block, 0, stream, pdl, a));
+  else if (rows <= 2)
+    MUI_CUDA_CHECK(mui_launch(append_e4m3_kernel<T, D, ALIGNED, 2>, dim3((unsigned)n), block, 0, stream, pdl, a));
+  else if (rows <= 4)
+    MUI_CUDA_CHECK(mui_launch(append_e4m3_kernel<T, D, ALIGNED, 4>, dim3((unsigned)n), block, 0, stream, pdl, a));
+  else
+    MUI_CUDA_CHECK(mui_launch(append_e4m3_kernel<T, D, ALIGNED, 8>, dim3((unsigned)n), block, 0, stream, pdl, a));
+  return MUI_OK;
+}
+
+bool row_aligned(const void* p, const mui_strides2_t& s) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (s.tok & 7) == 0 && (s.head & 7) == 0;
+}
+
+}  // namespace
+
+extern "C" mui_status_t mui_paged_kv_append(void* stream, mui_dtype_t dtype, const mui_paged_kv_t* cache,
+                                            int num_q_heads, const float* freqs, int max_positions, int rotary_dim,
+                                            int interleaved, const int64_t* position_ids, const void* q,
+                                            mui_strides2_t q_strides, const void* k, mui_strides2_t k_strides,
+                                            const void* v, mui_strides2_t v_strides, void* q_out, unsigned flags) {
+  if (mui_status_t s = paged_check(dtype, cache)) return s;
+  MUI_REQUIRE(num_q_heads >= 0, MUI_ERR_INVALID_ARG, "num_q_heads=%d", num_q_heads);
+  MUI_REQUIRE(freqs == nullptr || (max_positions >= 1 && rotary_dim >= 2 && rotary_dim <= cache->head_dim &&
+                                   (rotary_dim & 1) == 0),
+              MUI_ERR_INVALID_ARG, "rotary_dim=%d (even, 2..head_dim) or max_positions=%d (>= 1) out of range",
+              rotary_dim, max_positions);
+  if (cache->batch == 0 || cache->total_tokens == 0) return MUI_OK;
+  MUI_REQUIRE(k && v && (num_q_heads == 0 || (q && q_out)), MUI_ERR_INVALID_ARG, "q, k, v and q_out must be non-null");
+  MUI_REQUIRE((reinterpret_cast<uintptr_t>(q_out) & 15) == 0, MUI_ERR_INVALID_ARG, "q_out must be 16-byte aligned");
+  AppendArgs a = {};
+  a.kv = paged_view(*cache);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.qs = q_strides;
+  a.ks = k_strides;
+  a.vs = v_strides;
+  a.q_out = q_out;
+  a.freqs = freqs;
+  a.position_ids = position_ids;
+  a.Hq = num_q_heads;
+  a.max_positions = max_positions;
+  a.rotary = freqs ? rotary_dim : 0;
+  a.interleaved = interleaved != 0;
+  const bool aligned = (num_q_heads == 0 || row_aligned(q, q_strides)) && row_aligned(k, k_strides) &&
+                       row_aligned(v, v_strides) && (a.interleaved || (a.rotary & 15) == 0);
+  const bool e4m3 = cache->format == MUI_KV_E4M3;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int ps = cache->page_size;
+#define PC_GO(T, D) \
+  (aligned ? launch_append<T, D, true>(st, a, e4m3, ps, flags) : launch_append<T, D, false>(st, a, e4m3, ps, flags))
+  if (dtype == MUI_F16) return cache->head_dim == 128 ? PC_GO(__half, 128) : PC_GO(__half, 64);
+  return cache->head_dim == 128 ? PC_GO(__nv_bfloat16, 128) : PC_GO(__nv_bfloat16, 64);
+#undef PC_GO
+}

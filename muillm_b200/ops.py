@@ -529,3 +529,182 @@ def muillm_add_tokens_check_finished(input_ids, next_tokens, unfinished_sequence
         1 if has_max_length_stopping_criteria else 0, int(max_length if max_length is not None else -1), _ptr(out),
         _ptr(unf), flags))
     return out, unf
+
+
+# ---- paged KV cache and sampling --------------------------------------------------------------------------------
+
+
+def _check_on(device, t, name, dtype):
+    """t must be a contiguous `dtype` tensor on CUDA device number `device`."""
+    if t.get_device() != device:
+        raise RuntimeError(f"{name} must be on CUDA device {device}, the device of the other tensors")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must be of type {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+
+
+def _current_device_of(t, name):
+    device = t.get_device()
+    if device < 0:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if device != torch.cuda.current_device():
+        raise RuntimeError(f"{name} is on CUDA device {device}, which is not the current one")
+    return device
+
+
+def _check_rows3(device, t, name, total, heads, dim, dtype):
+    """A [total, heads, dim] view whose innermost stride is 1; returns its strides."""
+    if t.get_device() != device:
+        raise RuntimeError(f"{name} must be on CUDA device {device}, the device of the other tensors")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{name} must be of type {dtype}, got {t.dtype}")
+    if t.dim() != 3 or t.shape[0] != total or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise RuntimeError(f"{name} must be [{total}, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
+    s = t.stride()
+    if s[2] != 1 and t.numel():
+        raise RuntimeError(f"{name} must have innermost stride 1")
+    return capi.Strides2(s[0], s[1])
+
+
+def _paged_kv(device, dtype, total, k_pages, v_pages, block_table, context_lens, cu_tokens, k_scales, v_scales):
+    """Checks the tensors of a paged cache and describes them for the C ABI."""
+    if k_pages.dim() != 4:
+        raise RuntimeError("pages must be [num_pages, kv_heads, page_size, head_dim]")
+    num_pages, kv_heads, page_size, head_dim = k_pages.shape
+    if v_pages.shape != k_pages.shape:
+        raise RuntimeError("k_pages and v_pages must have the same shape")
+    e4m3 = k_pages.dtype == torch.float8_e4m3fn
+    page_dtype = torch.float8_e4m3fn if e4m3 else dtype
+    _check_on(device, k_pages, "k_pages", page_dtype)
+    _check_on(device, v_pages, "v_pages", page_dtype)
+    if e4m3:
+        if k_scales is None or v_scales is None:
+            raise RuntimeError("float8_e4m3fn pages need k_scales and v_scales")
+        _check_on(device, k_scales, "k_scales", torch.float32)
+        _check_on(device, v_scales, "v_scales", torch.float32)
+        if k_scales.shape != (num_pages, kv_heads) or v_scales.shape != (num_pages, kv_heads):
+            raise RuntimeError(f"scales must be [{num_pages}, {kv_heads}]")
+    elif k_scales is not None or v_scales is not None:
+        raise RuntimeError("16-bit pages take no scales")
+    _check_on(device, context_lens, "context_lens", torch.int32)
+    _check_on(device, block_table, "block_table", torch.int32)
+    batch = context_lens.shape[0]
+    if context_lens.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != batch:
+        raise RuntimeError("context_lens must be [batch] and block_table [batch, pages]")
+    if cu_tokens is not None:
+        _check_on(device, cu_tokens, "cu_tokens", torch.int32)
+        if cu_tokens.shape != (batch + 1,):
+            raise RuntimeError(f"cu_tokens must be [{batch + 1}]")
+    elif total != batch:
+        raise RuntimeError(f"without cu_tokens there is one new token per sequence: {total} rows for {batch} sequences")
+    return capi.PagedKV(
+        capi.MUI_KV_E4M3 if e4m3 else capi.MUI_KV_16BIT, num_pages, page_size, kv_heads, head_dim, batch,
+        block_table.shape[1], total, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
+        block_table.data_ptr(), context_lens.data_ptr(), _ptr(cu_tokens))
+
+
+def paged_kv_append(k_pages, v_pages, block_table, context_lens, q, k, v, freqs=None, cu_tokens=None, rotary_dim=None,
+                    interleaved=False, k_scales=None, v_scales=None, position_ids=None, q_out=None, flags=0):
+    """Writes the new tokens' rotated keys and their values to a paged cache and returns the rotated q.
+
+    k_pages, v_pages [num_pages, kv_heads, page_size, head_dim] of the model's 16-bit dtype, or float8_e4m3fn with fp32
+    scales [num_pages, kv_heads] (powers of two, kept by this call); block_table [batch, pages] int32; context_lens
+    [batch] int32, the tokens each sequence has in the cache before this call. q [total, Hq, head_dim], k and v [total,
+    kv_heads, head_dim] are views with innermost stride 1 (slices of the packed QKV projection): the new tokens of all
+    sequences one after the other, split by cu_tokens [batch + 1] int32, or one token per sequence without it. q may be
+    None. freqs [positions, rotary_dim / 2, 2] fp32 holds (cos, sin) pairs; the first rotary_dim elements of a head
+    (default: as many as freqs has) are turned in the half or the interleaved layout; position_ids [total] int64 stands
+    in for the cache positions as rotary positions. mui_paged_kv_append in the C ABI."""
+    device = _current_device_of(k, "k")
+    total = k.shape[0]
+    if k.dim() != 3 or k_pages.dim() != 4:
+        raise RuntimeError("k must be [total, kv_heads, head_dim] and pages [num_pages, kv_heads, page_size, head_dim]")
+    kv = _paged_kv(device, k.dtype, total, k_pages, v_pages, block_table, context_lens, cu_tokens, k_scales, v_scales)
+    D = kv.head_dim
+    ks = _check_rows3(device, k, "k", total, kv.kv_heads, D, k.dtype)
+    vs = _check_rows3(device, v, "v", total, kv.kv_heads, D, k.dtype)
+    heads, qs = 0, ks
+    if q is not None:
+        heads, qs = q.shape[1], _check_rows3(device, q, "q", total, None, D, k.dtype)
+        if q_out is None:
+            q_out = torch.empty((total, heads, D), dtype=k.dtype, device=k.device)
+        else:
+            _check_on(device, q_out, "q_out", k.dtype)
+            if q_out.shape != (total, heads, D):
+                raise RuntimeError(f"q_out must be [{total}, {heads}, {D}]")
+    max_pos = rot = 0
+    if freqs is not None:
+        _check_on(device, freqs, "freqs", torch.float32)
+        if freqs.dim() != 3 or freqs.shape[2] != 2 or (rotary_dim is not None and rotary_dim != 2 * freqs.shape[1]):
+            raise RuntimeError("freqs must be [positions, rotary_dim / 2, 2]")
+        max_pos, rot = freqs.shape[0], 2 * freqs.shape[1]
+    if position_ids is not None:
+        _check_on(device, position_ids, "position_ids", torch.int64)
+        if position_ids.shape != (total,):
+            raise RuntimeError(f"position_ids must be [{total}]")
+    capi.check(capi.lib().mui_paged_kv_append(
+        _stream(), _dtype_code(k), ctypes.byref(kv), heads, _ptr(freqs), max_pos, rot, 1 if interleaved else 0,
+        _ptr(position_ids), _ptr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ptr(q_out), flags))
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, block_table, context_lens, cu_tokens=None, max_new_tokens=None, k_scales=None,
+                    v_scales=None, scale=None, window=0, sinks=0, max_context=None, out=None, flags=0):
+    """Causal attention of the new tokens' queries over a paged cache that already holds their own rows (paged_kv_append
+    of the same description). q [total, Hq, head_dim] (a view with innermost stride 1), the cache tensors, context_lens
+    and cu_tokens as in paged_kv_append; max_new_tokens bounds the new tokens of every sequence (default: 1 without
+    cu_tokens, else total). window > 0 limits a token at position p to the rows j > p - window and the first `sinks`
+    rows. max_context is the longest sequence expected, a hint for the split of the work (default: the block table's
+    reach). Returns [total, Hq, head_dim]. mui_paged_attention in the C ABI."""
+    device = _current_device_of(q, "q")
+    total = q.shape[0]
+    kv = _paged_kv(device, q.dtype, total, k_pages, v_pages, block_table, context_lens, cu_tokens, k_scales, v_scales)
+    D = kv.head_dim
+    qs = _check_rows3(device, q, "q", total, None, D, q.dtype)
+    heads = q.shape[1]
+    if out is None:
+        out = torch.empty((total, heads, D), dtype=q.dtype, device=q.device)
+    else:
+        _check_on(device, out, "out", q.dtype)
+        if out.shape != (total, heads, D):
+            raise RuntimeError(f"out must be [{total}, {heads}, {D}]")
+    if max_new_tokens is None:
+        max_new_tokens = 1 if cu_tokens is None else max(1, total)
+    if max_context is None:
+        max_context = kv.table_stride * kv.page_size
+    lib = capi.lib()
+    # scratch of its own for every call: calls on several streams, or captured in several graphs, share nothing
+    nbytes = lib.mui_paged_attention_workspace_bytes(total, kv.batch, heads, kv.kv_heads, D, max_new_tokens, max_context,
+                                                     window, sinks)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    capi.check(lib.mui_paged_attention(
+        _stream(), _dtype_code(q), ctypes.byref(kv), heads, max_new_tokens, max_context, window, sinks,
+        scale if scale is not None else 1.0 / math.sqrt(D), q.data_ptr(), qs, out.data_ptr(), _ptr(ws), nbytes, flags))
+    return out
+
+
+def sample_tokens(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, flags=0):
+    """Draws one token per row of logits [rows, vocab] (fp16, bf16 or fp32, rows may be strided) from the given uniform
+    numbers [rows] in [0, 1): temperature, then the top_k largest logits (ties by index), of those the shortest run that
+    holds top_p of their probability, of those the ones with at least min_p times the largest probability; the token is
+    the first one in index order at which the running probability exceeds the uniform number. Parameters are per-row
+    tensors on the device (fp32; top_k int32) or None for off; a temperature of 0 takes the largest logit. Returns
+    (tokens int64 [rows], logprobs fp32 [rows] of the drawn tokens among the kept ones). mui_sample_tokens in the C ABI."""
+    device = _current_device_of(logits, "logits")
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise RuntimeError("logits must be [rows, vocab] with innermost stride 1")
+    rows, vocab = logits.shape
+    code = capi.MUI_COMM_F32 if logits.dtype == torch.float32 else _dtype_code(logits)
+    for t, name in ((uniforms, "uniforms"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"),
+                    (top_k, "top_k")):
+        if t is not None:
+            _check_on(device, t, name, torch.int32 if name == "top_k" else torch.float32)
+            if t.shape != (rows,):
+                raise RuntimeError(f"{name} must be [{rows}]")
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    capi.check(capi.lib().mui_sample_tokens(
+        _stream(), code, rows, vocab, logits.data_ptr(), logits.stride(0), _ptr(temperature), _ptr(top_k), _ptr(top_p),
+        _ptr(min_p), uniforms.data_ptr(), tokens.data_ptr(), logprobs.data_ptr(), flags))
+    return tokens, logprobs
