@@ -526,7 +526,7 @@ MUI_API mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const 
  * For each row of logits [rows, vocab] (row_stride in elements; dtype MUI_F16, MUI_BF16 or MUI_COMM_F32): with z =
  * (logit - largest logit) / temperature and weights w = exp(z), tokens are ranked by logit, equal ones by index; kept are
  * the first top_k of them, of those the shortest run from the front whose weights reach top_p of the top_k's weight (one
- * token at least), and of those the ones with w >= min_p. The drawn token is the first one, in index order, at which the
+ * token at least), and of those the ones with w >= min(min_p, 1). The drawn token is the first one, in index order, at which the
  * running weight of the kept ones exceeds uniform * their weight. temperature, top_k, top_p, min_p and uniforms ([rows];
  * fp32, top_k int32) live on the device; NULL means 1, off, off, off; top_k <= 0, top_p >= 1 and min_p <= 0 are off too;
  * a temperature that is not above 0 takes the largest logit (lowest index). Logits of -infinity or NaN are never drawn

@@ -108,10 +108,6 @@ __device__ __forceinline__ void load_tile(const PaArgs& a, Tile<KV8, D>& t, int 
   const bool there = page >= 0;
   const unsigned char* kp = reinterpret_cast<const unsigned char*>(a.kv.k_pages) + row0 * (D * ES) + q * 16;
   const unsigned char* vp = reinterpret_cast<const unsigned char*>(a.kv.v_pages) + row0 * (D * ES);
-  if (KV8) {
-    t.ks = there ? __ldcg(a.kv.k_scales + head) : 0.f;
-    t.vs = there ? __ldcg(a.kv.v_scales + head) : 0.f;
-  }
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     // a row that nobody sees is not read: what it holds (another owner's bytes, NaN) must not matter
@@ -237,25 +233,44 @@ __global__ void __launch_bounds__(PA_THREADS) paged_decode_kernel(const PaArgs a
     for (int j = 0; j < MT; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.f;
   }
 
+  // The warp's tiles in the order in which it takes them: U neighbours, then the next U that are its own. Pages and scales of 32
+  // of them are looked up at a time, one per lane, so that K and V do not wait for the block table tile by tile.
   const int32_t* table = a.kv.block_table + static_cast<size_t>(b) * a.kv.table_stride;
-  auto page_of = [&](int tile) {
-    const int page = __ldcg(table + (tile * PA_TILE >> a.kv.page_shift));
-    if (page < 0 || page >= a.kv.num_pages) {
-      if (lane == 0) mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(b));
-      return -1;
+  constexpr int STEP = PA_WARPS * U;
+  const int i_begin = split * per + warp * U;
+  int my_page = -1, my_tb = -1;
+  float my_ks = 0.f, my_vs = 0.f;
+  auto look_up = [&](int n0) {
+    const int n = n0 + lane, i = i_begin + (n / U) * STEP + n % U;
+    my_page = my_tb = -1;
+    my_ks = my_vs = 0.f;
+    if (i < i_end) {
+      const int tile = span_tile(sp, i);
+      const int page = __ldcg(table + (tile * PA_TILE >> a.kv.page_shift));
+      if (page >= 0 && page < a.kv.num_pages) {
+        my_page = page;
+        my_tb = tile * PA_TILE;
+        if (KV8) {
+          const size_t head = static_cast<size_t>(page) * a.kv.kv_heads + kvh;
+          my_ks = __ldcg(a.kv.k_scales + head);
+          my_vs = __ldcg(a.kv.v_scales + head);
+        }
+      } else {
+        mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(b));
+      }
     }
-    return page;
   };
-  // U tiles at a time per warp; tiles beyond the end are given page -1 (all of them masked)
-  auto fetch = [&](int i, Tile<KV8, D>(&t)[U], int (&tb)[U]) {
+  // tiles n .. n + U - 1 of the warp; those beyond the end have page -1 (all of them masked). n rises from call to call.
+  auto fetch = [&](int n, Tile<KV8, D>(&t)[U], int (&tb)[U]) {
+    if ((n & 31) == 0) look_up(n);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      int page = -1;
-      tb[u] = -1;
-      if (i + u < i_end) {
-        const int tile = span_tile(sp, i + u);
-        page = page_of(tile);
-        tb[u] = page < 0 ? -1 : tile * PA_TILE;
+      const int from = (n + u) & 31;
+      const int page = __shfl_sync(MUI_FULL_MASK, my_page, from);
+      tb[u] = __shfl_sync(MUI_FULL_MASK, my_tb, from);
+      if (KV8) {
+        t[u].ks = __shfl_sync(MUI_FULL_MASK, my_ks, from);
+        t[u].vs = __shfl_sync(MUI_FULL_MASK, my_vs, from);
       }
       load_tile<KV8, D>(a, t[u], page, kvh, max(tb[u], 0), sp.kv_len, sp.lo_min);
     }
@@ -399,15 +414,15 @@ __global__ void __launch_bounds__(PA_THREADS) paged_decode_kernel(const PaArgs a
     // two register sets: the loads of one are in flight while the other is multiplied
     Tile<KV8, D> t0[U], t1[U];
     int tb0[U], tb1[U];
-    int i = split * per + warp * U;
-    constexpr int STEP = PA_WARPS * U;
-    fetch(i, t0, tb0);
-    for (; i < i_end; i += 2 * STEP) {
-      fetch(i + STEP, t1, tb1);
+    int n = 0;
+    fetch(n, t0, tb0);
+    for (int i = i_begin; i < i_end; i += 2 * STEP) {
+      fetch(n + U, t1, tb1);
       consume(t0, tb0);
       if (i + STEP >= i_end) break;
-      fetch(i + 2 * STEP, t0, tb0);
+      fetch(n + 2 * U, t0, tb0);
       consume(t1, tb1);
+      n += 2 * U;
     }
   }
 

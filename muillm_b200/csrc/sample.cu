@@ -1,23 +1,45 @@
 // Drawing a token from each row of logits: temperature, top-k, top-p, min-p, inverse transform of a given uniform number.
 //
-// With d = (logit - largest) / temperature and w = exp(d), the kept tokens are a run from the front of the ranking by
-// (logit descending, index ascending): all tokens above a threshold logit and the first few at it. No sort is needed, only
-// the threshold: the largest key T for which the tokens >= T number top_k, or weigh top_p of the total.
+// With z = (logit - largest) / temperature and w = exp(z), the kept tokens are a run from the front of the ranking by
+// (logit descending, index ascending), so two numbers describe them: kept is key > T, or key == T and index <= T_idx. No
+// sort is needed, only that threshold.
 //
 // Sums of weights decide which token is drawn, so they must not depend on the order in which threads add: w is taken in
-// fp64 and rounded once to a 64-bit integer with S fraction bits (S = 62 - ceil(log2 vocab), 44 for 200 k tokens: no sum
-// overflows), and integers are summed. Against real arithmetic a boundary is off by at most vocab * 2^-(S+1) of the largest
-// weight, about 1e-8 in the worst case and sqrt(vocab) * 2^-S in practice.
+// fp64 and rounded once to an integer with S fraction bits (S = min(50, 62 - ceil(log2 vocab)); 44 for 200 k tokens; no sum
+// overflows), and integers are summed. A weight that rounds to 0 can never be drawn. Against real arithmetic a boundary is
+// off by sqrt(vocab) * 2^-S of the largest weight or so, 3e-11 for 200 k tokens.
+//
+// A cluster of up to eight CTAs works on a row (one CTA when there are rows enough to fill the GPU). Passes over the row:
+//   1. the largest logit (from HBM; the later passes find the row in L2);
+//   2. a histogram of z in 2048 equal bins down to the smallest z that still has weight. Counts give the bin that holds
+//      the top_k-th token exactly; counts times the bin centre's weight tell the bin in which top_p ends, nearly always;
+//   3. exact sums of the weight above and between these two bins; the bins' own tokens (some hundred) are collected in rank
+//      0's shared memory, ranked by comparing all pairs, and give T and T_idx;
+//   4. the kept weight of every run of 256 tokens; the run that holds the drawn point is then walked by one warp.
+// Without top-k and top-p only 1 and 4 run. Where a bin has more tokens than the list holds (long ties, high temperatures)
+// or the estimate of 2 was a bin off, T and T_idx are found by bisection over keys and indices instead: slower, same result.
+//
+// Bound: rows * vocab * size bytes for large batches, then 13 fp64 operations a weight; for few rows the chain of passes and
+// cluster barriers.
 #include "common.cuh"
 
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 MUI_STATUS_ACCESSOR(sample)
 
 namespace {
 
+typedef unsigned long long u64;
+
 constexpr int SM_THREADS = 1024;
 constexpr int SM_WARPS = SM_THREADS / 32;
+constexpr int SM_CHUNK = 256;    // tokens of one warp step: eight consecutive ones per lane
+constexpr int SM_BINS = 2048;
+constexpr int SM_LIST = 2048;    // tokens collected per boundary bin
+constexpr int SM_RUNS = 1024;    // runs of chunks whose kept weight a CTA holds
+constexpr int SM_MAX_CLUSTER = 8;
 
 struct SampleArgs {
   const void* logits;
@@ -26,17 +48,8 @@ struct SampleArgs {
   const int32_t* top_k;
   int64_t* tokens;
   float* logprobs;
-  int V, frac_bits;
+  int V, frac_bits, cluster, chunks_per_run;
 };
-
-template <typename T>
-__device__ __forceinline__ float logit_at(const T* row, int i) {
-  return ld_act_f32<T>(row + i);
-}
-template <>
-__device__ __forceinline__ float logit_at<float>(const float* row, int i) {
-  return __ldcg(row + i);
-}
 
 // order-preserving key of a logit: larger logit, larger key; -0 equals +0; NaN is below everything (key 0)
 __device__ __forceinline__ uint32_t logit_key(float x) {
@@ -47,213 +60,665 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
 __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-constexpr uint32_t KEY_NEG_INF = 0x007fffffu;  // key of -infinity; at or below it a token has no weight
 
-struct Weigh {
-  double inv_t;
-  float top;
-  double one;  // 2^frac_bits
-  __device__ __forceinline__ double real(float x) const {
-    if (x == top) return 1.0;
-    return exp((static_cast<double>(x) - static_cast<double>(top)) * inv_t);
-  }
-  __device__ __forceinline__ unsigned long long operator()(uint32_t key) const {
-    if (key <= KEY_NEG_INF) return 0ull;
-    return static_cast<unsigned long long>(__double2ll_rn(real(key_logit(key)) * one));
-  }
-};
-
-struct Sums {
-  unsigned long long count, mass;
-};
-// block-wide sum over all tokens with key >= pivot
-template <typename T>
-__device__ Sums sum_from(const T* row, int V, uint32_t pivot, const Weigh& w, bool want_mass, Sums* s_part) {
-  Sums r = {0, 0};
-  for (int i = threadIdx.x; i < V; i += SM_THREADS) {
-    const uint32_t k = logit_key(logit_at<T>(row, i));
-    if (k >= pivot) {
-      r.count += 1;
-      if (want_mass) r.mass += w(k);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    r.count += __shfl_xor_sync(MUI_FULL_MASK, r.count, o);
-    r.mass += __shfl_xor_sync(MUI_FULL_MASK, r.mass, o);
-  }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = r;
-  __syncthreads();
-  r = {0, 0};
-  for (int i = 0; i < SM_WARPS; ++i) {
-    r.count += s_part[i].count;
-    r.mass += s_part[i].mass;
-  }
+// ---- cluster helpers (also right for a cluster of one) ----
+__device__ __forceinline__ unsigned cta_rank() {
+  unsigned r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t peer_addr(const void* local, unsigned rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ uint32_t peer_u32(const uint32_t* local, unsigned rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_addr(local, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ u64 peer_u64(const u64* local, unsigned rank) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer_addr(local, rank)) : "memory");
+  return v;
+}
 
+struct Shared {
+  uint32_t bins[SM_BINS];    // this CTA's counts
+  u64 list[2][SM_LIST];      // rank 0: key << 32 | ~index of the tokens in the two boundary bins: larger ranks first
+  u64 list_w[SM_LIST];
+  u64 runs[SM_RUNS];
+  u64 part[SM_WARPS][3];
+  u64 sums[2][3];            // this CTA's sums, two turns so that one barrier per exchange is enough
+  u64 fwarp[SM_WARPS];
+  double mwarp[SM_WARPS];
+  uint32_t list_n[2];
+  uint32_t verdict;          // rank 0: threshold found
+  uint32_t T, T_idx;
+  int bin_k, bin_p;
+  uint32_t before_k;
+  double est_total;
+  int hit;
+};
+
+// The eight tokens from i on as fp32; NaN behind the end of the row.
 template <typename T>
-__global__ void __launch_bounds__(SM_THREADS) sample_kernel(const SampleArgs a) {
-  __shared__ Sums s_part[SM_WARPS];
-  __shared__ uint32_t s_key[SM_WARPS];
-  __shared__ int s_idx[SM_WARPS];
-  pdl_wait_prior_grid();
-  pdl_launch_dependents();
-  const int r = blockIdx.x, V = a.V, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const T* row = reinterpret_cast<const T*>(a.logits) + r * a.stride;
-  // largest key, lowest index
-  uint32_t best = 0;
-  int best_i = 0x7fffffff;
-  for (int i = tid; i < V; i += SM_THREADS) {
-    const uint32_t k = logit_key(logit_at<T>(row, i));
-    if (k > best || (k == best && i < best_i)) {
-      best = k;
-      best_i = i;
-    }
-  }
-  auto fold = [&](uint32_t ok, int oi) {
-    if (ok > best || (ok == best && oi < best_i)) {
-      best = ok;
-      best_i = oi;
-    }
-  };
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    fold(__shfl_xor_sync(MUI_FULL_MASK, best, o), __shfl_xor_sync(MUI_FULL_MASK, best_i, o));
-  if (lane == 0) {
-    s_key[warp] = best;
-    s_idx[warp] = best_i;
-  }
-  __syncthreads();
-  for (int i = 0; i < SM_WARPS; ++i) fold(s_key[i], s_idx[i]);
-  const float t = a.temperature ? __ldcg(a.temperature + r) : 1.f;
-  if (best <= KEY_NEG_INF || !(t > 0.f)) {
-    if (tid == 0) {
-      a.tokens[r] = best <= KEY_NEG_INF ? 0 : best_i;
-      if (a.logprobs) a.logprobs[r] = best <= KEY_NEG_INF ? -INFINITY : 0.f;
+__device__ __forceinline__ void load8(const T* row, int i, int V, bool vec, float (&x)[8]) {
+  if (vec && i + 8 <= V) {
+    if (sizeof(T) == 4) {
+      const uint4 a = ld_act16(reinterpret_cast<const char*>(row) + static_cast<size_t>(i) * 4);
+      const uint4 b = ld_act16(reinterpret_cast<const char*>(row) + static_cast<size_t>(i) * 4 + 16);
+      x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+      x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
+    } else {
+      using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
+      unpack8<H>(ld_act16(row + i), x);
     }
     return;
   }
-  Weigh w;
-  w.inv_t = 1.0 / static_cast<double>(t);
-  w.top = key_logit(best);
-  w.one = static_cast<double>(1ull << a.frac_bits);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = __int_as_float(0x7fffffff);
+    if (i + e < V) {
+      if (sizeof(T) == 4) x[e] = __ldcg(reinterpret_cast<const float*>(row) + i + e);
+      else {
+        using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
+        x[e] = ld_act_f32<H>(reinterpret_cast<const H*>(row) + i + e);
+      }
+    }
+  }
+}
 
-  // top-k: largest T with at least k tokens at or above it
-  const int k_raw = a.top_k ? __ldcg(a.top_k + r) : 0;
-  const bool use_k = k_raw > 0 && k_raw < V;
-  const float top_p = a.top_p ? __ldcg(a.top_p + r) : 1.f;
-  const float min_p = a.min_p ? __ldcg(a.min_p + r) : 0.f;
-  uint32_t T_key = 0;                     // kept: key > T_key, and the first `ties` at it
-  unsigned long long ties = ~0ull;
-  unsigned long long above_mass = 0;
+// Weights of one row. table: lane j of every warp holds 2^(j / 32).
+struct Weigh {
+  float top, bin_scale;
+  double inv_t, table;
+  int frac_bits;
+  // bin of z; SM_BINS and above: the weight rounds to 0. Non-decreasing in the distance from the largest logit.
+  __device__ __forceinline__ int bin(float x) const {
+    if (x == top) return 0;
+    const float b = (top - x) * bin_scale;
+    return b < static_cast<float>(SM_BINS) ? static_cast<int>(b) : SM_BINS;  // NaN: SM_BINS
+  }
+  // 2^S exp(z), rounded; whole warp, x of lanes with use == false is not looked at. z = (32 n + j) ln2 / 32 + r with |r| <=
+  // ln2 / 64: exp(z) = 2^n * 2^(j/32) * exp(r), the last one by its Taylor polynomial of degree 5 (r^6 / 720 < 3e-15).
+  __device__ __forceinline__ u64 operator()(float x, bool use) const {
+    const double z = use && x != top ? (static_cast<double>(x) - static_cast<double>(top)) * inv_t : 0.0;
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number, in the low bits
+    const double km = fma(z, 46.166241308446828, magic);  // 32 / ln 2
+    const int k = __double2loint(km);
+    const double r = fma(km - magic, -0.021660849392498290, z);  // ln 2 / 32
+    double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    p *= __shfl_sync(MUI_FULL_MASK, table, k & 31);
+    p = __hiloint2double(__double2hiint(p) + (((k >> 5) + frac_bits) << 20), __double2loint(p));
+    // p < 2^51: adding 2^52 leaves the rounded integer in the mantissa
+    const u64 bits = static_cast<u64>(__double_as_longlong(p + 4503599627370496.0)) & 0xfffffffffffffull;
+    return use ? bits : 0ull;
+  }
+};
+
+__device__ __forceinline__ u64 warp_sum_u64(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(MUI_FULL_MASK, v, o);
+  return v;
+}
+
+template <typename T>
+struct Row {
+  const T* p;
+  int V, c0, c1;  // this CTA's chunks
+  bool vec;
+  // f(first token of the lane, its eight logits) for every chunk of this CTA; warps take chunks in turn
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int c = c0 + warp;
+    for (; c + SM_WARPS < c1; c += 2 * SM_WARPS) {  // two chunks of loads in flight
+      float x[8], y[8];
+      load8<T>(p, c * SM_CHUNK + lane * 8, V, vec, x);
+      load8<T>(p, (c + SM_WARPS) * SM_CHUNK + lane * 8, V, vec, y);
+      f(c * SM_CHUNK + lane * 8, x);
+      f((c + SM_WARPS) * SM_CHUNK + lane * 8, y);
+    }
+    if (c < c1) {
+      float x[8];
+      load8<T>(p, c * SM_CHUNK + lane * 8, V, vec, x);
+      f(c * SM_CHUNK + lane * 8, x);
+    }
+  }
+};
+
+// Sums of three numbers over the cluster; every thread gets them. `turn` alternates from call to call.
+__device__ __forceinline__ void cluster_sum3(Shared& s, int cluster, int& turn, u64 (&v)[3]) {
+  const int warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) v[i] = warp_sum_u64(v[i]);
+  if ((threadIdx.x & 31) == 0)
+    for (int i = 0; i < 3; ++i) s.part[warp][i] = v[i];
+  __syncthreads();
+  if (threadIdx.x < 3) {
+    u64 t = 0;
+    for (int w = 0; w < SM_WARPS; ++w) t += s.part[w][threadIdx.x];
+    s.sums[turn][threadIdx.x] = t;
+  }
+  if (cluster > 1) cluster_sync();
+  else __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    v[i] = 0;
+    for (int r = 0; r < cluster; ++r) v[i] += cluster > 1 ? peer_u64(&s.sums[turn][i], r) : s.sums[turn][i];
+  }
+  turn ^= 1;
+}
+
+// The boundary of top-k and top-p by bisection: 32 steps over keys for each, then over indices for the ties.
+template <typename T>
+__device__ void threshold_by_bisection(Shared& s, const SampleArgs& a, const Row<T>& row, const Weigh& w, int& turn,
+                                       uint32_t best, bool use_k, uint32_t k, bool use_p, double top_p, uint32_t& T_key,
+                                       uint32_t& T_idx) {
+  // count and weight of the tokens with key >= pivot
+  auto from = [&](uint32_t pivot, u64& count, u64& mass) {
+    u64 v[3] = {0, 0, 0};
+    row.each([&](int i, float(&x)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = i + e < a.V && logit_key(x[e]) >= pivot;
+        v[0] += in;
+        v[1] += w(x[e], in && w.bin(x[e]) < SM_BINS);
+      }
+    });
+    cluster_sum3(s, a.cluster, turn, v);
+    count = v[0];
+    mass = v[1];
+  };
+  auto weight_of = [&](uint32_t key) {
+    const float x = key_logit(key);
+    return w(x, x == x && w.bin(x) < SM_BINS);
+  };
+  u64 ties = ~0ull, total = 0, n, m;
+  T_key = 0;
   if (use_k) {
-    uint32_t lo = 0, hi = best;  // count(>= lo) >= k
+    uint32_t lo = 0, hi = best;
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (sum_from<T>(row, V, mid, w, false, s_part).count >= static_cast<unsigned long long>(k_raw)) lo = mid;
+      from(mid, n, m);
+      if (n >= k) lo = mid;
       else hi = mid - 1;
     }
     T_key = lo;
-    const Sums up = lo == 0xffffffffu ? Sums{0, 0} : sum_from<T>(row, V, lo + 1, w, true, s_part);
-    ties = k_raw - up.count;
-    above_mass = up.mass;
+    from(lo + 1, n, m);  // lo <= best < 2^32 - 1 (a NaN has key 0)
+    ties = k - n;
+    total = m + ties * weight_of(lo);
+  } else if (use_p) {
+    from(0, n, total);
   }
-  if (top_p < 1.f) {
-    const unsigned long long total =
-        use_k ? above_mass + ties * w(T_key) : sum_from<T>(row, V, 0, w, true, s_part).mass;
-    const double target = static_cast<double>(top_p) * static_cast<double>(total);
-    // largest P whose tokens at or above (within the top-k) weigh the target
-    auto mass_from = [&](uint32_t p) {
-      if (use_k && p <= T_key) return total;
-      return sum_from<T>(row, V, p, w, true, s_part).mass;
-    };
+  if (use_p) {
+    const double target = top_p * static_cast<double>(total);
     uint32_t lo = T_key, hi = best;
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (static_cast<double>(mass_from(mid)) >= target) lo = mid;
+      from(mid, n, m);
+      if (static_cast<double>(m) >= target) lo = mid;
       else hi = mid - 1;
     }
-    const Sums up = lo == 0xffffffffu ? Sums{0, 0} : sum_from<T>(row, V, lo + 1, w, true, s_part);
-    const double each = static_cast<double>(w(lo));
-    unsigned long long n = 1;
+    from(lo + 1, n, m);
+    const double each = static_cast<double>(weight_of(lo));
+    u64 need = 1;
     if (each > 0.0) {
-      const double need = ceil((target - static_cast<double>(up.mass)) / each);
-      n = need < 1.0 ? 1ull : (need > 4.0e9 ? ~0ull : static_cast<unsigned long long>(need));
+      const double q = ceil((target - static_cast<double>(m)) / each);
+      need = q < 1.0 ? 1ull : (q > 4.0e9 ? ~0ull : static_cast<u64>(q));
     }
-    if (lo > T_key || !use_k) {
-      T_key = lo;
-      ties = n;
-    } else {
-      ties = n < ties ? n : ties;
+    ties = lo > T_key || need < ties ? need : ties;
+    T_key = lo;
+  }
+  // index of the last tie that is kept
+  uint32_t lo = 0, hi = a.V - 1;
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    u64 v[3] = {0, 0, 0};
+    row.each([&](int i, float(&x)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[0] += i + e < a.V && i + e <= static_cast<int>(mid) && logit_key(x[e]) == T_key;
+    });
+    cluster_sum3(s, a.cluster, turn, v);
+    if (v[0] >= ties) hi = mid;
+    else lo = mid + 1;
+  }
+  T_idx = lo;
+}
+
+// Ranks the tokens of a collected bin by comparing all pairs. kept(rank, weight of the bin's tokens before) says whether a
+// token is kept; the last kept one becomes the threshold. Returns the kept weight. One CTA.
+template <typename K>
+__device__ u64 settle_bin(Shared& s, const u64* list, int n, const Weigh& w, K kept) {
+  for (int base = 0; base < n; base += SM_THREADS) {
+    const int i = base + threadIdx.x;
+    const u64 x = w(i < n ? key_logit(static_cast<uint32_t>(list[i] >> 32)) : 0.f, i < n);
+    if (i < n) s.list_w[i] = x;
+  }
+  if (threadIdx.x == 0) {
+    s.T = 0xffffffffu;
+    s.T_idx = 0;
+  }
+  __syncthreads();
+  u64 sum = 0, last = ~0ull;  // smallest kept entry = last in the ranking
+  for (int i = threadIdx.x; i < n; i += SM_THREADS) {
+    const u64 me = list[i];
+    u64 before = 0;
+    uint32_t rank = 0;
+    for (int j = 0; j < n; ++j) {
+      const bool front = list[j] > me;
+      rank += front;
+      before += front ? s.list_w[j] : 0ull;
+    }
+    if (kept(rank, before)) {
+      sum += s.list_w[i];
+      last = me < last ? me : last;
     }
   }
-  // the smallest key that min-p keeps is found by evaluating w itself
-  const double min_w = min_p > 0.f ? static_cast<double>(min_p) : -1.0;
-  auto keeps = [&](uint32_t k) { return k > KEY_NEG_INF && (min_w < 0.0 || w.real(key_logit(k)) >= min_w || k == best); };
+  sum = warp_sum_u64(sum);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const u64 y = __shfl_xor_sync(MUI_FULL_MASK, last, o);
+    last = y < last ? y : last;
+  }
+  if ((threadIdx.x & 31) == 0) {
+    s.part[threadIdx.x >> 5][0] = sum;
+    s.fwarp[threadIdx.x >> 5] = last;
+  }
+  __syncthreads();
+  sum = 0;
+  last = ~0ull;
+  for (int i = 0; i < SM_WARPS; ++i) {
+    sum += s.part[i][0];
+    last = s.fwarp[i] < last ? s.fwarp[i] : last;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s.T = static_cast<uint32_t>(last >> 32);
+    s.T_idx = ~static_cast<uint32_t>(last);
+  }
+  __syncthreads();
+  return sum;
+}
 
-  // each warp takes a run of the row: ties and weight above the threshold in it
-  const int per = (V + SM_WARPS - 1) / SM_WARPS, i0 = warp * per, i1 = min(V, i0 + per);
-  Sums mine = {0, 0};
-  for (int i = i0 + lane; i < i1; i += 32) {
-    const uint32_t k = logit_key(logit_at<T>(row, i));
-    if (k == T_key) mine.count += 1;
-    else if (k > T_key && keeps(k)) mine.mass += w(k);
+template <typename T>
+__global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs a) {
+  extern __shared__ __align__(16) unsigned char sample_smem[];
+  Shared& s = *reinterpret_cast<Shared*>(sample_smem);
+  const int C = a.cluster, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const unsigned rank = C > 1 ? cta_rank() : 0;
+  const int r = blockIdx.x / C;
+  int turn = 0;
+  pdl_wait_prior_grid();
+  pdl_launch_dependents();
+
+  Row<T> row;
+  row.p = reinterpret_cast<const T*>(a.logits) + r * a.stride;
+  row.V = a.V;
+  row.vec = (reinterpret_cast<uintptr_t>(row.p) & 15) == 0;
+  const int chunks = (a.V + SM_CHUNK - 1) / SM_CHUNK, per_cta = (chunks + C - 1) / C;
+  row.c0 = min(chunks, static_cast<int>(rank) * per_cta);
+  row.c1 = min(chunks, row.c0 + per_cta);
+  const float t = a.temperature ? __ldcg(a.temperature + r) : 1.f;
+  const int k_raw = a.top_k ? __ldcg(a.top_k + r) : 0;
+  const float top_p = a.top_p ? __ldcg(a.top_p + r) : 1.f;
+  const float min_p = a.min_p ? __ldcg(a.min_p + r) : 0.f;
+  const bool use_k = k_raw > 0 && k_raw < a.V, use_p = top_p < 1.f, greedy = !(t > 0.f);
+
+  // 1. the largest logit; its lowest index where that is the answer
+  u64 best = 0;  // key << 32 | ~index
+  if (greedy) {
+    row.each([&](int i, float(&x)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const u64 v = static_cast<u64>(logit_key(x[e])) << 32 | ~static_cast<uint32_t>(i + e);
+        best = i + e < a.V && v > best ? v : best;
+      }
+    });
+  } else {
+    float m = -INFINITY;
+    row.each([&](int, float(&x)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+    });
+    best = static_cast<u64>(logit_key(m)) << 32 | 0xffffffffu;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    mine.count += __shfl_xor_sync(MUI_FULL_MASK, mine.count, o);
-    mine.mass += __shfl_xor_sync(MUI_FULL_MASK, mine.mass, o);
+    const u64 y = __shfl_xor_sync(MUI_FULL_MASK, best, o);
+    best = y > best ? y : best;
   }
+  if (lane == 0) s.fwarp[warp] = best;
+  for (int i = tid; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0;
+  if (tid < 2) s.list_n[tid] = 0;
   __syncthreads();
-  if (lane == 0) s_part[warp] = mine;
-  __syncthreads();
-  const unsigned long long tie_w = keeps(T_key) ? w(T_key) : 0ull;
-  unsigned long long left = ties, before = 0, total = 0, my_left = 0;
-  for (int i = 0; i < SM_WARPS; ++i) {
-    if (i == warp) {
-      my_left = left;
-      before = total;
+  for (int i = 0; i < SM_WARPS; ++i) best = s.fwarp[i] > best ? s.fwarp[i] : best;
+  if (C > 1) {
+    if (tid == 0) s.sums[1][0] = best;
+    cluster_sync();
+    for (int i = 0; i < C; ++i) {
+      const u64 y = peer_u64(&s.sums[1][0], i);
+      best = y > best ? y : best;
     }
-    const unsigned long long n = s_part[i].count < left ? s_part[i].count : left;
-    left -= n;
-    total += s_part[i].mass + n * tie_w;
-    if (i == warp) mine.mass = s_part[i].mass + n * tie_w;
   }
-  const float u = a.uniforms ? __ldcg(a.uniforms + r) : 0.f;
-  // uniform numbers lie in [0, 1); what does not is brought to the nearest fp32 that does
-  const double want = static_cast<double>(fminf(fmaxf(u, 0.f), 0.99999994f)) * static_cast<double>(total);
-  // the warp whose run holds the point walks it
-  if (mine.mass == 0 || static_cast<double>(before) > want || static_cast<double>(before + mine.mass) <= want) return;
-  unsigned long long run = before;
-  for (int base = i0; base < i1; base += 32) {
-    const int i = base + lane;
-    const uint32_t k = i < i1 ? logit_key(logit_at<T>(row, i)) : 0u;
-    const unsigned tie_mask = __ballot_sync(MUI_FULL_MASK, i < i1 && k == T_key);
-    const unsigned long long rank = __popc(tie_mask & ((1u << lane) - 1));
-    unsigned long long x = 0;
-    if (i < i1) {
-      if (k == T_key) x = rank < my_left ? tie_w : 0ull;
-      else if (k > T_key && keeps(k)) x = w(k);
+  const uint32_t best_key = static_cast<uint32_t>(best >> 32);
+  Weigh w;
+  w.top = key_logit(best_key);
+  const bool nothing = !(w.top > -INFINITY);  // key 0 (all NaN) reads as NaN
+  if (greedy || nothing) {
+    if (rank == 0 && tid == 0) {
+      a.tokens[r] = nothing ? 0 : static_cast<int64_t>(~static_cast<uint32_t>(best));
+      if (a.logprobs) a.logprobs[r] = nothing ? -INFINITY : 0.f;
     }
-    my_left -= min(my_left, static_cast<unsigned long long>(__popc(tie_mask)));
-    unsigned long long c = x;
+    if (C > 1) cluster_sync();  // peers may still be reading this CTA's memory
+    return;
+  }
+  w.frac_bits = a.frac_bits;
+  w.inv_t = 1.0 / static_cast<double>(t);
+  w.table = exp2(static_cast<double>(lane) / 32.0);
+  // z below -(S + 2) ln 2 has a weight under a quarter of the last bit
+  const float z_range = (a.frac_bits + 2) * 0.693147181f;
+  w.bin_scale = static_cast<float>(SM_BINS) / z_range / t;
+  const u64 one = 1ull << a.frac_bits;
+  // min-p in the integers of the weights; the largest token has weight 1 and always stays
+  const u64 w_min = min_p > 0.f ? static_cast<u64>(ceil(fmin(static_cast<double>(min_p), 1.0) * static_cast<double>(one))) : 1ull;
+
+  uint32_t T_key = 0, T_idx = 0;  // nothing to cut: every key that has weight is above 0
+  if (use_k || use_p) {
+    // 2. histogram
+    row.each([&](int, float(&x)[8]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int b = w.bin(x[e]);
+        if (b < SM_BINS) atomicAdd(&s.bins[b], 1u);
+      }
+    });
+    if (tid == 0) {
+      s.bin_k = s.bin_p = SM_BINS;
+      s.before_k = 0;
+      s.verdict = 0;
+    }
+    if (C > 1) cluster_sync();
+    else __syncthreads();
+    // prefix sums over the cluster's bins, two per thread: counts, and weights of the bin centres
+    uint32_t n[2];
+    double m[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      n[h] = 0;
+      for (int i = 0; i < C; ++i) n[h] += C > 1 ? peer_u32(&s.bins[2 * tid + h], i) : s.bins[2 * tid + h];
+      m[h] = n[h] * static_cast<double>(exp2f(-(2 * tid + h + 0.5f) * (z_range * 1.44269504f / SM_BINS)));
+    }
+    uint32_t nc = n[0] + n[1];
+    double mc = m[0] + m[1];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const unsigned long long y = __shfl_up_sync(MUI_FULL_MASK, c, o);
+      const uint32_t y = __shfl_up_sync(MUI_FULL_MASK, nc, o);
+      const double q = __shfl_up_sync(MUI_FULL_MASK, mc, o);
+      if (lane >= o) {
+        nc += y;
+        mc += q;
+      }
+    }
+    if (lane == 31) {
+      s.fwarp[warp] = nc;
+      s.mwarp[warp] = mc;
+    }
+    __syncthreads();
+    double all = 0.0;
+    for (int i = 0; i < SM_WARPS; ++i) {
+      if (i < warp) {
+        nc += static_cast<uint32_t>(s.fwarp[i]);
+        mc += s.mwarp[i];
+      }
+      all += s.mwarp[i];
+    }
+    const uint32_t n_before = nc - n[0] - n[1];
+    const double m_before = mc - m[0] - m[1];
+    if (use_k) {
+      const uint32_t k = static_cast<uint32_t>(k_raw);
+      if (tid == 0) s.est_total = all;
+      __syncthreads();
+      uint32_t nb = n_before;
+      double mb = m_before;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (nb < k && nb + n[h] >= k) {  // one thread at most
+          s.bin_k = 2 * tid + h;
+          s.before_k = nb;
+          s.est_total = mb + m[h] * (k - nb) / n[h];
+        }
+        nb += n[h];
+        mb += m[h];
+      }
+      __syncthreads();
+      all = s.est_total;
+    }
+    if (use_p) {
+      const double target = static_cast<double>(top_p) * all;
+      double mb = m_before;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // the bin where the sum passes the target; the first occupied one when the target is not above 0
+        if (n[h] > 0 && mb + m[h] >= target && (mb < target || n_before + (h ? n[0] : 0) == 0)) atomicMin(&s.bin_p, 2 * tid + h);
+        mb += m[h];
+      }
+      __syncthreads();
+    }
+    const int bin_k = s.bin_k;
+    const int bin_p = use_p ? min(s.bin_p, bin_k) : bin_k;
+    if (bin_p < SM_BINS) {
+      // 3. exact sums: [0] above bin_p, [1] between the bins; tokens of the bins go to rank 0
+      u64 v[3] = {0, 0, 0};
+      const uint32_t count_at[2] = {peer_addr(&s.list_n[0], 0), peer_addr(&s.list_n[1], 0)};
+      const uint32_t list_at[2] = {peer_addr(&s.list[0][0], 0), peer_addr(&s.list[1][0], 0)};
+      row.each([&](int i, float(&x)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int b = w.bin(x[e]);
+          const bool sum = use_p && b < bin_k && b != bin_p && b < SM_BINS;
+          if (__any_sync(MUI_FULL_MASK, sum)) {
+            const u64 q = w(x[e], sum);
+            v[0] += b < bin_p ? q : 0ull;
+            v[1] += b < bin_p ? 0ull : q;
+          }
+          if (b < SM_BINS && (b == bin_p || b == bin_k)) {
+            const int which = b == bin_p ? 0 : 1;
+            uint32_t at;
+            asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count_at[which]) : "memory");
+            if (at < SM_LIST) {
+              const u64 entry = static_cast<u64>(logit_key(x[e])) << 32 | ~static_cast<uint32_t>(i + e);
+              asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list_at[which] + at * 8), "l"(entry) : "memory");
+            }
+          }
+        }
+      });
+      cluster_sum3(s, C, turn, v);  // its barrier also publishes the lists
+      if (rank == 0) {
+        const int n0 = s.list_n[0], n1 = s.list_n[1];
+        const bool same = bin_p == bin_k;
+        bool ok = n0 <= SM_LIST && n1 <= SM_LIST;
+        if (ok) {
+          u64 kept_k = 0;
+          const uint32_t left = static_cast<uint32_t>(k_raw) - s.before_k;  // of bin_k (only used with top-k)
+          if (bin_k < SM_BINS)
+            kept_k = settle_bin(s, s.list[same ? 0 : 1], same ? n0 : n1, w,
+                                [&](uint32_t rk, u64) { return rk < left; });
+          if (use_p) {
+            u64 in_p = kept_k;
+            if (!same) {
+              in_p = 0;
+              for (int base = 0; base < n0; base += SM_THREADS) {
+                const int i = base + tid;
+                in_p += w(i < n0 ? key_logit(static_cast<uint32_t>(s.list[0][i] >> 32)) : 0.f, i < n0);
+              }
+              in_p = warp_sum_u64(in_p);
+              if (lane == 0) s.part[warp][1] = in_p;
+              __syncthreads();
+              in_p = 0;
+              for (int i = 0; i < SM_WARPS; ++i) in_p += s.part[i][1];
+            }
+            const u64 total = v[0] + v[1] + in_p + (same ? 0 : kept_k);
+            const double target = static_cast<double>(top_p) * static_cast<double>(total);
+            // the estimate must have named the right bin
+            ok = (v[0] == 0 || static_cast<double>(v[0]) < target) && static_cast<double>(v[0] + in_p) >= target;
+            if (ok)
+              settle_bin(s, s.list[0], n0, w, [&](uint32_t rk, u64 before) {
+                if (same && rk >= left) return false;
+                return (v[0] == 0 && rk == 0) || static_cast<double>(v[0] + before) < target;
+              });
+          }
+        }
+        if (tid == 0) s.verdict = ok ? 1u : 0u;
+      }
+      if (C > 1) cluster_sync();
+      else __syncthreads();
+      const bool ok = C > 1 ? peer_u32(&s.verdict, 0) != 0 : s.verdict != 0;
+      if (ok) {
+        T_key = C > 1 ? peer_u32(&s.T, 0) : s.T;
+        T_idx = C > 1 ? peer_u32(&s.T_idx, 0) : s.T_idx;
+      } else {
+        threshold_by_bisection<T>(s, a, row, w, turn, best_key, use_k, static_cast<uint32_t>(k_raw), use_p,
+                                  static_cast<double>(top_p), T_key, T_idx);
+      }
+    } else if (use_p) {
+      // no bin reaches the target by the estimate (a top_p next to 1)
+      threshold_by_bisection<T>(s, a, row, w, turn, best_key, use_k, static_cast<uint32_t>(k_raw), use_p,
+                                static_cast<double>(top_p), T_key, T_idx);
+    }
+  }
+
+  // 4. kept weight by runs of chunks
+  __syncthreads();
+  for (int i = tid; i < SM_RUNS; i += SM_THREADS) s.runs[i] = 0;
+  __syncthreads();
+  const float T_logit = T_key ? key_logit(T_key) : -INFINITY;
+  auto kept_weight = [&](float x, int i) {
+    const bool in = w.bin(x) < SM_BINS && (x > T_logit || (x == T_logit && i <= static_cast<int>(T_idx)));
+    u64 q = 0;
+    if (__any_sync(MUI_FULL_MASK, in)) q = w(x, in);
+    return q >= w_min ? q : 0ull;
+  };
+  u64 v[3] = {0, 0, 0};
+  row.each([&](int i, float(&x)[8]) {
+    u64 q = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q += kept_weight(x[e], i + e);
+    if (__any_sync(MUI_FULL_MASK, q != 0)) {
+      v[0] += q;
+      q = warp_sum_u64(q);
+      if (lane == 0) atomicAdd(&s.runs[(i / SM_CHUNK - row.c0) / a.chunks_per_run], q);
+    }
+  });
+  const int my_turn = turn;
+  cluster_sum3(s, C, turn, v);
+  const u64 total = v[0];
+  u64 before = 0, mine = 0;
+  for (int i = 0; i < C; ++i) {
+    const u64 y = C > 1 ? peer_u64(&s.sums[my_turn][0], i) : s.sums[my_turn][0];
+    if (i < static_cast<int>(rank)) before += y;
+    if (i == static_cast<int>(rank)) mine = y;
+  }
+  // uniform numbers lie in [0, 1); what does not is brought to the nearest fp32 that does
+  const float u = fminf(fmaxf(__ldcg(a.uniforms + r), 0.f), 0.99999994f);
+  const double want = static_cast<double>(u) * static_cast<double>(total);
+  if (C > 1) cluster_sync();  // the last look at a peer's memory
+  if (mine == 0 || static_cast<double>(before) > want || static_cast<double>(before + mine) <= want) return;
+
+  // this CTA holds the drawn point: first its run, then its chunk and token
+  {
+    u64 q = tid < SM_RUNS ? s.runs[tid] : 0;
+    u64 c = q;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 y = __shfl_up_sync(MUI_FULL_MASK, c, o);
       if (lane >= o) c += y;
     }
-    const unsigned hit = __ballot_sync(MUI_FULL_MASK, static_cast<double>(run + c) > want);
+    if (lane == 31) s.fwarp[warp] = c;
+    __syncthreads();
+    u64 at = before;
+    for (int i = 0; i < warp; ++i) at += s.fwarp[i];
+    if (q != 0 && static_cast<double>(at + c) > want && static_cast<double>(at + c - q) <= want) {
+      s.hit = tid;
+      s.sums[my_turn ^ 1][0] = at + c - q;  // weight in front of the run
+    }
+    __syncthreads();
+  }
+  if (warp != 0) return;
+  u64 at = s.sums[my_turn ^ 1][0];
+  const int first = row.c0 + s.hit * a.chunks_per_run, last = min(row.c1, first + a.chunks_per_run);
+  for (int c = first; c < last; ++c) {
+    float x[8];
+    u64 q[8], sum = 0;
+    const int i = c * SM_CHUNK + lane * 8;
+    load8<T>(row.p, i, a.V, row.vec, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q[e] = kept_weight(x[e], i + e);
+      sum += q[e];
+    }
+    u64 run = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 y = __shfl_up_sync(MUI_FULL_MASK, run, o);
+      if (lane >= o) run += y;
+    }
+    const unsigned hit = __ballot_sync(MUI_FULL_MASK, sum != 0 && static_cast<double>(at + run) > want);
     if (hit) {
       if (lane == __ffs(hit) - 1) {
-        a.tokens[r] = i;
-        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(x) / static_cast<double>(total)));
+        u64 p = at + run - sum;
+        int e = 0;
+#pragma unroll
+        for (int h = 7; h >= 0; --h) {  // the first token at which the running weight exceeds the point
+          u64 upto = p;
+          for (int j = 0; j <= h; ++j) upto += q[j];
+          if (q[h] != 0 && static_cast<double>(upto) > want) e = h;
+        }
+        a.tokens[r] = i + e;
+        u64 mine_w = 0;
+#pragma unroll
+        for (int h = 0; h < 8; ++h) mine_w = h == e ? q[h] : mine_w;
+        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(mine_w) / static_cast<double>(total)));
       }
       return;
     }
-    run += __shfl_sync(MUI_FULL_MASK, c, 31);
+    at += __shfl_sync(MUI_FULL_MASK, run, 31);
   }
+}
+
+template <typename T>
+mui_status_t launch_sample(cudaStream_t stream, const SampleArgs& a, int rows, int pdl, int device) {
+  static std::atomic<u64> configured{0};  // one bit per device
+  const u64 bit = 1ull << (device & 63);
+  if (!(configured.load() & bit)) {
+    MUI_CUDA_CHECK(cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(sizeof(Shared))));
+    configured.fetch_or(bit);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows) * a.cluster);
+  cfg.blockDim = dim3(SM_THREADS);
+  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = a.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  MUI_CUDA_CHECK(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a));
+  return MUI_OK;
 }
 
 }  // namespace
@@ -264,10 +729,13 @@ extern "C" mui_status_t mui_sample_tokens(void* stream, int dtype, int rows, int
                                           int64_t* tokens, float* logprobs, unsigned flags) {
   MUI_REQUIRE(dtype == MUI_F16 || dtype == MUI_BF16 || dtype == MUI_COMM_F32, MUI_ERR_UNSUPPORTED,
               "dtype %d unsupported", dtype);
-  MUI_REQUIRE(rows >= 0 && vocab >= 1 && vocab <= (1 << 24) && row_stride >= 0, MUI_ERR_INVALID_ARG,
-              "bad sizes rows=%d vocab=%d (1..2^24) row_stride=%lld", rows, vocab, (long long)row_stride);
+  MUI_REQUIRE(rows >= 0 && rows <= (1 << 24) && vocab >= 1 && vocab <= (1 << 24) && row_stride >= 0,
+              MUI_ERR_INVALID_ARG, "bad sizes rows=%d (0..2^24) vocab=%d (1..2^24) row_stride=%lld", rows, vocab,
+              (long long)row_stride);
   if (rows == 0) return MUI_OK;
   MUI_REQUIRE(logits && uniforms && tokens, MUI_ERR_INVALID_ARG, "logits, uniforms and tokens must be non-null");
+  const MuiDeviceInfo* di = mui_current_device_info();
+  if (!di) return MUI_ERR_CUDA;
   SampleArgs a;
   a.logits = logits;
   a.stride = row_stride;
@@ -281,16 +749,17 @@ extern "C" mui_status_t mui_sample_tokens(void* stream, int dtype, int rows, int
   a.V = vocab;
   int lg = 0;
   while ((1 << lg) < vocab) ++lg;
-  a.frac_bits = 62 - lg;
+  a.frac_bits = 62 - lg < 50 ? 62 - lg : 50;
+  // CTAs per row: as many as the rows leave SMs for, each with two steps of all its warps at least
+  a.cluster = 1;
+  while (a.cluster < SM_MAX_CLUSTER && rows * static_cast<long long>(a.cluster) * 2 <= di->sm_count &&
+         vocab > a.cluster * SM_CHUNK * SM_WARPS)
+    a.cluster *= 2;
+  const int chunks = (vocab + SM_CHUNK - 1) / SM_CHUNK, per_cta = (chunks + a.cluster - 1) / a.cluster;
+  a.chunks_per_run = (per_cta + SM_RUNS - 1) / SM_RUNS;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int pdl = (flags & MUI_FLAG_PDL) ? 1 : 0;
-  const dim3 grid(rows), block(SM_THREADS);
-  if (dtype == MUI_F16) {
-    MUI_CUDA_CHECK(mui_launch(sample_kernel<__half>, grid, block, 0, st, pdl, a));
-  } else if (dtype == MUI_BF16) {
-    MUI_CUDA_CHECK(mui_launch(sample_kernel<__nv_bfloat16>, grid, block, 0, st, pdl, a));
-  } else {
-    MUI_CUDA_CHECK(mui_launch(sample_kernel<float>, grid, block, 0, st, pdl, a));
-  }
-  return MUI_OK;
+  if (dtype == MUI_F16) return launch_sample<__half>(st, a, rows, pdl, di->device);
+  if (dtype == MUI_BF16) return launch_sample<__nv_bfloat16>(st, a, rows, pdl, di->device);
+  return launch_sample<float>(st, a, rows, pdl, di->device);
 }

@@ -155,7 +155,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
         before = torch.cumsum(w[order], 0) - w[order]
         order = order[: max(1, int((before < top_p * w[order].sum()).sum()))]
     if min_p is not None and min_p > 0:
-        order = order[(w[order] >= min_p) | (order == best)]
+        order = order[w[order] >= min(min_p, 1.0)]
     kept = torch.sort(order[w[order] > 0]).values
     run = torch.cumsum(w[kept], 0)
     at = int((run <= u * run[-1]).sum())
