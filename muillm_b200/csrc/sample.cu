@@ -11,13 +11,13 @@
 //
 // A cluster of up to eight CTAs works on a row (one CTA when there are rows enough to fill the GPU). Passes over the row:
 //   1. the largest logit (from HBM; the later passes find the row in L2);
-//   2. a histogram of z in 2048 equal bins down to the smallest z that still has weight. Counts give the bin that holds
+//   2. a histogram of z in 4096 equal bins down to the smallest z that still has weight. Counts give the bin that holds
 //      the top_k-th token exactly; counts times the bin centre's weight tell the bin in which top_p ends, nearly always;
 //   3. exact sums of the weight above and between these two bins; the bins' own tokens (some hundred) are collected in rank
-//      0's shared memory, ranked by comparing all pairs, and give T and T_idx;
+//      0's shared memory, sorted, and give T and T_idx; where the estimate was off, again with the neighbouring bin;
 //   4. the kept weight of every run of 256 tokens; the run that holds the drawn point is then walked by one warp.
-// Without top-k and top-p only 1 and 4 run. Where a bin has more tokens than the list holds (long ties, high temperatures)
-// or the estimate of 2 was a bin off, T and T_idx are found by bisection over keys and indices instead: slower, same result.
+// Without top-k and top-p only 1 and 4 run. Where a bin has more tokens than the list holds (long ties, very high
+// temperatures) T and T_idx are found by bisection over keys and indices instead: slower, same result.
 //
 // Bound: rows * vocab * size bytes for large batches, then 13 fp64 operations a weight; for few rows the chain of passes and
 // cluster barriers.
@@ -36,10 +36,12 @@ typedef unsigned long long u64;
 constexpr int SM_THREADS = 1024;
 constexpr int SM_WARPS = SM_THREADS / 32;
 constexpr int SM_CHUNK = 256;    // tokens of one warp step: eight consecutive ones per lane
-constexpr int SM_BINS = 2048;
-constexpr int SM_LIST = 2048;    // tokens collected per boundary bin
+constexpr int SM_BINS = 4096;
+constexpr int SM_LIST = 4096;    // tokens collected per boundary bin
 constexpr int SM_RUNS = 1024;    // runs of chunks whose kept weight a CTA holds
 constexpr int SM_MAX_CLUSTER = 8;
+// what rank 0 finds in the collected bins: the threshold, that top-p ends further up or down the ranking, or too many tokens
+enum : uint32_t { SM_FOUND, SM_UP, SM_DOWN, SM_BISECT };
 
 struct SampleArgs {
   const void* logits;
@@ -295,59 +297,55 @@ __device__ void threshold_by_bisection(Shared& s, const SampleArgs& a, const Row
   T_idx = lo;
 }
 
-// Ranks the tokens of a collected bin by comparing all pairs. kept(rank, weight of the bin's tokens before) says whether a
-// token is kept; the last kept one becomes the threshold. Returns the kept weight. One CTA.
-template <typename K>
-__device__ u64 settle_bin(Shared& s, const u64* list, int n, const Weigh& w, K kept) {
-  for (int base = 0; base < n; base += SM_THREADS) {
-    const int i = base + threadIdx.x;
-    const u64 x = w(i < n ? key_logit(static_cast<uint32_t>(list[i] >> 32)) : 0.f, i < n);
-    if (i < n) s.list_w[i] = x;
-  }
-  if (threadIdx.x == 0) {
-    s.T = 0xffffffffu;
-    s.T_idx = 0;
-  }
+// Sorts a collected bin into ranking order and leaves in list_w[i] the weight of its tokens before the i-th; returns the
+// weight of all of them. One CTA. A bitonic sort: 8192 exchanges of the largest list are 2 per thread and step.
+__device__ u64 rank_bin(Shared& s, u64* list, int n, const Weigh& w) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int m = 2;
+  while (m < n) m <<= 1;
+  for (int i = n + tid; i < m; i += SM_THREADS) list[i] = 0;
   __syncthreads();
-  u64 sum = 0, last = ~0ull;  // smallest kept entry = last in the ranking
-  for (int i = threadIdx.x; i < n; i += SM_THREADS) {
-    const u64 me = list[i];
-    u64 before = 0;
-    uint32_t rank = 0;
-    for (int j = 0; j < n; ++j) {
-      const bool front = list[j] > me;
-      rank += front;
-      before += front ? s.list_w[j] : 0ull;
+  for (int k = 2; k <= m; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int p = tid; p < m / 2; p += SM_THREADS) {
+        const int i = 2 * p - (p & (j - 1)), o = i + j;
+        const u64 x = list[i], y = list[o];
+        if ((x < y) == ((i & k) == 0)) {
+          list[i] = y;
+          list[o] = x;
+        }
+      }
+      __syncthreads();
     }
-    if (kept(rank, before)) {
-      sum += s.list_w[i];
-      last = me < last ? me : last;
-    }
-  }
-  sum = warp_sum_u64(sum);
+  constexpr int PER = SM_LIST / SM_THREADS;
+  u64 q[PER], sum = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 y = __shfl_xor_sync(MUI_FULL_MASK, last, o);
-    last = y < last ? y : last;
+  for (int e = 0; e < PER; ++e) {
+    const int i = tid * PER + e;
+    q[e] = w(i < n ? key_logit(static_cast<uint32_t>(list[i] >> 32)) : 0.f, i < n);
+    sum += q[e];
   }
-  if ((threadIdx.x & 31) == 0) {
-    s.part[threadIdx.x >> 5][0] = sum;
-    s.fwarp[threadIdx.x >> 5] = last;
+  u64 run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(MUI_FULL_MASK, run, o);
+    if (lane >= o) run += y;
   }
+  if (lane == 31) s.fwarp[warp] = run;
   __syncthreads();
-  sum = 0;
-  last = ~0ull;
+  u64 all = 0;
+  run -= sum;
   for (int i = 0; i < SM_WARPS; ++i) {
-    sum += s.part[i][0];
-    last = s.fwarp[i] < last ? s.fwarp[i] : last;
+    if (i < warp) run += s.fwarp[i];
+    all += s.fwarp[i];
+  }
+#pragma unroll
+  for (int e = 0; e < PER; ++e) {
+    s.list_w[tid * PER + e] = run;
+    run += q[e];
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    s.T = static_cast<uint32_t>(last >> 32);
-    s.T_idx = ~static_cast<uint32_t>(last);
-  }
-  __syncthreads();
-  return sum;
+  return all;
 }
 
 template <typename T>
@@ -445,78 +443,83 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     if (tid == 0) {
       s.bin_k = s.bin_p = SM_BINS;
       s.before_k = 0;
-      s.verdict = 0;
     }
     if (C > 1) cluster_sync();
     else __syncthreads();
-    // prefix sums over the cluster's bins, two per thread: counts, and weights of the bin centres
-    uint32_t n[2];
-    double m[2];
+    // prefix sums over the cluster's bins, four per thread: counts, and weights of the bin centres
+    constexpr int PER = SM_BINS / SM_THREADS;
+    uint32_t n[PER], nc = 0;
+    double m[PER], mc = 0.0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < PER; ++h) {
       n[h] = 0;
-      for (int i = 0; i < C; ++i) n[h] += C > 1 ? peer_u32(&s.bins[2 * tid + h], i) : s.bins[2 * tid + h];
-      m[h] = n[h] * static_cast<double>(exp2f(-(2 * tid + h + 0.5f) * (z_range * 1.44269504f / SM_BINS)));
+      for (int i = 0; i < C; ++i) n[h] += C > 1 ? peer_u32(&s.bins[PER * tid + h], i) : s.bins[PER * tid + h];
+      m[h] = n[h] * static_cast<double>(exp2f(-(PER * tid + h + 0.5f) * (z_range * 1.44269504f / SM_BINS)));
+      nc += n[h];
+      mc += m[h];
     }
-    uint32_t nc = n[0] + n[1];
-    double mc = m[0] + m[1];
+    uint32_t nb = nc;
+    double mb = mc;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(MUI_FULL_MASK, nc, o);
-      const double q = __shfl_up_sync(MUI_FULL_MASK, mc, o);
+      const uint32_t y = __shfl_up_sync(MUI_FULL_MASK, nb, o);
+      const double q = __shfl_up_sync(MUI_FULL_MASK, mb, o);
       if (lane >= o) {
-        nc += y;
-        mc += q;
+        nb += y;
+        mb += q;
       }
     }
     if (lane == 31) {
-      s.fwarp[warp] = nc;
-      s.mwarp[warp] = mc;
+      s.fwarp[warp] = nb;
+      s.mwarp[warp] = mb;
     }
     __syncthreads();
     double all = 0.0;
+    nb -= nc;
+    mb -= mc;
     for (int i = 0; i < SM_WARPS; ++i) {
       if (i < warp) {
-        nc += static_cast<uint32_t>(s.fwarp[i]);
-        mc += s.mwarp[i];
+        nb += static_cast<uint32_t>(s.fwarp[i]);
+        mb += s.mwarp[i];
       }
       all += s.mwarp[i];
     }
-    const uint32_t n_before = nc - n[0] - n[1];
-    const double m_before = mc - m[0] - m[1];
+    const uint32_t k = static_cast<uint32_t>(k_raw);
     if (use_k) {
-      const uint32_t k = static_cast<uint32_t>(k_raw);
       if (tid == 0) s.est_total = all;
       __syncthreads();
-      uint32_t nb = n_before;
-      double mb = m_before;
+      uint32_t at = nb;
+      double am = mb;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if (nb < k && nb + n[h] >= k) {  // one thread at most
-          s.bin_k = 2 * tid + h;
-          s.before_k = nb;
-          s.est_total = mb + m[h] * (k - nb) / n[h];
+      for (int h = 0; h < PER; ++h) {
+        if (at < k && at + n[h] >= k) {  // one thread at most
+          s.bin_k = PER * tid + h;
+          s.before_k = at;
+          s.est_total = am + m[h] * (k - at) / n[h];
         }
-        nb += n[h];
-        mb += m[h];
+        at += n[h];
+        am += m[h];
       }
       __syncthreads();
       all = s.est_total;
     }
     if (use_p) {
       const double target = static_cast<double>(top_p) * all;
-      double mb = m_before;
+      uint32_t at = nb;
+      double am = mb;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // the bin where the sum passes the target; the first occupied one when the target is not above 0
-        if (n[h] > 0 && mb + m[h] >= target && (mb < target || n_before + (h ? n[0] : 0) == 0)) atomicMin(&s.bin_p, 2 * tid + h);
-        mb += m[h];
+      for (int h = 0; h < PER; ++h) {
+        // the first occupied bin with which the sum reaches the target
+        if (n[h] > 0 && am + m[h] >= target && (am < target || at == 0)) atomicMin(&s.bin_p, PER * tid + h);
+        at += n[h];
+        am += m[h];
       }
       __syncthreads();
     }
     const int bin_k = s.bin_k;
-    const int bin_p = use_p ? min(s.bin_p, bin_k) : bin_k;
-    if (bin_p < SM_BINS) {
+    int bin_p = use_p ? min(s.bin_p, bin_k) : bin_k;
+    uint32_t verdict = use_p || bin_k < SM_BINS ? SM_BISECT : SM_FOUND;  // a top_p next to 1 may end in no bin
+    for (int attempt = 0; attempt < 4 && bin_p < SM_BINS; ++attempt) {
       // 3. exact sums: [0] above bin_p, [1] between the bins; tokens of the bins go to rank 0
       u64 v[3] = {0, 0, 0};
       const uint32_t count_at[2] = {peer_addr(&s.list_n[0], 0), peer_addr(&s.list_n[1], 0)};
@@ -546,54 +549,75 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
       if (rank == 0) {
         const int n0 = s.list_n[0], n1 = s.list_n[1];
         const bool same = bin_p == bin_k;
-        bool ok = n0 <= SM_LIST && n1 <= SM_LIST;
-        if (ok) {
-          u64 kept_k = 0;
-          const uint32_t left = static_cast<uint32_t>(k_raw) - s.before_k;  // of bin_k (only used with top-k)
-          if (bin_k < SM_BINS)
-            kept_k = settle_bin(s, s.list[same ? 0 : 1], same ? n0 : n1, w,
-                                [&](uint32_t rk, u64) { return rk < left; });
-          if (use_p) {
-            u64 in_p = kept_k;
-            if (!same) {
-              in_p = 0;
-              for (int base = 0; base < n0; base += SM_THREADS) {
-                const int i = base + tid;
-                in_p += w(i < n0 ? key_logit(static_cast<uint32_t>(s.list[0][i] >> 32)) : 0.f, i < n0);
+        uint32_t say = SM_BISECT;
+        if (n0 <= SM_LIST && n1 <= SM_LIST) {
+          const uint32_t left = k - s.before_k;  // tokens of bin_k within the top-k
+          u64 in_k = 0;
+          u64 last = 0;
+          if (!same && bin_k < SM_BINS) {
+            const u64 bin_mass = rank_bin(s, s.list[1], n1, w);
+            in_k = left < static_cast<uint32_t>(n1) ? s.list_w[left] : bin_mass;
+            __syncthreads();
+          }
+          const int n_p = same ? static_cast<int>(min(left, static_cast<uint32_t>(n0))) : n0;  // of bin_p within the top-k
+          u64 in_p = rank_bin(s, s.list[0], n0, w);
+          if (n_p < n0) in_p = s.list_w[n_p];
+          if (!use_p) {
+            last = s.list[0][n_p - 1];
+            say = SM_FOUND;
+          } else {
+            const double target = static_cast<double>(top_p) * static_cast<double>(v[0] + v[1] + in_p + in_k);
+            // the estimate of step 2 may be a bin off
+            if (v[0] != 0 && static_cast<double>(v[0]) >= target) say = SM_UP;
+            else if (static_cast<double>(v[0] + in_p) < target) say = SM_DOWN;
+            else {
+              // tokens whose predecessors do not reach the target are kept, the first of all in any case
+              int lo = 1, hi = n_p;
+              while (lo < hi) {
+                const int mid = (lo + hi + 1) / 2;
+                if (static_cast<double>(v[0] + s.list_w[mid - 1]) < target) lo = mid;
+                else hi = mid - 1;
               }
-              in_p = warp_sum_u64(in_p);
-              if (lane == 0) s.part[warp][1] = in_p;
-              __syncthreads();
-              in_p = 0;
-              for (int i = 0; i < SM_WARPS; ++i) in_p += s.part[i][1];
+              last = s.list[0][lo - 1];
+              say = SM_FOUND;
             }
-            const u64 total = v[0] + v[1] + in_p + (same ? 0 : kept_k);
-            const double target = static_cast<double>(top_p) * static_cast<double>(total);
-            // the estimate must have named the right bin
-            ok = (v[0] == 0 || static_cast<double>(v[0]) < target) && static_cast<double>(v[0] + in_p) >= target;
-            if (ok)
-              settle_bin(s, s.list[0], n0, w, [&](uint32_t rk, u64 before) {
-                if (same && rk >= left) return false;
-                return (v[0] == 0 && rk == 0) || static_cast<double>(v[0] + before) < target;
-              });
+          }
+          if (tid == 0) {
+            s.T = static_cast<uint32_t>(last >> 32);
+            s.T_idx = ~static_cast<uint32_t>(last);
           }
         }
-        if (tid == 0) s.verdict = ok ? 1u : 0u;
+        __syncthreads();
+        if (tid == 0) s.verdict = say;
+        if (tid < 2) s.list_n[tid] = 0;
       }
       if (C > 1) cluster_sync();
       else __syncthreads();
-      const bool ok = C > 1 ? peer_u32(&s.verdict, 0) != 0 : s.verdict != 0;
-      if (ok) {
+      verdict = C > 1 ? peer_u32(&s.verdict, 0) : s.verdict;
+      if (verdict != SM_UP && verdict != SM_DOWN) break;
+      // the neighbour that holds tokens (every CTA finds the same one)
+      const int was = bin_p;
+      if (tid == 0) s.bin_p = verdict == SM_UP ? -1 : SM_BINS;
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < PER; ++h) {
+        const int bin = PER * tid + h;
+        if (n[h] > 0 && verdict == SM_UP && bin < was) atomicMax(&s.bin_p, bin);
+        if (n[h] > 0 && verdict == SM_DOWN && bin > was) atomicMin(&s.bin_p, bin);
+      }
+      __syncthreads();
+      bin_p = s.bin_p;
+      verdict = SM_BISECT;
+      if (bin_p < 0 || bin_p > bin_k) break;
+      if (C > 1) cluster_sync();  // rank 0's list is empty before anyone adds to it; verdicts have been read
+    }
+    if (verdict == SM_FOUND) {
+      if (bin_p < SM_BINS) {
         T_key = C > 1 ? peer_u32(&s.T, 0) : s.T;
         T_idx = C > 1 ? peer_u32(&s.T_idx, 0) : s.T_idx;
-      } else {
-        threshold_by_bisection<T>(s, a, row, w, turn, best_key, use_k, static_cast<uint32_t>(k_raw), use_p,
-                                  static_cast<double>(top_p), T_key, T_idx);
       }
-    } else if (use_p) {
-      // no bin reaches the target by the estimate (a top_p next to 1)
-      threshold_by_bisection<T>(s, a, row, w, turn, best_key, use_k, static_cast<uint32_t>(k_raw), use_p,
-                                static_cast<double>(top_p), T_key, T_idx);
+    } else {
+      threshold_by_bisection<T>(s, a, row, w, turn, best_key, use_k, k, use_p, static_cast<double>(top_p), T_key, T_idx);
     }
   }
 
