@@ -4,11 +4,12 @@
 // K and V are read once per KV head; the query heads of the group (and the new tokens of a sequence) are the rows that
 // share them. Softmax is taken in one pass with a running maximum and sum in fp32.
 //
-// Two kernels. Up to 32 rows per KV head (decode): paged_decode_kernel, bound by the bytes of K and V; the visible tokens are
-// split over CTAs and joined by paged_merge_kernel. More rows (prompts): paged_prompt_kernel, bound by the tensor cores.
+// Two kernels. Up to 32 rows per KV head (decode): paged_decode_kernel, bound by the bytes of K and V; the visible rows of all
+// sequences are dealt out to the CTAs evenly, and what several CTAs share is joined by paged_merge_kernel. More rows (prompts): paged_prompt_kernel, bound by the tensor cores.
 #include "paged_common.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 MUI_STATUS_ACCESSOR(paged_attention)
@@ -18,8 +19,9 @@ namespace {
 constexpr int PA_TILE = 16;        // tokens per tile: never crosses a page
 constexpr int PA_THREADS = 128;
 constexpr int PA_WARPS = PA_THREADS / 32;
-constexpr int PA_MIN_TILES = 16;   // tiles per split at least (256 tokens)
-constexpr int PA_MAX_SPLITS = 128;
+constexpr int PA_MIN_TILES = 16;   // tiles per CTA at least (256 tokens)
+// What beginning and joining a triple costs a CTA, in the time of 4 KiB of K or V: the runs are cut by this measure
+constexpr int PA_TRIPLE_COST = 16;
 constexpr int PA_MAX_DECODE_ROWS = 32;
 
 struct PaArgs {
@@ -27,8 +29,8 @@ struct PaArgs {
   const void* q;
   mui_strides2_t qs;
   void* out;
-  float* partials;  // [total * Hq, splits, D + 2]: maximum, sum, unnormalised output
-  int Hq, G, splits, max_new, window, sinks;
+  float* partials;  // [ctas, 2, rows per block, D + 2]: maximum, sum, unnormalised output
+  int Hq, G, ctas, row_blocks, lead, max_new, window, sinks;
   float scale_log2;
 };
 
@@ -47,12 +49,6 @@ __device__ __forceinline__ Span visible_span(const PaArgs& a, int ctx, int count
   return s;
 }
 __device__ __forceinline__ int span_tile(const Span& s, int i) { return i < s.n_sink ? i : i - s.n_sink + s.first; }
-
-// tiles per split and the splits that have any, for a sequence of n tiles
-__device__ __forceinline__ int split_tiles(int n, int splits) {
-  const int t = (n + splits - 1) / splits;
-  return max(PA_MIN_TILES, (t + PA_WARPS - 1) / PA_WARPS * PA_WARPS);
-}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -77,452 +73,637 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint4 ld_kv16(const void* p) { return ld_stream16(p); }
 __device__ __forceinline__ uint2 ld_kv8(const void* p) {
   uint2 v;
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 
-// One tile of 16 cache rows in registers, as the tensor-core fragments want it. K as the A operand of S^T = K q^T: a lane
-// holds rows g and g + 8 (g = lane / 4), of each block of 32 (16-bit) or 64 (e4m3) head-dim elements the 16 bytes number
-// t = lane % 4; which head-dim element counts as which k index of an MMA is free as long as q agrees. V as the A operand
-// of O^T = V^T P^T: a lane holds rows 2t, 2t + 1, 2t + 8, 2t + 9 and of each the 16 bytes number g of every block of 128
-// bytes, so its elements e and e + 1 are rows g and g + 8 of an MMA's 16 output dims. Nothing passes through shared memory.
+// ---------------------------------------------------------------------------------------------------------------------
+// decode: few rows per KV head
+// ---------------------------------------------------------------------------------------------------------------------
+// The tiles of all (sequence, KV head, block of rows) triples are laid end to end and dealt out in equal runs, so that every
+// CTA streams the same number of bytes whatever the lengths are. A run that covers a triple whole writes its output; the
+// others leave partial results, at most two per CTA (the triple that the run starts in and the one it ends in), which
+// paged_merge_kernel joins in order.
+struct Run {
+  int seq;          // sequence at the run's first place
+  long long begin;  // place at which that sequence begins
+};
+
+// Length of a sequence's triples in places: `lead` places for their beginning, then one for each tile; 0: nothing to do
+__device__ __forceinline__ int seq_places(const PaArgs& a, int b) {
+  int first, count;
+  paged_new_tokens(a.kv, b, first, count);
+  const int ctx = __ldcg(a.kv.context_lens + b);
+  if (count == 0 || ctx < 0 || count > a.max_new) return 0;
+  const int n = visible_span(a, ctx, count).n;
+  return n ? a.lead + n : 0;
+}
+
+// Places of all triples, and the place at which the sequences of this thread (blocks of `per_thread`) begin. CTA-wide.
+__device__ __forceinline__ long long scan_sequences(const PaArgs& a, int per_thread, long long& mine_begin,
+                                                    long long* s_warp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int b0 = threadIdx.x * per_thread;
+  long long sum = 0;
+  for (int i = 0; i < per_thread; ++i)
+    if (b0 + i < a.kv.batch) sum += seq_places(a, b0 + i);
+  sum *= static_cast<long long>(a.kv.kv_heads) * a.row_blocks;
+  long long run = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(MUI_FULL_MASK, run, o);
+    if (lane >= o) run += y;
+  }
+  if (lane == 31) s_warp[warp] = run;
+  __syncthreads();
+  long long all = 0;
+  run -= sum;
+#pragma unroll
+  for (int w = 0; w < PA_WARPS; ++w) {
+    if (w < warp) run += s_warp[w];
+    all += s_warp[w];
+  }
+  mine_begin = run;
+  return all;
+}
+__device__ __forceinline__ long long run_length(long long total, int ctas) {
+  return max(static_cast<long long>(PA_MIN_TILES), (total + ctas - 1) / ctas);  // more than `lead`
+}
+
+// K and V pass through shared memory in items of 4 KiB, a ring of four per warp (K, V, K, V), copied asynchronously: three
+// items are in flight while one is multiplied, 12 KiB per warp and 144 KiB per SM with three CTAs.
+//
+// Fragments: K is the A operand of S^T = K q^T; a lane holds rows g and g + 8 (g = lane / 4) of a tile, of each block of 64
+// bytes the 16 bytes number t = lane % 4. Which head-dim element counts as which k index of an MMA is free as long as q
+// agrees. V is the A operand of O^T = V^T P^T; a lane reads rows 2t, 2t + 1, 2t + 8, 2t + 9, of each block of 128 bytes the 16
+// bytes number g, and pairs the rows' elements with byte permutes, its elements e and e + 1 being rows g and g + 8 of an MMA's 16
+// output dims. Both reads are free of bank conflicts when row r's 16-byte chunks are stored at chunk ^ swizzle(r).
 template <bool KV8, int D>
-struct Tile {
-  static constexpr int KB = KV8 ? D / 64 : D / 32;   // 16-byte pieces per K row and lane
-  static constexpr int VW = KV8 ? D / 32 : D / 16;   // 32-bit words per V row and lane
-  uint4 k[KB][2];
-  uint32_t v[4][VW];
+struct Item {
+  static constexpr int ES = KV8 ? 1 : 2;
+  static constexpr int RB = D * ES;            // bytes of a row
+  static constexpr int CPR = RB / 16;          // chunks of a row
+  static constexpr int TOKENS = 4096 / RB;     // 16, 32 or 64
+  static constexpr int U = TOKENS / PA_TILE;   // tiles
+  static constexpr int KB = RB / 64;           // 16-byte pieces of a K row per lane
+  static constexpr int KS = KV8 ? 4 : 2;       // k16 steps of such a piece
+  static constexpr int VW = KV8 ? D / 32 : D / 16;  // 32-bit words of a V row per lane
+  static __device__ __forceinline__ int swizzle(int row) {
+    if (CPR == 4) return (row >> 1) & 3;
+    return (row & 2) | (((row >> 2) ^ row) & 1) << 2;
+  }
+};
+constexpr int PA_ITEM = 4096, PA_RING = 4;
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+struct TileMeta {
+  int tb;        // first cache row, -1: nothing to see
   float ks, vs;  // page scales (e4m3)
 };
 
-template <bool KV8, int D>
-__device__ __forceinline__ void load_tile(const PaArgs& a, Tile<KV8, D>& t, int page, int kvh, int tb, int kv_len,
-                                          int lo_min) {
-  constexpr int ES = KV8 ? 1 : 2;
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const size_t head = static_cast<size_t>(page) * a.kv.kv_heads + kvh;
-  const size_t row0 = (head << a.kv.page_shift) + (tb & ((1 << a.kv.page_shift) - 1));
-  const bool there = page >= 0;
-  const unsigned char* kp = reinterpret_cast<const unsigned char*>(a.kv.k_pages) + row0 * (D * ES) + q * 16;
-  const unsigned char* vp = reinterpret_cast<const unsigned char*>(a.kv.v_pages) + row0 * (D * ES);
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    // a row that nobody sees is not read: what it holds (another owner's bytes, NaN) must not matter
-    const int j = tb + g + 8 * r;
-    const bool ok = there && j < kv_len && (j >= lo_min || j < a.sinks);
-#pragma unroll
-    for (int c = 0; c < Tile<KV8, D>::KB; ++c)
-      t.k[c][r] = ok ? ld_kv16(kp + (g + 8 * r) * (D * ES) + c * 64) : make_uint4(0, 0, 0, 0);
-  }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int slot = 2 * q + (r & 1) + (r >> 1) * 8;
-    const int j = tb + slot;
-    const bool ok = there && j < kv_len && (j >= lo_min || j < a.sinks);
-    const unsigned char* p = vp + slot * (D * ES);
-    if (KV8 && D == 64) {
-      const uint2 w = ok ? ld_kv8(p + g * 8) : make_uint2(0, 0);
-      t.v[r][0] = w.x;
-      t.v[r][1] = w.y;
-    } else {
-#pragma unroll
-      for (int c = 0; c < Tile<KV8, D>::VW / 4; ++c) {
-        const uint4 w = ok ? ld_kv16(p + c * 128 + g * 16) : make_uint4(0, 0, 0, 0);
-        t.v[r][4 * c] = w.x;
-        t.v[r][4 * c + 1] = w.y;
-        t.v[r][4 * c + 2] = w.z;
-        t.v[r][4 * c + 3] = w.w;
-      }
-    }
-  }
-}
-
-// grid (splits, KV heads, sequences); 4 warps that take the split's tiles in turn (U at a time) and are joined at the end.
-// NT: blocks of eight rows (row = new token * G + head in the group).
-template <typename T, bool KV8, int D, int NT, int U>
-__global__ void __launch_bounds__(PA_THREADS) paged_decode_kernel(const PaArgs a) {
+// 4 warps; row = new token * G + head in the group; NT blocks of eight rows per CTA
+template <typename T, bool KV8, int D, int NT>
+__global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kernel(const PaArgs a) {
+  using I = Item<KV8, D>;
   // e4m3 goes through the tensor cores as fp16, which holds every e4m3 value; so do q, after a power-of-two scaling per
   // row that brings its largest element near 1, and the probabilities
   using M = typename std::conditional<KV8, __half, T>::type;
   constexpr bool SPLIT_P = std::is_same<M, __nv_bfloat16>::value;  // probabilities as bf16 value + bf16 rest
-  constexpr int KB = Tile<KV8, D>::KB, KS = KV8 ? 4 : 2;           // k16 steps per 16-byte piece
-  constexpr int MT = D / 16;                                       // 16-dim blocks of the output
-  extern __shared__ float pa_smem[];                               // [PA_WARPS][NT * 8][D] then m, l
-  float* sm_o = pa_smem;
-  float* sm_m = pa_smem + PA_WARPS * NT * 8 * D;
-  float* sm_l = sm_m + PA_WARPS * NT * 8;
+  constexpr int U = I::U, KB = I::KB, KS = I::KS, MT = D / 16;
+  extern __shared__ __align__(128) unsigned char pa_smem[];        // [warp][PA_RING][PA_ITEM]; the join reuses it
+  __shared__ float sm_m[PA_WARPS][NT * 8], sm_l[PA_WARPS][NT * 8];
+  __shared__ TileMeta sm_meta[PA_WARPS][2][U];
+  __shared__ long long s_warp[PA_WARPS];
+  __shared__ Run s_run;
 
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-  const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z;
-  int first, count;
-  paged_new_tokens(a.kv, b, first, count);
-  const int ctx = __ldcg(a.kv.context_lens + b);
-  if (count == 0 || ctx < 0) {
-    if (ctx < 0 && threadIdx.x == 0) mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx));
-    return;
-  }
-  const int R = count * a.G;
-  if (count > a.max_new || R > NT * 8) {
-    if (threadIdx.x == 0) mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(count));
-    return;
-  }
-  const Span sp = visible_span(a, ctx, count);
-  if (sp.kv_len < ctx + count && threadIdx.x == 0) mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx + count));
-  const int per = split_tiles(sp.n, a.splits);
-  const int active = max(1, (sp.n + per - 1) / per);
-  if (split >= active) return;
-  const int i_end = min(sp.n, (split + 1) * per);
 
-  // q fragments (B operand: n = row g of the block, k in the order of K's pieces) and the rows' visible range
-  uint32_t qf[NT][KB * KS][2];
-  float qs[NT][2];        // e4m3: scale_log2 times the row's power of two, for the lane's two rows
-  int hi[NT][2], lo[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int r = n * 8 + g;
-    const T* qp = nullptr;
-    if (r < R) qp = reinterpret_cast<const T*>(a.q) + (first + r / a.G) * a.qs.tok + (kvh * a.G + r % a.G) * a.qs.head;
-    float amax = 0.f;
-    float qv[KB][KS * 4];
-#pragma unroll
-    for (int c = 0; c < KB; ++c)
-#pragma unroll
-      for (int e = 0; e < KS * 4; ++e) {
-        const int d = c * (KS * 16) + tq * (KS * 4) + e;
-        qv[c][e] = qp ? ld_act_f32<T>(qp + d) : 0.f;
-        amax = fmaxf(amax, fabsf(qv[c][e]));
-      }
-    float mul = 1.f, back = 1.f;
-    if (KV8) {
-      amax = fmaxf(amax, __shfl_xor_sync(MUI_FULL_MASK, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(MUI_FULL_MASK, amax, 2));
-      const int e = min(100, max(-100, static_cast<int>(__float_as_uint(amax) >> 23) - 127));
-      mul = exp2_int(-e);
-      back = exp2_int(e);
+  // this CTA's run
+  const int pairs = a.kv.kv_heads * a.row_blocks;
+  const int per_thread = (a.kv.batch + PA_THREADS - 1) / PA_THREADS;
+  long long begin;
+  const long long total = scan_sequences(a, per_thread, begin, s_warp);
+  if (blockIdx.x == 0)  // sequences that cannot be served have no tiles: say so
+    for (int i = 0; i < per_thread; ++i) {
+      const int s = threadIdx.x * per_thread + i;
+      if (s >= a.kv.batch) break;
+      int first, count;
+      paged_new_tokens(a.kv, s, first, count);
+      const int ctx = __ldcg(a.kv.context_lens + s);
+      if (count > a.max_new || (count > 0 && ctx < 0))
+        mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx < 0 ? ctx : count));
     }
-#pragma unroll
-    for (int c = 0; c < KB; ++c)
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        qf[n][c * KS + s][0] = Elt<M>::pack2(qv[c][4 * s] * mul, qv[c][4 * s + 1] * mul);
-        qf[n][c * KS + s][1] = Elt<M>::pack2(qv[c][4 * s + 2] * mul, qv[c][4 * s + 3] * mul);
-      }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int rr = n * 8 + 2 * tq + i;
-      const int p = ctx + rr / a.G;
-      hi[n][i] = rr < R ? p : -1;
-      lo[n][i] = a.window > 0 ? p - a.window + 1 : 0;
-      // the scale of row 2 tq + i sits in the lanes with g = 2 tq + i
-      qs[n][i] = a.scale_log2 * (KV8 ? __shfl_sync(MUI_FULL_MASK, back, (2 * tq + i) * 4) : 1.f);
+  const long long len = run_length(total, gridDim.x);
+  long long place = len * blockIdx.x;
+  const long long place_end = min(total, place + len);
+  if (place >= place_end) return;
+  for (int i = 0; i < per_thread; ++i) {
+    const int b = threadIdx.x * per_thread + i;
+    if (b >= a.kv.batch) break;
+    const long long n = static_cast<long long>(seq_places(a, b)) * pairs;
+    if (place >= begin && place < begin + n) {
+      s_run.seq = b;
+      s_run.begin = begin;
     }
+    begin += n;
   }
-  const int lo_max = a.window > 0 ? ctx + count - a.window : 0;  // first row the last new token's window holds
+  __syncthreads();
+  int b = s_run.seq;
+  long long seq_begin = s_run.begin;
 
-  float m[NT][2], l[NT][2], o[MT][NT][4], vref = 0.f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
-    l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int j = 0; j < MT; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.f;
-  }
+  const uint32_t ring = smem_u32(pa_smem) + warp * (PA_RING * PA_ITEM);
+  while (true) {
+    int first, count;
+    paged_new_tokens(a.kv, b, first, count);
+    const int ctx = __ldcg(a.kv.context_lens + b);
+    const Span sp = visible_span(a, ctx, count);
+    if (sp.kv_len < ctx + count && threadIdx.x == 0)
+      mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx + count));
+    const int places = a.lead + sp.n;
+    const int pair = static_cast<int>((place - seq_begin) / places);
+    const int kvh = pair / a.row_blocks, rblock = (pair % a.row_blocks) * (NT * 8);
+    const int at = static_cast<int>(place - seq_begin - static_cast<long long>(pair) * places);
+    const int at_end = static_cast<int>(min(static_cast<long long>(places), at + (place_end - place)));
+    const int i_begin = max(0, at - a.lead), i_end = max(0, at_end - a.lead);
+    const int R = count * a.G - rblock;  // rows from this block on; none left: the tiles are walked past
 
-  // The warp's tiles in the order in which it takes them: U neighbours, then the next U that are its own. Pages and scales of 32
-  // of them are looked up at a time, one per lane, so that K and V do not wait for the block table tile by tile.
-  const int32_t* table = a.kv.block_table + static_cast<size_t>(b) * a.kv.table_stride;
-  constexpr int STEP = PA_WARPS * U;
-  const int i_begin = split * per + warp * U;
-  int my_page = -1, my_tb = -1;
-  float my_ks = 0.f, my_vs = 0.f;
-  auto look_up = [&](int n0) {
-    const int n = n0 + lane, i = i_begin + (n / U) * STEP + n % U;
-    my_page = my_tb = -1;
-    my_ks = my_vs = 0.f;
-    if (i < i_end) {
-      const int tile = span_tile(sp, i);
-      const int page = __ldcg(table + (tile * PA_TILE >> a.kv.page_shift));
-      if (page >= 0 && page < a.kv.num_pages) {
-        my_page = page;
-        my_tb = tile * PA_TILE;
-        if (KV8) {
-          const size_t head = static_cast<size_t>(page) * a.kv.kv_heads + kvh;
-          my_ks = __ldcg(a.kv.k_scales + head);
-          my_vs = __ldcg(a.kv.v_scales + head);
-        }
-      } else {
-        mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(b));
-      }
-    }
-  };
-  // tiles n .. n + U - 1 of the warp; those beyond the end have page -1 (all of them masked). n rises from call to call.
-  auto fetch = [&](int n, Tile<KV8, D>(&t)[U], int (&tb)[U]) {
-    if ((n & 31) == 0) look_up(n);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int from = (n + u) & 31;
-      const int page = __shfl_sync(MUI_FULL_MASK, my_page, from);
-      tb[u] = __shfl_sync(MUI_FULL_MASK, my_tb, from);
-      if (KV8) {
-        t[u].ks = __shfl_sync(MUI_FULL_MASK, my_ks, from);
-        t[u].vs = __shfl_sync(MUI_FULL_MASK, my_vs, from);
-      }
-      load_tile<KV8, D>(a, t[u], page, kvh, max(tb[u], 0), sp.kv_len, sp.lo_min);
-    }
-  };
-
-  auto consume = [&](Tile<KV8, D>(&t)[U], int (&tb)[U]) {
-    float s[U][NT][4];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < KB; ++c) {
-        const uint32_t* r0 = reinterpret_cast<const uint32_t*>(&t[u].k[c][0]);
-        const uint32_t* r1 = reinterpret_cast<const uint32_t*>(&t[u].k[c][1]);
-#pragma unroll
-        for (int st = 0; st < KS; ++st) {
-          uint32_t a0, a1, a2, a3;
+    if (R > 0 && i_end > i_begin) {
+    // The warp's groups of U tiles: every fourth. Pages and scales of 32 tiles are looked up at a time, one per lane, so that
+    // K and V do not wait for the block table tile by tile.
+    const int32_t* table = a.kv.block_table + static_cast<size_t>(b) * a.kv.table_stride;
+    const int groups = (i_end - i_begin + U - 1) / U;           // of all warps
+    const int my_groups = groups > warp ? (groups - warp + PA_WARPS - 1) / PA_WARPS : 0;
+    int my_page = -1, my_tb = -1;
+    float my_ks = 0.f, my_vs = 0.f;
+    auto look_up = [&](int grp) {
+      const int i = i_begin + ((grp + lane / U) * PA_WARPS + warp) * U + lane % U;
+      my_page = my_tb = -1;
+      my_ks = my_vs = 0.f;
+      if (i < i_end) {
+        const int tile = span_tile(sp, i);
+        const int page = __ldcg(table + (tile * PA_TILE >> a.kv.page_shift));
+        if (page >= 0 && page < a.kv.num_pages) {
+          my_page = page;
+          my_tb = tile * PA_TILE;
           if (KV8) {
-            a0 = e4m3_to_half2(static_cast<uint16_t>(r0[st]));
-            a1 = e4m3_to_half2(static_cast<uint16_t>(r1[st]));
-            a2 = e4m3_to_half2(static_cast<uint16_t>(r0[st] >> 16));
-            a3 = e4m3_to_half2(static_cast<uint16_t>(r1[st] >> 16));
-          } else {
-            a0 = r0[2 * st];
-            a1 = r1[2 * st];
-            a2 = r0[2 * st + 1];
-            a3 = r1[2 * st + 1];
+            const size_t head = static_cast<size_t>(page) * a.kv.kv_heads + kvh;
+            my_ks = __ldcg(a.kv.k_scales + head);
+            my_vs = __ldcg(a.kv.v_scales + head);
           }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816<M>(s[u][n], a0, a1, a2, a3, qf[n][c * KS + st][0], qf[n][c * KS + st][1]);
+        } else {
+          mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(b));
         }
       }
-      const float ks = KV8 ? t[u].ks : 1.f;
-      const bool open = tb[u] >= 0 && tb[u] + PA_TILE - 1 <= ctx && (tb[u] >= lo_max || tb[u] + PA_TILE <= a.sinks);
+    };
+    // starts the copy of group grp's K (which == 0) or V; always closes one copy group
+    auto issue = [&](int grp, int which) {
+      if (grp < my_groups) {
+        if (which == 0) {
+          if ((grp * U & 31) == 0) look_up(grp);
+          if ((grp * U & 31) / U == lane / U) {
+            TileMeta& t = sm_meta[warp][grp & 1][lane % U];
+            t.tb = my_tb;
+            t.ks = my_ks;
+            t.vs = my_vs;
+          }
+        }
+        const unsigned char* base = reinterpret_cast<const unsigned char*>(which == 0 ? a.kv.k_pages : a.kv.v_pages);
+        const uint32_t slot = ring + ((grp & 1) * 2 + which) * PA_ITEM;
+        constexpr int RPI = 32 / I::CPR;  // rows per copy instruction
+        const int ch = lane % I::CPR;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int page = __shfl_sync(MUI_FULL_MASK, my_page, (grp * U + u) & 31);
+          const int tb = __shfl_sync(MUI_FULL_MASK, my_tb, (grp * U + u) & 31);
+          const size_t row0 = ((static_cast<size_t>(max(page, 0)) * a.kv.kv_heads + kvh) << a.kv.page_shift) +
+                              (max(tb, 0) & ((1 << a.kv.page_shift) - 1));
+          const unsigned char* src = base + row0 * I::RB + (lane / I::CPR) * I::RB + ch * 16;
+          // a row that nobody sees is not read (zeros stand for it): what it holds, another owner's bytes or NaN, must not matter
+          const bool whole = tb >= 0 && tb + PA_TILE <= sp.kv_len && (tb >= sp.lo_min || tb + PA_TILE <= a.sinks);
+#pragma unroll
+          for (int i = 0; i < PA_TILE / RPI; ++i) {
+            const int row = u * PA_TILE + i * RPI + lane / I::CPR;
+            const uint32_t dst = slot + row * I::RB + ((ch ^ I::swizzle(row)) << 4);
+            int bytes = 16;
+            if (!whole) {
+              const int j = tb + (row & (PA_TILE - 1));
+              bytes = tb >= 0 && j < sp.kv_len && (j >= sp.lo_min || j < a.sinks) ? 16 : 0;
+            }
+            copy16(dst, src + i * RPI * I::RB, bytes);
+          }
+        }
+      }
+      copy_commit();
+    };
+
+    issue(0, 0);
+    issue(0, 1);
+    issue(1, 0);
+    issue(1, 1);
+
+    // q fragments (B operand: n = row g of the block, k in the order of K's pieces) and the rows' visible range
+    uint32_t qf[NT][KB * KS][2];
+    float qs[NT][2];  // scale_log2 (e4m3: times the row's power of two) for the lane's two rows
+    int hi[NT][2], lo[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = n * 8 + g;
+      const T* qp = nullptr;
+      if (r < R)
+        qp = reinterpret_cast<const T*>(a.q) + (first + (rblock + r) / a.G) * a.qs.tok +
+             (kvh * a.G + (rblock + r) % a.G) * a.qs.head;
+      float amax = 0.f;
+      float qv[KB][KS * 4];
+#pragma unroll
+      for (int c = 0; c < KB; ++c)
+#pragma unroll
+        for (int e = 0; e < KS * 4; ++e) {
+          const int d = c * (KS * 16) + tq * (KS * 4) + e;
+          qv[c][e] = qp ? ld_act_f32<T>(qp + d) : 0.f;
+          amax = fmaxf(amax, fabsf(qv[c][e]));
+        }
+      float mul = 1.f, back = 1.f;
+      if (KV8) {
+        amax = fmaxf(amax, __shfl_xor_sync(MUI_FULL_MASK, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(MUI_FULL_MASK, amax, 2));
+        const int e = min(100, max(-100, static_cast<int>(__float_as_uint(amax) >> 23) - 127));
+        mul = exp2_int(-e);
+        back = exp2_int(e);
+      }
+#pragma unroll
+      for (int c = 0; c < KB; ++c)
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          qf[n][c * KS + s][0] = Elt<M>::pack2(qv[c][4 * s] * mul, qv[c][4 * s + 1] * mul);
+          qf[n][c * KS + s][1] = Elt<M>::pack2(qv[c][4 * s + 2] * mul, qv[c][4 * s + 3] * mul);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int rr = n * 8 + 2 * tq + i;
+        const int p = ctx + (rblock + rr) / a.G;
+        hi[n][i] = rr < R ? p : -1;
+        lo[n][i] = a.window > 0 ? p - a.window + 1 : 0;
+        // the scale of row 2 tq + i sits in the lanes with g = 2 tq + i
+        qs[n][i] = a.scale_log2 * (KV8 ? __shfl_sync(MUI_FULL_MASK, back, (2 * tq + i) * 4) : 1.f);
+      }
+    }
+    const int lo_max = a.window > 0 ? ctx + count - a.window : 0;  // first row the last new token's window holds
+
+    float m[NT][2], l[NT][2], o[MT][NT][4], vref = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.f;
+    }
+
+    for (int grp = 0; grp < my_groups; ++grp) {
+      const uint32_t kslot = ring + (grp & 1) * 2 * PA_ITEM, vslot = kslot + PA_ITEM;
+      copy_wait<3>();
+      __syncwarp();
+      float s[U][NT][4];
+      TileMeta meta[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        meta[u] = sm_meta[warp][grp & 1][u];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
+#pragma unroll
+        for (int c = 0; c < KB; ++c) {
+          const uint32_t at = kslot + (u * PA_TILE + g) * I::RB + (((c * 4 + tq) ^ I::swizzle(g)) << 4);
+          const uint4 k0 = lds16(at), k1 = lds16(at + 8 * I::RB);
+          const uint32_t r0[4] = {k0.x, k0.y, k0.z, k0.w}, r1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+          for (int st = 0; st < KS; ++st) {
+            uint32_t a0, a1, a2, a3;
+            if (KV8) {
+              a0 = e4m3_to_half2(static_cast<uint16_t>(r0[st]));
+              a1 = e4m3_to_half2(static_cast<uint16_t>(r1[st]));
+              a2 = e4m3_to_half2(static_cast<uint16_t>(r0[st] >> 16));
+              a3 = e4m3_to_half2(static_cast<uint16_t>(r1[st] >> 16));
+            } else {
+              a0 = r0[2 * st & 3];
+              a1 = r1[2 * st & 3];
+              a2 = r0[(2 * st + 1) & 3];
+              a3 = r1[(2 * st + 1) & 3];
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma16816<M>(s[u][n], a0, a1, a2, a3, qf[n][c * KS + st][0], qf[n][c * KS + st][1]);
+          }
+        }
+      }
+      __syncwarp();
+      issue(grp + 2, 0);
+
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int tb = meta[u].tb;
+        const float ks = KV8 ? meta[u].ks : 1.f;
+        const bool open = tb >= 0 && tb + PA_TILE - 1 <= ctx && (tb >= lo_max || tb + PA_TILE <= a.sinks);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[u][n][e] *= KV8 ? qs[n][e & 1] * ks : qs[n][e & 1];
+            if (!open) {
+              const int j = tb + g + (e >> 1) * 8;
+              const bool see = tb >= 0 && j <= hi[n][e & 1] && (j >= lo[n][e & 1] || j < a.sinks);
+              if (!see) s[u][n][e] = -INFINITY;
+            }
+          }
+      }
+      float turn = 1.f;  // e4m3: change of the reference scale of the output
+      if (KV8) {
+        float v = vref;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (meta[u].tb >= 0) v = fmaxf(v, meta[u].vs);
+        if (v > vref) {
+          turn = vref / v;
+          vref = v;
+        }
+      }
+      bool moved = turn != 1.f;
+      float corr[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[u][n][e] *= qs[n][e & 1] * ks;
-          if (!open) {
-            const int j = tb[u] + g + (e >> 1) * 8;
-            const bool see = tb[u] >= 0 && j <= hi[n][e & 1] && (j >= lo[n][e & 1] || j < a.sinks);
-            if (!see) s[u][n][e] = -INFINITY;
+        for (int i = 0; i < 2; ++i) {
+          float mx = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(s[u][n][i], s[u][n][2 + i]));
+          mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 16));
+          const float mn = fmaxf(m[n][i], mx);
+          const float use = mn == -INFINITY ? 0.f : mn;
+          corr[n][i] = ex2(m[n][i] - use);
+          moved |= mn != m[n][i];
+          m[n][i] = mn;
+          float sum = 0.f;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            s[u][n][i] = ex2(s[u][n][i] - use);
+            s[u][n][2 + i] = ex2(s[u][n][2 + i] - use);
+            sum += s[u][n][i] + s[u][n][2 + i];
+          }
+          l[n][i] = l[n][i] * corr[n][i] + sum;
+        }
+      if (__any_sync(MUI_FULL_MASK, moved)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float c0 = corr[n][0] * turn, c1 = corr[n][1] * turn;
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            o[j][n][0] *= c0;
+            o[j][n][1] *= c1;
+            o[j][n][2] *= c0;
+            o[j][n][3] *= c1;
           }
         }
-    }
-    float turn = 1.f;  // e4m3: change of the reference scale of the output
-    if (KV8) {
-      float v = vref;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (tb[u] >= 0) v = fmaxf(v, t[u].vs);
-      if (v > vref) {
-        turn = vref / v;
-        vref = v;
       }
+      uint32_t pb[U][NT][2], pr[U][NT][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float f = KV8 ? (meta[u].tb >= 0 && vref > 0.f ? meta[u].vs / vref : 0.f) : 1.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float p0 = KV8 ? s[u][n][2 * h] * f : s[u][n][2 * h], p1 = KV8 ? s[u][n][2 * h + 1] * f : s[u][n][2 * h + 1];
+            const uint32_t x = Elt<M>::pack2(p0, p1);
+            pb[u][n][h] = movmatrix(x);
+            if (SPLIT_P) {
+              const float2 back = Elt<M>::unpack2(x);
+              pr[u][n][h] = movmatrix(Elt<M>::pack2(p0 - back.x, p1 - back.y));
+            }
+          }
+      }
+
+      copy_wait<3>();
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint32_t v[4][I::VW];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int slot = 2 * tq + (r & 1) + (r >> 1) * 8;
+          const uint32_t at = vslot + (u * PA_TILE + slot) * I::RB;
+          if (I::CPR == 4) {
+            lds_v2(at + (((g >> 1) ^ I::swizzle(slot)) << 4) + (g & 1) * 8, v[r][0], v[r][1]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < I::VW / 4; ++c) {
+              const uint4 w = lds16(at + (((c * 8 + g) ^ I::swizzle(slot)) << 4));
+              v[r][4 * c] = w.x;
+              v[r][4 * c + 1] = w.y;
+              v[r][4 * c + 2] = w.z;
+              v[r][4 * c + 3] = w.w;
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          uint32_t a0, a1, a2, a3;
+          if (KV8) {
+            // word j / 2 of the four rows holds dims 4 (j / 2) .. + 3 of the lane's; bytes of two rows side by side
+            const uint32_t p01 = __byte_perm(v[0][j >> 1], v[1][j >> 1], (j & 1) ? 0x7362 : 0x5140);
+            const uint32_t p89 = __byte_perm(v[2][j >> 1], v[3][j >> 1], (j & 1) ? 0x7362 : 0x5140);
+            a0 = e4m3_to_half2(static_cast<uint16_t>(p01));
+            a1 = e4m3_to_half2(static_cast<uint16_t>(p01 >> 16));
+            a2 = e4m3_to_half2(static_cast<uint16_t>(p89));
+            a3 = e4m3_to_half2(static_cast<uint16_t>(p89 >> 16));
+          } else {
+            a0 = __byte_perm(v[0][j], v[1][j], 0x5410);
+            a1 = __byte_perm(v[0][j], v[1][j], 0x7632);
+            a2 = __byte_perm(v[2][j], v[3][j], 0x5410);
+            a3 = __byte_perm(v[2][j], v[3][j], 0x7632);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816<M>(o[j][n], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
+            if (SPLIT_P) mma16816<M>(o[j][n], a0, a1, a2, a3, pr[u][n][0], pr[u][n][1]);
+          }
+        }
+      }
+      __syncwarp();
+      issue(grp + 2, 1);
     }
-    bool moved = turn != 1.f;
-    float corr[NT][2];
+
+    // join the warps in shared memory (the ring is idle: what was issued last are empty copy groups)
+    copy_wait<0>();
+    __syncthreads();
+    float* sm_o = reinterpret_cast<float*>(pa_smem);  // [warp][NT * 8][D]
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float mx = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(s[u][n][i], s[u][n][2 + i]));
-        mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 16));
-        const float mn = fmaxf(m[n][i], mx);
-        const float use = mn == -INFINITY ? 0.f : mn;
-        corr[n][i] = ex2(m[n][i] - use);
-        moved |= mn != m[n][i];
-        m[n][i] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          s[u][n][i] = ex2(s[u][n][i] - use);
-          s[u][n][2 + i] = ex2(s[u][n][2 + i] - use);
-          sum += s[u][n][i] + s[u][n][2 + i];
+        float v = l[n][i];
+        v += __shfl_xor_sync(MUI_FULL_MASK, v, 4);
+        v += __shfl_xor_sync(MUI_FULL_MASK, v, 8);
+        v += __shfl_xor_sync(MUI_FULL_MASK, v, 16);
+        const int r = n * 8 + 2 * tq + i;
+        if (g == 0) {
+          sm_m[warp][r] = m[n][i];
+          sm_l[warp][r] = v;
         }
-        l[n][i] = l[n][i] * corr[n][i] + sum;
-      }
-    if (__any_sync(MUI_FULL_MASK, moved)) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float c0 = corr[n][0] * turn, c1 = corr[n][1] * turn;
+        const float f = KV8 ? vref : 1.f;
+        float* row = sm_o + (warp * NT * 8 + r) * D;
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          o[j][n][0] *= c0;
-          o[j][n][1] *= c1;
-          o[j][n][2] *= c0;
-          o[j][n][3] *= c1;
+          const int d = KV8 ? g * (D / 8) + 2 * j : (j >> 2) * 64 + g * 8 + 2 * (j & 3);
+          *reinterpret_cast<float2*>(row + d) = make_float2(o[j][n][i] * f, o[j][n][2 + i] * f);
         }
       }
-    }
+    __syncthreads();
+    const bool whole = i_begin == 0 && i_end == sp.n;
+    // partial results: slot 0 of a CTA for a triple that began before its run, slot 1 for one that goes on after it
+    float* part = a.partials + (static_cast<size_t>(blockIdx.x) * 2 + (i_begin == 0 ? 1 : 0)) * (NT * 8 * (D + 2));
+    T* out = reinterpret_cast<T*>(a.out);
+    for (int idx = threadIdx.x; idx < min(R, NT * 8) * D; idx += PA_THREADS) {
+      const int r = idx / D, d = idx % D;
+      float mm = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const float f = KV8 ? (tb[u] >= 0 && vref > 0.f ? t[u].vs / vref : 0.f) : 1.f;
-      uint32_t pb[NT][2], pr[NT][2];
+      for (int w = 0; w < PA_WARPS; ++w) mm = fmaxf(mm, sm_m[w][r]);
+      const float use = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f, oo = 0.f;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float p0 = s[u][n][2 * h] * f, p1 = s[u][n][2 * h + 1] * f;
-          const uint32_t x = Elt<M>::pack2(p0, p1);
-          pb[n][h] = movmatrix(x);
-          if (SPLIT_P) {
-            const float2 back = Elt<M>::unpack2(x);
-            pr[n][h] = movmatrix(Elt<M>::pack2(p0 - back.x, p1 - back.y));
-          }
+      for (int w = 0; w < PA_WARPS; ++w) {
+        const float f = ex2(sm_m[w][r] - use);
+        ll = fmaf(sm_l[w][r], f, ll);
+        oo = fmaf(sm_o[(w * NT * 8 + r) * D + d], f, oo);
+      }
+      if (whole) {
+        const int rr = rblock + r;
+        out[(static_cast<size_t>(first + rr / a.G) * a.Hq + kvh * a.G + rr % a.G) * D + d] =
+            Elt<T>::from_f32(ll != 0.f ? oo / ll : 0.f);
+      } else {
+        float* p = part + r * (D + 2);
+        if (d == 0) {
+          p[0] = mm;
+          p[1] = ll;
         }
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        uint32_t a0, a1, a2, a3;
-        if (KV8) {
-          // word j / 2 of the four rows holds dims 4 (j / 2) .. + 3 of the lane's; bytes of two rows side by side
-          const uint32_t lo01 = __byte_perm(t[u].v[0][j >> 1], t[u].v[1][j >> 1], (j & 1) ? 0x7362 : 0x5140);
-          const uint32_t lo89 = __byte_perm(t[u].v[2][j >> 1], t[u].v[3][j >> 1], (j & 1) ? 0x7362 : 0x5140);
-          a0 = e4m3_to_half2(static_cast<uint16_t>(lo01));
-          a1 = e4m3_to_half2(static_cast<uint16_t>(lo01 >> 16));
-          a2 = e4m3_to_half2(static_cast<uint16_t>(lo89));
-          a3 = e4m3_to_half2(static_cast<uint16_t>(lo89 >> 16));
-        } else {
-          a0 = __byte_perm(t[u].v[0][j], t[u].v[1][j], 0x5410);
-          a1 = __byte_perm(t[u].v[0][j], t[u].v[1][j], 0x7632);
-          a2 = __byte_perm(t[u].v[2][j], t[u].v[3][j], 0x5410);
-          a3 = __byte_perm(t[u].v[2][j], t[u].v[3][j], 0x7632);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mma16816<M>(o[j][n], a0, a1, a2, a3, pb[n][0], pb[n][1]);
-          if (SPLIT_P) mma16816<M>(o[j][n], a0, a1, a2, a3, pr[n][0], pr[n][1]);
-        }
+        p[2 + d] = oo;
       }
     }
-  };
+    __syncthreads();
+    }
 
-  {
-    // two register sets: the loads of one are in flight while the other is multiplied
-    Tile<KV8, D> t0[U], t1[U];
-    int tb0[U], tb1[U];
-    int n = 0;
-    fetch(n, t0, tb0);
-    for (int i = i_begin; i < i_end; i += 2 * STEP) {
-      fetch(n + U, t1, tb1);
-      consume(t0, tb0);
-      if (i + STEP >= i_end) break;
-      fetch(n + 2 * U, t0, tb0);
-      consume(t1, tb1);
-      n += 2 * U;
-    }
-  }
-
-  // join the warps: sums over the lanes of a column first
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float v = l[n][i];
-      v += __shfl_xor_sync(MUI_FULL_MASK, v, 4);
-      v += __shfl_xor_sync(MUI_FULL_MASK, v, 8);
-      v += __shfl_xor_sync(MUI_FULL_MASK, v, 16);
-      const int r = n * 8 + 2 * tq + i;
-      if (g == 0) {
-        sm_m[warp * NT * 8 + r] = m[n][i];
-        sm_l[warp * NT * 8 + r] = v;
-      }
-      const float f = KV8 ? vref : 1.f;
-      float* row = sm_o + (warp * NT * 8 + r) * D;
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int d = KV8 ? g * (D / 8) + 2 * j : (j >> 2) * 64 + g * 8 + 2 * (j & 3);
-        row[d] = o[j][n][i] * f;
-        row[d + 1] = o[j][n][2 + i] * f;
-      }
-    }
-  __syncthreads();
-  T* out = reinterpret_cast<T*>(a.out);
-  for (int idx = threadIdx.x; idx < R * D; idx += PA_THREADS) {
-    const int r = idx / D, d = idx % D;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) mm = fmaxf(mm, sm_m[w * NT * 8 + r]);
-    const float use = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f, oo = 0.f;
-#pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) {
-      const float f = ex2(sm_m[w * NT * 8 + r] - use);
-      ll = fmaf(sm_l[w * NT * 8 + r], f, ll);
-      oo = fmaf(sm_o[(w * NT * 8 + r) * D + d], f, oo);
-    }
-    const size_t row = static_cast<size_t>(first + r / a.G) * a.Hq + kvh * a.G + r % a.G;
-    if (active == 1) {
-      out[row * D + d] = Elt<T>::from_f32(ll != 0.f ? oo / ll : 0.f);
-    } else {
-      float* p = a.partials + (row * a.splits + split) * (D + 2);
-      if (d == 0) {
-        p[0] = mm;
-        p[1] = ll;
-      }
-      p[2 + d] = oo;
+    place += at_end - at;
+    if (place >= place_end) break;
+    if (place - seq_begin >= static_cast<long long>(places) * pairs) {  // next sequence that has tiles
+      seq_begin += static_cast<long long>(places) * pairs;
+      do ++b;
+      while (b < a.kv.batch && seq_places(a, b) == 0);
     }
   }
 }
 
-// Joins the splits of a row in split order: a warp per (new token, query head).
-template <typename T, int D>
+// Joins the partial results of the triples that several CTAs shared. A CTA per (triple, row): its warps take the partial
+// results in turn and are joined in shared memory, always in the same order.
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a) {
+  __shared__ long long s_warp[PA_WARPS];
+  __shared__ long long s_begin;
+  __shared__ float sm_m[PA_WARPS], sm_l[PA_WARPS], sm_o[PA_WARPS][D];
   pdl_wait_prior_grid();
   pdl_launch_dependents();
-  const int lane = threadIdx.x & 31;
-  const long long row = static_cast<long long>(blockIdx.x) * PA_WARPS + (threadIdx.x >> 5);
-  const int t = static_cast<int>(row / a.Hq);
-  if (t >= a.kv.total) return;
-  int b = t;
-  if (a.kv.cu != nullptr) {
-    const int32_t* cu = a.kv.cu;
-    b = warp_count_le(a.kv.batch, t, [&](int k) { return __ldcg(cu + 1 + k); });
-    if (b >= a.kv.batch) return;
-  }
+  const int pairs = a.kv.kv_heads * a.row_blocks;
+  const int r = blockIdx.x % (NT * 8), triple = blockIdx.x / (NT * 8);
+  const int b = triple / pairs, pair = triple % pairs;
+  const int kvh = pair / a.row_blocks, rblock = (pair % a.row_blocks) * (NT * 8);
   int first, count;
   paged_new_tokens(a.kv, b, first, count);
-  const int ctx = __ldcg(a.kv.context_lens + b);
-  if (count == 0 || ctx < 0 || count > a.max_new) return;
-  const Span sp = visible_span(a, ctx, count);
-  const int per = split_tiles(sp.n, a.splits);
-  const int active = (sp.n + per - 1) / per;
-  if (active <= 1) return;
-  const float* p = a.partials + static_cast<size_t>(row) * a.splits * (D + 2);
-  float mm = -INFINITY;
-  for (int s = lane; s < active; s += 32) mm = fmaxf(mm, __ldcg(p + static_cast<size_t>(s) * (D + 2)));
-  mm = warp_max(mm);
-  const float use = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, o[D / 32] = {};
-#pragma unroll 4
-  for (int s = 0; s < active; ++s) {
-    const float* ps = p + static_cast<size_t>(s) * (D + 2);
-    const float f = ex2(__ldcg(ps) - use);
-    ll = fmaf(__ldcg(ps + 1), f, ll);
+  if (rblock + r >= count * a.G) return;
+  const int per_thread = (a.kv.batch + PA_THREADS - 1) / PA_THREADS;
+  long long begin;
+  const long long total = scan_sequences(a, per_thread, begin, s_warp);
+  if (b / per_thread == static_cast<int>(threadIdx.x)) {
+    for (int i = threadIdx.x * per_thread; i < b; ++i) begin += static_cast<long long>(seq_places(a, i)) * pairs;
+    s_begin = begin;
+  }
+  __syncthreads();
+  const int places = seq_places(a, b);
+  if (places == 0) return;
+  const long long len = run_length(total, a.ctas);
+  const long long at = s_begin + static_cast<long long>(pair) * places;
+  // the runs of the first and of the last tile; the first one left slot 1 (the triple begins in it), the others slot 0
+  const int c0 = static_cast<int>((at + a.lead) / len), c1 = static_cast<int>((at + places - 1) / len);
+  if (c0 == c1) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float mm = -INFINITY, ll = 0.f, o[D / 32] = {};
+  for (int c = c0 + warp; c <= c1; c += 4 * PA_WARPS) {
+    float pm[4], pl[4];
+    float2 v[4][D / 64];
 #pragma unroll
-    for (int e = 0; e < D / 64; ++e) {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(ps + 2) + e * 32 + lane);
-      o[2 * e] = fmaf(v.x, f, o[2 * e]);
-      o[2 * e + 1] = fmaf(v.y, f, o[2 * e + 1]);
+    for (int i = 0; i < 4; ++i) {  // four partial results of loads in flight
+      const int cc = c + i * PA_WARPS;
+      pm[i] = -INFINITY;
+      pl[i] = 0.f;
+      if (cc <= c1) {
+        const float* p = a.partials + ((static_cast<size_t>(cc) * 2 + (cc == c0 ? 1 : 0)) * (NT * 8) + r) * (D + 2);
+        pm[i] = __ldcg(p);
+        pl[i] = __ldcg(p + 1);
+#pragma unroll
+        for (int e = 0; e < D / 64; ++e) v[i][e] = __ldcg(reinterpret_cast<const float2*>(p + 2) + e * 32 + lane);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (pm[i] == -INFINITY) continue;
+      const float mn = fmaxf(mm, pm[i]), f0 = ex2(mm - mn), f1 = ex2(pm[i] - mn);
+      mm = mn;
+      ll = ll * f0 + pl[i] * f1;
+#pragma unroll
+      for (int e = 0; e < D / 64; ++e) {
+        o[2 * e] = o[2 * e] * f0 + v[i][e].x * f1;
+        o[2 * e + 1] = o[2 * e + 1] * f0 + v[i][e].y * f1;
+      }
     }
   }
-  const float inv = ll != 0.f ? 1.f / ll : 0.f;
-  uint32_t* out = reinterpret_cast<uint32_t*>(a.out) + static_cast<size_t>(row) * (D / 2);
+  if (lane == 0) {
+    sm_m[warp] = mm;
+    sm_l[warp] = ll;
+  }
 #pragma unroll
-  for (int e = 0; e < D / 64; ++e) out[e * 32 + lane] = Elt<T>::pack2(o[2 * e] * inv, o[2 * e + 1] * inv);
+  for (int e = 0; e < D / 64; ++e)
+    *reinterpret_cast<float2*>(&sm_o[warp][(e * 32 + lane) * 2]) = make_float2(o[2 * e], o[2 * e + 1]);
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += PA_THREADS) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) m = fmaxf(m, sm_m[w]);
+    const float use = m == -INFINITY ? 0.f : m;
+    float l = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) {
+      const float f = ex2(sm_m[w] - use);
+      l = fmaf(sm_l[w], f, l);
+      x = fmaf(sm_o[w][d], f, x);
+    }
+    const int rr = rblock + r;
+    reinterpret_cast<T*>(a.out)[(static_cast<size_t>(first + rr / a.G) * a.Hq + kvh * a.G + rr % a.G) * D + d] =
+        Elt<T>::from_f32(l != 0.f ? x / l : 0.f);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -663,8 +844,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_prompt_kernel(const PaArgs a
             v4 = make_uint4(e4m3_to_half2((uint16_t)v2.x), e4m3_to_half2((uint16_t)(v2.x >> 16)),
                             e4m3_to_half2((uint16_t)v2.y), e4m3_to_half2((uint16_t)(v2.y >> 16)));
           } else {
-            k4 = ld_kv16(kp);
-            v4 = ld_kv16(vp);
+            k4 = ld_stream16(kp);
+            v4 = ld_stream16(vp);
           }
         }
         const int at = (warp * 16 + row) * CH + (ch ^ (row & 7));
@@ -768,44 +949,46 @@ __global__ void __launch_bounds__(PA_THREADS) paged_prompt_kernel(const PaArgs a
 // ---------------------------------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
-// Splits per sequence: enough CTAs to fill the GPU, each with PA_MIN_TILES tiles at least for the longest span.
-int pa_splits(int sm_count, int batch, int kv_heads, int max_new, int max_context, int window, int sinks) {
+// rows per block of the decode kernel: one block of eight, else blocks of sixteen
+int pa_block_rows(int G, int max_new) { return G * max_new <= 8 ? 8 : 16; }
+// CTAs of the decode kernel: as many as fit the GPU at once, fewer when the longest sequence expected leaves them without
+// PA_MIN_TILES tiles each
+int pa_ctas(int sm_count, int batch, int kv_heads, int G, int max_new, int max_context, int window, int sinks) {
   long long span = max_context;
   if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + max_new + sinks);
-  const long long tiles = (span + PA_TILE - 1) / PA_TILE + 1;
-  const long long most = std::max<long long>(1, (tiles + PA_MIN_TILES - 1) / PA_MIN_TILES);
-  const long long base = std::max(1, batch * kv_heads);
-  const long long want = (static_cast<long long>(sm_count) * 4 + base - 1) / base;
-  return static_cast<int>(std::max<long long>(1, std::min<long long>({want, most, PA_MAX_SPLITS})));
+  const int block = pa_block_rows(G, max_new);
+  const long long tiles = ((span + PA_TILE - 1) / PA_TILE + 2) * batch * kv_heads * ((G * max_new + block - 1) / block);
+  const long long most = static_cast<long long>(sm_count) * (block == 8 ? 3 : 2);
+  return static_cast<int>(std::max<long long>(1, std::min(most, (tiles + PA_MIN_TILES - 1) / PA_MIN_TILES)));
+}
+size_t pa_workspace(int ctas, int block, int D) {
+  return ctas == 1 ? 0 : static_cast<size_t>(ctas) * 2 * block * (D + 2) * sizeof(float);
 }
 
 bool pa_decode(int G, int max_new) { return static_cast<long long>(G) * max_new <= PA_MAX_DECODE_ROWS; }
 
-template <typename T, bool KV8, int D, int NT, int U>
-mui_status_t launch_decode(cudaStream_t stream, const PaArgs& a, int pdl) {
-  const size_t smem = sizeof(float) * PA_WARPS * NT * 8 * (D + 2);
-  if (smem > 48 * 1024)
-    MUI_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_kernel<T, KV8, D, NT, U>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+template <typename T, bool KV8, int D, int NT>
+mui_status_t launch_decode(cudaStream_t stream, const PaArgs& a, int pdl, int device) {
+  constexpr size_t smem = PA_WARPS * PA_RING * PA_ITEM;
+  static std::atomic<unsigned long long> configured{0};  // one bit per device
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(configured.load() & bit)) {
+    MUI_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_kernel<T, KV8, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         static_cast<int>(smem)));
-  MUI_CUDA_CHECK(mui_launch(paged_decode_kernel<T, KV8, D, NT, U>, dim3(a.splits, a.kv.kv_heads, a.kv.batch),
-                            dim3(PA_THREADS), smem, stream, pdl, a));
-  if (a.splits > 1) {
-    const long long rows = static_cast<long long>(a.kv.total) * a.Hq;
-    MUI_CUDA_CHECK(mui_launch(paged_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + PA_WARPS - 1) / PA_WARPS)),
-                              dim3(PA_THREADS), 0, stream, 1, a));
+    configured.fetch_or(bit);
   }
+  MUI_CUDA_CHECK(mui_launch(paged_decode_kernel<T, KV8, D, NT>, dim3(a.ctas), dim3(PA_THREADS), smem, stream, pdl, a));
+  if (a.ctas > 1)
+    MUI_CUDA_CHECK(mui_launch(paged_merge_kernel<T, D, NT>, dim3(static_cast<unsigned>(a.kv.batch) * a.kv.kv_heads * a.row_blocks * NT * 8),
+                              dim3(PA_THREADS), 0, stream, 1, a));
   return MUI_OK;
 }
 
 template <typename T, bool KV8, int D>
-mui_status_t launch_attention(cudaStream_t stream, const PaArgs& a, int pdl) {
-  constexpr int U = KV8 ? 2 : 1;
-  if (pa_decode(a.G, a.max_new)) {
-    const int rows = a.G * a.max_new;
-    if (rows <= 8) return launch_decode<T, KV8, D, 1, U>(stream, a, pdl);
-    if (rows <= 16) return launch_decode<T, KV8, D, 2, U>(stream, a, pdl);
-    return launch_decode<T, KV8, D, 4, U>(stream, a, pdl);
-  }
+mui_status_t launch_attention(cudaStream_t stream, const PaArgs& a, int pdl, int device) {
+  if (pa_decode(a.G, a.max_new))
+    return pa_block_rows(a.G, a.max_new) == 8 ? launch_decode<T, KV8, D, 1>(stream, a, pdl, device)
+                                              : launch_decode<T, KV8, D, 2>(stream, a, pdl, device);
   const long long tiles = a.kv.cu ? static_cast<long long>(a.kv.total) * a.G / PP_ROWS + a.kv.batch
                                   : static_cast<long long>(a.kv.batch) * ((a.G + PP_ROWS - 1) / PP_ROWS);
   MUI_REQUIRE(tiles <= 0x7fffffff, MUI_ERR_UNSUPPORTED, "too many rows");
@@ -826,9 +1009,9 @@ size_t mui_paged_attention_workspace_bytes(int total_tokens, int batch, int num_
   if (!pa_decode(num_q_heads / kv_heads, max_new_tokens)) return 0;
   const MuiDeviceInfo* di = mui_current_device_info();
   if (!di) return 0;
-  const int splits = pa_splits(di->sm_count, batch, kv_heads, max_new_tokens, max_context, window, sinks);
-  if (splits == 1) return 0;
-  return static_cast<size_t>(total_tokens) * num_q_heads * splits * (head_dim + 2) * sizeof(float);
+  const int G = num_q_heads / kv_heads;
+  return pa_workspace(pa_ctas(di->sm_count, batch, kv_heads, G, max_new_tokens, max_context, window, sinks),
+                      pa_block_rows(G, max_new_tokens), head_dim);
 }
 
 mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_paged_kv_t* cache, int num_q_heads,
@@ -859,12 +1042,16 @@ mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_page
   a.window = window;
   a.sinks = sinks;
   a.scale_log2 = scale * 1.44269504088896341f;
-  a.splits = 1;
+  a.ctas = a.row_blocks = 1;
+  // a tile is 16 rows of K and of V
+  a.lead = PA_TRIPLE_COST * 4096 / (2 * PA_TILE * cache->head_dim * (cache->format == MUI_KV_E4M3 ? 1 : 2));
   if (pa_decode(G, max_new_tokens)) {
-    a.splits = pa_splits(di->sm_count, cache->batch, cache->kv_heads, max_new_tokens, max_context, window, sinks);
-    const size_t need = a.splits == 1 ? 0
-                                      : static_cast<size_t>(cache->total_tokens) * num_q_heads * a.splits *
-                                            (cache->head_dim + 2) * sizeof(float);
+    const int block = pa_block_rows(G, max_new_tokens);
+    a.row_blocks = (G * max_new_tokens + block - 1) / block;
+    a.ctas = pa_ctas(di->sm_count, cache->batch, cache->kv_heads, G, max_new_tokens, max_context, window, sinks);
+    const size_t need = pa_workspace(a.ctas, block, cache->head_dim);
+    MUI_REQUIRE(static_cast<long long>(cache->batch) * cache->kv_heads * a.row_blocks * block <= 0x7fffffff, MUI_ERR_UNSUPPORTED,
+                "batch=%d times kv_heads=%d is too large", cache->batch, cache->kv_heads);
     MUI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need &&
                               (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                 MUI_ERR_INVALID_ARG, "workspace of %zu bytes (16-byte aligned) needed, %zu given", need,
@@ -874,8 +1061,8 @@ mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_page
   const int pdl = (flags & MUI_FLAG_PDL) ? 1 : 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define PA_GO(T, D)                                                            \
-  (cache->format == MUI_KV_E4M3 ? launch_attention<T, true, D>(st, a, pdl) \
-                                : launch_attention<T, false, D>(st, a, pdl))
+  (cache->format == MUI_KV_E4M3 ? launch_attention<T, true, D>(st, a, pdl, di->device) \
+                                : launch_attention<T, false, D>(st, a, pdl, di->device))
   if (dtype == MUI_F16) return cache->head_dim == 128 ? PA_GO(__half, 128) : PA_GO(__half, 64);
   return cache->head_dim == 128 ? PA_GO(__nv_bfloat16, 128) : PA_GO(__nv_bfloat16, 64);
 #undef PA_GO
