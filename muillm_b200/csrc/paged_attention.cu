@@ -21,7 +21,7 @@ constexpr int PA_THREADS = 128;
 constexpr int PA_WARPS = PA_THREADS / 32;
 constexpr int PA_MIN_TILES = 16;   // tiles per CTA at least (256 tokens)
 // What beginning and joining a triple costs a CTA, in the time of 4 KiB of K or V: the runs are cut by this measure
-constexpr int PA_TRIPLE_COST = 16;
+constexpr int PA_TRIPLE_COST = 24;
 constexpr int PA_MAX_DECODE_ROWS = 32;
 
 struct PaArgs {
@@ -30,7 +30,7 @@ struct PaArgs {
   mui_strides2_t qs;
   void* out;
   float* partials;  // [ctas, 2, rows per block, D + 2]: maximum, sum, unnormalised output
-  int Hq, G, ctas, row_blocks, lead, max_new, window, sinks;
+  int Hq, G, ctas, row_blocks, lead, max_new, window, sinks, q_vec;
   float scale_log2;
 };
 
@@ -87,18 +87,22 @@ __device__ __forceinline__ uint2 ld_kv8(const void* p) {
 // others leave partial results, at most two per CTA (the triple that the run starts in and the one it ends in), which
 // paged_merge_kernel joins in order.
 struct Run {
-  int seq;          // sequence at the run's first place
-  long long begin;  // place at which that sequence begins
+  int seq, first, count, ctx;  // sequence at the run's first place
+  long long begin;             // place at which that sequence begins
 };
 
 // Length of a sequence's triples in places: `lead` places for their beginning, then one for each tile; 0: nothing to do
-__device__ __forceinline__ int seq_places(const PaArgs& a, int b) {
-  int first, count;
-  paged_new_tokens(a.kv, b, first, count);
-  const int ctx = __ldcg(a.kv.context_lens + b);
-  if (count == 0 || ctx < 0 || count > a.max_new) return 0;
-  const int n = visible_span(a, ctx, count).n;
+__device__ __forceinline__ int seq_places(const PaArgs& a, int b, Run& r) {
+  paged_new_tokens(a.kv, b, r.first, r.count);
+  r.ctx = __ldcg(a.kv.context_lens + b);
+  r.seq = b;
+  if (r.count == 0 || r.ctx < 0 || r.count > a.max_new) return 0;
+  const int n = visible_span(a, r.ctx, r.count).n;
   return n ? a.lead + n : 0;
+}
+__device__ __forceinline__ int seq_places(const PaArgs& a, int b) {
+  Run r;
+  return seq_places(a, b, r);
 }
 
 // Places of all triples, and the place at which the sequences of this thread (blocks of `per_thread`) begin. CTA-wide.
@@ -171,6 +175,19 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   return v;
 }
 
+// eight consecutive elements of a q row (zeros for a row that does not exist); vec: rows are 16-byte aligned
+template <typename T>
+__device__ __forceinline__ uint4 load_q8(const T* p, int vec) {
+  if (p == nullptr) return make_uint4(0, 0, 0, 0);
+  if (vec) return ld_act16(p);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = __ldcg(reinterpret_cast<const unsigned short*>(p) + 2 * i) |
+           static_cast<uint32_t>(__ldcg(reinterpret_cast<const unsigned short*>(p) + 2 * i + 1)) << 16;
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 struct TileMeta {
   int tb;        // first cache row, -1: nothing to see
   float ks, vs;  // page scales (e4m3)
@@ -200,46 +217,38 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
   const int per_thread = (a.kv.batch + PA_THREADS - 1) / PA_THREADS;
   long long begin;
   const long long total = scan_sequences(a, per_thread, begin, s_warp);
-  if (blockIdx.x == 0)  // sequences that cannot be served have no tiles: say so
-    for (int i = 0; i < per_thread; ++i) {
-      const int s = threadIdx.x * per_thread + i;
-      if (s >= a.kv.batch) break;
-      int first, count;
-      paged_new_tokens(a.kv, s, first, count);
-      const int ctx = __ldcg(a.kv.context_lens + s);
-      if (count > a.max_new || (count > 0 && ctx < 0))
-        mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx < 0 ? ctx : count));
-    }
   const long long len = run_length(total, gridDim.x);
   long long place = len * blockIdx.x;
   const long long place_end = min(total, place + len);
-  if (place >= place_end) return;
+  if (place >= place_end && blockIdx.x != 0) return;
   for (int i = 0; i < per_thread; ++i) {
-    const int b = threadIdx.x * per_thread + i;
-    if (b >= a.kv.batch) break;
-    const long long n = static_cast<long long>(seq_places(a, b)) * pairs;
+    const int s = threadIdx.x * per_thread + i;
+    if (s >= a.kv.batch) break;
+    Run r;
+    const long long n = static_cast<long long>(seq_places(a, s, r)) * pairs;
+    // sequences that cannot be served have no places: say so
+    if (blockIdx.x == 0 && n == 0 && r.count > 0 && (r.ctx < 0 || r.count > a.max_new))
+      mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(r.ctx < 0 ? r.ctx : r.count));
     if (place >= begin && place < begin + n) {
-      s_run.seq = b;
-      s_run.begin = begin;
+      r.begin = begin;
+      s_run = r;
     }
     begin += n;
   }
+  if (place >= place_end) return;
   __syncthreads();
-  int b = s_run.seq;
-  long long seq_begin = s_run.begin;
+  Run run = s_run;
 
   const uint32_t ring = smem_u32(pa_smem) + warp * (PA_RING * PA_ITEM);
   while (true) {
-    int first, count;
-    paged_new_tokens(a.kv, b, first, count);
-    const int ctx = __ldcg(a.kv.context_lens + b);
+    const int b = run.seq, first = run.first, count = run.count, ctx = run.ctx;
     const Span sp = visible_span(a, ctx, count);
     if (sp.kv_len < ctx + count && threadIdx.x == 0)
       mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx + count));
     const int places = a.lead + sp.n;
-    const int pair = static_cast<int>((place - seq_begin) / places);
+    const int pair = static_cast<int>((place - run.begin) / places);
     const int kvh = pair / a.row_blocks, rblock = (pair % a.row_blocks) * (NT * 8);
-    const int at = static_cast<int>(place - seq_begin - static_cast<long long>(pair) * places);
+    const int at = static_cast<int>(place - run.begin - static_cast<long long>(pair) * places);
     const int at_end = static_cast<int>(min(static_cast<long long>(places), at + (place_end - place)));
     const int i_begin = max(0, at - a.lead), i_end = max(0, at_end - a.lead);
     const int R = count * a.G - rblock;  // rows from this block on; none left: the tiles are walked past
@@ -250,33 +259,46 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
     const int32_t* table = a.kv.block_table + static_cast<size_t>(b) * a.kv.table_stride;
     const int groups = (i_end - i_begin + U - 1) / U;           // of all warps
     const int my_groups = groups > warp ? (groups - warp + PA_WARPS - 1) / PA_WARPS : 0;
-    int my_page = -1, my_tb = -1;
-    float my_ks = 0.f, my_vs = 0.f;
-    auto look_up = [&](int grp) {
+    // The next 32 are begun half a batch ahead: pages first, their scales once the pages are there.
+    int my_page = -1, my_tb = -1, next_page = -1, next_tb = -1;
+    float my_ks = 0.f, my_vs = 0.f, next_ks = 0.f, next_vs = 0.f;
+    auto ask_pages = [&](int grp) {
       const int i = i_begin + ((grp + lane / U) * PA_WARPS + warp) * U + lane % U;
-      my_page = my_tb = -1;
-      my_ks = my_vs = 0.f;
+      next_page = next_tb = -1;
       if (i < i_end) {
-        const int tile = span_tile(sp, i);
-        const int page = __ldcg(table + (tile * PA_TILE >> a.kv.page_shift));
-        if (page >= 0 && page < a.kv.num_pages) {
-          my_page = page;
-          my_tb = tile * PA_TILE;
-          if (KV8) {
-            const size_t head = static_cast<size_t>(page) * a.kv.kv_heads + kvh;
-            my_ks = __ldcg(a.kv.k_scales + head);
-            my_vs = __ldcg(a.kv.v_scales + head);
-          }
-        } else {
-          mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(b));
-        }
+        next_tb = span_tile(sp, i) * PA_TILE;
+        next_page = __ldcg(table + (next_tb >> a.kv.page_shift));
+      }
+    };
+    auto ask_scales = [&]() {
+      if (next_tb >= 0 && (next_page < 0 || next_page >= a.kv.num_pages)) {
+        mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(b));
+        next_page = next_tb = -1;
+      }
+      next_ks = next_vs = 0.f;
+      if (KV8 && next_tb >= 0) {
+        const size_t head = static_cast<size_t>(next_page) * a.kv.kv_heads + kvh;
+        next_ks = __ldcg(a.kv.k_scales + head);
+        next_vs = __ldcg(a.kv.v_scales + head);
       }
     };
     // starts the copy of group grp's K (which == 0) or V; always closes one copy group
     auto issue = [&](int grp, int which) {
       if (grp < my_groups) {
         if (which == 0) {
-          if ((grp * U & 31) == 0) look_up(grp);
+          const int phase = grp * U & 31;
+          if (phase == 0) {
+            if (grp == 0) {
+              ask_pages(0);
+              ask_scales();
+            }
+            my_page = next_page;
+            my_tb = next_tb;
+            my_ks = next_ks;
+            my_vs = next_vs;
+          }
+          if (phase == 16) ask_pages(grp + 16 / U);
+          if (phase == 24) ask_scales();
           if ((grp * U & 31) / U == lane / U) {
             TileMeta& t = sm_meta[warp][grp & 1][lane % U];
             t.tb = my_tb;
@@ -313,6 +335,20 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
       copy_commit();
     };
 
+    // q is requested before the first copies, which would delay it by microseconds, and converted after them
+    uint4 q_raw[NT][KB][KS / 2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = rblock + n * 8 + g;
+      const T* qp = nullptr;
+      if (r < count * a.G)
+        qp = reinterpret_cast<const T*>(a.q) + (first + r / a.G) * a.qs.tok + (kvh * a.G + r % a.G) * a.qs.head;
+#pragma unroll
+      for (int c = 0; c < KB; ++c)
+#pragma unroll
+        for (int e = 0; e < KS / 2; ++e)
+          q_raw[n][c][e] = load_q8<T>(qp ? qp + c * (KS * 16) + tq * (KS * 4) + e * 8 : nullptr, a.q_vec);
+    }
     issue(0, 0);
     issue(0, 1);
     issue(1, 0);
@@ -324,20 +360,19 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
     int hi[NT][2], lo[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = n * 8 + g;
-      const T* qp = nullptr;
-      if (r < R)
-        qp = reinterpret_cast<const T*>(a.q) + (first + (rblock + r) / a.G) * a.qs.tok +
-             (kvh * a.G + (rblock + r) % a.G) * a.qs.head;
       float amax = 0.f;
       float qv[KB][KS * 4];
 #pragma unroll
       for (int c = 0; c < KB; ++c)
 #pragma unroll
-        for (int e = 0; e < KS * 4; ++e) {
-          const int d = c * (KS * 16) + tq * (KS * 4) + e;
-          qv[c][e] = qp ? ld_act_f32<T>(qp + d) : 0.f;
-          amax = fmaxf(amax, fabsf(qv[c][e]));
+        for (int e = 0; e < KS / 2; ++e) {
+          float x[8];
+          unpack8<T>(q_raw[n][c][e], x);
+#pragma unroll
+          for (int h = 0; h < 8; ++h) {
+            qv[c][8 * e + h] = x[h];
+            amax = fmaxf(amax, fabsf(x[h]));
+          }
         }
       float mul = 1.f, back = 1.f;
       if (KV8) {
@@ -610,10 +645,11 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
 
     place += at_end - at;
     if (place >= place_end) break;
-    if (place - seq_begin >= static_cast<long long>(places) * pairs) {  // next sequence that has tiles
-      seq_begin += static_cast<long long>(places) * pairs;
-      do ++b;
-      while (b < a.kv.batch && seq_places(a, b) == 0);
+    if (place - run.begin >= static_cast<long long>(places) * pairs) {  // next sequence that has tiles
+      const long long next = run.begin + static_cast<long long>(places) * pairs;
+      int s = b + 1;
+      while (s < a.kv.batch && seq_places(a, s, run) == 0) ++s;
+      run.begin = next;
     }
   }
 }
@@ -625,7 +661,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
   __shared__ long long s_warp[PA_WARPS];
   __shared__ long long s_begin;
   __shared__ float sm_m[PA_WARPS], sm_l[PA_WARPS], sm_o[PA_WARPS][D];
-  pdl_wait_prior_grid();
+  // Lengths were there before the attention kernel began (it waits for its predecessors before it lets this one start), so
+  // they are read while it still runs; its partial results only after the wait. Every CTA waits, also one without work: this
+  // grid must not be done before the attention kernel is.
   pdl_launch_dependents();
   const int pairs = a.kv.kv_heads * a.row_blocks;
   const int r = blockIdx.x % (NT * 8), triple = blockIdx.x / (NT * 8);
@@ -633,7 +671,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
   const int kvh = pair / a.row_blocks, rblock = (pair % a.row_blocks) * (NT * 8);
   int first, count;
   paged_new_tokens(a.kv, b, first, count);
-  if (rblock + r >= count * a.G) return;
+  if (rblock + r >= count * a.G) {
+    pdl_wait_prior_grid();
+    return;
+  }
   const int per_thread = (a.kv.batch + PA_THREADS - 1) / PA_THREADS;
   long long begin;
   const long long total = scan_sequences(a, per_thread, begin, s_warp);
@@ -643,12 +684,12 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
   }
   __syncthreads();
   const int places = seq_places(a, b);
-  if (places == 0) return;
   const long long len = run_length(total, a.ctas);
   const long long at = s_begin + static_cast<long long>(pair) * places;
   // the runs of the first and of the last tile; the first one left slot 1 (the triple begins in it), the others slot 0
   const int c0 = static_cast<int>((at + a.lead) / len), c1 = static_cast<int>((at + places - 1) / len);
-  if (c0 == c1) return;
+  pdl_wait_prior_grid();
+  if (places == 0 || c0 >= c1) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float mm = -INFINITY, ll = 0.f, o[D / 32] = {};
   for (int c = c0 + warp; c <= c1; c += 4 * PA_WARPS) {
@@ -1039,6 +1080,7 @@ mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_page
   a.Hq = num_q_heads;
   a.G = G;
   a.max_new = max_new_tokens;
+  a.q_vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (q_strides.tok & 7) == 0 && (q_strides.head & 7) == 0;
   a.window = window;
   a.sinks = sinks;
   a.scale_log2 = scale * 1.44269504088896341f;
