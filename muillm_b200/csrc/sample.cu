@@ -1,26 +1,29 @@
 // Drawing a token from each row of logits: temperature, top-k, top-p, min-p, inverse transform of a given uniform number.
 //
 // With z = (logit - largest) / temperature and w = exp(z), the kept tokens are a run from the front of the ranking by
-// (logit descending, index ascending), so two numbers describe them: kept is key > T, or key == T and index <= T_idx. No
-// sort is needed, only that threshold.
+// (logit descending, index ascending), so two numbers describe them: kept is key > T, or key == T and index <= T_idx.
 //
 // Sums of weights decide which token is drawn, so they must not depend on the order in which threads add: w is taken in
-// fp64 and rounded once to an integer with S fraction bits (S = min(50, 62 - ceil(log2 vocab)); 44 for 200 k tokens; no sum
+// fp64 and rounded once to an integer with S fraction bits (S = min(48, 62 - ceil(log2 vocab)); 44 for 200 k tokens; no sum
 // overflows), and integers are summed. A weight that rounds to 0 can never be drawn. Against real arithmetic a boundary is
 // off by sqrt(vocab) * 2^-S of the largest weight or so, 3e-11 for 200 k tokens.
 //
 // A cluster of up to eight CTAs works on a row (one CTA when there are rows enough to fill the GPU). Passes over the row:
 //   1. the largest logit (from HBM; the later passes find the row in L2);
-//   2. a histogram of z in 4096 equal bins down to the smallest z that still has weight. Counts give the bin that holds
-//      the top_k-th token exactly; counts times the bin centre's weight tell the bin in which top_p ends, nearly always;
-//   3. exact sums of the weight above and between these two bins; the bins' own tokens (some hundred) are collected in rank
-//      0's shared memory, sorted, and give T and T_idx; where the estimate was off, again with the neighbouring bin;
-//   4. the kept weight of every run of 256 tokens; the run that holds the drawn point is then walked by one warp.
-// Without top-k and top-p only 1 and 4 run. Where a bin has more tokens than the list holds (long ties, very high
-// temperatures) T and T_idx are found by bisection over keys and indices instead: slower, same result.
+//   2. with top-k or top-p, a histogram of z in 4096 equal bins down to the smallest z that still has weight. Counts give the
+//      bin that holds the top_k-th token exactly; counts times the bin centre's weight tell the bin in which top_p ends,
+//      nearly always. Not needed where min-p alone leaves few tokens;
+//   3. all tokens up to that bin (or above min-p's cut) are collected in rank 0's shared memory if they are at most 4096, with
+//      the weight of the whole row where top-p asks for it. Sorted by rank they give T and T_idx, sorted by index the token.
+// More tokens than that (a nucleus of thousands, a temperature without cuts):
+//   3'. exact sums of the weight above and between the boundary bins, whose own tokens are collected and sorted to give T and
+//      T_idx; where the estimate of 2 was off, again with the neighbouring bin;
+//   4'. the kept weight of every run of 256 tokens; the run that holds the drawn point is then walked by one warp.
+// Where even one bin has more tokens than the list holds (long ties, very high temperatures) T and T_idx are found by
+// bisection over keys and indices instead: slower, same result.
 //
-// Bound: rows * vocab * size bytes for large batches, then 13 fp64 operations a weight; for few rows the chain of passes and
-// cluster barriers.
+// Bound: rows * vocab * size bytes for large batches, then eleven fp64 operations a weight (fp64 runs at half the fp32 rate);
+// for few rows the chain of passes and cluster barriers.
 #include "common.cuh"
 
 #include <atomic>
@@ -37,10 +40,10 @@ constexpr int SM_THREADS = 1024;
 constexpr int SM_WARPS = SM_THREADS / 32;
 constexpr int SM_CHUNK = 256;    // tokens of one warp step: eight consecutive ones per lane
 constexpr int SM_BINS = 4096;
-constexpr int SM_LIST = 4096;    // tokens collected per boundary bin
+constexpr int SM_LIST = 4096;    // tokens collected at most
 constexpr int SM_RUNS = 1024;    // runs of chunks whose kept weight a CTA holds
 constexpr int SM_MAX_CLUSTER = 8;
-// what rank 0 finds in the collected bins: the threshold, that top-p ends further up or down the ranking, or too many tokens
+// what rank 0 finds in the collected tokens: the threshold, that top-p ends further up or down the ranking, or too many tokens
 enum : uint32_t { SM_FOUND, SM_UP, SM_DOWN, SM_BISECT };
 
 struct SampleArgs {
@@ -62,6 +65,10 @@ __device__ __forceinline__ uint32_t logit_key(float x) {
 __device__ __forceinline__ float key_logit(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
+// a token in ranking order: larger is further in front
+__device__ __forceinline__ u64 rank_entry(float x, int i) {
+  return static_cast<u64>(logit_key(x)) << 32 | ~static_cast<uint32_t>(i);
+}
 
 // ---- cluster helpers (also right for a cluster of one) ----
 __device__ __forceinline__ unsigned cta_rank() {
@@ -69,101 +76,158 @@ __device__ __forceinline__ unsigned cta_rank() {
   asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
+__device__ __forceinline__ void cluster_sync(int cluster) {
+  if (cluster == 1) {
+    __syncthreads();
+    return;
+  }
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t peer_addr(const void* local, unsigned rank) {
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ uint32_t peer_u32(const uint32_t* local, unsigned rank) {
+__device__ __forceinline__ uint32_t peer_u32(const void* local, unsigned rank) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_addr(local, rank)) : "memory");
   return v;
 }
-__device__ __forceinline__ u64 peer_u64(const u64* local, unsigned rank) {
-  u64 v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(peer_addr(local, rank)) : "memory");
-  return v;
+__device__ __forceinline__ void store_peer_u64(u64* local, unsigned rank, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_addr(local, rank)), "l"(v) : "memory");
 }
 
 struct Shared {
-  uint32_t bins[SM_BINS];    // this CTA's counts
-  u64 list[2][SM_LIST];      // rank 0: key << 32 | ~index of the tokens in the two boundary bins: larger ranks first
+  uint32_t bins[SM_BINS];              // rank 0: the cluster's counts
+  u64 list[2][SM_LIST];                // rank 0: rank_entry of collected tokens
   u64 list_w[SM_LIST];
   u64 runs[SM_RUNS];
   u64 part[SM_WARPS][3];
-  u64 sums[2][3];            // this CTA's sums, two turns so that one barrier per exchange is enough
-  u64 fwarp[SM_WARPS];
-  double mwarp[SM_WARPS];
+  u64 sums[2][SM_MAX_CLUSTER][3];      // every CTA's sums, two turns so that one barrier per exchange is enough
+  u64 best[SM_MAX_CLUSTER];
+  u64 warp_u64[SM_WARPS];
+  float warp_f32[SM_WARPS];
+  uint32_t warp_u32[SM_WARPS];
   uint32_t list_n[2];
-  uint32_t verdict;          // rank 0: threshold found
   uint32_t T, T_idx;
-  int bin_k, bin_p;
-  uint32_t before_k;
-  double est_total;
+  // rank 0's findings, read by its peers
+  struct {
+    uint32_t verdict, before_k, collect;
+    int bin_k, bin_p;
+  } say;
+  float est_total;
   int hit;
 };
 
-// The eight tokens from i on as fp32; NaN behind the end of the row.
+// Eight consecutive tokens as they sit in memory: 16 or 32 bytes.
+struct Raw {
+  uint4 a, b;
+};
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int i, int V, bool vec, float (&x)[8]) {
+__device__ __forceinline__ Raw load_raw(const T* row, int i, int V, bool vec) {
+  Raw r;
   if (vec && i + 8 <= V) {
-    if (sizeof(T) == 4) {
-      const uint4 a = ld_act16(reinterpret_cast<const char*>(row) + static_cast<size_t>(i) * 4);
-      const uint4 b = ld_act16(reinterpret_cast<const char*>(row) + static_cast<size_t>(i) * 4 + 16);
-      x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
-      x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
-    } else {
-      using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
-      unpack8<H>(ld_act16(row + i), x);
-    }
-    return;
+    const char* p = reinterpret_cast<const char*>(row) + static_cast<size_t>(i) * sizeof(T);
+    r.a = ld_act16(p);
+    if (sizeof(T) == 4) r.b = ld_act16(p + 16);
+    return r;
   }
+  uint32_t w[8];  // NaN behind the end of the row
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    x[e] = __int_as_float(0x7fffffff);
-    if (i + e < V) {
-      if (sizeof(T) == 4) x[e] = __ldcg(reinterpret_cast<const float*>(row) + i + e);
-      else {
-        using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
-        x[e] = ld_act_f32<H>(reinterpret_cast<const H*>(row) + i + e);
-      }
-    }
+    if (sizeof(T) == 4) w[e] = i + e < V ? __ldcg(reinterpret_cast<const uint32_t*>(row) + i + e) : 0x7fffffffu;
+    else w[e] = i + e < V ? __ldcg(reinterpret_cast<const unsigned short*>(row) + i + e) : 0x7fffu;
+  }
+  if (sizeof(T) == 4) {
+    r.a = make_uint4(w[0], w[1], w[2], w[3]);
+    r.b = make_uint4(w[4], w[5], w[6], w[7]);
+  } else {
+    r.a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack_raw(const Raw& r, float (&x)[8]) {
+  if (sizeof(T) == 4) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
+  } else {
+    using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
+    unpack8<H>(r.a, x);
   }
 }
 
+template <typename T>
+struct Row {
+  const T* p;
+  int V, c0, c1;  // this CTA's chunks
+  bool vec;
+  bool inf;       // the largest logit is +infinity: 0 stands for it then, and -infinity for every other one
+  __device__ __forceinline__ void unpack(const Raw& r, float (&x)[8]) const {
+    unpack_raw<T>(r, x);
+    if (inf) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
+    }
+  }
+  // f(first token of the lane, its eight logits) for every chunk of this CTA; warps take chunks in turn, the next one's load
+  // in flight
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    const int lane = threadIdx.x & 31;
+    int c = c0 + (threadIdx.x >> 5);
+    if (c >= c1) return;
+    Raw cur = load_raw<T>(p, c * SM_CHUNK + lane * 8, V, vec);
+    while (true) {
+      const int n = c + SM_WARPS;
+      Raw next;
+      if (n < c1) next = load_raw<T>(p, n * SM_CHUNK + lane * 8, V, vec);
+      float x[8];
+      unpack(cur, x);
+      f(c * SM_CHUNK + lane * 8, x);
+      if (n >= c1) break;
+      cur = next;
+      c = n;
+    }
+  }
+};
+
 // Weights of one row. table: lane j of every warp holds 2^(j / 32).
 struct Weigh {
-  float top, bin_scale;
-  double inv_t, table;
+  float top, floor, bin_scale;  // floor: at and below it a weight rounds to 0
+  double scale, table;          // 32 / (ln 2 * temperature)
   int frac_bits;
-  // bin of z; SM_BINS and above: the weight rounds to 0. Non-decreasing in the distance from the largest logit.
+  // bin of z; SM_BINS and above: no weight. Non-decreasing in the distance from the largest logit.
   __device__ __forceinline__ int bin(float x) const {
-    if (x == top) return 0;
     const float b = (top - x) * bin_scale;
     return b < static_cast<float>(SM_BINS) ? static_cast<int>(b) : SM_BINS;  // NaN: SM_BINS
   }
-  // 2^S exp(z), rounded; whole warp, x of lanes with use == false is not looked at. z = (32 n + j) ln2 / 32 + r with |r| <=
-  // ln2 / 64: exp(z) = 2^n * 2^(j/32) * exp(r), the last one by its Taylor polynomial of degree 5 (r^6 / 720 < 3e-15).
-  __device__ __forceinline__ u64 operator()(float x, bool use) const {
-    const double z = use && x != top ? (static_cast<double>(x) - static_cast<double>(top)) * inv_t : 0.0;
+  // 2^S exp(z) before rounding, x above the floor; whole warp. (logit - largest) * scale = 32 n + j + f, |f| <= 1/2: the weight is
+  // 2^n * 2^(j/32) * 2^(f/32), the last one by its Taylor polynomial of degree 4 (error below 1.3e-12).
+  __device__ __forceinline__ double value(float x) const {
+    const double d = static_cast<double>(fmaxf(x, floor)) - static_cast<double>(top);
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number, in the low bits
-    const double km = fma(z, 46.166241308446828, magic);  // 32 / ln 2
+    const double km = fma(d, scale, magic);
     const int k = __double2loint(km);
-    const double r = fma(km - magic, -0.021660849392498290, z);  // ln 2 / 32
-    double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    p *= __shfl_sync(MUI_FULL_MASK, table, k & 31);
-    p = __hiloint2double(__double2hiint(p) + (((k >> 5) + frac_bits) << 20), __double2loint(p));
-    // p < 2^51: adding 2^52 leaves the rounded integer in the mantissa
-    const u64 bits = static_cast<u64>(__double_as_longlong(p + 4503599627370496.0)) & 0xfffffffffffffull;
-    return use ? bits : 0ull;
+    const double f = fma(d, scale, magic - km);
+    constexpr double L = 0.021660849392498290;  // ln 2 / 32
+    double p = fma(f, L * L * L * L / 24.0, L * L * L / 6.0);
+    p = fma(p, f, L * L / 2.0);
+    p = fma(p, f, L);
+    p = fma(p, f, 1.0);
+    p *= __shfl_sync(MUI_FULL_MASK, table, k);
+    return __hiloint2double(__double2hiint(p) + ((k >> 5) + frac_bits) * (1 << 20), __double2loint(p));
+  }
+  // values below 2^51 added to 2^52 leave their rounded sum in the mantissa
+  static __device__ __forceinline__ u64 bits(double v) {
+    return static_cast<u64>(__double_as_longlong(v)) & 0xfffffffffffffull;
+  }
+  // the weight as an integer; whole warp
+  __device__ __forceinline__ u64 operator()(float x, bool use) const {
+    const u64 q = bits(value(x) + 4503599627370496.0);
+    return use ? q : 0ull;
   }
 };
 
@@ -172,59 +236,54 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(MUI_FULL_MASK, v, o);
   return v;
 }
-
-template <typename T>
-struct Row {
-  const T* p;
-  int V, c0, c1;  // this CTA's chunks
-  bool vec;
-  // f(first token of the lane, its eight logits) for every chunk of this CTA; warps take chunks in turn
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int c = c0 + warp;
-    for (; c + SM_WARPS < c1; c += 2 * SM_WARPS) {  // two chunks of loads in flight
-      float x[8], y[8];
-      load8<T>(p, c * SM_CHUNK + lane * 8, V, vec, x);
-      load8<T>(p, (c + SM_WARPS) * SM_CHUNK + lane * 8, V, vec, y);
-      f(c * SM_CHUNK + lane * 8, x);
-      f((c + SM_WARPS) * SM_CHUNK + lane * 8, y);
-    }
-    if (c < c1) {
-      float x[8];
-      load8<T>(p, c * SM_CHUNK + lane * 8, V, vec, x);
-      f(c * SM_CHUNK + lane * 8, x);
-    }
+template <typename V>
+__device__ __forceinline__ V warp_scan(V v) {  // inclusive
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V y = __shfl_up_sync(MUI_FULL_MASK, v, o);
+    if (lane >= o) v += y;
   }
-};
+  return v;
+}
+// Exclusive sum over the CTA's threads; s_warp: one element per warp, free again after the next barrier.
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V* s_warp, V& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const V inc = warp_scan(v);
+  if (lane == 31) s_warp[warp] = inc;
+  __syncthreads();
+  const V w = warp_scan(s_warp[lane]);
+  all = __shfl_sync(MUI_FULL_MASK, w, 31);
+  const V before = __shfl_sync(MUI_FULL_MASK, w, warp - 1);
+  return inc - v + (warp ? before : V(0));
+}
 
 // Sums of three numbers over the cluster; every thread gets them. `turn` alternates from call to call.
-__device__ __forceinline__ void cluster_sum3(Shared& s, int cluster, int& turn, u64 (&v)[3]) {
-  const int warp = threadIdx.x >> 5;
+__device__ __forceinline__ void cluster_sum3(Shared& s, int cluster, unsigned rank, int& turn, u64 (&v)[3]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < 3; ++i) v[i] = warp_sum_u64(v[i]);
-  if ((threadIdx.x & 31) == 0)
+  if (lane == 0)
     for (int i = 0; i < 3; ++i) s.part[warp][i] = v[i];
   __syncthreads();
-  if (threadIdx.x < 3) {
-    u64 t = 0;
-    for (int w = 0; w < SM_WARPS; ++w) t += s.part[w][threadIdx.x];
-    s.sums[turn][threadIdx.x] = t;
+  if (warp < 3) {
+    const u64 t = warp_sum_u64(s.part[lane][warp]);
+    if (lane < cluster) store_peer_u64(&s.sums[turn][rank][warp], lane, t);
   }
-  if (cluster > 1) cluster_sync();
-  else __syncthreads();
+  cluster_sync(cluster);
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     v[i] = 0;
-    for (int r = 0; r < cluster; ++r) v[i] += cluster > 1 ? peer_u64(&s.sums[turn][i], r) : s.sums[turn][i];
+    for (int r = 0; r < cluster; ++r) v[i] += s.sums[turn][r][i];
   }
   turn ^= 1;
 }
 
 // The boundary of top-k and top-p by bisection: 32 steps over keys for each, then over indices for the ties.
 template <typename T>
-__device__ void threshold_by_bisection(Shared& s, const SampleArgs& a, const Row<T>& row, const Weigh& w, int& turn,
-                                       uint32_t best, bool use_k, uint32_t k, bool use_p, double top_p, uint32_t& T_key,
+__device__ void threshold_by_bisection(Shared& s, const SampleArgs& a, const Row<T>& row, const Weigh& w, unsigned rank,
+                                       int& turn, uint32_t best, bool use_k, uint32_t k, bool use_p, double top_p, uint32_t& T_key,
                                        uint32_t& T_idx) {
   // count and weight of the tokens with key >= pivot
   auto from = [&](uint32_t pivot, u64& count, u64& mass) {
@@ -237,7 +296,7 @@ __device__ void threshold_by_bisection(Shared& s, const SampleArgs& a, const Row
         v[1] += w(x[e], in && w.bin(x[e]) < SM_BINS);
       }
     });
-    cluster_sum3(s, a.cluster, turn, v);
+    cluster_sum3(s, a.cluster, rank, turn, v);
     count = v[0];
     mass = v[1];
   };
@@ -290,17 +349,16 @@ __device__ void threshold_by_bisection(Shared& s, const SampleArgs& a, const Row
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[0] += i + e < a.V && i + e <= static_cast<int>(mid) && logit_key(x[e]) == T_key;
     });
-    cluster_sum3(s, a.cluster, turn, v);
+    cluster_sum3(s, a.cluster, rank, turn, v);
     if (v[0] >= ties) hi = mid;
     else lo = mid + 1;
   }
   T_idx = lo;
 }
 
-// Sorts a collected bin into ranking order and leaves in list_w[i] the weight of its tokens before the i-th; returns the
-// weight of all of them. One CTA. A bitonic sort: 8192 exchanges of the largest list are 2 per thread and step.
-__device__ u64 rank_bin(Shared& s, u64* list, int n, const Weigh& w) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// Sorts n entries, largest first. One CTA. A bitonic sort: two exchanges per thread and step for the largest list.
+__device__ void sort_list(u64* list, int n) {
+  const int tid = threadIdx.x;
   int m = 2;
   while (m < n) m <<= 1;
   for (int i = n + tid; i < m; i += SM_THREADS) list[i] = 0;
@@ -315,37 +373,43 @@ __device__ u64 rank_bin(Shared& s, u64* list, int n, const Weigh& w) {
           list[o] = x;
         }
       }
-      __syncthreads();
+      // exchanges closer than 64 entries stay within a warp, as does the step after such a one
+      if (j > 32 || (j == 1 && 2 * k > 64)) __syncthreads();
+      else __syncwarp();
     }
+  __syncthreads();
+}
+
+// Leaves in list_w[i] the weight of the sorted list's tokens before the i-th; returns the weight of all of them. One CTA.
+__device__ u64 weigh_list(Shared& s, const u64* list, int n, const Weigh& w) {
   constexpr int PER = SM_LIST / SM_THREADS;
-  u64 q[PER], sum = 0;
+  u64 q[PER], sum = 0, all;
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    const int i = tid * PER + e;
+    const int i = threadIdx.x * PER + e;
     q[e] = w(i < n ? key_logit(static_cast<uint32_t>(list[i] >> 32)) : 0.f, i < n);
     sum += q[e];
   }
-  u64 run = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = __shfl_up_sync(MUI_FULL_MASK, run, o);
-    if (lane >= o) run += y;
-  }
-  if (lane == 31) s.fwarp[warp] = run;
-  __syncthreads();
-  u64 all = 0;
-  run -= sum;
-  for (int i = 0; i < SM_WARPS; ++i) {
-    if (i < warp) run += s.fwarp[i];
-    all += s.fwarp[i];
-  }
+  u64 run = block_scan(sum, s.warp_u64, all);
 #pragma unroll
   for (int e = 0; e < PER; ++e) {
-    s.list_w[tid * PER + e] = run;
+    s.list_w[threadIdx.x * PER + e] = run;
     run += q[e];
   }
   __syncthreads();
   return all;
+}
+
+// number of leading entries i < n for which test(i) holds (it holds for a run from the front)
+template <typename F>
+__device__ __forceinline__ int leading(int n, F test) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (test(mid)) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
 }
 
 template <typename T>
@@ -363,74 +427,187 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   row.p = reinterpret_cast<const T*>(a.logits) + r * a.stride;
   row.V = a.V;
   row.vec = (reinterpret_cast<uintptr_t>(row.p) & 15) == 0;
+  row.inf = false;
   const int chunks = (a.V + SM_CHUNK - 1) / SM_CHUNK, per_cta = (chunks + C - 1) / C;
   row.c0 = min(chunks, static_cast<int>(rank) * per_cta);
   row.c1 = min(chunks, row.c0 + per_cta);
-  const float t = a.temperature ? __ldcg(a.temperature + r) : 1.f;
+  float t = a.temperature ? __ldcg(a.temperature + r) : 1.f;
   const int k_raw = a.top_k ? __ldcg(a.top_k + r) : 0;
   const float top_p = a.top_p ? __ldcg(a.top_p + r) : 1.f;
   const float min_p = a.min_p ? __ldcg(a.min_p + r) : 0.f;
+  const float uniform = __ldcg(a.uniforms + r);
   const bool use_k = k_raw > 0 && k_raw < a.V, use_p = top_p < 1.f, greedy = !(t > 0.f);
 
   // 1. the largest logit; its lowest index where that is the answer
-  u64 best = 0;  // key << 32 | ~index
+  for (int i = tid; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0;
+  if (tid < 2) s.list_n[tid] = 0;
+  u64 best = 0;
   if (greedy) {
     row.each([&](int i, float(&x)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const u64 v = static_cast<u64>(logit_key(x[e])) << 32 | ~static_cast<uint32_t>(i + e);
+        const u64 v = rank_entry(x[e], i + e);
         best = i + e < a.V && v > best ? v : best;
       }
     });
   } else {
     float m = -INFINITY;
-    row.each([&](int, float(&x)[8]) {
+    int c = row.c0 + warp;
+    for (; c + 3 * SM_WARPS < row.c1; c += 4 * SM_WARPS) {  // four chunks of loads in flight
+      Raw q[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) q[h] = load_raw<T>(row.p, (c + h * SM_WARPS) * SM_CHUNK + lane * 8, a.V, row.vec);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        float x[8];
+        unpack_raw<T>(q[h], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+      }
+    }
+    for (; c < row.c1; c += SM_WARPS) {
+      float x[8];
+      unpack_raw<T>(load_raw<T>(row.p, c * SM_CHUNK + lane * 8, a.V, row.vec), x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
-    });
-    best = static_cast<u64>(logit_key(m)) << 32 | 0xffffffffu;
+    }
+    best = rank_entry(m, 0);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const u64 y = __shfl_xor_sync(MUI_FULL_MASK, best, o);
     best = y > best ? y : best;
   }
-  if (lane == 0) s.fwarp[warp] = best;
-  for (int i = tid; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0;
-  if (tid < 2) s.list_n[tid] = 0;
+  if (lane == 0) s.warp_u64[warp] = best;
   __syncthreads();
-  for (int i = 0; i < SM_WARPS; ++i) best = s.fwarp[i] > best ? s.fwarp[i] : best;
-  if (C > 1) {
-    if (tid == 0) s.sums[1][0] = best;
-    cluster_sync();
-    for (int i = 0; i < C; ++i) {
-      const u64 y = peer_u64(&s.sums[1][0], i);
+  if (warp == 0) {
+    best = s.warp_u64[lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const u64 y = __shfl_xor_sync(MUI_FULL_MASK, best, o);
       best = y > best ? y : best;
     }
+    if (lane < C) store_peer_u64(&s.best[rank], lane, best);
   }
-  const uint32_t best_key = static_cast<uint32_t>(best >> 32);
+  cluster_sync(C);
+  best = 0;
+  for (int i = 0; i < C; ++i) best = s.best[i] > best ? s.best[i] : best;
   Weigh w;
-  w.top = key_logit(best_key);
+  w.top = key_logit(static_cast<uint32_t>(best >> 32));
   const bool nothing = !(w.top > -INFINITY);  // key 0 (all NaN) reads as NaN
   if (greedy || nothing) {
     if (rank == 0 && tid == 0) {
       a.tokens[r] = nothing ? 0 : static_cast<int64_t>(~static_cast<uint32_t>(best));
       if (a.logprobs) a.logprobs[r] = nothing ? -INFINITY : 0.f;
     }
-    if (C > 1) cluster_sync();  // peers may still be reading this CTA's memory
     return;
   }
+  if (w.top == INFINITY) {
+    row.inf = true;
+    w.top = 0.f;
+  }
+  const uint32_t best_key = logit_key(w.top);
   w.frac_bits = a.frac_bits;
-  w.inv_t = 1.0 / static_cast<double>(t);
-  w.table = exp2(static_cast<double>(lane) / 32.0);
-  // z below -(S + 2) ln 2 has a weight under a quarter of the last bit
+  // z below -(S + 2) ln 2 has a weight under a quarter of the last bit. A temperature so small that the next smaller logit
+  // lies beyond that, or so large that all logits are alike, is brought to where this is just the case.
   const float z_range = (a.frac_bits + 2) * 0.693147181f;
+  t = fminf(fmaxf(fmaxf(t, (w.top - key_logit(best_key - 1)) / z_range), 1.17549435e-38f), 1e30f);
+  w.floor = fmaxf(fminf(w.top - z_range * t, key_logit(best_key - 1)), -3.402823466e38f);
+  w.scale = 46.166241308446828 / static_cast<double>(t);  // 32 / ln 2
+  w.table = exp2(static_cast<double>(lane) / 32.0);
   w.bin_scale = static_cast<float>(SM_BINS) / z_range / t;
   const u64 one = 1ull << a.frac_bits;
-  // min-p in the integers of the weights; the largest token has weight 1 and always stays
-  const u64 w_min = min_p > 0.f ? static_cast<u64>(ceil(fmin(static_cast<double>(min_p), 1.0) * static_cast<double>(one))) : 1ull;
+  // min-p in the integers of the weights (the largest token has weight 1 and always stays), and a logit safely below its cut
+  const float min_w = fminf(min_p, 1.f);
+  const u64 w_min = min_p > 0.f ? static_cast<u64>(ceil(static_cast<double>(min_w) * static_cast<double>(one))) : 1ull;
+  const float x_min = min_p > 0.f ? w.top + t * (logf(min_w) - 1e-3f) - fabsf(w.top) * 1e-6f : -INFINITY;
+  // uniform numbers lie in [0, 1); what does not is brought to the nearest fp32 that does
+  const double u = static_cast<double>(fminf(fmaxf(uniform, 0.f), 0.99999994f));
+
+  // Rank 0 turns a complete list of the tokens in front (n of them, `total` the weight of the row for top-p without top-k) into
+  // the drawn token. cut_p: the list ends where top-p was expected to end; false is returned when it does not.
+  auto finish = [&](int n, u64 total, bool cut_p) {
+    sort_list(s.list[0], n);
+    const u64 all = weigh_list(s, s.list[0], n, w);
+    auto before = [&](int i) { return i < n ? s.list_w[i] : all; };
+    int keep = use_k ? min(n, k_raw) : n;
+    if (use_p) {
+      const double target = static_cast<double>(top_p) * static_cast<double>(use_k ? before(keep) : total);
+      if (cut_p && static_cast<double>(all) < target) return false;
+      keep = max(1, leading(keep, [&](int i) { return static_cast<double>(before(i)) < target; }));
+    }
+    keep = leading(keep, [&](int i) { return before(i + 1) - before(i) >= w_min; });
+    const u64 mass = before(keep);
+    const double want = u * static_cast<double>(mass);
+    // the kept ones by index
+    for (int i = tid; i < keep; i += SM_THREADS)
+      s.list[1][i] = (s.list[0][i] << 32) | static_cast<uint32_t>(i);  // ~index, place
+    __syncthreads();
+    sort_list(s.list[1], keep);
+    constexpr int PER = SM_LIST / SM_THREADS;
+    u64 q[PER], sum = 0, unused;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const int i = tid * PER + e;
+      q[e] = 0;
+      if (i < keep) {
+        const int at = static_cast<int>(s.list[1][i] & 0xffffffffu);
+        q[e] = before(at + 1) - before(at);
+      }
+      sum += q[e];
+    }
+    u64 run = block_scan(sum, s.warp_u64, unused);
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      // the first token at which the running weight exceeds the point
+      if (q[e] != 0 && static_cast<double>(run + q[e]) > want && static_cast<double>(run) <= want) {
+        a.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.list[1][tid * PER + e] >> 32));
+        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(q[e]) / static_cast<double>(mass)));
+      }
+      run += q[e];
+    }
+    return true;
+  };
+  // Collects the tokens that in(x) names in rank 0's list, with the weight of the whole row if asked for. Returns their number
+  // (over SM_LIST: the list is incomplete); the weight is left in v[0].
+  const uint32_t count_at[2] = {peer_addr(&s.list_n[0], 0), peer_addr(&s.list_n[1], 0)};
+  const uint32_t list_at[2] = {peer_addr(&s.list[0][0], 0), peer_addr(&s.list[1][0], 0)};
+  auto put = [&](int which, float x, int i) {
+    uint32_t at;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count_at[which]) : "memory");
+    if (at < SM_LIST)
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list_at[which] + at * 8), "l"(rank_entry(x, i)) : "memory");
+  };
+  u64 v[3];
+  auto collect = [&](auto in, bool weigh) {
+    v[0] = v[1] = v[2] = 0;
+    row.each([&](int i, float(&x)[8]) {
+      if (weigh) {
+        double sum = 4503599627370496.0;  // 2^52
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += w.value(x[e]);
+        v[0] += Weigh::bits(sum);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (in(x[e])) put(0, x[e], i + e);
+    });
+    cluster_sum3(s, C, rank, turn, v);  // its barrier also publishes the list
+  };
 
   uint32_t T_key = 0, T_idx = 0;  // nothing to cut: every key that has weight is above 0
+  bool bisect = false;
+  if (min_p > 0.f && !use_k) {
+    collect([&](float x) { return x >= x_min; }, use_p);
+    const uint32_t n = peer_u32(&s.list_n[0], 0);
+    if (n <= SM_LIST) {
+      if (rank == 0) finish(static_cast<int>(n), v[0], false);
+      if (C > 1) cluster_sync(C);  // rank 0's count has been read
+      return;
+    }
+    cluster_sync(C);
+    if (tid == 0) s.list_n[0] = 0;
+  }
   if (use_k || use_p) {
     // 2. histogram
     row.each([&](int, float(&x)[8]) {
@@ -440,127 +617,144 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
         if (b < SM_BINS) atomicAdd(&s.bins[b], 1u);
       }
     });
-    if (tid == 0) {
-      s.bin_k = s.bin_p = SM_BINS;
-      s.before_k = 0;
+    if (rank != 0) {
+      __syncthreads();
+      for (int i = tid; i < SM_BINS; i += SM_THREADS)
+        if (const uint32_t n = s.bins[i])
+          asm volatile("red.shared::cluster.add.u32 [%0], %1;" ::"r"(peer_addr(&s.bins[i], 0)), "r"(n) : "memory");
     }
-    if (C > 1) cluster_sync();
-    else __syncthreads();
-    // prefix sums over the cluster's bins, four per thread: counts, and weights of the bin centres
+    cluster_sync(C);
     constexpr int PER = SM_BINS / SM_THREADS;
-    uint32_t n[PER], nc = 0;
-    double m[PER], mc = 0.0;
-#pragma unroll
-    for (int h = 0; h < PER; ++h) {
-      n[h] = 0;
-      for (int i = 0; i < C; ++i) n[h] += C > 1 ? peer_u32(&s.bins[PER * tid + h], i) : s.bins[PER * tid + h];
-      m[h] = n[h] * static_cast<double>(exp2f(-(PER * tid + h + 0.5f) * (z_range * 1.44269504f / SM_BINS)));
-      nc += n[h];
-      mc += m[h];
-    }
-    uint32_t nb = nc;
-    double mb = mc;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t y = __shfl_up_sync(MUI_FULL_MASK, nb, o);
-      const double q = __shfl_up_sync(MUI_FULL_MASK, mb, o);
-      if (lane >= o) {
-        nb += y;
-        mb += q;
-      }
-    }
-    if (lane == 31) {
-      s.fwarp[warp] = nb;
-      s.mwarp[warp] = mb;
-    }
-    __syncthreads();
-    double all = 0.0;
-    nb -= nc;
-    mb -= mc;
-    for (int i = 0; i < SM_WARPS; ++i) {
-      if (i < warp) {
-        nb += static_cast<uint32_t>(s.fwarp[i]);
-        mb += s.mwarp[i];
-      }
-      all += s.mwarp[i];
-    }
     const uint32_t k = static_cast<uint32_t>(k_raw);
-    if (use_k) {
-      if (tid == 0) s.est_total = all;
-      __syncthreads();
-      uint32_t at = nb;
-      double am = mb;
+    if (rank == 0) {
+      // prefix sums over the bins, four per thread: counts, and weights of the bin centres
+      if (tid == 0) {
+        s.say.bin_k = s.say.bin_p = SM_BINS;
+        s.say.before_k = 0;
+      }
+      uint32_t n[PER], nc = 0, n_all;
+      float m[PER], mc = 0.f, all;
 #pragma unroll
       for (int h = 0; h < PER; ++h) {
-        if (at < k && at + n[h] >= k) {  // one thread at most
-          s.bin_k = PER * tid + h;
-          s.before_k = at;
-          s.est_total = am + m[h] * (k - at) / n[h];
+        n[h] = s.bins[PER * tid + h];
+        m[h] = n[h] * exp2f(-(PER * tid + h + 0.5f) * (z_range * 1.44269504f / SM_BINS));
+        nc += n[h];
+        mc += m[h];
+      }
+      const uint32_t nb = block_scan(nc, s.warp_u32, n_all);
+      const float mb = block_scan(mc, s.warp_f32, all);
+      if (use_k) {
+        if (tid == 0) s.est_total = all;
+        __syncthreads();
+        uint32_t at = nb;
+        float am = mb;
+#pragma unroll
+        for (int h = 0; h < PER; ++h) {
+          if (at < k && at + n[h] >= k) {  // one thread at most
+            s.say.bin_k = PER * tid + h;
+            s.say.before_k = at;
+            s.est_total = am + m[h] * (k - at) / n[h];
+          }
+          at += n[h];
+          am += m[h];
         }
-        at += n[h];
-        am += m[h];
+        __syncthreads();
+        all = s.est_total;
       }
-      __syncthreads();
-      all = s.est_total;
-    }
-    if (use_p) {
-      const double target = static_cast<double>(top_p) * all;
-      uint32_t at = nb;
-      double am = mb;
+      const int bin_k = s.say.bin_k;
+      if (use_p) {
+        const float target = top_p * all;
+        uint32_t at = nb;
+        float am = mb;
 #pragma unroll
-      for (int h = 0; h < PER; ++h) {
-        // the first occupied bin with which the sum reaches the target
-        if (n[h] > 0 && am + m[h] >= target && (am < target || at == 0)) atomicMin(&s.bin_p, PER * tid + h);
-        at += n[h];
-        am += m[h];
+        for (int h = 0; h < PER; ++h) {
+          // the first occupied bin with which the sum reaches the target
+          if (n[h] > 0 && am + m[h] >= target && (am < target || at == 0)) atomicMin(&s.say.bin_p, PER * tid + h);
+          at += n[h];
+          am += m[h];
+        }
+        __syncthreads();
+      }
+      const int bin_p = use_p ? min(s.say.bin_p, bin_k) : bin_k;
+      // tokens up to the last bin that matters; top-p without top-k takes a bin more, since it is an estimate
+      const int last = use_k ? bin_k : min(bin_p + 1, SM_BINS);
+      if (last < SM_BINS && tid == last / PER) {
+        uint32_t upto = nb;
+#pragma unroll
+        for (int h = 0; h < PER; ++h)
+          if (PER * tid + h <= last) upto += n[h];
+        s.say.collect = upto <= SM_LIST;
+      } else if (last >= SM_BINS && tid == 0) {
+        s.say.collect = n_all <= SM_LIST;
       }
       __syncthreads();
+      if (tid == 0) s.say.bin_p = bin_p;
     }
-    const int bin_k = s.bin_k;
-    int bin_p = use_p ? min(s.bin_p, bin_k) : bin_k;
-    uint32_t verdict = use_p || bin_k < SM_BINS ? SM_BISECT : SM_FOUND;  // a top_p next to 1 may end in no bin
+    cluster_sync(C);
+    const int bin_k = static_cast<int>(peer_u32(&s.say.bin_k, 0));
+    int bin_p = static_cast<int>(peer_u32(&s.say.bin_p, 0));
+    const uint32_t before_k = peer_u32(&s.say.before_k, 0);
+    if (peer_u32(&s.say.collect, 0)) {
+      // 3. the tokens in front
+      const int last = use_k ? bin_k : min(bin_p + 1, SM_BINS);
+      collect([&](float x) { return w.bin(x) < SM_BINS && w.bin(x) <= last; }, use_p && !use_k);
+      if (rank == 0) {
+        const bool ok = finish(static_cast<int>(s.list_n[0]), v[0], use_p && !use_k && last < SM_BINS);
+        __syncthreads();
+        if (tid == 0) {
+          s.say.verdict = ok ? SM_FOUND : SM_UP;
+          s.list_n[0] = 0;
+        }
+      }
+      cluster_sync(C);
+      const bool ok = peer_u32(&s.say.verdict, 0) == SM_FOUND;
+      if (C > 1) cluster_sync(C);  // the verdict has been read
+      if (ok) return;
+    }
+    bisect = use_p || bin_k < SM_BINS;  // a top_p next to 1 may end in no bin
     for (int attempt = 0; attempt < 4 && bin_p < SM_BINS; ++attempt) {
-      // 3. exact sums: [0] above bin_p, [1] between the bins; tokens of the bins go to rank 0
-      u64 v[3] = {0, 0, 0};
-      const uint32_t count_at[2] = {peer_addr(&s.list_n[0], 0), peer_addr(&s.list_n[1], 0)};
-      const uint32_t list_at[2] = {peer_addr(&s.list[0][0], 0), peer_addr(&s.list[1][0], 0)};
+      // 3'. exact sums: [0] above bin_p, [1] between the bins; tokens of the bins go to rank 0
+      v[0] = v[1] = v[2] = 0;
       row.each([&](int i, float(&x)[8]) {
+        double above = 4503599627370496.0, between = above;
+        bool mine = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int b = w.bin(x[e]);
-          const bool sum = use_p && b < bin_k && b != bin_p && b < SM_BINS;
-          if (__any_sync(MUI_FULL_MASK, sum)) {
-            const u64 q = w(x[e], sum);
-            v[0] += b < bin_p ? q : 0ull;
-            v[1] += b < bin_p ? 0ull : q;
+          mine |= use_p && b < bin_k && b != bin_p && b < SM_BINS;
+          if (b < SM_BINS && (b == bin_p || b == bin_k)) put(b == bin_p ? 0 : 1, x[e], i + e);
+        }
+        if (__any_sync(MUI_FULL_MASK, mine)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int b = w.bin(x[e]);
+            const double p = w.value(x[e]);
+            above += b < bin_p ? p : 0.0;
+            between += b > bin_p && b < bin_k ? p : 0.0;
           }
-          if (b < SM_BINS && (b == bin_p || b == bin_k)) {
-            const int which = b == bin_p ? 0 : 1;
-            uint32_t at;
-            asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count_at[which]) : "memory");
-            if (at < SM_LIST) {
-              const u64 entry = static_cast<u64>(logit_key(x[e])) << 32 | ~static_cast<uint32_t>(i + e);
-              asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list_at[which] + at * 8), "l"(entry) : "memory");
-            }
-          }
+          v[0] += Weigh::bits(above);
+          v[1] += Weigh::bits(between);
         }
       });
-      cluster_sum3(s, C, turn, v);  // its barrier also publishes the lists
+      cluster_sum3(s, C, rank, turn, v);  // its barrier also publishes the lists
       if (rank == 0) {
         const int n0 = s.list_n[0], n1 = s.list_n[1];
         const bool same = bin_p == bin_k;
         uint32_t say = SM_BISECT;
+        int next = bin_p;
         if (n0 <= SM_LIST && n1 <= SM_LIST) {
-          const uint32_t left = k - s.before_k;  // tokens of bin_k within the top-k
+          const uint32_t left = k - before_k;  // tokens of bin_k within the top-k
           u64 in_k = 0;
           u64 last = 0;
           if (!same && bin_k < SM_BINS) {
-            const u64 bin_mass = rank_bin(s, s.list[1], n1, w);
+            sort_list(s.list[1], n1);
+            const u64 bin_mass = weigh_list(s, s.list[1], n1, w);
             in_k = left < static_cast<uint32_t>(n1) ? s.list_w[left] : bin_mass;
             __syncthreads();
           }
           const int n_p = same ? static_cast<int>(min(left, static_cast<uint32_t>(n0))) : n0;  // of bin_p within the top-k
-          u64 in_p = rank_bin(s, s.list[0], n0, w);
+          sort_list(s.list[0], n0);
+          u64 in_p = weigh_list(s, s.list[0], n0, w);
           if (n_p < n0) in_p = s.list_w[n_p];
           if (!use_p) {
             last = s.list[0][n_p - 1];
@@ -572,15 +766,16 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
             else if (static_cast<double>(v[0] + in_p) < target) say = SM_DOWN;
             else {
               // tokens whose predecessors do not reach the target are kept, the first of all in any case
-              int lo = 1, hi = n_p;
-              while (lo < hi) {
-                const int mid = (lo + hi + 1) / 2;
-                if (static_cast<double>(v[0] + s.list_w[mid - 1]) < target) lo = mid;
-                else hi = mid - 1;
-              }
-              last = s.list[0][lo - 1];
+              const int kept = leading(n_p, [&](int i) { return static_cast<double>(v[0] + s.list_w[i]) < target; });
+              last = s.list[0][max(1, kept) - 1];
               say = SM_FOUND;
             }
+          }
+          if (say == SM_UP || say == SM_DOWN) {  // the neighbour that holds tokens
+            const int step = say == SM_UP ? -1 : 1;
+            do next += step;
+            while (next >= 0 && next < SM_BINS && s.bins[next] == 0);
+            if (next < 0 || next > bin_k || next >= SM_BINS) say = SM_BISECT;
           }
           if (tid == 0) {
             s.T = static_cast<uint32_t>(last >> 32);
@@ -588,130 +783,101 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
           }
         }
         __syncthreads();
-        if (tid == 0) s.verdict = say;
+        if (tid == 0) {
+          s.say.verdict = say;
+          s.say.bin_p = next;
+        }
         if (tid < 2) s.list_n[tid] = 0;
       }
-      if (C > 1) cluster_sync();
-      else __syncthreads();
-      verdict = C > 1 ? peer_u32(&s.verdict, 0) : s.verdict;
-      if (verdict != SM_UP && verdict != SM_DOWN) break;
-      // the neighbour that holds tokens (every CTA finds the same one)
-      const int was = bin_p;
-      if (tid == 0) s.bin_p = verdict == SM_UP ? -1 : SM_BINS;
-      __syncthreads();
-#pragma unroll
-      for (int h = 0; h < PER; ++h) {
-        const int bin = PER * tid + h;
-        if (n[h] > 0 && verdict == SM_UP && bin < was) atomicMax(&s.bin_p, bin);
-        if (n[h] > 0 && verdict == SM_DOWN && bin > was) atomicMin(&s.bin_p, bin);
-      }
-      __syncthreads();
-      bin_p = s.bin_p;
-      verdict = SM_BISECT;
-      if (bin_p < 0 || bin_p > bin_k) break;
-      if (C > 1) cluster_sync();  // rank 0's list is empty before anyone adds to it; verdicts have been read
+      cluster_sync(C);
+      const uint32_t verdict = peer_u32(&s.say.verdict, 0);
+      bin_p = static_cast<int>(peer_u32(&s.say.bin_p, 0));
+      T_key = peer_u32(&s.T, 0);
+      T_idx = peer_u32(&s.T_idx, 0);
+      cluster_sync(C);  // rank 0's findings have been read
+      bisect = verdict != SM_FOUND;
+      if (verdict == SM_FOUND || verdict == SM_BISECT) break;
     }
-    if (verdict == SM_FOUND) {
-      if (bin_p < SM_BINS) {
-        T_key = C > 1 ? peer_u32(&s.T, 0) : s.T;
-        T_idx = C > 1 ? peer_u32(&s.T_idx, 0) : s.T_idx;
-      }
-    } else {
-      threshold_by_bisection<T>(s, a, row, w, turn, best_key, use_k, k, use_p, static_cast<double>(top_p), T_key, T_idx);
-    }
+    if (bisect)
+      threshold_by_bisection<T>(s, a, row, w, rank, turn, best_key, use_k, k, use_p, static_cast<double>(top_p), T_key, T_idx);
   }
 
-  // 4. kept weight by runs of chunks
-  __syncthreads();
+  // 4'. kept weight by runs of chunks
   for (int i = tid; i < SM_RUNS; i += SM_THREADS) s.runs[i] = 0;
   __syncthreads();
   const float T_logit = T_key ? key_logit(T_key) : -INFINITY;
-  auto kept_weight = [&](float x, int i) {
-    const bool in = w.bin(x) < SM_BINS && (x > T_logit || (x == T_logit && i <= static_cast<int>(T_idx)));
-    u64 q = 0;
-    if (__any_sync(MUI_FULL_MASK, in)) q = w(x, in);
-    return q >= w_min ? q : 0ull;
-  };
-  u64 v[3] = {0, 0, 0};
-  row.each([&](int i, float(&x)[8]) {
-    u64 q = 0;
+  const float x_low = fmaxf(fmaxf(T_logit, x_min), w.floor);
+  // weights of the lane's eight tokens that are kept; whole warp
+  auto kept_weights = [&](int i, const float(&x)[8], u64(&q)[8]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q += kept_weight(x[e], i + e);
-    if (__any_sync(MUI_FULL_MASK, q != 0)) {
-      v[0] += q;
-      q = warp_sum_u64(q);
-      if (lane == 0) atomicAdd(&s.runs[(i / SM_CHUNK - row.c0) / a.chunks_per_run], q);
+    for (int e = 0; e < 8; ++e) {
+      const bool in = x[e] > T_logit || (x[e] == T_logit && i + e <= static_cast<int>(T_idx));
+      q[e] = w(x[e], in);
+      q[e] = q[e] >= w_min ? q[e] : 0ull;
+    }
+  };
+  v[0] = v[1] = v[2] = 0;
+  row.each([&](int i, float(&x)[8]) {
+    bool some = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) some |= x[e] >= x_low;
+    if (__any_sync(MUI_FULL_MASK, some)) {
+      u64 q[8], sum = 0;
+      kept_weights(i, x, q);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += q[e];
+      v[0] += sum;
+      sum = warp_sum_u64(sum);
+      if (lane == 0 && sum) atomicAdd(&s.runs[(i / SM_CHUNK - row.c0) / a.chunks_per_run], sum);
     }
   });
   const int my_turn = turn;
-  cluster_sum3(s, C, turn, v);
-  const u64 total = v[0];
-  u64 before = 0, mine = 0;
-  for (int i = 0; i < C; ++i) {
-    const u64 y = C > 1 ? peer_u64(&s.sums[my_turn][0], i) : s.sums[my_turn][0];
-    if (i < static_cast<int>(rank)) before += y;
-    if (i == static_cast<int>(rank)) mine = y;
-  }
-  // uniform numbers lie in [0, 1); what does not is brought to the nearest fp32 that does
-  const float u = fminf(fmaxf(__ldcg(a.uniforms + r), 0.f), 0.99999994f);
-  const double want = static_cast<double>(u) * static_cast<double>(total);
-  if (C > 1) cluster_sync();  // the last look at a peer's memory
+  cluster_sum3(s, C, rank, turn, v);
+  const u64 total = v[0], mine = s.sums[my_turn][rank][0];
+  u64 before = 0;
+  for (unsigned i = 0; i < rank; ++i) before += s.sums[my_turn][i][0];
+  const double want = u * static_cast<double>(total);
   if (mine == 0 || static_cast<double>(before) > want || static_cast<double>(before + mine) <= want) return;
 
   // this CTA holds the drawn point: first its run, then its chunk and token
   {
-    u64 q = tid < SM_RUNS ? s.runs[tid] : 0;
-    u64 c = q;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(MUI_FULL_MASK, c, o);
-      if (lane >= o) c += y;
-    }
-    if (lane == 31) s.fwarp[warp] = c;
-    __syncthreads();
-    u64 at = before;
-    for (int i = 0; i < warp; ++i) at += s.fwarp[i];
-    if (q != 0 && static_cast<double>(at + c) > want && static_cast<double>(at + c - q) <= want) {
+    const u64 q = s.runs[tid];
+    u64 all;
+    const u64 at = before + block_scan(q, s.warp_u64, all);
+    if (q != 0 && static_cast<double>(at + q) > want && static_cast<double>(at) <= want) {
       s.hit = tid;
-      s.sums[my_turn ^ 1][0] = at + c - q;  // weight in front of the run
+      s.best[0] = at;  // weight in front of the run
     }
     __syncthreads();
   }
   if (warp != 0) return;
-  u64 at = s.sums[my_turn ^ 1][0];
+  u64 at = s.best[0];
   const int first = row.c0 + s.hit * a.chunks_per_run, last = min(row.c1, first + a.chunks_per_run);
   for (int c = first; c < last; ++c) {
     float x[8];
     u64 q[8], sum = 0;
     const int i = c * SM_CHUNK + lane * 8;
-    load8<T>(row.p, i, a.V, row.vec, x);
+    row.unpack(load_raw<T>(row.p, i, a.V, row.vec), x);
+    kept_weights(i, x, q);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      q[e] = kept_weight(x[e], i + e);
-      sum += q[e];
-    }
-    u64 run = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(MUI_FULL_MASK, run, o);
-      if (lane >= o) run += y;
-    }
+    for (int e = 0; e < 8; ++e) sum += q[e];
+    const u64 run = warp_scan(sum);
     const unsigned hit = __ballot_sync(MUI_FULL_MASK, sum != 0 && static_cast<double>(at + run) > want);
     if (hit) {
       if (lane == __ffs(hit) - 1) {
-        u64 p = at + run - sum;
-        int e = 0;
+        u64 upto = at + run;
+        int token = 0;
+        u64 weight = 0;
 #pragma unroll
-        for (int h = 7; h >= 0; --h) {  // the first token at which the running weight exceeds the point
-          u64 upto = p;
-          for (int j = 0; j <= h; ++j) upto += q[j];
-          if (q[h] != 0 && static_cast<double>(upto) > want) e = h;
+        for (int e = 7; e >= 0; --e) {  // the first token at which the running weight exceeds the point
+          if (q[e] != 0 && static_cast<double>(upto) > want) {
+            token = i + e;
+            weight = q[e];
+          }
+          upto -= q[e];
         }
-        a.tokens[r] = i + e;
-        u64 mine_w = 0;
-#pragma unroll
-        for (int h = 0; h < 8; ++h) mine_w = h == e ? q[h] : mine_w;
-        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(mine_w) / static_cast<double>(total)));
+        a.tokens[r] = token;
+        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(weight) / static_cast<double>(total)));
       }
       return;
     }
@@ -773,7 +939,7 @@ extern "C" mui_status_t mui_sample_tokens(void* stream, int dtype, int rows, int
   a.V = vocab;
   int lg = 0;
   while ((1 << lg) < vocab) ++lg;
-  a.frac_bits = 62 - lg < 50 ? 62 - lg : 50;
+  a.frac_bits = 62 - lg < 48 ? 62 - lg : 48;
   // CTAs per row: as many as the rows leave SMs for, each with two steps of all its warps at least
   a.cluster = 1;
   while (a.cluster < SM_MAX_CLUSTER && rows * static_cast<long long>(a.cluster) * 2 <= di->sm_count &&
