@@ -523,7 +523,8 @@ MUI_API mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const 
                                          size_t workspace_bytes, unsigned flags);
 
 /* ---- drawing tokens from logits -----------------------------------------------------------------------------
- * For each row of logits [rows, vocab] (row_stride in elements; dtype MUI_F16, MUI_BF16 or MUI_COMM_F32): with z =
+ * For each row of logits [rows, vocab] (vocab up to 2^22; row_stride in elements; dtype MUI_F16, MUI_BF16
+ * or MUI_COMM_F32): with z =
  * (logit - largest logit) / temperature and weights w = exp(z), tokens are ranked by logit, equal ones by index; kept are
  * the first top_k of them, of those the shortest run from the front whose weights reach top_p of the top_k's weight (one
  * token at least), and of those the ones with w >= min(min_p, 1). The drawn token is the first one, in index order, at which the

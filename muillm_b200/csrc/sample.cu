@@ -10,12 +10,13 @@
 //
 // A cluster of up to eight CTAs works on a row (one CTA when there are rows enough to fill the GPU). Passes over the row:
 //   1. the largest logit (from HBM; the later passes find the row in L2);
-//   2. with top-k or top-p, a histogram of z in 4096 equal bins down to the smallest z that still has weight. Counts give the
+//   2. with top-k or top-p, a histogram of z in 2048 equal bins down to the smallest z that still has weight. Counts give the
 //      bin that holds the top_k-th token exactly; counts times the bin centre's weight tell the bin in which top_p ends,
 //      nearly always. Not needed where min-p alone leaves few tokens;
-//   3. all tokens up to that bin (or above min-p's cut) are collected in rank 0's shared memory if they are at most 4096, with
-//      the weight of the whole row where top-p asks for it. Sorted by rank they give T and T_idx, sorted by index the token.
-// More tokens than that (a nucleus of thousands, a temperature without cuts):
+//   3. all tokens up to that bin (or above min-p's cut) are collected in rank 0's shared memory if they are at most 12288, with
+//      the weight of the whole row where top-p asks for it. Rank 0 sums them by bins of z, sorts the bins in which top-k and
+//      top-p end, sums the kept ones by parts of the index range and sorts the part that holds the drawn point.
+// More tokens than that (a wide nucleus, a temperature without cuts):
 //   3'. exact sums of the weight above and between the boundary bins, whose own tokens are collected and sorted to give T and
 //      T_idx; where the estimate of 2 was off, again with the neighbouring bin;
 //   4'. the kept weight of every run of 256 tokens; the run that holds the drawn point is then walked by one warp.
@@ -36,12 +37,14 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int SM_THREADS = 1024;
+constexpr int SM_THREADS = 512;
 constexpr int SM_WARPS = SM_THREADS / 32;
 constexpr int SM_CHUNK = 256;    // tokens of one warp step: eight consecutive ones per lane
-constexpr int SM_BINS = 4096;
-constexpr int SM_LIST = 4096;    // tokens collected at most
-constexpr int SM_RUNS = 1024;    // runs of chunks whose kept weight a CTA holds
+constexpr int SM_BINS = 2048;
+constexpr int SM_LIST = 12288;   // tokens collected at most
+constexpr int SM_SMALL = 4096;   // tokens of one bin at most
+constexpr int SM_MAX_VOCAB = 1 << 22;  // a part of an index range in SM_BINS parts fits the small list
+constexpr int SM_RUNS = SM_THREADS;  // runs of chunks whose kept weight a CTA holds
 constexpr int SM_MAX_CLUSTER = 8;
 // what rank 0 finds in the collected tokens: the threshold, that top-p ends further up or down the ranking, or too many tokens
 enum : uint32_t { SM_FOUND, SM_UP, SM_DOWN, SM_BISECT };
@@ -99,9 +102,12 @@ __device__ __forceinline__ void store_peer_u64(u64* local, unsigned rank, u64 v)
 }
 
 struct Shared {
+  u64 list[SM_LIST];                   // rank 0: rank_entry of collected tokens
+  u64 small[SM_SMALL];                 // rank 0: those of one bin
+  u64 small_w[SM_SMALL];               // weight of the sorted small list in front of each
+  u64 mass[SM_BINS];
+  uint32_t count[SM_BINS];
   uint32_t bins[SM_BINS];              // rank 0: the cluster's counts
-  u64 list[2][SM_LIST];                // rank 0: rank_entry of collected tokens
-  u64 list_w[SM_LIST];
   u64 runs[SM_RUNS];
   u64 part[SM_WARPS][3];
   u64 sums[2][SM_MAX_CLUSTER][3];      // every CTA's sums, two turns so that one barrier per exchange is enough
@@ -117,6 +123,10 @@ struct Shared {
     int bin_k, bin_p;
   } say;
   float est_total;
+  // a bin that rank 0 looks for, with what lies in front of it
+  int bin;
+  uint32_t bin_count, small_n;
+  u64 bin_mass;
   int hit;
 };
 
@@ -172,24 +182,27 @@ struct Row {
       for (int e = 0; e < 8; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
     }
   }
-  // f(first token of the lane, its eight logits) for every chunk of this CTA; warps take chunks in turn, the next one's load
-  // in flight
+  // f(first token of the lane, its eight logits) for every chunk of this CTA; warps take chunks in turn, the next four in
+  // flight (64 KiB per CTA of fp32 logits: a round trip to L2 takes about a microsecond)
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
     const int lane = threadIdx.x & 31;
     int c = c0 + (threadIdx.x >> 5);
-    if (c >= c1) return;
-    Raw cur = load_raw<T>(p, c * SM_CHUNK + lane * 8, V, vec);
-    while (true) {
-      const int n = c + SM_WARPS;
-      Raw next;
-      if (n < c1) next = load_raw<T>(p, n * SM_CHUNK + lane * 8, V, vec);
+    auto get = [&](int n) {
+      Raw q = {};
+      if (n < c1) q = load_raw<T>(p, n * SM_CHUNK + lane * 8, V, vec);
+      return q;
+    };
+    Raw q0 = get(c), q1 = get(c + SM_WARPS), q2 = get(c + 2 * SM_WARPS), q3 = get(c + 3 * SM_WARPS);
+#pragma unroll 1
+    for (; c < c1; c += SM_WARPS) {
       float x[8];
-      unpack(cur, x);
+      unpack(q0, x);
+      q0 = q1;
+      q1 = q2;
+      q2 = q3;
+      q3 = get(c + 4 * SM_WARPS);
       f(c * SM_CHUNK + lane * 8, x);
-      if (n >= c1) break;
-      cur = next;
-      c = n;
     }
   }
 };
@@ -253,7 +266,7 @@ __device__ __forceinline__ V block_scan(V v, V* s_warp, V& all) {
   const V inc = warp_scan(v);
   if (lane == 31) s_warp[warp] = inc;
   __syncthreads();
-  const V w = warp_scan(s_warp[lane]);
+  const V w = warp_scan(lane < SM_WARPS ? s_warp[lane] : V(0));
   all = __shfl_sync(MUI_FULL_MASK, w, 31);
   const V before = __shfl_sync(MUI_FULL_MASK, w, warp - 1);
   return inc - v + (warp ? before : V(0));
@@ -268,7 +281,7 @@ __device__ __forceinline__ void cluster_sum3(Shared& s, int cluster, unsigned ra
     for (int i = 0; i < 3; ++i) s.part[warp][i] = v[i];
   __syncthreads();
   if (warp < 3) {
-    const u64 t = warp_sum_u64(s.part[lane][warp]);
+    const u64 t = warp_sum_u64(lane < SM_WARPS ? s.part[lane][warp] : 0ull);
     if (lane < cluster) store_peer_u64(&s.sums[turn][rank][warp], lane, t);
   }
   cluster_sync(cluster);
@@ -380,22 +393,27 @@ __device__ void sort_list(u64* list, int n) {
   __syncthreads();
 }
 
-// Leaves in list_w[i] the weight of the sorted list's tokens before the i-th; returns the weight of all of them. One CTA.
-__device__ u64 weigh_list(Shared& s, const u64* list, int n, const Weigh& w) {
-  constexpr int PER = SM_LIST / SM_THREADS;
-  u64 q[PER], sum = 0, all;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    const int i = threadIdx.x * PER + e;
-    q[e] = w(i < n ? key_logit(static_cast<uint32_t>(list[i] >> 32)) : 0.f, i < n);
-    sum += q[e];
+// Leaves in w_before[i] the weight of the sorted list's tokens in front of the i-th; returns the weight of all of them. SHIFT:
+// where the keys sit in the entries. One CTA.
+template <int SHIFT>
+__device__ u64 weigh_list(Shared& s, const u64* list, u64* w_before, int n, const Weigh& w) {
+  const int per = (n + SM_THREADS - 1) / SM_THREADS, i0 = threadIdx.x * per;
+  u64 sum = 0, all;
+#pragma unroll 1
+  for (int e = 0; e < per; ++e) {
+    const bool in = i0 + e < n;
+    const u64 q = w(in ? key_logit(static_cast<uint32_t>(list[i0 + e] >> SHIFT)) : 0.f, in);
+    if (in) w_before[i0 + e] = q;
+    sum += q;
   }
   u64 run = block_scan(sum, s.warp_u64, all);
-#pragma unroll
-  for (int e = 0; e < PER; ++e) {
-    s.list_w[threadIdx.x * PER + e] = run;
-    run += q[e];
-  }
+#pragma unroll 1
+  for (int e = 0; e < per; ++e)
+    if (i0 + e < n) {
+      const u64 q = w_before[i0 + e];
+      w_before[i0 + e] = run;
+      run += q;
+    }
   __syncthreads();
   return all;
 }
@@ -481,7 +499,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   if (lane == 0) s.warp_u64[warp] = best;
   __syncthreads();
   if (warp == 0) {
-    best = s.warp_u64[lane];
+    best = lane < SM_WARPS ? s.warp_u64[lane] : 0ull;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const u64 y = __shfl_xor_sync(MUI_FULL_MASK, best, o);
@@ -527,55 +545,174 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   // Rank 0 turns a complete list of the tokens in front (n of them, `total` the weight of the row for top-p without top-k) into
   // the drawn token. cut_p: the list ends where top-p was expected to end; false is returned when it does not.
   auto finish = [&](int n, u64 total, bool cut_p) {
-    sort_list(s.list[0], n);
-    const u64 all = weigh_list(s, s.list[0], n, w);
-    auto before = [&](int i) { return i < n ? s.list_w[i] : all; };
-    int keep = use_k ? min(n, k_raw) : n;
-    if (use_p) {
-      const double target = static_cast<double>(top_p) * static_cast<double>(use_k ? before(keep) : total);
-      if (cut_p && static_cast<double>(all) < target) return false;
-      keep = max(1, leading(keep, [&](int i) { return static_cast<double>(before(i)) < target; }));
+    constexpr int PER = SM_BINS / SM_THREADS;
+    uint32_t cn[PER], cb = 0;
+    u64 mn[PER], mb = 0, all = 0;
+    auto clear = [&]() {
+      for (int i = tid; i < SM_BINS; i += SM_THREADS) {
+        s.mass[i] = 0;
+        s.count[i] = 0;
+      }
+      if (tid == 0) {
+        s.bin = SM_BINS;
+        s.small_n = 0;
+      }
+      __syncthreads();
+    };
+    // g(entry, its weight) for every token of the list; whole warps
+    auto tokens = [&](auto g) {
+#pragma unroll 1
+      for (int base = 0; base < n; base += SM_THREADS) {
+        const int i = base + tid;
+        const u64 e = i < n ? s.list[i] : 0;
+        const u64 q = w(i < n ? key_logit(static_cast<uint32_t>(e >> 32)) : 0.f, i < n);
+        if (i < n) g(e, q);
+      }
+    };
+    auto prefix = [&]() {
+      __syncthreads();
+      cb = 0;
+      mb = 0;
+#pragma unroll
+      for (int h = 0; h < PER; ++h) {
+        cn[h] = s.count[tid * PER + h];
+        mn[h] = s.mass[tid * PER + h];
+        cb += cn[h];
+        mb += mn[h];
+      }
+      uint32_t unused;
+      cb = block_scan(cb, s.warp_u32, unused);
+      mb = block_scan(mb, s.warp_u64, all);
+    };
+    // the first bin for which hit(count in front, its count, weight in front, its weight) holds
+    auto find = [&](auto hit) {
+      uint32_t c = cb;
+      u64 m = mb;
+#pragma unroll
+      for (int h = 0; h < PER; ++h) {
+        if (cn[h] > 0 && hit(c, cn[h], m, mn[h])) atomicMin(&s.bin, tid * PER + h);
+        c += cn[h];
+        m += mn[h];
+      }
+      __syncthreads();
+      c = cb;
+      m = mb;
+#pragma unroll
+      for (int h = 0; h < PER; ++h) {
+        if (s.bin == tid * PER + h) {
+          s.bin_count = c;
+          s.bin_mass = m;
+        }
+        c += cn[h];
+        m += mn[h];
+      }
+      __syncthreads();
+      return s.bin;
+    };
+    auto bin_of = [&](u64 e) { return min(w.bin(key_logit(static_cast<uint32_t>(e >> 32))), SM_BINS - 1); };
+    // the tokens of a bin, sorted, with the weight in front of each; their number, over SM_SMALL: too many
+    auto open_bin = [&](int bin) {
+      for (int i = tid; i < n; i += SM_THREADS)
+        if (bin_of(s.list[i]) == bin) {
+          const uint32_t at = atomicAdd(&s.small_n, 1u);
+          if (at < SM_SMALL) s.small[at] = s.list[i];
+        }
+      __syncthreads();
+      const int m = s.small_n;
+      __syncthreads();
+      if (tid == 0) {
+        s.small_n = 0;
+        s.bin = SM_BINS;
+      }
+      if (m <= SM_SMALL) {
+        sort_list(s.small, m);
+        weigh_list<32>(s, s.small, s.small_w, m, w);
+      }
+      return m;
+    };
+
+    u64 edge = 0;  // entries from here on are kept
+    if (use_k || use_p) {
+      clear();
+      tokens([&](u64 e, u64 q) {
+        const int b = bin_of(e);
+        atomicAdd(&s.count[b], 1u);
+        atomicAdd(&s.mass[b], q);
+      });
+      prefix();
+      u64 within = use_k ? all : total;
+      if (use_k && n > k_raw) {
+        const uint32_t k = static_cast<uint32_t>(k_raw);
+        const int bin = find([&](uint32_t c, uint32_t nc, u64, u64) { return c < k && c + nc >= k; });
+        const uint32_t left = k - s.bin_count;
+        const u64 front = s.bin_mass;
+        const int m = open_bin(bin);
+        if (m > SM_SMALL) return false;
+        edge = s.small[left - 1];
+        const u64 last = w(key_logit(static_cast<uint32_t>(edge >> 32)), true);
+        within = front + s.small_w[left - 1] + last;
+        __syncthreads();
+      }
+      if (use_p) {
+        const double target = static_cast<double>(top_p) * static_cast<double>(within);
+        if (cut_p && static_cast<double>(all) < target) return false;
+        const int bin = find([&](uint32_t c, uint32_t, u64 f, u64 m) {
+          return static_cast<double>(f + m) >= target && (static_cast<double>(f) < target || c == 0);
+        });
+        if (bin < SM_BINS) {
+          const u64 front = s.bin_mass;
+          const int m = open_bin(bin);
+          if (m > SM_SMALL) return false;
+          // tokens whose predecessors do not reach the target are kept, the first of all in any case
+          const int kept = max(1, leading(m, [&](int i) { return static_cast<double>(front + s.small_w[i]) < target; }));
+          const u64 e = s.small[kept - 1];
+          edge = e > edge ? e : edge;
+          __syncthreads();
+        }
+      }
     }
-    keep = leading(keep, [&](int i) { return before(i + 1) - before(i) >= w_min; });
-    const u64 mass = before(keep);
-    const double want = u * static_cast<double>(mass);
     // the kept ones by index
-    for (int i = tid; i < keep; i += SM_THREADS)
-      s.list[1][i] = (s.list[0][i] << 32) | static_cast<uint32_t>(i);  // ~index, place
+    clear();
+    int shift = 0;
+    while ((a.V - 1) >> shift >= SM_BINS) ++shift;
+    auto index_of = [](u64 e) { return static_cast<int>(~static_cast<uint32_t>(e)); };
+    tokens([&](u64 e, u64 q) {
+      if (e >= edge && q >= w_min) {
+        atomicAdd(&s.count[index_of(e) >> shift], 1u);
+        atomicAdd(&s.mass[index_of(e) >> shift], q);
+      }
+    });
+    prefix();
+    const double want = u * static_cast<double>(all);
+    const int part = find([&](uint32_t, uint32_t, u64 f, u64 m) {
+      return static_cast<double>(f + m) > want && static_cast<double>(f) <= want;
+    });
+    tokens([&](u64 e, u64 q) {
+      if (e >= edge && q >= w_min && index_of(e) >> shift == part)
+        s.small[atomicAdd(&s.small_n, 1u)] = e << 32 | e >> 32;  // ~index, key
+    });
     __syncthreads();
-    sort_list(s.list[1], keep);
-    constexpr int PER = SM_LIST / SM_THREADS;
-    u64 q[PER], sum = 0, unused;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int i = tid * PER + e;
-      q[e] = 0;
-      if (i < keep) {
-        const int at = static_cast<int>(s.list[1][i] & 0xffffffffu);
-        q[e] = before(at + 1) - before(at);
-      }
-      sum += q[e];
-    }
-    u64 run = block_scan(sum, s.warp_u64, unused);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
+    const int m = s.small_n;
+    sort_list(s.small, m);
+    const u64 in_part = weigh_list<0>(s, s.small, s.small_w, m, w);
+    for (int i = tid; i < m; i += SM_THREADS) {
       // the first token at which the running weight exceeds the point
-      if (q[e] != 0 && static_cast<double>(run + q[e]) > want && static_cast<double>(run) <= want) {
-        a.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.list[1][tid * PER + e] >> 32));
-        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(q[e]) / static_cast<double>(mass)));
+      const u64 from = s.bin_mass + s.small_w[i], to = s.bin_mass + (i + 1 < m ? s.small_w[i + 1] : in_part);
+      if (static_cast<double>(to) > want && static_cast<double>(from) <= want) {
+        a.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.small[i] >> 32));
+        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(to - from) / static_cast<double>(all)));
       }
-      run += q[e];
     }
     return true;
   };
-  // Collects the tokens that in(x) names in rank 0's list, with the weight of the whole row if asked for. Returns their number
-  // (over SM_LIST: the list is incomplete); the weight is left in v[0].
+  // Collects the tokens that in(x) names in rank 0's list. v[0]: the weight of the whole row if asked for, v[1]: their number
+  // (over SM_LIST: the list is incomplete).
   const uint32_t count_at[2] = {peer_addr(&s.list_n[0], 0), peer_addr(&s.list_n[1], 0)};
-  const uint32_t list_at[2] = {peer_addr(&s.list[0][0], 0), peer_addr(&s.list[1][0], 0)};
-  auto put = [&](int which, float x, int i) {
+  const uint32_t list_at[2] = {peer_addr(s.list, 0), peer_addr(s.small, 0)};
+  auto put = [&](int which, float x, int i, uint32_t room) {
     uint32_t at;
     asm volatile("atom.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(count_at[which]) : "memory");
-    if (at < SM_LIST)
+    if (at < room)
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list_at[which] + at * 8), "l"(rank_entry(x, i)) : "memory");
   };
   u64 v[3];
@@ -590,7 +727,10 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (in(x[e])) put(0, x[e], i + e);
+        if (in(x[e])) {
+          put(0, x[e], i + e, SM_LIST);
+          ++v[1];
+        }
     });
     cluster_sum3(s, C, rank, turn, v);  // its barrier also publishes the list
   };
@@ -599,14 +739,11 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   bool bisect = false;
   if (min_p > 0.f && !use_k) {
     collect([&](float x) { return x >= x_min; }, use_p);
-    const uint32_t n = peer_u32(&s.list_n[0], 0);
-    if (n <= SM_LIST) {
-      if (rank == 0) finish(static_cast<int>(n), v[0], false);
-      if (C > 1) cluster_sync(C);  // rank 0's count has been read
+    if (v[1] <= SM_LIST) {
+      if (rank == 0) finish(static_cast<int>(v[1]), v[0], false);
       return;
     }
-    cluster_sync(C);
-    if (tid == 0) s.list_n[0] = 0;
+    if (tid == 0) s.list_n[0] = 0;  // a barrier follows before the next token is put there
   }
   if (use_k || use_p) {
     // 2. histogram
@@ -722,7 +859,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
         for (int e = 0; e < 8; ++e) {
           const int b = w.bin(x[e]);
           mine |= use_p && b < bin_k && b != bin_p && b < SM_BINS;
-          if (b < SM_BINS && (b == bin_p || b == bin_k)) put(b == bin_p ? 0 : 1, x[e], i + e);
+          if (b < SM_BINS && (b == bin_p || b == bin_k)) put(b == bin_p ? 0 : 1, x[e], i + e, SM_SMALL);
         }
         if (__any_sync(MUI_FULL_MASK, mine)) {
 #pragma unroll
@@ -742,22 +879,22 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
         const bool same = bin_p == bin_k;
         uint32_t say = SM_BISECT;
         int next = bin_p;
-        if (n0 <= SM_LIST && n1 <= SM_LIST) {
+        if (n0 <= SM_SMALL && n1 <= SM_SMALL) {
           const uint32_t left = k - before_k;  // tokens of bin_k within the top-k
           u64 in_k = 0;
           u64 last = 0;
           if (!same && bin_k < SM_BINS) {
-            sort_list(s.list[1], n1);
-            const u64 bin_mass = weigh_list(s, s.list[1], n1, w);
-            in_k = left < static_cast<uint32_t>(n1) ? s.list_w[left] : bin_mass;
+            sort_list(s.small, n1);
+            const u64 bin_mass = weigh_list<32>(s, s.small, s.small_w, n1, w);
+            in_k = left < static_cast<uint32_t>(n1) ? s.small_w[left] : bin_mass;
             __syncthreads();
           }
           const int n_p = same ? static_cast<int>(min(left, static_cast<uint32_t>(n0))) : n0;  // of bin_p within the top-k
-          sort_list(s.list[0], n0);
-          u64 in_p = weigh_list(s, s.list[0], n0, w);
-          if (n_p < n0) in_p = s.list_w[n_p];
+          sort_list(s.list, n0);
+          u64 in_p = weigh_list<32>(s, s.list, s.small_w, n0, w);
+          if (n_p < n0) in_p = s.small_w[n_p];
           if (!use_p) {
-            last = s.list[0][n_p - 1];
+            last = s.list[n_p - 1];
             say = SM_FOUND;
           } else {
             const double target = static_cast<double>(top_p) * static_cast<double>(v[0] + v[1] + in_p + in_k);
@@ -766,8 +903,8 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
             else if (static_cast<double>(v[0] + in_p) < target) say = SM_DOWN;
             else {
               // tokens whose predecessors do not reach the target are kept, the first of all in any case
-              const int kept = leading(n_p, [&](int i) { return static_cast<double>(v[0] + s.list_w[i]) < target; });
-              last = s.list[0][max(1, kept) - 1];
+              const int kept = leading(n_p, [&](int i) { return static_cast<double>(v[0] + s.small_w[i]) < target; });
+              last = s.list[max(1, kept) - 1];
               say = SM_FOUND;
             }
           }
@@ -919,8 +1056,8 @@ extern "C" mui_status_t mui_sample_tokens(void* stream, int dtype, int rows, int
                                           int64_t* tokens, float* logprobs, unsigned flags) {
   MUI_REQUIRE(dtype == MUI_F16 || dtype == MUI_BF16 || dtype == MUI_COMM_F32, MUI_ERR_UNSUPPORTED,
               "dtype %d unsupported", dtype);
-  MUI_REQUIRE(rows >= 0 && rows <= (1 << 24) && vocab >= 1 && vocab <= (1 << 24) && row_stride >= 0,
-              MUI_ERR_INVALID_ARG, "bad sizes rows=%d (0..2^24) vocab=%d (1..2^24) row_stride=%lld", rows, vocab,
+  MUI_REQUIRE(rows >= 0 && rows <= (1 << 24) && vocab >= 1 && vocab <= SM_MAX_VOCAB && row_stride >= 0,
+              MUI_ERR_INVALID_ARG, "bad sizes rows=%d (0..2^24) vocab=%d (1..2^22) row_stride=%lld", rows, vocab,
               (long long)row_stride);
   if (rows == 0) return MUI_OK;
   MUI_REQUIRE(logits && uniforms && tokens, MUI_ERR_INVALID_ARG, "logits, uniforms and tokens must be non-null");

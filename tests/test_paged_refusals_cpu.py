@@ -85,7 +85,7 @@ def test_sample_arguments_are_refused():
 
     inv = capi.MUI_ERR_INVALID_ARG
     assert call(dtype=5) == capi.MUI_ERR_UNSUPPORTED
-    for kw in (dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(stride=-1), dict(logits=None), dict(u=None),
+    for kw in (dict(rows=-1), dict(vocab=0), dict(vocab=(1 << 22) + 1), dict(stride=-1), dict(logits=None), dict(u=None),
                dict(tokens=None)):
         assert call(**kw) == inv, kw
     assert call(rows=0, logits=None) == capi.MUI_OK
