@@ -130,23 +130,33 @@ struct Shared {
   int hit;
 };
 
-// Eight consecutive tokens as they sit in memory: 16 or 32 bytes.
+// Eight tokens as they sit in memory: 16 bytes, or twice 16 bytes of fp32. A lane's eight tokens of a chunk are consecutive
+// 16-bit ones, or four and another four half a chunk on, so that a warp reads whole lines: token e is i + e + gap<T>(e).
 struct Raw {
   uint4 a, b;
 };
 template <typename T>
+__device__ __forceinline__ constexpr int gap(int e) {
+  return sizeof(T) == 4 && e >= 4 ? SM_CHUNK / 2 - 4 : 0;
+}
+template <typename T>
+__device__ __forceinline__ int lane_first(int chunk) {  // the lane's first token of a chunk
+  return chunk * SM_CHUNK + static_cast<int>(threadIdx.x & 31) * (sizeof(T) == 4 ? 4 : 8);
+}
+template <typename T>
 __device__ __forceinline__ Raw load_raw(const T* row, int i, int V, bool vec) {
   Raw r;
-  if (vec && i + 8 <= V) {
+  if (vec && i + 8 + gap<T>(7) <= V) {
     const char* p = reinterpret_cast<const char*>(row) + static_cast<size_t>(i) * sizeof(T);
     r.a = ld_act16(p);
-    if (sizeof(T) == 4) r.b = ld_act16(p + 16);
+    if (sizeof(T) == 4) r.b = ld_act16(p + SM_CHUNK * 2);
     return r;
   }
   uint32_t w[8];  // NaN behind the end of the row
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    if (sizeof(T) == 4) w[e] = i + e < V ? __ldcg(reinterpret_cast<const uint32_t*>(row) + i + e) : 0x7fffffffu;
+    const int n = i + e + gap<T>(e);
+    if (sizeof(T) == 4) w[e] = n < V ? __ldcg(reinterpret_cast<const uint32_t*>(row) + n) : 0x7fffffffu;
     else w[e] = i + e < V ? __ldcg(reinterpret_cast<const unsigned short*>(row) + i + e) : 0x7fffu;
   }
   if (sizeof(T) == 4) {
@@ -186,11 +196,10 @@ struct Row {
   // flight (64 KiB per CTA of fp32 logits: a round trip to L2 takes about a microsecond)
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    const int lane = threadIdx.x & 31;
     int c = c0 + (threadIdx.x >> 5);
     auto get = [&](int n) {
       Raw q = {};
-      if (n < c1) q = load_raw<T>(p, n * SM_CHUNK + lane * 8, V, vec);
+      if (n < c1) q = load_raw<T>(p, lane_first<T>(n), V, vec);
       return q;
     };
     Raw q0 = get(c), q1 = get(c + SM_WARPS), q2 = get(c + 2 * SM_WARPS), q3 = get(c + 3 * SM_WARPS);
@@ -202,7 +211,7 @@ struct Row {
       q1 = q2;
       q2 = q3;
       q3 = get(c + 4 * SM_WARPS);
-      f(c * SM_CHUNK + lane * 8, x);
+      f(lane_first<T>(c), x);
     }
   }
 };
@@ -217,21 +226,34 @@ struct Weigh {
     const float b = (top - x) * bin_scale;
     return b < static_cast<float>(SM_BINS) ? static_cast<int>(b) : SM_BINS;  // NaN: SM_BINS
   }
-  // 2^S exp(z) before rounding, x above the floor; whole warp. (logit - largest) * scale = 32 n + j + f, |f| <= 1/2: the weight is
-  // 2^n * 2^(j/32) * 2^(f/32), the last one by its Taylor polynomial of degree 4 (error below 1.3e-12).
-  __device__ __forceinline__ double value(float x) const {
-    const double d = static_cast<double>(fmaxf(x, floor)) - static_cast<double>(top);
-    const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to a whole number, in the low bits
-    const double km = fma(d, scale, magic);
-    const int k = __double2loint(km);
-    const double f = fma(d, scale, magic - km);
+  // 2^S exp(z) before rounding of N logits, x above the floor; whole warp. (logit - largest) * scale = 32 n + j + f, |f| <= 1/2: the
+  // weight is 2^n * 2^(j/32) * 2^(f/32), the last one by its Taylor polynomial of degree 4 (error below 1.3e-12). Step by step
+  // for all N, since one of these chains takes some 250 cycles.
+  template <int N>
+  __device__ __forceinline__ void values(const float (&x)[N], double (&p)[N]) const {
     constexpr double L = 0.021660849392498290;  // ln 2 / 32
-    double p = fma(f, L * L * L * L / 24.0, L * L * L / 6.0);
-    p = fma(p, f, L * L / 2.0);
-    p = fma(p, f, L);
-    p = fma(p, f, 1.0);
-    p *= __shfl_sync(MUI_FULL_MASK, table, k);
-    return __hiloint2double(__double2hiint(p) + ((k >> 5) + frac_bits) * (1 << 20), __double2loint(p));
+    const double magic = 6755399441055744.0;    // 1.5 * 2^52: adding it rounds to a whole number, in the low bits
+    double d[N], km[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] = static_cast<double>(fmaxf(x[e], floor)) - static_cast<double>(top);
+#pragma unroll
+    for (int e = 0; e < N; ++e) km[e] = fma(d[e], scale, magic);
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] = fma(d[e], scale, magic - km[e]);
+#pragma unroll
+    for (int e = 0; e < N; ++e) p[e] = fma(d[e], L * L * L * L / 24.0, L * L * L / 6.0);
+#pragma unroll
+    for (int e = 0; e < N; ++e) p[e] = fma(p[e], d[e], L * L / 2.0);
+#pragma unroll
+    for (int e = 0; e < N; ++e) p[e] = fma(p[e], d[e], L);
+#pragma unroll
+    for (int e = 0; e < N; ++e) p[e] = fma(p[e], d[e], 1.0);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int k = __double2loint(km[e]);
+      p[e] *= __shfl_sync(MUI_FULL_MASK, table, k);
+      p[e] = __hiloint2double(__double2hiint(p[e]) + ((k >> 5) + frac_bits) * (1 << 20), __double2loint(p[e]));
+    }
   }
   // values below 2^51 added to 2^52 leave their rounded sum in the mantissa
   static __device__ __forceinline__ u64 bits(double v) {
@@ -239,8 +261,10 @@ struct Weigh {
   }
   // the weight as an integer; whole warp
   __device__ __forceinline__ u64 operator()(float x, bool use) const {
-    const u64 q = bits(value(x) + 4503599627370496.0);
-    return use ? q : 0ull;
+    const float in[1] = {x};
+    double p[1];
+    values(in, p);
+    return use ? bits(p[0] + 4503599627370496.0) : 0ull;
   }
 };
 
@@ -304,7 +328,7 @@ __device__ void threshold_by_bisection(Shared& s, const SampleArgs& a, const Row
     row.each([&](int i, float(&x)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const bool in = i + e < a.V && logit_key(x[e]) >= pivot;
+        const bool in = i + e + gap<T>(e) < a.V && logit_key(x[e]) >= pivot;
         v[0] += in;
         v[1] += w(x[e], in && w.bin(x[e]) < SM_BINS);
       }
@@ -360,7 +384,10 @@ __device__ void threshold_by_bisection(Shared& s, const SampleArgs& a, const Row
     u64 v[3] = {0, 0, 0};
     row.each([&](int i, float(&x)[8]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[0] += i + e < a.V && i + e <= static_cast<int>(mid) && logit_key(x[e]) == T_key;
+      for (int e = 0; e < 8; ++e) {
+        const int n = i + e + gap<T>(e);
+        v[0] += n < a.V && n <= static_cast<int>(mid) && logit_key(x[e]) == T_key;
+      }
     });
     cluster_sum3(s, a.cluster, rank, turn, v);
     if (v[0] >= ties) hi = mid;
@@ -464,19 +491,20 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     row.each([&](int i, float(&x)[8]) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const u64 v = rank_entry(x[e], i + e);
-        best = i + e < a.V && v > best ? v : best;
+        const int n = i + e + gap<T>(e);
+        const u64 v = rank_entry(x[e], n);
+        best = n < a.V && v > best ? v : best;
       }
     });
   } else {
     float m = -INFINITY;
     int c = row.c0 + warp;
-    for (; c + 3 * SM_WARPS < row.c1; c += 4 * SM_WARPS) {  // four chunks of loads in flight
-      Raw q[4];
+    for (; c + 7 * SM_WARPS < row.c1; c += 8 * SM_WARPS) {  // eight chunks of loads in flight, 128 KiB per CTA of fp32
+      Raw q[8];
 #pragma unroll
-      for (int h = 0; h < 4; ++h) q[h] = load_raw<T>(row.p, (c + h * SM_WARPS) * SM_CHUNK + lane * 8, a.V, row.vec);
+      for (int h = 0; h < 8; ++h) q[h] = load_raw<T>(row.p, lane_first<T>(c + h * SM_WARPS), a.V, row.vec);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
+      for (int h = 0; h < 8; ++h) {
         float x[8];
         unpack_raw<T>(q[h], x);
 #pragma unroll
@@ -485,7 +513,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     }
     for (; c < row.c1; c += SM_WARPS) {
       float x[8];
-      unpack_raw<T>(load_raw<T>(row.p, c * SM_CHUNK + lane * 8, a.V, row.vec), x);
+      unpack_raw<T>(load_raw<T>(row.p, lane_first<T>(c), a.V, row.vec), x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
     }
@@ -720,15 +748,16 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     v[0] = v[1] = v[2] = 0;
     row.each([&](int i, float(&x)[8]) {
       if (weigh) {
-        double sum = 4503599627370496.0;  // 2^52
+        double p[8], sum = 4503599627370496.0;  // 2^52
+        w.values(x, p);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += w.value(x[e]);
+        for (int e = 0; e < 8; ++e) sum += p[e];
         v[0] += Weigh::bits(sum);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (in(x[e])) {
-          put(0, x[e], i + e, SM_LIST);
+          put(0, x[e], i + e + gap<T>(e), SM_LIST);
           ++v[1];
         }
     });
@@ -859,15 +888,16 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
         for (int e = 0; e < 8; ++e) {
           const int b = w.bin(x[e]);
           mine |= use_p && b < bin_k && b != bin_p && b < SM_BINS;
-          if (b < SM_BINS && (b == bin_p || b == bin_k)) put(b == bin_p ? 0 : 1, x[e], i + e, SM_SMALL);
+          if (b < SM_BINS && (b == bin_p || b == bin_k)) put(b == bin_p ? 0 : 1, x[e], i + e + gap<T>(e), SM_SMALL);
         }
         if (__any_sync(MUI_FULL_MASK, mine)) {
+          double p[8];
+          w.values(x, p);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int b = w.bin(x[e]);
-            const double p = w.value(x[e]);
-            above += b < bin_p ? p : 0.0;
-            between += b > bin_p && b < bin_k ? p : 0.0;
+            above += b < bin_p ? p[e] : 0.0;
+            between += b > bin_p && b < bin_k ? p[e] : 0.0;
           }
           v[0] += Weigh::bits(above);
           v[1] += Weigh::bits(between);
@@ -946,11 +976,13 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   const float x_low = fmaxf(fmaxf(T_logit, x_min), w.floor);
   // weights of the lane's eight tokens that are kept; whole warp
   auto kept_weights = [&](int i, const float(&x)[8], u64(&q)[8]) {
+    double p[8];
+    w.values(x, p);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const bool in = x[e] > T_logit || (x[e] == T_logit && i + e <= static_cast<int>(T_idx));
-      q[e] = w(x[e], in);
-      q[e] = q[e] >= w_min ? q[e] : 0ull;
+      const bool in = x[e] > T_logit || (x[e] == T_logit && i + e + gap<T>(e) <= static_cast<int>(T_idx));
+      q[e] = Weigh::bits(p[e] + 4503599627370496.0);
+      q[e] = in && q[e] >= w_min ? q[e] : 0ull;
     }
   };
   v[0] = v[1] = v[2] = 0;
@@ -992,33 +1024,40 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   const int first = row.c0 + s.hit * a.chunks_per_run, last = min(row.c1, first + a.chunks_per_run);
   for (int c = first; c < last; ++c) {
     float x[8];
-    u64 q[8], sum = 0;
-    const int i = c * SM_CHUNK + lane * 8;
+    u64 q[8];
+    const int i = lane_first<T>(c);
     row.unpack(load_raw<T>(row.p, i, a.V, row.vec), x);
     kept_weights(i, x, q);
+    // tokens in index order: all eight of a lane, or the first four of all lanes and then the other four
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, N = 8 / PARTS;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum += q[e];
-    const u64 run = warp_scan(sum);
-    const unsigned hit = __ballot_sync(MUI_FULL_MASK, sum != 0 && static_cast<double>(at + run) > want);
-    if (hit) {
-      if (lane == __ffs(hit) - 1) {
-        u64 upto = at + run;
-        int token = 0;
-        u64 weight = 0;
+    for (int h = 0; h < PARTS; ++h) {
+      u64 sum = 0;
 #pragma unroll
-        for (int e = 7; e >= 0; --e) {  // the first token at which the running weight exceeds the point
-          if (q[e] != 0 && static_cast<double>(upto) > want) {
-            token = i + e;
-            weight = q[e];
+      for (int e = 0; e < N; ++e) sum += q[h * N + e];
+      const u64 run = warp_scan(sum);
+      const unsigned hit = __ballot_sync(MUI_FULL_MASK, sum != 0 && static_cast<double>(at + run) > want);
+      if (hit) {
+        if (lane == __ffs(hit) - 1) {
+          u64 upto = at + run;
+          int token = 0;
+          u64 weight = 0;
+#pragma unroll
+          for (int e = N - 1; e >= 0; --e) {  // the first token at which the running weight exceeds the point
+            const u64 mine_w = q[h * N + e];
+            if (mine_w != 0 && static_cast<double>(upto) > want) {
+              token = i + h * N + e + gap<T>(h * N + e);
+              weight = mine_w;
+            }
+            upto -= mine_w;
           }
-          upto -= q[e];
+          a.tokens[r] = token;
+          if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(weight) / static_cast<double>(total)));
         }
-        a.tokens[r] = token;
-        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(weight) / static_cast<double>(total)));
+        return;
       }
-      return;
+      at += __shfl_sync(MUI_FULL_MASK, run, 31);
     }
-    at += __shfl_sync(MUI_FULL_MASK, run, 31);
   }
 }
 
