@@ -30,7 +30,7 @@ struct PaArgs {
   mui_strides2_t qs;
   void* out;
   float* partials;  // [ctas, 2, rows per block, D + 2]: maximum, sum, unnormalised output
-  int Hq, G, ctas, row_blocks, lead, max_new, window, sinks, q_vec;
+  int Hq, G, ctas, row_blocks, splits, mixed, lead, max_new, window, sinks, q_vec;
   float scale_log2;
 };
 
@@ -73,11 +73,6 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint2 ld_kv8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // decode: few rows per KV head
@@ -97,6 +92,7 @@ __device__ __forceinline__ int seq_places(const PaArgs& a, int b, Run& r) {
   r.ctx = __ldcg(a.kv.context_lens + b);
   r.seq = b;
   if (r.count == 0 || r.ctx < 0 || r.count > a.max_new) return 0;
+  if (a.mixed && r.count * a.G > PA_MAX_DECODE_ROWS) return 0;  // the prompt kernel's
   const int n = visible_span(a, r.ctx, r.count).n;
   return n ? a.lead + n : 0;
 }
@@ -748,265 +744,639 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// prompts: 64 rows per CTA (16 per warp), 64 cache rows at a time through shared memory
+// prompts: many rows per KV head, on the tcgen05 tensor cores
 // ---------------------------------------------------------------------------------------------------------------------
-constexpr int PP_ROWS = 64, PP_KEYS = 64;
+// A CTA owns 256 rows (two groups of 128, row = new token * G + head in the group) of one sequence and KV head and walks the
+// cache rows that they see, 128 at a time:
+//   S_g = Q_g K^T    (128 x 128, K = D)   both operands in shared memory, K-major with the 128-byte swizzle
+//   P_g = exp2(S_g * scale - reference)   one thread per row, tensor memory to tensor memory, P over S
+//   O_g += P_g V     (128 x D, K = 128)   P from tensor memory, V as it lies in the cache (its head dims contiguous: MN-major)
+// All of tensor memory is taken: S 2 x 128 columns, O 2 x D columns. One thread issues the MMAs, two warpgroups (one per group
+// of rows) take the softmax, four warps bring K and V (16-bit pages: asynchronous copies; e4m3 pages: converted to fp16, exact, on
+// the way) into a ring of four 128-row tiles. While one group's softmax runs, the tensor cores work for the other.
+//
+// The reference of a row's exponents is its running maximum, but moves only when the maximum is more than 8 (a factor 256)
+// above it: then O is rescaled in tensor memory, which is rare after the first tiles; P stays below 2^8 and the sums are right in
+// any case. P is rounded once to the type of the tensor-core operands (half a step is 2^-9 of it for bf16, 2^-12 for fp16).
+// Bound: exp2 (16 a cycle and SM) and the MMAs need about 2050 cycles a step each.
+constexpr int PT_ROWS = 256, PT_GROUP = 128, PT_KEYS = 128;
+constexpr int PT_SUB = PT_KEYS / PA_TILE;          // 16-row tiles of a step
+constexpr int PT_SLOTS = 4;                        // ring of K and V tiles
+constexpr int PT_MMA_WARP = 8, PT_LOAD_WARP = 9, PT_LOAD_WARPS = 4;
+constexpr int PT_LOADERS = PT_LOAD_WARPS * 32;
+constexpr int PT_THREADS = (PT_LOAD_WARP + PT_LOAD_WARPS) * 32;  // 416
+constexpr int PT_MAX_SPLITS = 16;
+constexpr float PT_SLACK = 8.f;
 
-__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit_to(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
+// D[tmem] (+)= A[smem] B[smem]^T
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 consecutive 32-bit columns of this thread's tensor-memory lane
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory matrix descriptor, 128-byte swizzle: rows of 128 bytes, groups of eight rows 1024 bytes apart. K-major: a row
+// is 64 elements along K; the leading offset is not used. MN-major: a row is 64 elements along N, the rows run along K, and
+// `lead` is the distance from one block of 64 to the next along N.
+__device__ __forceinline__ uint64_t sw128_desc(uint32_t addr, uint32_t lead) {
+  return static_cast<uint64_t>((addr & 0x3ffffu) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+// kind::f16 with fp32 accumulators: M = 128; b_mn: B is MN-major
+__device__ __forceinline__ uint32_t f16_idesc(int is_bf16, int n, int b_mn) {
+  return 1u << 4 | static_cast<uint32_t>(is_bf16) << 7 | static_cast<uint32_t>(is_bf16) << 10 |
+         static_cast<uint32_t>(b_mn) << 16 | static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(128 >> 4) << 24;
+}
+
+// Which rows a CTA owns and what they see. false: nothing to do.
+struct PromptTile {
+  int b, first, count, ctx, r0, R;
+  Span sp;
+  int steps, per, active;  // steps of 128 cache rows; steps per split; splits that have any
+};
+__device__ __forceinline__ bool prompt_tile(const PaArgs& a, int x, PromptTile& t) {
+  int tile;
+  if (a.kv.cu != nullptr) {
+    // tiles are numbered through: sequence b's start at floor(cu[b] * G / 256) + b
+    const int32_t* cu = a.kv.cu;
+    auto start = [&](int k) { return static_cast<int>(static_cast<long long>(__ldcg(cu + k)) * a.G / PT_ROWS) + k; };
+    t.b = warp_count_le(a.kv.batch, x, [&](int k) { return start(k + 1); });
+    if (t.b >= a.kv.batch) return false;
+    tile = x - start(t.b);
+  } else {
+    t.b = x;  // one new token: at most 32 rows
+    tile = 0;
+  }
+  paged_new_tokens(a.kv, t.b, t.first, t.count);
+  t.ctx = __ldcg(a.kv.context_lens + t.b);
+  t.r0 = tile * PT_ROWS;
+  t.R = t.count * a.G;
+  if (tile < 0 || t.r0 >= t.R) return false;
+  if (t.ctx < 0 || t.count > a.max_new) {
+    if ((threadIdx.x & 31) == 0) mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(t.ctx < 0 ? t.ctx : t.count));
+    return false;
+  }
+  if (a.mixed && t.R <= PA_MAX_DECODE_ROWS) return false;  // the decode kernel's
+  const int lo = t.r0 / a.G, hi = (min(t.R, t.r0 + PT_ROWS) - 1) / a.G;  // new tokens of this tile
+  t.sp = visible_span(a, t.ctx + lo, hi - lo + 1);
+  t.steps = (t.sp.n + PT_SUB - 1) / PT_SUB;
+  t.per = max(2, (t.steps + a.splits - 1) / a.splits);
+  t.active = max(1, (t.steps + t.per - 1) / t.per);
+  return true;
 }
 
 template <typename T, bool KV8, int D>
-__global__ void __launch_bounds__(PA_THREADS) paged_prompt_kernel(const PaArgs a) {
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArgs a) {
   using M = typename std::conditional<KV8, __half, T>::type;
-  constexpr int CH = D / 8;  // 16-byte chunks per row, stored at chunk ^ (row & 7)
-  __shared__ __align__(16) uint4 sk[PP_KEYS * CH];
-  __shared__ __align__(16) uint4 sv[PP_KEYS * CH];
-  __shared__ float s_ks[PP_KEYS / PA_TILE], s_vs[PP_KEYS / PA_TILE];
-  __shared__ int s_tb[PP_KEYS / PA_TILE];
+  constexpr int QT = PT_GROUP * D * 2;                 // bytes of a group's Q
+  constexpr int KT = PT_KEYS * D * 2;                  // bytes of a K or V tile
+  constexpr int BLOCK = PT_KEYS * 128;                 // bytes of one 64-element block of a tile (Q, K or V)
+  constexpr uint32_t TM_S = 0, TM_O = 2 * PT_KEYS;     // tensor-memory columns
+  extern __shared__ unsigned char pt_raw[];
+  __shared__ uint64_t kv_full[PT_SLOTS], kv_empty[PT_SLOTS], s_full[2], p_full[2], pv_done[2];
+  __shared__ float q_back[PT_ROWS];
+  __shared__ uint32_t tmem_s;
+  __shared__ int abort_s;
+  const uint32_t tiles = (smem_u32(pt_raw) + 1023u) & ~1023u;  // Q0, Q1, then the ring
+  const uint32_t ring = tiles + 2 * QT;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kvh = blockIdx.y, split = blockIdx.z;
+  volatile int* abort_flag = &abort_s;
+
   pdl_wait_prior_grid();
   pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-  const int kvh = blockIdx.y;
-  // row tiles are numbered through: sequence b's start at floor(cu[b] * G / 64) + b
-  int b = 0, tile_in_seq = 0;
-  const int x = gridDim.x - 1 - blockIdx.x;  // the longest spans first
-  if (a.kv.cu != nullptr) {
-    const int32_t* cu = a.kv.cu;
-    auto start = [&](int k) {
-      return static_cast<int>(static_cast<long long>(__ldcg(cu + k)) * a.G / PP_ROWS) + k;
-    };
-    b = warp_count_le(a.kv.batch, x, [&](int k) { return start(k + 1); });
-    if (b >= a.kv.batch) return;
-    tile_in_seq = x - start(b);
-  } else {
-    const int tiles = (a.G + PP_ROWS - 1) / PP_ROWS;
-    b = x / tiles;
-    tile_in_seq = x % tiles;
-  }
-  int first, count;
-  paged_new_tokens(a.kv, b, first, count);
-  const int ctx = __ldcg(a.kv.context_lens + b);
-  const int R = count * a.G, r0 = tile_in_seq * PP_ROWS;
-  if (count > a.max_new || ctx < 0) {
-    if (threadIdx.x == 0) mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx < 0 ? ctx : count));
-    return;
-  }
-  if (r0 >= R) return;
-  const int tok_lo = r0 / a.G, tok_hi = (min(R, r0 + PP_ROWS) - 1) / a.G;  // new tokens of this tile
-  const Span sp = visible_span(a, ctx + tok_lo, tok_hi - tok_lo + 1);
-  if (sp.kv_len < ctx + tok_hi + 1 && threadIdx.x == 0)
-    mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx + tok_hi + 1));
+  PromptTile t;
+  if (!prompt_tile(a, gridDim.x - 1 - blockIdx.x, t)) return;
+  if (split >= t.active) return;
+  const int i_begin = split * t.per * PT_SUB, i_end = min(t.sp.n, i_begin + t.per * PT_SUB);  // 16-row tiles of this split
+  const int n = (i_end - i_begin + PT_SUB - 1) / PT_SUB;
+  const bool two = t.R - t.r0 > PT_GROUP;  // the second group has rows
+  if (t.sp.kv_len < t.ctx + (min(t.R, t.r0 + PT_ROWS) - 1) / a.G + 1 && tid == 0)
+    mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(t.sp.kv_len));
 
-  // q fragments (A operand): rows g and g + 8 of the warp's sixteen
-  uint32_t qf[D / 16][4];
-  float qs[2];
-  int hi[2], lo[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = r0 + warp * 16 + g + 8 * h;
-    const T* qp = nullptr;
-    if (r < R) qp = reinterpret_cast<const T*>(a.q) + (first + r / a.G) * a.qs.tok + (kvh * a.G + r % a.G) * a.qs.head;
-    float v[D / 16][4], amax = 0.f;
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        v[c][e] = qp ? ld_act_f32<T>(qp + c * 16 + (e >> 1) * 8 + tq * 2 + (e & 1)) : 0.f;
-        amax = fmaxf(amax, fabsf(v[c][e]));
-      }
-    float mul = 1.f, back = 1.f;
-    if (KV8) {
-      amax = fmaxf(amax, __shfl_xor_sync(MUI_FULL_MASK, amax, 1));
-      amax = fmaxf(amax, __shfl_xor_sync(MUI_FULL_MASK, amax, 2));
-      const int e = min(100, max(-100, static_cast<int>(__float_as_uint(amax) >> 23) - 127));
-      mul = exp2_int(-e);
-      back = exp2_int(e);
+  if (tid == 0) {
+    for (int i = 0; i < PT_SLOTS; ++i) {
+      mbar_init(&kv_full[i], PT_LOADERS);
+      mbar_init(&kv_empty[i], 1);
     }
-#pragma unroll
-    for (int c = 0; c < D / 16; ++c) {
-      qf[c][h] = Elt<M>::pack2(v[c][0] * mul, v[c][1] * mul);
-      qf[c][2 + h] = Elt<M>::pack2(v[c][2] * mul, v[c][3] * mul);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_full[g], PT_GROUP);
+      mbar_init(&pv_done[g], 1);
     }
-    qs[h] = a.scale_log2 * back;
-    const int p = ctx + r / a.G;
-    hi[h] = r < R ? p : -1;
-    lo[h] = a.window > 0 ? p - a.window + 1 : 0;
+    abort_s = 0;
+    mbar_fence_init();
   }
-
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4], vref = 0.f;
+  if (warp == PT_MMA_WARP) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_s)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // Q into shared memory: eight lanes (D = 64) or sixteen per row. e4m3 pages: as fp16, brought near 1 by a power of two per row.
+  {
+    constexpr int LPR = D / 8;
+    for (int i = tid; i < PT_ROWS * LPR; i += PT_THREADS) {  // 416 is a multiple of 16 and so is the row count: whole rows
+      const int r = i / LPR, ch = i % LPR, rr = t.r0 + r;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (rr < t.R)
+        w = load_q8<T>(reinterpret_cast<const T*>(a.q) + (t.first + rr / a.G) * a.qs.tok + (kvh * a.G + rr % a.G) * a.qs.head + ch * 8,
+                       a.q_vec);
+      if (KV8) {
+        float x[8], amax = 0.f;
+        unpack8<T>(w, x);
 #pragma unroll
-  for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  const int32_t* table = a.kv.block_table + static_cast<size_t>(b) * a.kv.table_stride;
-  constexpr int ES = KV8 ? 1 : 2;
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+        const unsigned mask = LPR == 16 ? 0xffffu << (lane & 16) : 0xffu << (lane & 24);
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(mask, amax, o));
+        const int e2 = min(100, max(-100, static_cast<int>(__float_as_uint(amax) >> 23) - 127));
+        const float mul = exp2_int(-e2);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] *= mul;
+        w = pack8<__half>(x);
+        if (ch == 0) q_back[r] = exp2_int(e2);
+      }
+      const int c = ch & 7;
+      const uint32_t dst = tiles + (r / PT_GROUP) * QT + (ch >> 3) * BLOCK + (r % PT_GROUP) * 128 + ((c ^ (r & 7)) << 4);
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_s;
+  // a wait that runs out records itself once and makes every other one give up
+  auto wait = [&](uint64_t* bar, int phase, unsigned what) {
+    if (mbar_wait_bounded(bar, phase & 1, abort_flag)) return true;
+    if (!*abort_flag) mui_dev_set_status(MUI_DEV_TIMEOUT_FULL, 0x800000u | what);
+    *abort_flag = 1;
+    return false;
+  };
+  const int32_t* table = a.kv.block_table + static_cast<size_t>(t.b) * a.kv.table_stride;
+  // lanes 0-7: page (-1: none) and first row (-1) of the 16-row tiles of step j
+  auto find_tile = [&](int j, int& page, int& tb, bool record) {
+    const int i = i_begin + j * PT_SUB + lane;
+    page = tb = -1;
+    if (lane < PT_SUB && i < i_end) {
+      const int row = span_tile(t.sp, i) * PA_TILE;
+      const int p = __ldcg(table + (row >> a.kv.page_shift));
+      if (p >= 0 && p < a.kv.num_pages) {
+        page = p;
+        tb = row;
+      } else if (record) {
+        mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(t.b));
+      }
+    }
+  };
 
-  for (int i0 = 0; i0 < sp.n; i0 += PP_KEYS / PA_TILE) {
-    __syncthreads();
-    // each warp brings one tile of 16 rows
-    {
-      int tb = -1, page = -1;
-      if (i0 + warp < sp.n) {
-        const int tile = span_tile(sp, i0 + warp);
-        page = __ldcg(table + (tile * PA_TILE >> a.kv.page_shift));
-        if (page < 0 || page >= a.kv.num_pages) {
-          if (lane == 0) mui_dev_set_status(MUI_DEV_BAD_PAGE, static_cast<unsigned>(b));
-          page = -1;
-        } else {
-          tb = tile * PA_TILE;
-        }
-      }
-      const size_t head = static_cast<size_t>(max(page, 0)) * a.kv.kv_heads + kvh;
-      const size_t off = ((head << a.kv.page_shift) + (max(tb, 0) & ((1 << a.kv.page_shift) - 1))) * (D * ES);
-      if (lane == 0) {
-        s_tb[warp] = tb;
-        if (KV8) {
-          s_ks[warp] = tb >= 0 ? __ldcg(a.kv.k_scales + head) : 0.f;
-          s_vs[warp] = tb >= 0 ? __ldcg(a.kv.v_scales + head) : 0.f;
-        }
-      }
-      for (int c = lane; c < 16 * CH; c += 32) {
-        const int row = c / CH, ch = c % CH, j = tb + row;
-        const bool ok = tb >= 0 && j < sp.kv_len && (j >= sp.lo_min || j < a.sinks);
-        uint4 k4 = make_uint4(0, 0, 0, 0), v4 = k4;
-        if (ok) {
-          const unsigned char* kp = reinterpret_cast<const unsigned char*>(a.kv.k_pages) + off + (row * D + ch * 8) * ES;
-          const unsigned char* vp = reinterpret_cast<const unsigned char*>(a.kv.v_pages) + off + (row * D + ch * 8) * ES;
+  if (warp >= PT_LOAD_WARP) {
+    // ------------------------------ K and V ------------------------------
+    const int lt = tid - PT_LOAD_WARP * 32;
+    constexpr int ES = KV8 ? 1 : 2, RB = D * ES, CPR = RB / 16;  // bytes and 16-byte chunks of a cache row
+    constexpr int IT = PT_KEYS * CPR / PT_LOADERS;               // chunks of a tile per thread
+    constexpr int RPI = PT_LOADERS / CPR;                        // rows per turn
+    const int ch = lt % CPR, row0 = lt / CPR;
+    int page, tb, next_page, next_tb;
+    find_tile(0, page, tb, true);
+    uint4 hold[KV8 ? IT : 1];
+    bool ok = true;
+    for (int j = 0; j < n && ok; ++j) {
+      next_page = next_tb = -1;
+      if (j + 1 < n) find_tile(j + 1, next_page, next_tb, true);
+      for (int which = 0; which < 2 && ok; ++which) {
+        const int it = 2 * j + which, slot = it % PT_SLOTS;
+        const unsigned char* base = reinterpret_cast<const unsigned char*>(which == 0 ? a.kv.k_pages : a.kv.v_pages) + ch * 16;
+        const uint32_t dst = ring + slot * KT;
+        // e4m3: the loads do not need the slot
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+          const int row = i * RPI + row0, sub = row / PA_TILE;
+          const int pg = __shfl_sync(MUI_FULL_MASK, page, sub), b0 = __shfl_sync(MUI_FULL_MASK, tb, sub);
+          const int jr = b0 + (row & (PA_TILE - 1));
+          // rows that nobody of this tile sees are zeros: what they hold must not matter
+          const bool see = b0 >= 0 && jr < t.sp.kv_len && (jr >= t.sp.lo_min || jr < a.sinks);
+          const size_t at = ((static_cast<size_t>(max(pg, 0)) * a.kv.kv_heads + kvh) << a.kv.page_shift) +
+                            (max(b0, 0) & ((1 << a.kv.page_shift) - 1)) + (row & (PA_TILE - 1));
+          const unsigned char* src = base + at * RB;
           if (KV8) {
-            const uint2 k2 = ld_kv8(kp), v2 = ld_kv8(vp);
-            k4 = make_uint4(e4m3_to_half2((uint16_t)k2.x), e4m3_to_half2((uint16_t)(k2.x >> 16)),
-                            e4m3_to_half2((uint16_t)k2.y), e4m3_to_half2((uint16_t)(k2.y >> 16)));
-            v4 = make_uint4(e4m3_to_half2((uint16_t)v2.x), e4m3_to_half2((uint16_t)(v2.x >> 16)),
-                            e4m3_to_half2((uint16_t)v2.y), e4m3_to_half2((uint16_t)(v2.y >> 16)));
+            hold[KV8 ? i : 0] = see ? ld_stream16(src) : make_uint4(0, 0, 0, 0);
           } else {
-            k4 = ld_stream16(kp);
-            v4 = ld_stream16(vp);
+            if (i == 0 && it >= PT_SLOTS) {
+              ok = wait(&kv_empty[slot], it / PT_SLOTS - 1, 0x100 + slot);
+              ok = __all_sync(MUI_FULL_MASK, ok);
+              if (!ok) break;
+            }
+            copy16(dst + (ch >> 3) * BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4), src, see ? 16 : 0);
           }
         }
-        const int at = (warp * 16 + row) * CH + (ch ^ (row & 7));
-        sk[at] = k4;
-        sv[at] = v4;
+        if (!ok) break;
+        if (KV8) {
+          if (it >= PT_SLOTS) {
+            ok = wait(&kv_empty[slot], it / PT_SLOTS - 1, 0x100 + slot);
+            ok = __all_sync(MUI_FULL_MASK, ok);
+            if (!ok) break;
+          }
+#pragma unroll
+          for (int i = 0; i < (KV8 ? IT : 0); ++i) {
+            const int row = i * RPI + row0;
+            const uint32_t w[4] = {hold[i].x, hold[i].y, hold[i].z, hold[i].w};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = 2 * ch + h;  // 16-bit chunk
+              const uint32_t at = dst + (c >> 3) * BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+              const uint32_t w0 = w[2 * h], w1 = w[2 * h + 1];
+              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(e4m3_to_half2((uint16_t)w0)),
+                           "r"(e4m3_to_half2((uint16_t)(w0 >> 16))), "r"(e4m3_to_half2((uint16_t)w1)),
+                           "r"(e4m3_to_half2((uint16_t)(w1 >> 16)))
+                           : "memory");
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(&kv_full[slot]);
+        } else {
+          copy_commit();
+          if (it >= 2) {  // two tiles stay in flight
+            copy_wait<2>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            mbar_arrive(&kv_full[(it - 2) % PT_SLOTS]);
+          }
+        }
+      }
+      page = next_page;
+      tb = next_tb;
+    }
+    if (!KV8) {
+      copy_wait<0>();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (ok)
+        for (int it = max(0, 2 * n - 2); it < 2 * n; ++it) mbar_arrive(&kv_full[it % PT_SLOTS]);
+    }
+  } else if (warp == PT_MMA_WARP) {
+    // ------------------------------ MMAs ------------------------------
+    if (lane == 0) {
+      const int bf = std::is_same<M, __nv_bfloat16>::value;
+      const uint32_t id_s = f16_idesc(bf, PT_KEYS, 0), id_o = f16_idesc(bf, D, 1);
+      auto scores = [&](int g, int slot) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * BLOCK + (k & 3) * 32;
+          mma_ss(tmem + TM_S + g * PT_KEYS, sw128_desc(tiles + g * QT + off, 16), sw128_desc(ring + slot * KT + off, 16), id_s, k != 0);
+        }
+      };
+      auto output = [&](int g, int slot, bool more) {
+#pragma unroll
+        for (int k = 0; k < PT_KEYS / 16; ++k)
+          mma_ts(tmem + TM_O + g * D, tmem + TM_S + g * PT_KEYS + k * 8, sw128_desc(ring + slot * KT + k * 2048, BLOCK), id_o,
+                 more || k != 0);
+      };
+      bool ok = n == 0 || wait(&kv_full[0], 0, 0x200);
+      if (ok && n > 0) {
+        tc_after();
+        scores(0, 0);
+        tc_commit_to(&s_full[0]);
+        if (two) {
+          scores(1, 0);
+          tc_commit_to(&s_full[1]);
+        }
+        tc_commit_to(&kv_empty[0]);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const int vi = 2 * j + 1, ki = 2 * j + 2, vs = vi % PT_SLOTS, ks = ki % PT_SLOTS;
+        ok = wait(&kv_full[vs], vi / PT_SLOTS, 0x210) && wait(&p_full[0], j, 0x220);
+        if (!ok) break;
+        tc_after();
+        output(0, vs, j > 0);
+        tc_commit_to(&pv_done[0]);
+        if (j + 1 < n) {
+          ok = wait(&kv_full[ks], ki / PT_SLOTS, 0x230);
+          if (!ok) break;
+          tc_after();
+          scores(0, ks);
+          tc_commit_to(&s_full[0]);
+        }
+        if (two) {
+          ok = wait(&p_full[1], j, 0x240);
+          if (!ok) break;
+          tc_after();
+          output(1, vs, j > 0);
+          tc_commit_to(&pv_done[1]);
+        }
+        tc_commit_to(&kv_empty[vs]);
+        if (j + 1 < n) {
+          if (two) {
+            scores(1, ks);
+            tc_commit_to(&s_full[1]);
+          }
+          tc_commit_to(&kv_empty[ks]);
+        }
+      }
+      if (!ok) {  // leave no MMA in flight behind (slot 0's barrier is not waited for by anyone any more)
+        tc_commit_to(&pv_done[0]);
+        const uint64_t t0 = global_timer_ns();
+        while (global_timer_ns() - t0 < 1000000ull) {
+        }
       }
     }
-    __syncthreads();
-    float s[PP_KEYS / 8][4];
+    __syncwarp();
+  } else {
+    // ------------------------------ softmax: a thread per row ------------------------------
+    const int g = warp >> 2, row = (warp & 3) * 32 + lane;
+    if (g == 0 || two) {
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t ts = tmem + lanes + TM_S + g * PT_KEYS, to = tmem + lanes + TM_O + g * D;
+      const int rr = t.r0 + g * PT_GROUP + row;
+      const bool mine = rr < t.R;
+      const int pos = t.ctx + (mine ? rr / a.G : 0);
+      const int hi = mine ? pos : -1, lo = a.window > 0 ? pos - a.window + 1 : 0;
+      // what all rows of the group see without looking: rows from lo_all (or sinks) to hi_all
+      const int last_row = min(t.R, t.r0 + (g + 1) * PT_GROUP) - 1;
+      const int hi_all = t.ctx + (t.r0 + g * PT_GROUP) / a.G;
+      const int lo_all = a.window > 0 ? t.ctx + last_row / a.G - a.window + 1 : 0;
+      const float sc = KV8 ? a.scale_log2 * q_back[g * PT_GROUP + row] : a.scale_log2;
+      float ref = -INFINITY, l = 0.f, vref = 0.f;
+      int page, tb, next_page, next_tb;
+      float ks = 0.f, vs = 0.f;
+      auto scales = [&](int p, float& k, float& v) {
+        k = v = 0.f;
+        if (KV8 && p >= 0) {
+          const size_t head = static_cast<size_t>(p) * a.kv.kv_heads + kvh;
+          k = __ldcg(a.kv.k_scales + head);
+          v = __ldcg(a.kv.v_scales + head);
+        }
+      };
+      find_tile(0, page, tb, false);
+      scales(page, ks, vs);
+      bool ok = true;
+      for (int j = 0; j < n; ++j) {
+        next_page = next_tb = -1;
+        if (j + 1 < n) find_tile(j + 1, next_page, next_tb, false);
+        // every row of the step is seen by every row of the group
+        const bool whole = lane >= PT_SUB || (tb >= 0 && tb + PA_TILE - 1 <= hi_all && (tb >= lo_all || tb + PA_TILE <= a.sinks));
+        const bool open = __all_sync(MUI_FULL_MASK, whole);
+        ok = __all_sync(MUI_FULL_MASK, wait(&s_full[g], j, 0x300 + g));
+        if (!ok) break;
+        tc_after();
+        // scaled scores of 32 columns
+        auto load_scores = [&](int c, float (&s)[32]) {
+          tmem_load32(ts + c * 32, s);
 #pragma unroll
-    for (int n = 0; n < PP_KEYS / 8; n += 2) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      s[n + 1][0] = s[n + 1][1] = s[n + 1][2] = s[n + 1][3] = 0.f;
+          for (int h = 0; h < 2; ++h) {
+            const float f = KV8 ? sc * __shfl_sync(MUI_FULL_MASK, ks, 2 * c + h) : sc;
+            const int b0 = __shfl_sync(MUI_FULL_MASK, tb, 2 * c + h);
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) {
-        // matrices: rows n*8.. chunk 2c, same rows chunk 2c+1, rows n*8+8.. chunk 2c, chunk 2c+1
-        const int row = n * 8 + (lane & 7) + ((lane >> 4) << 3), ch = 2 * c + ((lane >> 3) & 1);
-        uint32_t r[4];
-        ldmatrix_x4(r, smem_u32(&sk[row * CH + (ch ^ (row & 7))]));
-        mma16816<M>(s[n], qf[c][0], qf[c][1], qf[c][2], qf[c][3], r[0], r[1]);
-        mma16816<M>(s[n + 1], qf[c][0], qf[c][1], qf[c][2], qf[c][3], r[2], r[3]);
+            for (int e = 0; e < 16; ++e) {
+              s[16 * h + e] *= f;
+              if (!open) {
+                const int jr = b0 + e;
+                if (!(b0 >= 0 && jr <= hi && (jr >= lo || jr < a.sinks))) s[16 * h + e] = -INFINITY;
+              }
+            }
+          }
+        };
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s[32];
+          load_scores(c, s);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(s[e], s[e + 1]));
+        }
+        float turn = 1.f;  // e4m3: change of the output's reference scale
+        if (KV8) {
+          const float v = fmaxf(vref, warp_max(lane < PT_SUB ? vs : 0.f));
+          if (v > vref) {
+            turn = vref / v;
+            vref = v;
+          }
+        }
+        float factor = turn;
+        if (mx > ref + PT_SLACK || ref == -INFINITY) {
+          factor *= ref == -INFINITY ? 0.f : ex2(ref - mx);
+          l *= ref == -INFINITY ? 0.f : ex2(ref - mx);
+          ref = mx;
+        }
+        if (j > 0 && __any_sync(MUI_FULL_MASK, factor != 1.f)) {
+          ok = __all_sync(MUI_FULL_MASK, wait(&pv_done[g], j - 1, 0x310 + g));
+          if (!ok) break;
+          tc_after();
+          // a row without anything so far has nothing in O
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tmem_load32(to + c * 32, o);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t w[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[16 * h + e] * factor);
+              tmem_store16(to + c * 32 + 16 * h, w);
+            }
+          }
+        }
+        const float use = ref == -INFINITY ? 0.f : ref;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s[32];
+          load_scores(c, s);
+          uint32_t w[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float f = KV8 ? (vref > 0.f ? __shfl_sync(MUI_FULL_MASK, vs, 2 * c + h) / vref : 0.f) : 1.f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float p0 = ex2(s[16 * h + e] - use), p1 = ex2(s[16 * h + e + 1] - use);
+              l += p0 + p1;
+              w[8 * h + e / 2] = KV8 ? Elt<M>::pack2(p0 * f, p1 * f) : Elt<M>::pack2(p0, p1);
+            }
+          }
+          tmem_store16(ts + c * 16, w);  // columns that were read above
+        }
+        tmem_store_wait();
+        tc_before();
+        mbar_arrive(&p_full[g]);
+        page = next_page;
+        tb = next_tb;
+        scales(page, ks, vs);
       }
-    }
-    float mx[2] = {-INFINITY, -INFINITY};
+      if (ok && n > 0) ok = __all_sync(MUI_FULL_MASK, wait(&pv_done[g], n - 1, 0x320 + g));
+      tc_after();
+      if (ok) {
+        const bool direct = t.active == 1;
+        const float norm = (direct ? (l != 0.f ? 1.f / l : 0.f) : 1.f) * (KV8 ? vref : 1.f);
+        const size_t out_row = static_cast<size_t>(t.first + rr / a.G) * a.Hq + kvh * a.G + rr % a.G;
+        float* part = a.partials + (out_row * a.splits + split) * (D + 2);
+        if (mine && !direct) {
+          part[0] = ref;
+          part[1] = l;
+        }
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (n > 0) {
+            tmem_load32(to + c * 32, o);
+          } else {
 #pragma unroll
-    for (int n = 0; n < PP_KEYS / 8; ++n) {
-      const int tb = s_tb[n / 2];
-      const float ks = KV8 ? s_ks[n / 2] : 1.f;
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          if (!mine) continue;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int h = e >> 1, j = tb + (n & 1) * 8 + 2 * tq + (e & 1);
-        const bool see = tb >= 0 && j <= hi[h] && (j >= lo[h] || j < a.sinks);
-        s[n][e] = see ? s[n][e] * (qs[h] * ks) : -INFINITY;
-        mx[h] = fmaxf(mx[h], s[n][e]);
-      }
-    }
-    float turn = 1.f;
-    if (KV8) {
-      float v = vref;
+          for (int e = 0; e < 32; ++e) o[e] *= norm;
+          if (direct) {
+            uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + out_row * D + c * 32);
 #pragma unroll
-      for (int w = 0; w < PP_KEYS / PA_TILE; ++w) v = fmaxf(v, s_vs[w]);
-      if (v > vref) {
-        turn = vref / v;
-        vref = v;
-      }
-    }
+            for (int e = 0; e < 4; ++e)
+              out[e] = make_uint4(Elt<T>::pack2(o[8 * e], o[8 * e + 1]), Elt<T>::pack2(o[8 * e + 2], o[8 * e + 3]),
+                                  Elt<T>::pack2(o[8 * e + 4], o[8 * e + 5]), Elt<T>::pack2(o[8 * e + 6], o[8 * e + 7]));
+          } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(MUI_FULL_MASK, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(MUI_FULL_MASK, mx[h], 2));
-      const float mn = fmaxf(m[h], mx[h]);
-      const float use = mn == -INFINITY ? 0.f : mn;
-      const float corr = ex2(m[h] - use);
-      m[h] = mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int n = 0; n < PP_KEYS / 8; ++n) {
-        s[n][2 * h] = ex2(s[n][2 * h] - use);
-        s[n][2 * h + 1] = ex2(s[n][2 * h + 1] - use);
-        sum += s[n][2 * h] + s[n][2 * h + 1];
-      }
-      l[h] = l[h] * corr + sum;
-#pragma unroll
-      for (int j = 0; j < D / 8; ++j) {
-        o[j][2 * h] *= corr * turn;
-        o[j][2 * h + 1] *= corr * turn;
-      }
-    }
-#pragma unroll
-    for (int kk = 0; kk < PP_KEYS / 16; ++kk) {
-      // probabilities rounded once to the type of the cache's values (half a step, 2^-9 for bf16 and 2^-11 for fp16)
-      const float f = KV8 ? (vref > 0.f ? s_vs[kk] / vref : 0.f) : 1.f;
-      const uint32_t a0 = Elt<M>::pack2(s[2 * kk][0] * f, s[2 * kk][1] * f);
-      const uint32_t a1 = Elt<M>::pack2(s[2 * kk][2] * f, s[2 * kk][3] * f);
-      const uint32_t a2 = Elt<M>::pack2(s[2 * kk + 1][0] * f, s[2 * kk + 1][1] * f);
-      const uint32_t a3 = Elt<M>::pack2(s[2 * kk + 1][2] * f, s[2 * kk + 1][3] * f);
-#pragma unroll
-      for (int j = 0; j < D / 8; j += 2) {
-        const int row = kk * 16 + (lane & 15), ch = j + (lane >> 4);
-        uint32_t r[4];
-        ldmatrix_x4_trans(r, smem_u32(&sv[row * CH + (ch ^ (row & 7))]));
-        mma16816<M>(o[j], a0, a1, a2, a3, r[0], r[1]);
-        mma16816<M>(o[j + 1], a0, a1, a2, a3, r[2], r[3]);
+            for (int e = 0; e < 16; ++e)
+              *reinterpret_cast<float2*>(part + 2 + c * 32 + 2 * e) = make_float2(o[2 * e], o[2 * e + 1]);
+          }
+        }
       }
     }
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(MUI_FULL_MASK, l[h], 1);
-    l[h] += __shfl_xor_sync(MUI_FULL_MASK, l[h], 2);
-    const int r = r0 + warp * 16 + g + 8 * h;
-    if (r >= R) continue;
-    const float inv = (l[h] != 0.f ? 1.f / l[h] : 0.f) * (KV8 ? vref : 1.f);
-    uint32_t* out = reinterpret_cast<uint32_t*>(a.out) +
-                    (static_cast<size_t>(first + r / a.G) * a.Hq + kvh * a.G + r % a.G) * (D / 2);
-#pragma unroll
-    for (int j = 0; j < D / 8; ++j) out[j * 4 + tq] = Elt<T>::pack2(o[j][2 * h] * inv, o[j][2 * h + 1] * inv);
+  tc_before();
+  __syncthreads();
+  if (warp == PT_MMA_WARP) {
+    tc_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
+}
+
+// Joins the splits of the prompt kernel in order: a warp per (new token, query head).
+template <typename T, int D>
+__global__ void __launch_bounds__(PA_THREADS) paged_prompt_merge_kernel(const PaArgs a) {
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * PA_WARPS + (threadIdx.x >> 5);
+  const int tok = static_cast<int>(row / a.Hq), head = static_cast<int>(row % a.Hq);
+  int active = 0;
+  if (tok < a.kv.total) {
+    int b = tok;
+    const int32_t* cu = a.kv.cu;
+    if (cu != nullptr) b = warp_count_le(a.kv.batch, tok, [&](int k) { return __ldcg(cu + 1 + k); });
+    if (b < a.kv.batch) {
+      int first, count;
+      paged_new_tokens(a.kv, b, first, count);
+      const int x = ((tok - first) * a.G + head % a.G) / PT_ROWS;
+      PromptTile t;
+      const int start = cu != nullptr ? static_cast<int>(static_cast<long long>(__ldcg(cu + b)) * a.G / PT_ROWS) + b : b;
+      if (prompt_tile(a, start + x, t)) active = t.active;
+    }
+  }
+  pdl_wait_prior_grid();  // every thread, also one without work: this grid must not be done before the attention kernel is
+  if (active <= 1) return;
+  const float* p = a.partials + static_cast<size_t>(row) * a.splits * (D + 2);
+  float m[PT_MAX_SPLITS], mm = -INFINITY;
+#pragma unroll
+  for (int s = 0; s < PT_MAX_SPLITS; ++s) {
+    m[s] = s < active ? __ldcg(p + s * (D + 2)) : -INFINITY;
+    mm = fmaxf(mm, m[s]);
+  }
+  const float use = mm == -INFINITY ? 0.f : mm;
+  float l = 0.f, o[D / 32] = {};
+#pragma unroll
+  for (int s = 0; s < PT_MAX_SPLITS; ++s) {
+    if (s >= active) break;
+    const float f = ex2(m[s] - use);
+    l = fmaf(__ldcg(p + s * (D + 2) + 1), f, l);
+#pragma unroll
+    for (int e = 0; e < D / 64; ++e) {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(p + s * (D + 2) + 2) + e * 32 + lane);
+      o[2 * e] = fmaf(v.x, f, o[2 * e]);
+      o[2 * e + 1] = fmaf(v.y, f, o[2 * e + 1]);
+    }
+  }
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  uint32_t* out = reinterpret_cast<uint32_t*>(a.out) + static_cast<size_t>(row) * (D / 2);
+#pragma unroll
+  for (int e = 0; e < D / 64; ++e) out[e * 32 + lane] = Elt<T>::pack2(o[2 * e] * inv, o[2 * e + 1] * inv);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------------------------------
-// rows per block of the decode kernel: one block of eight, else blocks of sixteen
-int pa_block_rows(int G, int max_new) { return G * max_new <= 8 ? 8 : 16; }
-// CTAs of the decode kernel: as many as fit the GPU at once, fewer when the longest sequence expected leaves them without
-// PA_MIN_TILES tiles each
-int pa_ctas(int sm_count, int batch, int kv_heads, int G, int max_new, int max_context, int window, int sinks) {
+// What a call launches and the scratch it needs, from sizes alone.
+struct PaPlan {
+  // Up to 32 rows per sequence: the decode kernel; more: the prompt kernel. Where short and long sequences can meet in one call
+  // both run, each on its own (mixed).
+  bool decode, prompt;
+  int block, row_blocks, ctas;  // decode: rows per block (8, else blocks of 16)
+  int tiles, splits;            // prompt
+  size_t decode_bytes, bytes;
+};
+bool pa_plan(const MuiDeviceInfo& di, int total, int batch, int Hq, int kv_heads, int D, int max_new, int max_context,
+             int window, int sinks, PaPlan& p) {
+  const int G = Hq / kv_heads;
   long long span = max_context;
   if (window > 0) span = std::min<long long>(span, static_cast<long long>(window) + max_new + sinks);
-  const int block = pa_block_rows(G, max_new);
-  const long long tiles = ((span + PA_TILE - 1) / PA_TILE + 2) * batch * kv_heads * ((G * max_new + block - 1) / block);
-  const long long most = static_cast<long long>(sm_count) * (block == 8 ? 3 : 2);
-  return static_cast<int>(std::max<long long>(1, std::min(most, (tiles + PA_MIN_TILES - 1) / PA_MIN_TILES)));
+  p = {};
+  p.prompt = static_cast<long long>(G) * max_new > PA_MAX_DECODE_ROWS;
+  // at least one short sequence fits beside sequences of max_new tokens only if the total leaves room for it
+  p.decode = !p.prompt ||
+             (batch > 1 && total <= static_cast<long long>(batch - 1) * max_new + PA_MAX_DECODE_ROWS / G);
+  if (p.decode) {
+    const int rows = p.prompt ? PA_MAX_DECODE_ROWS : G * max_new;
+    p.block = rows <= 8 ? 8 : 16;
+    p.row_blocks = (rows + p.block - 1) / p.block;
+    const long long pairs = static_cast<long long>(batch) * kv_heads * p.row_blocks;
+    if (pairs * p.block > 0x7fffffff) return false;
+    // as many CTAs as fit the GPU at once, fewer when the longest sequence expected leaves them without PA_MIN_TILES tiles each
+    const long long tiles = ((span + PA_TILE - 1) / PA_TILE + 2) * pairs;
+    const long long most = static_cast<long long>(di.sm_count) * (p.block == 8 ? 3 : 2);
+    p.ctas = static_cast<int>(std::max<long long>(1, std::min(most, (tiles + PA_MIN_TILES - 1) / PA_MIN_TILES)));
+    if (p.ctas > 1) p.decode_bytes = (static_cast<size_t>(p.ctas) * 2 * p.block * (D + 2) * sizeof(float) + 255) / 256 * 256;
+  }
+  p.bytes = p.decode_bytes;
+  if (p.prompt) {
+    const long long tiles = static_cast<long long>(total) * G / PT_ROWS + batch;
+    if (tiles > 0x7fffffff) return false;
+    p.tiles = static_cast<int>(tiles);
+    // the rows' spans are split where whole ones would leave SMs idle
+    const long long fit = di.sm_count / std::max<long long>(1, tiles * kv_heads);
+    p.splits = static_cast<int>(std::max<long long>(1, std::min<long long>({fit, span / (2 * PT_KEYS), PT_MAX_SPLITS})));
+    if (p.splits > 1) p.bytes += static_cast<size_t>(total) * Hq * p.splits * (D + 2) * sizeof(float);
+  }
+  return true;
 }
-size_t pa_workspace(int ctas, int block, int D) {
-  return ctas == 1 ? 0 : static_cast<size_t>(ctas) * 2 * block * (D + 2) * sizeof(float);
-}
-
-bool pa_decode(int G, int max_new) { return static_cast<long long>(G) * max_new <= PA_MAX_DECODE_ROWS; }
 
 template <typename T, bool KV8, int D, int NT>
 mui_status_t launch_decode(cudaStream_t stream, const PaArgs& a, int pdl, int device) {
@@ -1026,16 +1396,37 @@ mui_status_t launch_decode(cudaStream_t stream, const PaArgs& a, int pdl, int de
 }
 
 template <typename T, bool KV8, int D>
-mui_status_t launch_attention(cudaStream_t stream, const PaArgs& a, int pdl, int device) {
-  if (pa_decode(a.G, a.max_new))
-    return pa_block_rows(a.G, a.max_new) == 8 ? launch_decode<T, KV8, D, 1>(stream, a, pdl, device)
-                                              : launch_decode<T, KV8, D, 2>(stream, a, pdl, device);
-  const long long tiles = a.kv.cu ? static_cast<long long>(a.kv.total) * a.G / PP_ROWS + a.kv.batch
-                                  : static_cast<long long>(a.kv.batch) * ((a.G + PP_ROWS - 1) / PP_ROWS);
-  MUI_REQUIRE(tiles <= 0x7fffffff, MUI_ERR_UNSUPPORTED, "too many rows");
-  MUI_CUDA_CHECK(mui_launch(paged_prompt_kernel<T, KV8, D>, dim3(static_cast<unsigned>(tiles), a.kv.kv_heads),
-                            dim3(PA_THREADS), 0, stream, pdl, a));
+mui_status_t launch_prompt(cudaStream_t stream, const PaArgs& a, int tiles, int pdl, int device) {
+  constexpr size_t smem = 2 * PT_GROUP * D * 2 + PT_SLOTS * PT_KEYS * D * 2 + 1024;
+  static std::atomic<unsigned long long> configured{0};  // one bit per device
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(configured.load() & bit)) {
+    MUI_CUDA_CHECK(cudaFuncSetAttribute(paged_prompt_kernel<T, KV8, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        static_cast<int>(smem)));
+    configured.fetch_or(bit);
+  }
+  MUI_CUDA_CHECK(mui_launch(paged_prompt_kernel<T, KV8, D>, dim3(tiles, a.kv.kv_heads, a.splits), dim3(PT_THREADS), smem,
+                            stream, pdl, a));
+  if (a.splits > 1) {
+    const long long rows = static_cast<long long>(a.kv.total) * a.Hq;
+    MUI_CUDA_CHECK(mui_launch(paged_prompt_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + PA_WARPS - 1) / PA_WARPS)),
+                              dim3(PA_THREADS), 0, stream, 1, a));
+  }
   return MUI_OK;
+}
+
+template <typename T, bool KV8, int D>
+mui_status_t launch_attention(cudaStream_t stream, PaArgs a, const PaPlan& p, void* workspace, int pdl, int device) {
+  if (p.decode) {
+    a.partials = reinterpret_cast<float*>(workspace);
+    const mui_status_t s = p.block == 8 ? launch_decode<T, KV8, D, 1>(stream, a, pdl, device)
+                                        : launch_decode<T, KV8, D, 2>(stream, a, pdl, device);
+    if (s != MUI_OK) return s;
+    pdl = 0;
+  }
+  if (!p.prompt) return MUI_OK;
+  a.partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + p.decode_bytes);
+  return launch_prompt<T, KV8, D>(stream, a, p.tiles, pdl, device);
 }
 
 }  // namespace
@@ -1047,12 +1438,12 @@ size_t mui_paged_attention_workspace_bytes(int total_tokens, int batch, int num_
   if (total_tokens <= 0 || batch <= 0 || num_q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || max_new_tokens <= 0 ||
       max_context <= 0)
     return 0;
-  if (!pa_decode(num_q_heads / kv_heads, max_new_tokens)) return 0;
   const MuiDeviceInfo* di = mui_current_device_info();
-  if (!di) return 0;
-  const int G = num_q_heads / kv_heads;
-  return pa_workspace(pa_ctas(di->sm_count, batch, kv_heads, G, max_new_tokens, max_context, window, sinks),
-                      pa_block_rows(G, max_new_tokens), head_dim);
+  PaPlan p;
+  if (num_q_heads < kv_heads || !di ||
+      !pa_plan(*di, total_tokens, batch, num_q_heads, kv_heads, head_dim, max_new_tokens, max_context, window, sinks, p))
+    return 0;
+  return p.bytes;
 }
 
 mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_paged_kv_t* cache, int num_q_heads,
@@ -1084,27 +1475,26 @@ mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_page
   a.window = window;
   a.sinks = sinks;
   a.scale_log2 = scale * 1.44269504088896341f;
-  a.ctas = a.row_blocks = 1;
   // a tile is 16 rows of K and of V
   a.lead = PA_TRIPLE_COST * 4096 / (2 * PA_TILE * cache->head_dim * (cache->format == MUI_KV_E4M3 ? 1 : 2));
-  if (pa_decode(G, max_new_tokens)) {
-    const int block = pa_block_rows(G, max_new_tokens);
-    a.row_blocks = (G * max_new_tokens + block - 1) / block;
-    a.ctas = pa_ctas(di->sm_count, cache->batch, cache->kv_heads, G, max_new_tokens, max_context, window, sinks);
-    const size_t need = pa_workspace(a.ctas, block, cache->head_dim);
-    MUI_REQUIRE(static_cast<long long>(cache->batch) * cache->kv_heads * a.row_blocks * block <= 0x7fffffff, MUI_ERR_UNSUPPORTED,
-                "batch=%d times kv_heads=%d is too large", cache->batch, cache->kv_heads);
-    MUI_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need &&
-                              (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
-                MUI_ERR_INVALID_ARG, "workspace of %zu bytes (16-byte aligned) needed, %zu given", need,
-                workspace ? workspace_bytes : static_cast<size_t>(0));
-    a.partials = reinterpret_cast<float*>(workspace);
-  }
+  PaPlan p;
+  MUI_REQUIRE(pa_plan(*di, cache->total_tokens, cache->batch, num_q_heads, cache->kv_heads, cache->head_dim, max_new_tokens,
+                      max_context, window, sinks, p),
+              MUI_ERR_UNSUPPORTED, "batch=%d, total_tokens=%d and kv_heads=%d are too large", cache->batch,
+              cache->total_tokens, cache->kv_heads);
+  MUI_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes &&
+                               (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+              MUI_ERR_INVALID_ARG, "workspace of %zu bytes (16-byte aligned) needed, %zu given", p.bytes,
+              workspace ? workspace_bytes : static_cast<size_t>(0));
+  a.row_blocks = p.row_blocks;
+  a.ctas = p.ctas;
+  a.splits = p.splits;
+  a.mixed = p.decode && p.prompt;
   const int pdl = (flags & MUI_FLAG_PDL) ? 1 : 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define PA_GO(T, D)                                                            \
-  (cache->format == MUI_KV_E4M3 ? launch_attention<T, true, D>(st, a, pdl, di->device) \
-                                : launch_attention<T, false, D>(st, a, pdl, di->device))
+  (cache->format == MUI_KV_E4M3 ? launch_attention<T, true, D>(st, a, p, workspace, pdl, di->device) \
+                                : launch_attention<T, false, D>(st, a, p, workspace, pdl, di->device))
   if (dtype == MUI_F16) return cache->head_dim == 128 ? PA_GO(__half, 128) : PA_GO(__half, 64);
   return cache->head_dim == 128 ? PA_GO(__nv_bfloat16, 128) : PA_GO(__nv_bfloat16, 64);
 #undef PA_GO

@@ -532,76 +532,90 @@ def muillm_add_tokens_check_finished(input_ids, next_tokens, unfinished_sequence
 
 
 # ---- paged KV cache and sampling --------------------------------------------------------------------------------
+# One call of these costs the GPU a few microseconds, so the checks below are written to cost the host as little: conditions
+# in line, and a function that finds the words for the error only where one fails.
+
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+_CODES = {torch.float16: capi.MUI_F16, torch.bfloat16: capi.MUI_BF16, torch.float32: capi.MUI_COMM_F32}
 
 
-def _check_on(device, t, name, dtype):
-    """t must be a contiguous `dtype` tensor on CUDA device number `device`."""
+def _refuse(t, name, device, dtype, shape=None):
+    """Raises the error of a tensor that is not a contiguous `dtype` tensor [of `shape`] on CUDA device `device`."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
     if t.get_device() != device:
-        raise RuntimeError(f"{name} must be on CUDA device {device}, the device of the other tensors")
+        raise RuntimeError(f"{name} must be on CUDA device {device}, the current device and the one of the other tensors")
     if t.dtype != dtype:
         raise RuntimeError(f"{name} must be of type {dtype}, got {t.dtype}")
-    if not t.is_contiguous():
-        raise RuntimeError(f"{name} must be contiguous")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    raise RuntimeError(f"{name} must be contiguous")
 
 
-def _current_device_of(t, name):
+def _device_of(t, name):
     device = t.get_device()
-    if device < 0:
-        raise RuntimeError(f"{name} must be a CUDA tensor")
-    if device != torch.cuda.current_device():
-        raise RuntimeError(f"{name} is on CUDA device {device}, which is not the current one")
+    if device < 0 or device != torch.cuda.current_device():
+        _refuse(t, name, torch.cuda.current_device() if t.is_cuda else -1, None)
     return device
 
 
-def _check_rows3(device, t, name, total, heads, dim, dtype):
-    """A [total, heads, dim] view whose innermost stride is 1; returns its strides."""
-    if t.get_device() != device:
-        raise RuntimeError(f"{name} must be on CUDA device {device}, the device of the other tensors")
-    if t.dtype != dtype:
-        raise RuntimeError(f"{name} must be of type {dtype}, got {t.dtype}")
-    if t.dim() != 3 or t.shape[0] != total or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise RuntimeError(f"{name} must be [{total}, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
-    s = t.stride()
-    if s[2] != 1 and t.numel():
+def _rows3(device, t, name, total, heads, dim, dtype):
+    """Strides of a [total, heads, dim] view whose innermost stride is 1."""
+    if t.get_device() != device or t.dtype != dtype:
+        _refuse(t, name, device, dtype)
+    if t.shape != (total, heads, dim):
+        raise RuntimeError(f"{name} must be [{total}, {heads}, {dim}], got {list(t.shape)}")
+    tok, head, inner = t.stride()
+    if inner != 1 and total and heads:
         raise RuntimeError(f"{name} must have innermost stride 1")
-    return capi.Strides2(s[0], s[1])
+    return capi.Strides2(tok, head)
 
 
 def _paged_kv(device, dtype, total, k_pages, v_pages, block_table, context_lens, cu_tokens, k_scales, v_scales):
     """Checks the tensors of a paged cache and describes them for the C ABI."""
-    if k_pages.dim() != 4:
+    shape = k_pages.shape
+    if len(shape) != 4:
         raise RuntimeError("pages must be [num_pages, kv_heads, page_size, head_dim]")
-    num_pages, kv_heads, page_size, head_dim = k_pages.shape
-    if v_pages.shape != k_pages.shape:
-        raise RuntimeError("k_pages and v_pages must have the same shape")
+    num_pages, kv_heads, page_size, head_dim = shape
     e4m3 = k_pages.dtype == torch.float8_e4m3fn
     page_dtype = torch.float8_e4m3fn if e4m3 else dtype
-    _check_on(device, k_pages, "k_pages", page_dtype)
-    _check_on(device, v_pages, "v_pages", page_dtype)
+    if k_pages.get_device() != device or k_pages.dtype != page_dtype or not k_pages.is_contiguous():
+        _refuse(k_pages, "k_pages", device, page_dtype)
+    if (v_pages.get_device() != device or v_pages.dtype != page_dtype or v_pages.shape != shape
+            or not v_pages.is_contiguous()):
+        _refuse(v_pages, "v_pages", device, page_dtype, shape)
+    ks = vs = None
     if e4m3:
         if k_scales is None or v_scales is None:
             raise RuntimeError("float8_e4m3fn pages need k_scales and v_scales")
-        _check_on(device, k_scales, "k_scales", torch.float32)
-        _check_on(device, v_scales, "v_scales", torch.float32)
-        if k_scales.shape != (num_pages, kv_heads) or v_scales.shape != (num_pages, kv_heads):
-            raise RuntimeError(f"scales must be [{num_pages}, {kv_heads}]")
+        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            if (t.get_device() != device or t.dtype != torch.float32 or t.shape != (num_pages, kv_heads)
+                    or not t.is_contiguous()):
+                _refuse(t, name, device, torch.float32, (num_pages, kv_heads))
+        ks, vs = k_scales.data_ptr(), v_scales.data_ptr()
     elif k_scales is not None or v_scales is not None:
         raise RuntimeError("16-bit pages take no scales")
-    _check_on(device, context_lens, "context_lens", torch.int32)
-    _check_on(device, block_table, "block_table", torch.int32)
-    batch = context_lens.shape[0]
-    if context_lens.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != batch:
+    if context_lens.dim() != 1 or block_table.dim() != 2 or block_table.shape[0] != context_lens.shape[0]:
         raise RuntimeError("context_lens must be [batch] and block_table [batch, pages]")
+    batch, table_stride = block_table.shape
+    if context_lens.get_device() != device or context_lens.dtype != torch.int32 or not context_lens.is_contiguous():
+        _refuse(context_lens, "context_lens", device, torch.int32)
+    if block_table.get_device() != device or block_table.dtype != torch.int32 or not block_table.is_contiguous():
+        _refuse(block_table, "block_table", device, torch.int32)
+    cu = None
     if cu_tokens is not None:
-        _check_on(device, cu_tokens, "cu_tokens", torch.int32)
-        if cu_tokens.shape != (batch + 1,):
-            raise RuntimeError(f"cu_tokens must be [{batch + 1}]")
+        if (cu_tokens.get_device() != device or cu_tokens.dtype != torch.int32 or cu_tokens.shape != (batch + 1,)
+                or not cu_tokens.is_contiguous()):
+            _refuse(cu_tokens, "cu_tokens", device, torch.int32, (batch + 1,))
+        cu = cu_tokens.data_ptr()
     elif total != batch:
         raise RuntimeError(f"without cu_tokens there is one new token per sequence: {total} rows for {batch} sequences")
     return capi.PagedKV(
-        capi.MUI_KV_E4M3 if e4m3 else capi.MUI_KV_16BIT, num_pages, page_size, kv_heads, head_dim, batch,
-        block_table.shape[1], total, k_pages.data_ptr(), v_pages.data_ptr(), _ptr(k_scales), _ptr(v_scales),
-        block_table.data_ptr(), context_lens.data_ptr(), _ptr(cu_tokens))
+        capi.MUI_KV_E4M3 if e4m3 else capi.MUI_KV_16BIT, num_pages, page_size, kv_heads, head_dim, batch, table_stride,
+        total, k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, block_table.data_ptr(), context_lens.data_ptr(), cu)
 
 
 def paged_kv_append(k_pages, v_pages, block_table, context_lens, q, k, v, freqs=None, cu_tokens=None, rotary_dim=None,
@@ -616,36 +630,42 @@ def paged_kv_append(k_pages, v_pages, block_table, context_lens, q, k, v, freqs=
     None. freqs [positions, rotary_dim / 2, 2] fp32 holds (cos, sin) pairs; the first rotary_dim elements of a head
     (default: as many as freqs has) are turned in the half or the interleaved layout; position_ids [total] int64 stands
     in for the cache positions as rotary positions. mui_paged_kv_append in the C ABI."""
-    device = _current_device_of(k, "k")
+    device, dtype = _device_of(k, "k"), k.dtype
+    if dtype not in _CODES:
+        _dtype_code(k)
     total = k.shape[0]
-    if k.dim() != 3 or k_pages.dim() != 4:
-        raise RuntimeError("k must be [total, kv_heads, head_dim] and pages [num_pages, kv_heads, page_size, head_dim]")
-    kv = _paged_kv(device, k.dtype, total, k_pages, v_pages, block_table, context_lens, cu_tokens, k_scales, v_scales)
-    D = kv.head_dim
-    ks = _check_rows3(device, k, "k", total, kv.kv_heads, D, k.dtype)
-    vs = _check_rows3(device, v, "v", total, kv.kv_heads, D, k.dtype)
-    heads, qs = 0, ks
+    kv = _paged_kv(device, dtype, total, k_pages, v_pages, block_table, context_lens, cu_tokens, k_scales, v_scales)
+    hkv, dim = kv.kv_heads, kv.head_dim
+    ks, vs = _rows3(device, k, "k", total, hkv, dim, dtype), _rows3(device, v, "v", total, hkv, dim, dtype)
+    heads, qs, q_ptr, out_ptr = 0, ks, None, None
     if q is not None:
-        heads, qs = q.shape[1], _check_rows3(device, q, "q", total, None, D, k.dtype)
+        if q.dim() != 3:
+            raise RuntimeError("q must be [total, heads, head_dim]")
+        heads = q.shape[1]
+        qs, q_ptr = _rows3(device, q, "q", total, heads, dim, dtype), q.data_ptr()
         if q_out is None:
-            q_out = torch.empty((total, heads, D), dtype=k.dtype, device=k.device)
-        else:
-            _check_on(device, q_out, "q_out", k.dtype)
-            if q_out.shape != (total, heads, D):
-                raise RuntimeError(f"q_out must be [{total}, {heads}, {D}]")
-    max_pos = rot = 0
+            q_out = k.new_empty((total, heads, dim))
+        elif (q_out.get_device() != device or q_out.dtype != dtype or q_out.shape != (total, heads, dim)
+              or not q_out.is_contiguous()):
+            _refuse(q_out, "q_out", device, dtype, (total, heads, dim))
+        out_ptr = q_out.data_ptr()
+    max_pos, rot, freqs_ptr, pos_ptr = 0, 0, None, None
     if freqs is not None:
-        _check_on(device, freqs, "freqs", torch.float32)
+        if freqs.get_device() != device or freqs.dtype != torch.float32 or not freqs.is_contiguous():
+            _refuse(freqs, "freqs", device, torch.float32)
         if freqs.dim() != 3 or freqs.shape[2] != 2 or (rotary_dim is not None and rotary_dim != 2 * freqs.shape[1]):
             raise RuntimeError("freqs must be [positions, rotary_dim / 2, 2]")
-        max_pos, rot = freqs.shape[0], 2 * freqs.shape[1]
+        max_pos, rot, freqs_ptr = freqs.shape[0], 2 * freqs.shape[1], freqs.data_ptr()
     if position_ids is not None:
-        _check_on(device, position_ids, "position_ids", torch.int64)
-        if position_ids.shape != (total,):
-            raise RuntimeError(f"position_ids must be [{total}]")
-    capi.check(capi.lib().mui_paged_kv_append(
-        _stream(), _dtype_code(k), ctypes.byref(kv), heads, _ptr(freqs), max_pos, rot, 1 if interleaved else 0,
-        _ptr(position_ids), _ptr(q), qs, k.data_ptr(), ks, v.data_ptr(), vs, _ptr(q_out), flags))
+        if (position_ids.get_device() != device or position_ids.dtype != torch.int64 or position_ids.shape != (total,)
+                or not position_ids.is_contiguous()):
+            _refuse(position_ids, "position_ids", device, torch.int64, (total,))
+        pos_ptr = position_ids.data_ptr()
+    status = capi.lib().mui_paged_kv_append(
+        _raw_stream(device), _CODES[dtype], ctypes.byref(kv), heads, freqs_ptr, max_pos, rot, 1 if interleaved else 0,
+        pos_ptr, q_ptr, qs, k.data_ptr(), ks, v.data_ptr(), vs, out_ptr, flags)
+    if status:
+        capi.check(status)
     return q_out
 
 
@@ -655,32 +675,36 @@ def paged_attention(q, k_pages, v_pages, block_table, context_lens, cu_tokens=No
     of the same description). q [total, Hq, head_dim] (a view with innermost stride 1), the cache tensors, context_lens
     and cu_tokens as in paged_kv_append; max_new_tokens bounds the new tokens of every sequence (default: 1 without
     cu_tokens, else total). window > 0 limits a token at position p to the rows j > p - window and the first `sinks`
-    rows. max_context is the longest sequence expected, a hint for the split of the work (default: the block table's
-    reach). Returns [total, Hq, head_dim]. mui_paged_attention in the C ABI."""
-    device = _current_device_of(q, "q")
-    total = q.shape[0]
-    kv = _paged_kv(device, q.dtype, total, k_pages, v_pages, block_table, context_lens, cu_tokens, k_scales, v_scales)
-    D = kv.head_dim
-    qs = _check_rows3(device, q, "q", total, None, D, q.dtype)
-    heads = q.shape[1]
+    rows. max_context is the longest sequence expected, a hint for the number of CTAs (default: the block table's reach).
+    Returns [total, Hq, head_dim]. mui_paged_attention in the C ABI."""
+    device, dtype = _device_of(q, "q"), q.dtype
+    if dtype not in _CODES:
+        _dtype_code(q)
+    if q.dim() != 3:
+        raise RuntimeError("q must be [total, heads, head_dim]")
+    total, heads = q.shape[0], q.shape[1]
+    kv = _paged_kv(device, dtype, total, k_pages, v_pages, block_table, context_lens, cu_tokens, k_scales, v_scales)
+    dim = kv.head_dim
+    qs = _rows3(device, q, "q", total, heads, dim, dtype)
     if out is None:
-        out = torch.empty((total, heads, D), dtype=q.dtype, device=q.device)
-    else:
-        _check_on(device, out, "out", q.dtype)
-        if out.shape != (total, heads, D):
-            raise RuntimeError(f"out must be [{total}, {heads}, {D}]")
+        out = q.new_empty((total, heads, dim))
+    elif (out.get_device() != device or out.dtype != dtype or out.shape != (total, heads, dim)
+          or not out.is_contiguous()):
+        _refuse(out, "out", device, dtype, (total, heads, dim))
     if max_new_tokens is None:
         max_new_tokens = 1 if cu_tokens is None else max(1, total)
     if max_context is None:
         max_context = kv.table_stride * kv.page_size
     lib = capi.lib()
     # scratch of its own for every call: calls on several streams, or captured in several graphs, share nothing
-    nbytes = lib.mui_paged_attention_workspace_bytes(total, kv.batch, heads, kv.kv_heads, D, max_new_tokens, max_context,
+    nbytes = lib.mui_paged_attention_workspace_bytes(total, kv.batch, heads, kv.kv_heads, dim, max_new_tokens, max_context,
                                                      window, sinks)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    capi.check(lib.mui_paged_attention(
-        _stream(), _dtype_code(q), ctypes.byref(kv), heads, max_new_tokens, max_context, window, sinks,
-        scale if scale is not None else 1.0 / math.sqrt(D), q.data_ptr(), qs, out.data_ptr(), _ptr(ws), nbytes, flags))
+    ws = q.new_empty(nbytes // 2) if nbytes else None
+    status = lib.mui_paged_attention(
+        _raw_stream(device), _CODES[dtype], ctypes.byref(kv), heads, max_new_tokens, max_context, window, sinks,
+        scale if scale is not None else dim ** -0.5, q.data_ptr(), qs, out.data_ptr(), _ptr(ws), nbytes, flags)
+    if status:
+        capi.check(status)
     return out
 
 
@@ -691,20 +715,29 @@ def sample_tokens(logits, uniforms, temperature=None, top_k=None, top_p=None, mi
     the first one in index order at which the running probability exceeds the uniform number. Parameters are per-row
     tensors on the device (fp32; top_k int32) or None for off; a temperature of 0 takes the largest logit. Returns
     (tokens int64 [rows], logprobs fp32 [rows] of the drawn tokens among the kept ones). mui_sample_tokens in the C ABI."""
-    device = _current_device_of(logits, "logits")
+    device, dtype = _device_of(logits, "logits"), logits.dtype
+    if dtype not in _CODES:
+        raise RuntimeError(f"Unsupported dtype {dtype} (float16, bfloat16 or float32 expected)")
     if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise RuntimeError("logits must be [rows, vocab] with innermost stride 1")
     rows, vocab = logits.shape
-    code = capi.MUI_COMM_F32 if logits.dtype == torch.float32 else _dtype_code(logits)
-    for t, name in ((uniforms, "uniforms"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"),
-                    (top_k, "top_k")):
-        if t is not None:
-            _check_on(device, t, name, torch.int32 if name == "top_k" else torch.float32)
-            if t.shape != (rows,):
-                raise RuntimeError(f"{name} must be [{rows}]")
-    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
-    capi.check(capi.lib().mui_sample_tokens(
-        _stream(), code, rows, vocab, logits.data_ptr(), logits.stride(0), _ptr(temperature), _ptr(top_k), _ptr(top_p),
-        _ptr(min_p), uniforms.data_ptr(), tokens.data_ptr(), logprobs.data_ptr(), flags))
+
+    def ptr(t, name, dt):
+        if t is None:
+            return None
+        if t.get_device() != device or t.dtype != dt or t.shape != (rows,) or not t.is_contiguous():
+            _refuse(t, name, device, dt, (rows,))
+        return t.data_ptr()
+
+    f32 = torch.float32
+    if uniforms is None:
+        raise RuntimeError("uniforms must be given")
+    tokens = logits.new_empty(rows, dtype=torch.int64)
+    logprobs = logits.new_empty(rows, dtype=f32)
+    status = capi.lib().mui_sample_tokens(
+        _raw_stream(device), _CODES[dtype], rows, vocab, logits.data_ptr(), logits.stride(0),
+        ptr(temperature, "temperature", f32), ptr(top_k, "top_k", torch.int32), ptr(top_p, "top_p", f32),
+        ptr(min_p, "min_p", f32), ptr(uniforms, "uniforms", f32), tokens.data_ptr(), logprobs.data_ptr(), flags)
+    if status:
+        capi.check(status)
     return tokens, logprobs
