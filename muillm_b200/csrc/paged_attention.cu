@@ -31,6 +31,7 @@ struct PaArgs {
   void* out;
   float* partials;  // [ctas, 2, rows per block, D + 2]: maximum, sum, unnormalised output
   int Hq, G, ctas, row_blocks, splits, mixed, lead, max_new, window, sinks, q_vec;
+  uint32_t q_flip;  // sign bits turned over in q
   float scale_log2;
 };
 
@@ -363,7 +364,12 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
 #pragma unroll
         for (int e = 0; e < KS / 2; ++e) {
           float x[8];
-          unpack8<T>(q_raw[n][c][e], x);
+          uint4 w = q_raw[n][c][e];
+          w.x ^= a.q_flip;
+          w.y ^= a.q_flip;
+          w.z ^= a.q_flip;
+          w.w ^= a.q_flip;
+          unpack8<T>(w, x);
 #pragma unroll
           for (int h = 0; h < 8; ++h) {
             qv[c][8 * e + h] = x[h];
@@ -752,7 +758,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
 //   P_g = exp2(S_g * scale - reference)   one thread per row, tensor memory to tensor memory, P over S
 //   O_g += P_g V     (128 x D, K = 128)   P from tensor memory, V as it lies in the cache (its head dims contiguous: MN-major)
 // All of tensor memory is taken: S 2 x 128 columns, O 2 x D columns. One thread issues the MMAs, two warpgroups (one per group
-// of rows) take the softmax, four warps bring K and V (16-bit pages: asynchronous copies; e4m3 pages: converted to fp16, exact, on
+// of rows) take the softmax, three warps bring K and V (16-bit pages: asynchronous copies; e4m3 pages: converted to fp16, exact, on
 // the way) into a ring of four 128-row tiles. While one group's softmax runs, the tensor cores work for the other.
 //
 // The reference of a row's exponents is its running maximum, but moves only when the maximum is more than 8 (a factor 256)
@@ -762,9 +768,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
 constexpr int PT_ROWS = 256, PT_GROUP = 128, PT_KEYS = 128;
 constexpr int PT_SUB = PT_KEYS / PA_TILE;          // 16-row tiles of a step
 constexpr int PT_SLOTS = 4;                        // ring of K and V tiles
-constexpr int PT_MMA_WARP = 8, PT_LOAD_WARP = 9, PT_LOAD_WARPS = 4;
+constexpr int PT_MMA_WARP = 8, PT_LOAD_WARP = 9, PT_LOAD_WARPS = 3;
 constexpr int PT_LOADERS = PT_LOAD_WARPS * 32;
-constexpr int PT_THREADS = (PT_LOAD_WARP + PT_LOAD_WARPS) * 32;  // 416
+constexpr int PT_THREADS = (PT_LOAD_WARP + PT_LOAD_WARPS) * 32;  // 384: 168 registers a thread
 constexpr int PT_MAX_SPLITS = 16;
 constexpr float PT_SLACK = 8.f;
 
@@ -787,9 +793,8 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 32 consecutive 32-bit columns of this thread's tensor-memory lane
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-  uint32_t r[32];
+// 32 consecutive 32-bit columns of this thread's tensor-memory lane; there after tmem_load_wait
+__device__ __forceinline__ void tmem_ask32(uint32_t addr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
       "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -799,7 +804,22 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
         "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// the registers are named so that nothing that uses them moves above the wait
+__device__ __forceinline__ void tmem_load_wait(uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+        "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+        "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+        "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+      :
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_ask32(addr, r);
+  tmem_load_wait(r);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
@@ -911,12 +931,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
   // Q into shared memory: eight lanes (D = 64) or sixteen per row. e4m3 pages: as fp16, brought near 1 by a power of two per row.
   {
     constexpr int LPR = D / 8;
-    for (int i = tid; i < PT_ROWS * LPR; i += PT_THREADS) {  // 416 is a multiple of 16 and so is the row count: whole rows
+    for (int i = tid; i < PT_ROWS * LPR; i += PT_THREADS) {  // a row's lanes are neighbours in one warp, and whole warps take part
       const int r = i / LPR, ch = i % LPR, rr = t.r0 + r;
       uint4 w = make_uint4(0, 0, 0, 0);
       if (rr < t.R)
         w = load_q8<T>(reinterpret_cast<const T*>(a.q) + (t.first + rr / a.G) * a.qs.tok + (kvh * a.G + rr % a.G) * a.qs.head + ch * 8,
                        a.q_vec);
+      w.x ^= a.q_flip;
+      w.y ^= a.q_flip;
+      w.z ^= a.q_flip;
+      w.w ^= a.q_flip;
       if (KV8) {
         float x[8], amax = 0.f;
         unpack8<T>(w, x);
@@ -968,69 +992,92 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
 
   if (warp >= PT_LOAD_WARP) {
     // ------------------------------ K and V ------------------------------
-    const int lt = tid - PT_LOAD_WARP * 32;
+    const int lw = warp - PT_LOAD_WARP;
     constexpr int ES = KV8 ? 1 : 2, RB = D * ES, CPR = RB / 16;  // bytes and 16-byte chunks of a cache row
-    constexpr int IT = PT_KEYS * CPR / PT_LOADERS;               // chunks of a tile per thread
-    constexpr int RPI = PT_LOADERS / CPR;                        // rows per turn
-    const int ch = lt % CPR, row0 = lt / CPR;
+    constexpr int RPI = 32 / CPR;                                // rows a warp copies at a time
+    // A step is 16 units of eight rows; a warp takes every third one, so that addresses are worked out once per unit.
+    constexpr int UNITS = 2 * PT_SUB, TURNS = (UNITS + PT_LOAD_WARPS - 1) / PT_LOAD_WARPS, CPU = 8 / RPI;
+    const int ch = lane % CPR, row0 = lane / CPR;
+    // where this lane's chunks of a unit go: 16-bit chunk c of row r sits at block c / 8, row r, chunk (c % 8) ^ (r % 8)
+    auto place = [&](int r, int c) { return static_cast<uint32_t>((c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
+    uint32_t at[CPU][KV8 ? 2 : 1];
+#pragma unroll
+    for (int i = 0; i < CPU; ++i)
+#pragma unroll
+      for (int h = 0; h < (KV8 ? 2 : 1); ++h) at[i][h] = place(i * RPI + row0, KV8 ? 2 * ch + h : ch);
     int page, tb, next_page, next_tb;
     find_tile(0, page, tb, true);
-    uint4 hold[KV8 ? IT : 1];
     bool ok = true;
     for (int j = 0; j < n && ok; ++j) {
       next_page = next_tb = -1;
       if (j + 1 < n) find_tile(j + 1, next_page, next_tb, true);
-      for (int which = 0; which < 2 && ok; ++which) {
+#pragma unroll 1
+      for (int which = 0; which < 2; ++which) {
         const int it = 2 * j + which, slot = it % PT_SLOTS;
-        const unsigned char* base = reinterpret_cast<const unsigned char*>(which == 0 ? a.kv.k_pages : a.kv.v_pages) + ch * 16;
+        const unsigned char* pages = reinterpret_cast<const unsigned char*>(which == 0 ? a.kv.k_pages : a.kv.v_pages);
         const uint32_t dst = ring + slot * KT;
-        // e4m3: the loads do not need the slot
+        // calls f(turn, unit, lane's source, whole, first cache row) for the warp's units
+        auto units = [&](auto f) {
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-          const int row = i * RPI + row0, sub = row / PA_TILE;
-          const int pg = __shfl_sync(MUI_FULL_MASK, page, sub), b0 = __shfl_sync(MUI_FULL_MASK, tb, sub);
-          const int jr = b0 + (row & (PA_TILE - 1));
-          // rows that nobody of this tile sees are zeros: what they hold must not matter
-          const bool see = b0 >= 0 && jr < t.sp.kv_len && (jr >= t.sp.lo_min || jr < a.sinks);
-          const size_t at = ((static_cast<size_t>(max(pg, 0)) * a.kv.kv_heads + kvh) << a.kv.page_shift) +
-                            (max(b0, 0) & ((1 << a.kv.page_shift) - 1)) + (row & (PA_TILE - 1));
-          const unsigned char* src = base + at * RB;
-          if (KV8) {
-            hold[KV8 ? i : 0] = see ? ld_stream16(src) : make_uint4(0, 0, 0, 0);
-          } else {
-            if (i == 0 && it >= PT_SLOTS) {
-              ok = wait(&kv_empty[slot], it / PT_SLOTS - 1, 0x100 + slot);
-              ok = __all_sync(MUI_FULL_MASK, ok);
-              if (!ok) break;
-            }
-            copy16(dst + (ch >> 3) * BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4), src, see ? 16 : 0);
+          for (int k = 0; k < TURNS; ++k) {
+            const int u = k * PT_LOAD_WARPS + lw;
+            if (u >= UNITS) break;
+            const int pg = __shfl_sync(MUI_FULL_MASK, page, u >> 1), b0 = __shfl_sync(MUI_FULL_MASK, tb, u >> 1);
+            const int first = b0 < 0 ? -PA_TILE : b0 + (u & 1) * 8;
+            const size_t row = ((static_cast<size_t>(max(pg, 0)) * a.kv.kv_heads + kvh) << a.kv.page_shift) +
+                               (max(first, 0) & ((1 << a.kv.page_shift) - 1));
+            const bool whole = first >= 0 && first + 8 <= t.sp.kv_len && (first >= t.sp.lo_min || first + 8 <= a.sinks);
+            f(k, u, pages + (row + row0) * RB + ch * 16, whole, first);
           }
-        }
-        if (!ok) break;
+        };
+        // whether anybody of this tile sees a cache row; zeros stand for the others: what they hold must not matter
+        auto seen = [&](int first, int r) {
+          const int jr = first + r;
+          return first >= 0 && jr < t.sp.kv_len && (jr >= t.sp.lo_min || jr < a.sinks);
+        };
+        auto slot_free = [&]() {
+          if (it >= PT_SLOTS) ok = __all_sync(MUI_FULL_MASK, wait(&kv_empty[slot], it / PT_SLOTS - 1, 0x100 + slot));
+          return ok;
+        };
         if (KV8) {
-          if (it >= PT_SLOTS) {
-            ok = wait(&kv_empty[slot], it / PT_SLOTS - 1, 0x100 + slot);
-            ok = __all_sync(MUI_FULL_MASK, ok);
-            if (!ok) break;
-          }
+          uint4 hold[TURNS][CPU];  // requested before the slot is free
+          units([&](int k, int, const unsigned char* src, bool whole, int first) {
 #pragma unroll
-          for (int i = 0; i < (KV8 ? IT : 0); ++i) {
-            const int row = i * RPI + row0;
-            const uint32_t w[4] = {hold[i].x, hold[i].y, hold[i].z, hold[i].w};
+            for (int i = 0; i < CPU; ++i)
+              hold[k][i] = whole || seen(first, i * RPI + row0) ? ld_stream16(src + i * RPI * RB) : make_uint4(0, 0, 0, 0);
+          });
+          if (!slot_free()) break;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int c = 2 * ch + h;  // 16-bit chunk
-              const uint32_t at = dst + (c >> 3) * BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-              const uint32_t w0 = w[2 * h], w1 = w[2 * h + 1];
-              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(e4m3_to_half2((uint16_t)w0)),
-                           "r"(e4m3_to_half2((uint16_t)(w0 >> 16))), "r"(e4m3_to_half2((uint16_t)w1)),
-                           "r"(e4m3_to_half2((uint16_t)(w1 >> 16)))
-                           : "memory");
+          for (int k = 0; k < TURNS; ++k) {
+            const int u = k * PT_LOAD_WARPS + lw;
+            if (u >= UNITS) break;
+#pragma unroll
+            for (int i = 0; i < CPU; ++i) {
+              const uint32_t w[4] = {hold[k][i].x, hold[k][i].y, hold[k][i].z, hold[k][i].w};
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t w0 = w[2 * h], w1 = w[2 * h + 1];
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + u * 1024 + at[i][KV8 ? h : 0]),
+                             "r"(e4m3_to_half2((uint16_t)w0)), "r"(e4m3_to_half2((uint16_t)(w0 >> 16))),
+                             "r"(e4m3_to_half2((uint16_t)w1)), "r"(e4m3_to_half2((uint16_t)(w1 >> 16)))
+                             : "memory");
+              }
             }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           mbar_arrive(&kv_full[slot]);
         } else {
+          if (!slot_free()) break;
+          units([&](int, int u, const unsigned char* src, bool whole, int first) {
+            if (whole) {
+#pragma unroll
+              for (int i = 0; i < CPU; ++i) copy16(dst + u * 1024 + at[i][0], src + i * RPI * RB, 16);
+            } else {
+#pragma unroll
+              for (int i = 0; i < CPU; ++i)
+                copy16(dst + u * 1024 + at[i][0], src + i * RPI * RB, seen(first, i * RPI + row0) ? 16 : 0);
+            }
+          });
           copy_commit();
           if (it >= 2) {  // two tiles stay in flight
             copy_wait<2>();
@@ -1053,18 +1100,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
     if (lane == 0) {
       const int bf = std::is_same<M, __nv_bfloat16>::value;
       const uint32_t id_s = f16_idesc(bf, PT_KEYS, 0), id_o = f16_idesc(bf, D, 1);
+      // one thread issues: a descriptor per operand, its address field (16-byte units) moved on
       auto scores = [&](int g, int slot) {
+        const uint64_t da = sw128_desc(tiles + g * QT, 16), db = sw128_desc(ring + slot * KT, 16);
+        const uint32_t d = tmem + TM_S + g * PT_KEYS;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * BLOCK + (k & 3) * 32;
-          mma_ss(tmem + TM_S + g * PT_KEYS, sw128_desc(tiles + g * QT + off, 16), sw128_desc(ring + slot * KT + off, 16), id_s, k != 0);
+          const uint64_t off = ((k >> 2) * BLOCK + (k & 3) * 32) >> 4;
+          mma_ss(d, da + off, db + off, id_s, k != 0);
         }
       };
       auto output = [&](int g, int slot, bool more) {
+        const uint64_t db = sw128_desc(ring + slot * KT, BLOCK);
+        const uint32_t d = tmem + TM_O + g * D, p = tmem + TM_S + g * PT_KEYS;
+        mma_ts(d, p, db, id_o, more);
 #pragma unroll
-        for (int k = 0; k < PT_KEYS / 16; ++k)
-          mma_ts(tmem + TM_O + g * D, tmem + TM_S + g * PT_KEYS + k * 8, sw128_desc(ring + slot * KT + k * 2048, BLOCK), id_o,
-                 more || k != 0);
+        for (int k = 1; k < PT_KEYS / 16; ++k) mma_ts(d, p + k * 8, db + k * (2048 >> 4), id_o, 1);
       };
       bool ok = n == 0 || wait(&kv_full[0], 0, 0x200);
       if (ok && n > 0) {
@@ -1129,7 +1180,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
       const int last_row = min(t.R, t.r0 + (g + 1) * PT_GROUP) - 1;
       const int hi_all = t.ctx + (t.r0 + g * PT_GROUP) / a.G;
       const int lo_all = a.window > 0 ? t.ctx + last_row / a.G - a.window + 1 : 0;
-      const float sc = KV8 ? a.scale_log2 * q_back[g * PT_GROUP + row] : a.scale_log2;
+      const float sc = KV8 ? a.scale_log2 * q_back[g * PT_GROUP + row] : fmaxf(a.scale_log2, 1e-37f);
       float ref = -INFINITY, l = 0.f, vref = 0.f;
       int page, tb, next_page, next_tb;
       float ks = 0.f, vs = 0.f;
@@ -1153,30 +1204,58 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
         ok = __all_sync(MUI_FULL_MASK, wait(&s_full[g], j, 0x300 + g));
         if (!ok) break;
         tc_after();
-        // scaled scores of 32 columns
-        auto load_scores = [&](int c, float (&s)[32]) {
-          tmem_load32(ts + c * 32, s);
+        // factor of the scores of 16 columns; above 0, since -infinity stands for what a row does not see
+        auto factor_of = [&](int sub) { return KV8 ? fmaxf(sc * __shfl_sync(MUI_FULL_MASK, ks, sub), 1e-37f) : sc; };
+        float mx = -INFINITY;
+        if (open) {
+          uint32_t s0[32], s1[32];
+          auto top = [&](int c, const uint32_t(&s)[32]) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float f = KV8 ? sc * __shfl_sync(MUI_FULL_MASK, ks, 2 * c + h) : sc;
-            const int b0 = __shfl_sync(MUI_FULL_MASK, tb, 2 * c + h);
+            for (int h = 0; h < 2; ++h) {
+              float m0 = __uint_as_float(s[16 * h]), m1 = __uint_as_float(s[16 * h + 1]);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              s[16 * h + e] *= f;
-              if (!open) {
-                const int jr = b0 + e;
-                if (!(b0 >= 0 && jr <= hi && (jr >= lo || jr < a.sinks))) s[16 * h + e] = -INFINITY;
+              for (int e = 2; e < 16; e += 2) {
+                m0 = fmaxf(m0, __uint_as_float(s[16 * h + e]));
+                m1 = fmaxf(m1, __uint_as_float(s[16 * h + e + 1]));
               }
+              mx = fmaxf(mx, fmaxf(m0, m1) * factor_of(2 * c + h));
+            }
+          };
+          tmem_ask32(ts, s0);
+          tmem_load_wait(s0);
+          tmem_ask32(ts + 32, s1);
+          top(0, s0);
+          tmem_load_wait(s1);
+          tmem_ask32(ts + 64, s0);
+          top(1, s1);
+          tmem_load_wait(s0);
+          tmem_ask32(ts + 96, s1);
+          top(2, s0);
+          tmem_load_wait(s1);
+          top(3, s1);
+        } else {
+          // masked scores are written back, so that what follows need not know
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float s[32];
+            tmem_load32(ts + c * 32, s);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float f = factor_of(2 * c + h);
+              const int b0 = __shfl_sync(MUI_FULL_MASK, tb, 2 * c + h);
+              uint32_t w[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const int jr = b0 + e;
+                const bool see = b0 >= 0 && jr <= hi && (jr >= lo || jr < a.sinks);
+                const float x = see ? s[16 * h + e] : -INFINITY;
+                mx = fmaxf(mx, see ? x * f : -INFINITY);
+                w[e] = __float_as_uint(x);
+              }
+              tmem_store16(ts + c * 32 + 16 * h, w);
             }
           }
-        };
-        float mx = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float s[32];
-          load_scores(c, s);
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) mx = fmaxf(mx, fmaxf(s[e], s[e + 1]));
+          tmem_store_wait();
         }
         float turn = 1.f;  // e4m3: change of the output's reference scale
         if (KV8) {
@@ -1210,23 +1289,40 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
             }
           }
         }
-        const float use = ref == -INFINITY ? 0.f : ref;
+        const float use = ref == -INFINITY ? 0.f : -ref;
+        {
+          uint32_t s0[32], s1[32];
+          auto weigh = [&](int c, const uint32_t(&s)[32]) {
+            uint32_t w[16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float s[32];
-          load_scores(c, s);
-          uint32_t w[16];
+            for (int h = 0; h < 2; ++h) {
+              const float f = factor_of(2 * c + h);
+              const float pf = KV8 ? (vref > 0.f ? __shfl_sync(MUI_FULL_MASK, vs, 2 * c + h) / vref : 0.f) : 1.f;
+              float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float f = KV8 ? (vref > 0.f ? __shfl_sync(MUI_FULL_MASK, vs, 2 * c + h) / vref : 0.f) : 1.f;
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float p0 = ex2(s[16 * h + e] - use), p1 = ex2(s[16 * h + e + 1] - use);
-              l += p0 + p1;
-              w[8 * h + e / 2] = KV8 ? Elt<M>::pack2(p0 * f, p1 * f) : Elt<M>::pack2(p0, p1);
+              for (int e = 0; e < 16; e += 2) {
+                const float p0 = ex2(fmaf(__uint_as_float(s[16 * h + e]), f, use));
+                const float p1 = ex2(fmaf(__uint_as_float(s[16 * h + e + 1]), f, use));
+                l0 += p0;
+                l1 += p1;
+                w[8 * h + e / 2] = KV8 ? Elt<M>::pack2(p0 * pf, p1 * pf) : Elt<M>::pack2(p0, p1);
+              }
+              l += l0 + l1;
             }
-          }
-          tmem_store16(ts + c * 16, w);  // columns that were read above
+            tmem_store16(ts + c * 16, w);  // columns that have been read
+          };
+          tmem_ask32(ts, s0);
+          tmem_load_wait(s0);
+          tmem_ask32(ts + 32, s1);
+          weigh(0, s0);
+          tmem_load_wait(s1);
+          tmem_ask32(ts + 64, s0);
+          weigh(1, s1);
+          tmem_load_wait(s0);
+          tmem_ask32(ts + 96, s1);
+          weigh(2, s0);
+          tmem_load_wait(s1);
+          weigh(3, s1);
         }
         tmem_store_wait();
         tc_before();
@@ -1474,7 +1570,9 @@ mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_page
   a.q_vec = (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (q_strides.tok & 7) == 0 && (q_strides.head & 7) == 0;
   a.window = window;
   a.sinks = sinks;
-  a.scale_log2 = scale * 1.44269504088896341f;
+  // a negative scale is taken as a positive one of -q
+  a.q_flip = scale < 0.f ? 0x80008000u : 0u;
+  a.scale_log2 = (scale < 0.f ? -scale : scale) * 1.44269504088896341f;
   // a tile is 16 rows of K and of V
   a.lead = PA_TRIPLE_COST * 4096 / (2 * PA_TILE * cache->head_dim * (cache->format == MUI_KV_E4M3 ? 1 : 2));
   PaPlan p;
