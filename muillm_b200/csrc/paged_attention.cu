@@ -7,6 +7,7 @@
 // Two kernels. Up to 32 rows per KV head (decode): paged_decode_kernel, bound by the bytes of K and V; the visible rows of all
 // sequences are dealt out to the CTAs evenly, and what several CTAs share is joined by paged_merge_kernel. More rows (prompts): paged_prompt_kernel, bound by the tensor cores.
 #include "paged_common.cuh"
+#include "tensor_map.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -883,7 +884,8 @@ __device__ __forceinline__ bool prompt_tile(const PaArgs& a, int x, PromptTile& 
 }
 
 template <typename T, bool KV8, int D>
-__global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArgs a) {
+__global__ void __launch_bounds__(PT_THREADS, 1)
+    paged_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PaArgs a) {
   using M = typename std::conditional<KV8, __half, T>::type;
   constexpr int QT = PT_GROUP * D * 2;                 // bytes of a group's Q
   constexpr int KT = PT_KEYS * D * 2;                  // bytes of a K or V tile
@@ -913,7 +915,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
 
   if (tid == 0) {
     for (int i = 0; i < PT_SLOTS; ++i) {
-      mbar_init(&kv_full[i], PT_LOADERS);
+      mbar_init(&kv_full[i], KV8 ? PT_LOADERS : 33);
       mbar_init(&kv_empty[i], 1);
     }
     for (int g = 0; g < 2; ++g) {
@@ -990,21 +992,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
     }
   };
 
-  if (warp >= PT_LOAD_WARP) {
-    // ------------------------------ K and V ------------------------------
+  if (KV8 && warp >= PT_LOAD_WARP) {
+    // ------------------------------ K and V, e4m3: converted by three warps ------------------------------
     const int lw = warp - PT_LOAD_WARP;
-    constexpr int ES = KV8 ? 1 : 2, RB = D * ES, CPR = RB / 16;  // bytes and 16-byte chunks of a cache row
+    constexpr int RB = D, CPR = RB / 16;                         // bytes and 16-byte chunks of a cache row
     constexpr int RPI = 32 / CPR;                                // rows a warp copies at a time
     // A step is 16 units of eight rows; a warp takes every third one, so that addresses are worked out once per unit.
     constexpr int UNITS = 2 * PT_SUB, TURNS = (UNITS + PT_LOAD_WARPS - 1) / PT_LOAD_WARPS, CPU = 8 / RPI;
     const int ch = lane % CPR, row0 = lane / CPR;
     // where this lane's chunks of a unit go: 16-bit chunk c of row r sits at block c / 8, row r, chunk (c % 8) ^ (r % 8)
     auto place = [&](int r, int c) { return static_cast<uint32_t>((c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
-    uint32_t at[CPU][KV8 ? 2 : 1];
+    uint32_t at[CPU][2];
 #pragma unroll
     for (int i = 0; i < CPU; ++i)
 #pragma unroll
-      for (int h = 0; h < (KV8 ? 2 : 1); ++h) at[i][h] = place(i * RPI + row0, KV8 ? 2 * ch + h : ch);
+      for (int h = 0; h < 2; ++h) at[i][h] = place(i * RPI + row0, 2 * ch + h);
     int page, tb, next_page, next_tb;
     find_tile(0, page, tb, true);
     bool ok = true;
@@ -1039,7 +1041,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
           if (it >= PT_SLOTS) ok = __all_sync(MUI_FULL_MASK, wait(&kv_empty[slot], it / PT_SLOTS - 1, 0x100 + slot));
           return ok;
         };
-        if (KV8) {
+        {
           uint4 hold[TURNS][CPU];  // requested before the slot is free
           units([&](int k, int, const unsigned char* src, bool whole, int first) {
 #pragma unroll
@@ -1057,7 +1059,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 const uint32_t w0 = w[2 * h], w1 = w[2 * h + 1];
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + u * 1024 + at[i][KV8 ? h : 0]),
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst + u * 1024 + at[i][h]),
                              "r"(e4m3_to_half2((uint16_t)w0)), "r"(e4m3_to_half2((uint16_t)(w0 >> 16))),
                              "r"(e4m3_to_half2((uint16_t)w1)), "r"(e4m3_to_half2((uint16_t)(w1 >> 16)))
                              : "memory");
@@ -1066,34 +1068,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           mbar_arrive(&kv_full[slot]);
-        } else {
-          if (!slot_free()) break;
-          units([&](int, int u, const unsigned char* src, bool whole, int first) {
-            if (whole) {
-#pragma unroll
-              for (int i = 0; i < CPU; ++i) copy16(dst + u * 1024 + at[i][0], src + i * RPI * RB, 16);
-            } else {
-#pragma unroll
-              for (int i = 0; i < CPU; ++i)
-                copy16(dst + u * 1024 + at[i][0], src + i * RPI * RB, seen(first, i * RPI + row0) ? 16 : 0);
-            }
-          });
-          copy_commit();
-          if (it >= 2) {  // two tiles stay in flight
-            copy_wait<2>();
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(&kv_full[(it - 2) % PT_SLOTS]);
-          }
         }
       }
       page = next_page;
       tb = next_tb;
     }
-    if (!KV8) {
-      copy_wait<0>();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (ok)
-        for (int it = max(0, 2 * n - 2); it < 2 * n; ++it) mbar_arrive(&kv_full[it % PT_SLOTS]);
+  } else if (!KV8 && warp >= PT_LOAD_WARP) {
+    // ------------------------------ K and V, 16-bit: one warp, tile copies of 16 rows x 64 elements ------------------------------
+    if (warp == PT_LOAD_WARP) {
+      constexpr int RB = D * 2, CPR = RB / 16, RPI = 32 / CPR;
+      const int ch = lane % CPR, row0 = lane / CPR;
+      int page, tb, next_page, next_tb;
+      find_tile(0, page, tb, true);
+      bool ok = true;
+      for (int j = 0; j < n && ok; ++j) {
+        next_page = next_tb = -1;
+        if (j + 1 < n) find_tile(j + 1, next_page, next_tb, true);
+        // lanes 0-7, a 16-row tile each: seen whole by somebody of this CTA's rows, or to be copied row by row
+        const int row = ((max(page, 0) * a.kv.kv_heads + kvh) << a.kv.page_shift) + (max(tb, 0) & ((1 << a.kv.page_shift) - 1));
+        const bool whole = tb >= 0 && tb + PA_TILE <= t.sp.kv_len && (tb >= t.sp.lo_min || tb + PA_TILE <= a.sinks);
+        const unsigned mask = __ballot_sync(MUI_FULL_MASK, lane < PT_SUB && whole);
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+          const int it = 2 * j + which, slot = it % PT_SLOTS;
+          const uint32_t dst = ring + slot * KT;
+          if (it >= PT_SLOTS) ok = __all_sync(MUI_FULL_MASK, wait(&kv_empty[slot], it / PT_SLOTS - 1, 0x100 + slot));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], __popc(mask) * (PA_TILE * RB));
+          __syncwarp();
+          if (mask >> lane & 1) {
+            const CUtensorMap* map = which == 0 ? &map_k : &map_v;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+              asm volatile(
+                  "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                      dst + h * BLOCK + lane * (PA_TILE * 128)),
+                  "l"(reinterpret_cast<uint64_t>(map)), "r"(h * 64), "r"(row), "r"(smem_u32(&kv_full[slot]))
+                  : "memory");
+          }
+          // the others: rows that nobody of this tile sees are zeros (what they hold must not matter)
+          for (unsigned left = ~mask & ((1u << PT_SUB) - 1); left; left &= left - 1) {
+            const int sub = __ffs(left) - 1;
+            const int first = __shfl_sync(MUI_FULL_MASK, tb, sub), from = __shfl_sync(MUI_FULL_MASK, row, sub);
+            const unsigned char* src = reinterpret_cast<const unsigned char*>(which == 0 ? a.kv.k_pages : a.kv.v_pages) +
+                                       static_cast<size_t>(from) * RB + ch * 16;
+#pragma unroll
+            for (int r = row0; r < PA_TILE; r += RPI) {
+              const int jr = first + r;
+              const bool see = first >= 0 && jr < t.sp.kv_len && (jr >= t.sp.lo_min || jr < a.sinks);
+              copy16(dst + (ch >> 3) * BLOCK + (sub * PA_TILE + r) * 128 + (((ch & 7) ^ (r & 7)) << 4), src + r * RB, see ? 16 : 0);
+            }
+          }
+          // arrives when this lane's copies, if any, have landed
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&kv_full[slot])) : "memory");
+        }
+        page = next_page;
+        tb = next_tb;
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (!ok) {  // leave no tile copy in flight behind: the last four items that were begun
+        int none = 0;
+        for (int i = 0; i < PT_SLOTS; ++i) (void)mbar_wait_bounded(&kv_full[i], 0, &none);
+      }
     }
   } else if (warp == PT_MMA_WARP) {
     // ------------------------------ MMAs ------------------------------
@@ -1118,8 +1154,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
         for (int k = 1; k < PT_KEYS / 16; ++k) mma_ts(d, p + k * 8, db + k * (2048 >> 4), id_o, 1);
       };
       bool ok = n == 0 || wait(&kv_full[0], 0, 0x200);
-      if (ok && n > 0) {
+      // what cp.async wrote is ordered before the tensor cores' reads by a fence on this side (tile copies need none)
+      auto fence = [&]() {
         tc_after();
+        if (!KV8) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      };
+      if (ok && n > 0) {
+        fence();
         scores(0, 0);
         tc_commit_to(&s_full[0]);
         if (two) {
@@ -1132,13 +1173,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_prompt_kernel(const PaArg
         const int vi = 2 * j + 1, ki = 2 * j + 2, vs = vi % PT_SLOTS, ks = ki % PT_SLOTS;
         ok = wait(&kv_full[vs], vi / PT_SLOTS, 0x210) && wait(&p_full[0], j, 0x220);
         if (!ok) break;
-        tc_after();
+        fence();
         output(0, vs, j > 0);
         tc_commit_to(&pv_done[0]);
         if (j + 1 < n) {
           ok = wait(&kv_full[ks], ki / PT_SLOTS, 0x230);
           if (!ok) break;
-          tc_after();
+          fence();
           scores(0, ks);
           tc_commit_to(&s_full[0]);
         }
@@ -1501,8 +1542,24 @@ mui_status_t launch_prompt(cudaStream_t stream, const PaArgs& a, int tiles, int 
                                         static_cast<int>(smem)));
     configured.fetch_or(bit);
   }
+  CUtensorMap maps[2] = {};
+  if (!KV8) {
+    // the pool as rows of head_dim elements; boxes of 16 rows x 64 elements, which never cross a page
+    EncodeTiledFn enc = encode_tiled_fn();
+    MUI_REQUIRE(enc != nullptr, MUI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    const long long rows = (static_cast<long long>(a.kv.num_pages) * a.kv.kv_heads) << a.kv.page_shift;
+    MUI_REQUIRE(rows <= 0x7fffffff, MUI_ERR_UNSUPPORTED, "%lld cache rows in a pool (at most 2^31 - 1)", rows);
+    const cuuint64_t dims[2] = {D, static_cast<cuuint64_t>(rows)}, stride[1] = {D * 2};
+    const cuuint32_t box[2] = {64, PA_TILE}, step[2] = {1, 1};
+    for (int i = 0; i < 2; ++i) {
+      const CUresult r = enc(&maps[i], CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, i == 0 ? a.kv.k_pages : a.kv.v_pages, dims, stride, box,
+                             step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      MUI_REQUIRE(r == CUDA_SUCCESS, MUI_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", static_cast<int>(r));
+    }
+  }
   MUI_CUDA_CHECK(mui_launch(paged_prompt_kernel<T, KV8, D>, dim3(tiles, a.kv.kv_heads, a.splits), dim3(PT_THREADS), smem,
-                            stream, pdl, a));
+                            stream, pdl, maps[0], maps[1], a));
   if (a.splits > 1) {
     const long long rows = static_cast<long long>(a.kv.total) * a.Hq;
     MUI_CUDA_CHECK(mui_launch(paged_prompt_merge_kernel<T, D>, dim3(static_cast<unsigned>((rows + PA_WARPS - 1) / PA_WARPS)),

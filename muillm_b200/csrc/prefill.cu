@@ -17,12 +17,11 @@
 //  * Four warps read the accumulators back with tcgen05.ld and apply the epilogue.
 // Every wait is bounded: a wait that runs out records a device status code, the CTA waits (bounded) for its copies
 // and MMAs in flight, frees its tensor memory and returns. No cluster launch, no multicast.
-#include <cuda.h>
-
 #include <mutex>
 #include <type_traits>
 
 #include "common.cuh"
+#include "tensor_map.cuh"
 
 MUI_STATUS_ACCESSOR(prefill)
 
@@ -294,23 +293,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1)
 // ---------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point query (the library links no libcuda)
-EncodeTiledFn encode_tiled_fn() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
-
 // Tensor map of a row-major [rows, K] 16-bit matrix, tiles of [box_rows] x [64 elements of K], 128-byte swizzle;
 // out-of-range elements read as zero.
 mui_status_t make_map(CUtensorMap* m, mui_dtype_t dtype, const void* base, int rows, int K, int box_rows) {
