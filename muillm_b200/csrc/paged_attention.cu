@@ -780,6 +780,13 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 __device__ __forceinline__ void tc_commit_to(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// One lane of a converged warp. Unlike `lane == 0` it leaves the code around it warp-uniform, so that descriptors stay in
+// uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
 // D[tmem] (+)= A[smem] B[smem]^T
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -1133,13 +1140,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     }
   } else if (warp == PT_MMA_WARP) {
     // ------------------------------ MMAs ------------------------------
-    if (lane == 0) {
+    {
       const int bf = std::is_same<M, __nv_bfloat16>::value;
       const uint32_t id_s = f16_idesc(bf, PT_KEYS, 0), id_o = f16_idesc(bf, D, 1);
       // one thread issues: a descriptor per operand, its address field (16-byte units) moved on
       auto scores = [&](int g, int slot) {
         const uint64_t da = sw128_desc(tiles + g * QT, 16), db = sw128_desc(ring + slot * KT, 16);
         const uint32_t d = tmem + TM_S + g * PT_KEYS;
+        if (elect_one())
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint64_t off = ((k >> 2) * BLOCK + (k & 3) * 32) >> 4;
@@ -1149,11 +1157,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       auto output = [&](int g, int slot, bool more) {
         const uint64_t db = sw128_desc(ring + slot * KT, BLOCK);
         const uint32_t d = tmem + TM_O + g * D, p = tmem + TM_S + g * PT_KEYS;
-        mma_ts(d, p, db, id_o, more);
+        if (elect_one()) {
+          mma_ts(d, p, db, id_o, more);
 #pragma unroll
-        for (int k = 1; k < PT_KEYS / 16; ++k) mma_ts(d, p + k * 8, db + k * (2048 >> 4), id_o, 1);
+          for (int k = 1; k < PT_KEYS / 16; ++k) mma_ts(d, p + k * 8, db + k * (2048 >> 4), id_o, 1);
+        }
       };
-      bool ok = n == 0 || wait(&kv_full[0], 0, 0x200);
+      bool ok = n == 0 || __all_sync(MUI_FULL_MASK, wait(&kv_full[0], 0, 0x200));
+      // the whole warp waits and one lane, always the same, issues and commits
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc_commit_to(bar);
+        __syncwarp();
+      };
       // what cp.async wrote is ordered before the tensor cores' reads by a fence on this side (tile copies need none)
       auto fence = [&]() {
         tc_after();
@@ -1162,45 +1177,45 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       if (ok && n > 0) {
         fence();
         scores(0, 0);
-        tc_commit_to(&s_full[0]);
+        commit(&s_full[0]);
         if (two) {
           scores(1, 0);
-          tc_commit_to(&s_full[1]);
+          commit(&s_full[1]);
         }
-        tc_commit_to(&kv_empty[0]);
+        commit(&kv_empty[0]);
       }
       for (int j = 0; j < n && ok; ++j) {
         const int vi = 2 * j + 1, ki = 2 * j + 2, vs = vi % PT_SLOTS, ks = ki % PT_SLOTS;
-        ok = wait(&kv_full[vs], vi / PT_SLOTS, 0x210) && wait(&p_full[0], j, 0x220);
+        ok = __all_sync(MUI_FULL_MASK, wait(&kv_full[vs], vi / PT_SLOTS, 0x210) && wait(&p_full[0], j, 0x220));
         if (!ok) break;
         fence();
         output(0, vs, j > 0);
-        tc_commit_to(&pv_done[0]);
+        commit(&pv_done[0]);
         if (j + 1 < n) {
-          ok = wait(&kv_full[ks], ki / PT_SLOTS, 0x230);
+          ok = __all_sync(MUI_FULL_MASK, wait(&kv_full[ks], ki / PT_SLOTS, 0x230));
           if (!ok) break;
           fence();
           scores(0, ks);
-          tc_commit_to(&s_full[0]);
+          commit(&s_full[0]);
         }
         if (two) {
-          ok = wait(&p_full[1], j, 0x240);
+          ok = __all_sync(MUI_FULL_MASK, wait(&p_full[1], j, 0x240));
           if (!ok) break;
           tc_after();
           output(1, vs, j > 0);
-          tc_commit_to(&pv_done[1]);
+          commit(&pv_done[1]);
         }
-        tc_commit_to(&kv_empty[vs]);
+        commit(&kv_empty[vs]);
         if (j + 1 < n) {
           if (two) {
             scores(1, ks);
-            tc_commit_to(&s_full[1]);
+            commit(&s_full[1]);
           }
-          tc_commit_to(&kv_empty[ks]);
+          commit(&kv_empty[ks]);
         }
       }
       if (!ok) {  // leave no MMA in flight behind (slot 0's barrier is not waited for by anyone any more)
-        tc_commit_to(&pv_done[0]);
+        commit(&pv_done[0]);
         const uint64_t t0 = global_timer_ns();
         while (global_timer_ns() - t0 < 1000000ull) {
         }
@@ -1284,15 +1299,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             for (int h = 0; h < 2; ++h) {
               const float f = factor_of(2 * c + h);
               const int b0 = __shfl_sync(MUI_FULL_MASK, tb, 2 * c + h);
+              // bit e: this row sees column b0 + e
+              auto below = [&](int x) { return (1u << min(max(x, 0), PA_TILE)) - 1u; };
+              const unsigned see =
+                  b0 < 0 ? 0u : below(hi - b0 + 1) & (~below(lo - b0) | below(min(a.sinks, 0x7fffffff - PA_TILE) - b0));
               uint32_t w[16];
+              float top = -INFINITY;
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
-                const int jr = b0 + e;
-                const bool see = b0 >= 0 && jr <= hi && (jr >= lo || jr < a.sinks);
-                const float x = see ? s[16 * h + e] : -INFINITY;
-                mx = fmaxf(mx, see ? x * f : -INFINITY);
+                const float x = see >> e & 1 ? s[16 * h + e] : -INFINITY;
+                top = fmaxf(top, x);
                 w[e] = __float_as_uint(x);
               }
+              mx = fmaxf(mx, top * f);
               tmem_store16(ts + c * 32 + 16 * h, w);
             }
           }
