@@ -57,6 +57,22 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nmov.b64 z, {%6, %7};\n"
+      "fma.rn.f32x2 x, x, y, z;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%2, %3};\nmov.b64 y, {%4, %5};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -899,7 +915,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   constexpr int BLOCK = PT_KEYS * 128;                 // bytes of one 64-element block of a tile (Q, K or V)
   constexpr uint32_t TM_S = 0, TM_O = 2 * PT_KEYS;     // tensor-memory columns
   extern __shared__ unsigned char pt_raw[];
-  __shared__ uint64_t kv_full[PT_SLOTS], kv_empty[PT_SLOTS], s_full[2], p_full[2], pv_done[2];
+  __shared__ uint64_t kv_full[PT_SLOTS], kv_empty[PT_SLOTS], s_full[2], p_half[2], p_full[2], pv_done[2];
   __shared__ float q_back[PT_ROWS];
   __shared__ uint32_t tmem_s;
   __shared__ int abort_s;
@@ -927,6 +943,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&s_full[g], 1);
+      mbar_init(&p_half[g], PT_GROUP);
       mbar_init(&p_full[g], PT_GROUP);
       mbar_init(&pv_done[g], 1);
     }
@@ -1154,13 +1171,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           mma_ss(d, da + off, db + off, id_s, k != 0);
         }
       };
-      auto output = [&](int g, int slot, bool more) {
-        const uint64_t db = sw128_desc(ring + slot * KT, BLOCK);
-        const uint32_t d = tmem + TM_O + g * D, p = tmem + TM_S + g * PT_KEYS;
+      auto output = [&](int g, int slot, int half, bool more) {
+        const uint64_t db = sw128_desc(ring + slot * KT + half * (PT_KEYS / 2) * 128, BLOCK);
+        const uint32_t d = tmem + TM_O + g * D, p = tmem + TM_S + g * PT_KEYS + half * (PT_KEYS / 4);
         if (elect_one()) {
           mma_ts(d, p, db, id_o, more);
 #pragma unroll
-          for (int k = 1; k < PT_KEYS / 16; ++k) mma_ts(d, p + k * 8, db + k * (2048 >> 4), id_o, 1);
+          for (int k = 1; k < PT_KEYS / 32; ++k) mma_ts(d, p + k * 8, db + k * (2048 >> 4), id_o, 1);
         }
       };
       bool ok = n == 0 || __all_sync(MUI_FULL_MASK, wait(&kv_full[0], 0, 0x200));
@@ -1186,10 +1203,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       }
       for (int j = 0; j < n && ok; ++j) {
         const int vi = 2 * j + 1, ki = 2 * j + 2, vs = vi % PT_SLOTS, ks = ki % PT_SLOTS;
-        ok = __all_sync(MUI_FULL_MASK, wait(&kv_full[vs], vi / PT_SLOTS, 0x210) && wait(&p_full[0], j, 0x220));
+        ok = __all_sync(MUI_FULL_MASK, wait(&kv_full[vs], vi / PT_SLOTS, 0x210) && wait(&p_half[0], j, 0x220));
         if (!ok) break;
         fence();
-        output(0, vs, j > 0);
+        output(0, vs, 0, j > 0);
+        ok = __all_sync(MUI_FULL_MASK, wait(&p_full[0], j, 0x221));
+        if (!ok) break;
+        tc_after();
+        output(0, vs, 1, true);
         commit(&pv_done[0]);
         if (j + 1 < n) {
           ok = __all_sync(MUI_FULL_MASK, wait(&kv_full[ks], ki / PT_SLOTS, 0x230));
@@ -1199,10 +1220,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           commit(&s_full[0]);
         }
         if (two) {
-          ok = __all_sync(MUI_FULL_MASK, wait(&p_full[1], j, 0x240));
+          ok = __all_sync(MUI_FULL_MASK, wait(&p_half[1], j, 0x240));
           if (!ok) break;
           tc_after();
-          output(1, vs, j > 0);
+          output(1, vs, 0, j > 0);
+          ok = __all_sync(MUI_FULL_MASK, wait(&p_full[1], j, 0x241));
+          if (!ok) break;
+          tc_after();
+          output(1, vs, 1, true);
           commit(&pv_done[1]);
         }
         commit(&kv_empty[vs]);
@@ -1352,22 +1377,22 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         const float use = ref == -INFINITY ? 0.f : -ref;
         {
           uint32_t s0[32], s1[32];
+          float2 sum = make_float2(0.f, 0.f);
           auto weigh = [&](int c, const uint32_t(&s)[32]) {
             uint32_t w[16];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float f = factor_of(2 * c + h);
               const float pf = KV8 ? (vref > 0.f ? __shfl_sync(MUI_FULL_MASK, vs, 2 * c + h) / vref : 0.f) : 1.f;
-              float l0 = 0.f, l1 = 0.f;
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
-                const float p0 = ex2(fmaf(__uint_as_float(s[16 * h + e]), f, use));
-                const float p1 = ex2(fmaf(__uint_as_float(s[16 * h + e + 1]), f, use));
-                l0 += p0;
-                l1 += p1;
-                w[8 * h + e / 2] = KV8 ? Elt<M>::pack2(p0 * pf, p1 * pf) : Elt<M>::pack2(p0, p1);
+                float2 p = fma2(make_float2(__uint_as_float(s[16 * h + e]), __uint_as_float(s[16 * h + e + 1])),
+                                make_float2(f, f), make_float2(use, use));
+                p.x = ex2(p.x);
+                p.y = ex2(p.y);
+                sum = add2(sum, p);
+                w[8 * h + e / 2] = KV8 ? Elt<M>::pack2(p.x * pf, p.y * pf) : Elt<M>::pack2(p.x, p.y);
               }
-              l += l0 + l1;
             }
             tmem_store16(ts + c * 16, w);  // columns that have been read
           };
@@ -1379,10 +1404,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           tmem_ask32(ts + 64, s0);
           weigh(1, s1);
           tmem_load_wait(s0);
+          tmem_store_wait();
+          tc_before();
+          mbar_arrive(&p_half[g]);  // the first 64 cache rows can be multiplied
           tmem_ask32(ts + 96, s1);
           weigh(2, s0);
           tmem_load_wait(s1);
           weigh(3, s1);
+          l += sum.x + sum.y;
         }
         tmem_store_wait();
         tc_before();
