@@ -922,13 +922,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   const uint32_t tiles = (smem_u32(pt_raw) + 1023u) & ~1023u;  // Q0, Q1, then the ring
   const uint32_t ring = tiles + 2 * QT;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kvh = blockIdx.y, split = blockIdx.z;
+  // KV heads fastest, the longest spans first
+  const int kvh = blockIdx.x % a.kv.kv_heads, split = blockIdx.y;
   volatile int* abort_flag = &abort_s;
 
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   PromptTile t;
-  if (!prompt_tile(a, gridDim.x - 1 - blockIdx.x, t)) return;
+  if (!prompt_tile(a, static_cast<int>((gridDim.x - 1 - blockIdx.x) / a.kv.kv_heads), t)) return;
   if (split >= t.active) return;
   const int i_begin = split * t.per * PT_SUB, i_end = min(t.sp.n, i_begin + t.per * PT_SUB);  // 16-row tiles of this split
   const int n = (i_end - i_begin + PT_SUB - 1) / PT_SUB;
@@ -1553,7 +1554,7 @@ bool pa_plan(const MuiDeviceInfo& di, int total, int batch, int Hq, int kv_heads
   p.bytes = p.decode_bytes;
   if (p.prompt) {
     const long long tiles = static_cast<long long>(total) * G / PT_ROWS + batch;
-    if (tiles > 0x7fffffff) return false;
+    if (tiles * kv_heads > 0x7fffffff) return false;
     p.tiles = static_cast<int>(tiles);
     // the rows' spans are split where whole ones would leave SMs idle
     const long long fit = di.sm_count / std::max<long long>(1, tiles * kv_heads);
@@ -1606,7 +1607,7 @@ mui_status_t launch_prompt(cudaStream_t stream, const PaArgs& a, int tiles, int 
       MUI_REQUIRE(r == CUDA_SUCCESS, MUI_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", static_cast<int>(r));
     }
   }
-  MUI_CUDA_CHECK(mui_launch(paged_prompt_kernel<T, KV8, D>, dim3(tiles, a.kv.kv_heads, a.splits), dim3(PT_THREADS), smem,
+  MUI_CUDA_CHECK(mui_launch(paged_prompt_kernel<T, KV8, D>, dim3(tiles * a.kv.kv_heads, a.splits), dim3(PT_THREADS), smem,
                             stream, pdl, maps[0], maps[1], a));
   if (a.splits > 1) {
     const long long rows = static_cast<long long>(a.kv.total) * a.Hq;

@@ -30,28 +30,66 @@ struct AppendArgs {
   const float* freqs;
   const int64_t* position_ids;
   int Hq, max_positions, rotary, interleaved;
-  int head_blocks;  // row part: blocks of heads per token
+  int freqs_vec;    // the table can be read 16 bytes at a time: aligned, and a lane's eight elements all rotated or none
+  int head_blocks;  // row part: blocks of heads per token, each `steps` turns of a warp
+  int steps;
   int unit_blocks;  // CTAs of the e4m3 unit part
-  int units;        // (sequence, page) candidates of the e4m3 unit part
+  int unit_heads;   // KV heads per CTA of it
 };
 
-// (cos, sin) of the eight elements from d0 on of a head; identity outside the rotated part
+// (cos, sin) of the eight elements from d0 on of a head; identity outside the rotated part. The sine of the first element of a
+// pair is negated.
 struct Turn {
   float c[8], s[8];
 };
 __device__ __forceinline__ void load_turn(const AppendArgs& a, long long pos, int d0, Turn& t) {
   const int half = a.rotary >> 1;
-  const float* row = a.freqs + (a.freqs ? pos * a.rotary : 0);
+  if (a.freqs == nullptr || d0 >= a.rotary) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      t.c[i] = 1.f;
+      t.s[i] = 0.f;
+    }
+    return;
+  }
+  const float* row = a.freqs + pos * a.rotary;
+  if (a.freqs_vec) {
+    // the eight elements are four pairs (interleaved) or one element of eight pairs (half), side by side in the table
+    const float4* p = reinterpret_cast<const float4*>(row + (a.interleaved ? d0 : 2 * (d0 < half ? d0 : d0 - half)));
+    if (a.interleaved) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 v = __ldg(p + i);
+        t.c[4 * i] = t.c[4 * i + 1] = v.x;
+        t.s[4 * i] = -v.y;
+        t.s[4 * i + 1] = v.y;
+        t.c[4 * i + 2] = t.c[4 * i + 3] = v.z;
+        t.s[4 * i + 2] = -v.w;
+        t.s[4 * i + 3] = v.w;
+      }
+    } else {
+      const float sign = d0 < half ? -1.f : 1.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 v = __ldg(p + i);
+        t.c[2 * i] = v.x;
+        t.s[2 * i] = sign * v.y;
+        t.c[2 * i + 1] = v.z;
+        t.s[2 * i + 1] = sign * v.w;
+      }
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int d = d0 + i;
     t.c[i] = 1.f;
     t.s[i] = 0.f;
-    if (a.freqs != nullptr && d < a.rotary) {
+    if (d < a.rotary) {
       const int pair = a.interleaved ? d >> 1 : (d < half ? d : d - half);
       t.c[i] = row[2 * pair];
       t.s[i] = row[2 * pair + 1];
-      if (a.interleaved ? !(d & 1) : d < half) t.s[i] = -t.s[i];  // first of the pair: minus sine
+      if (a.interleaved ? !(d & 1) : d < half) t.s[i] = -t.s[i];
     }
   }
 }
@@ -135,14 +173,14 @@ __device__ __forceinline__ int find_page(const PagedView& kv, int b, long long p
   return page;
 }
 
-// Rows of token t and the heads [block * STEPS * rows per step, ...) of the concatenation q | k | v (q only with QONLY).
-// A warp loads the (cos, sin) row once for all its heads.
-template <typename T, int D, bool ALIGNED, int STEPS, bool QONLY>
+// Rows of token t and a block of the heads of the concatenation q | k | v (q only with QONLY): a warp looks the token up and
+// loads its (cos, sin) row once for all of them, and has four turns of rows in flight.
+template <typename T, int D, bool ALIGNED, bool QONLY>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, long long unit) {
   constexpr int LPR = D / 8, RPS = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int t = static_cast<int>(unit / a.head_blocks);
-  const int h0 = static_cast<int>(unit % a.head_blocks) * (STEPS * RPS) + lane / LPR;
+  const int block0 = static_cast<int>(unit % a.head_blocks) * (a.steps * RPS);
   const int d0 = (lane % LPR) * 8;
   if (t >= a.kv.total) return;
   int b, ctx, i;
@@ -164,41 +202,46 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, long long unit)
   }
   Turn turn;
   load_turn(a, pos, d0, turn);
+  const int block_end = min(heads, block0 + a.steps * RPS);
+#pragma unroll 1
+  for (int h0 = block0; h0 < block_end; h0 += 4 * RPS) {
 #pragma unroll
-  for (int st = 0; st < STEPS; ++st) {
-    int h = h0 + st * RPS;
-    const T* in = nullptr;
-    T* out = nullptr;
-    bool rot = true;
-    if (h < a.Hq) {
-      in = reinterpret_cast<const T*>(a.q) + t * a.qs.tok + h * a.qs.head;
-      out = reinterpret_cast<T*>(a.q_out) + (static_cast<size_t>(t) * a.Hq + h) * D + d0;
-    } else if (h < heads) {
-      h -= a.Hq;
-      rot = h < a.kv.kv_heads;
-      if (!rot) h -= a.kv.kv_heads;
-      in = rot ? reinterpret_cast<const T*>(a.k) + t * a.ks.tok + h * a.ks.head
-               : reinterpret_cast<const T*>(a.v) + t * a.vs.tok + h * a.vs.head;
-      out = rot ? krow : vrow;
-      if (out != nullptr) out += (static_cast<size_t>(h) << a.kv.page_shift) * D;
+    for (int st = 0; st < 4; ++st) {
+      if (h0 + st * RPS >= block_end) break;  // whole warps
+      int h = h0 + st * RPS + lane / LPR;
+      const T* in = nullptr;
+      T* out = nullptr;
+      bool rot = true;
+      if (h < a.Hq) {
+        in = reinterpret_cast<const T*>(a.q) + t * a.qs.tok + h * a.qs.head;
+        out = reinterpret_cast<T*>(a.q_out) + (static_cast<size_t>(t) * a.Hq + h) * D + d0;
+      } else if (h < heads) {
+        h -= a.Hq;
+        rot = h < a.kv.kv_heads;
+        if (!rot) h -= a.kv.kv_heads;
+        in = rot ? reinterpret_cast<const T*>(a.k) + t * a.ks.tok + h * a.ks.head
+                 : reinterpret_cast<const T*>(a.v) + t * a.vs.tok + h * a.vs.head;
+        out = rot ? krow : vrow;
+        if (out != nullptr) out += (static_cast<size_t>(h) << a.kv.page_shift) * D;
+      }
+      float y[8];
+      load_row8<T, D, ALIGNED>(a, in, d0, rot && a.freqs != nullptr, turn, y);
+      if (out != nullptr) *reinterpret_cast<uint4*>(out) = pack8<T>(y);
     }
-    float y[8];
-    load_row8<T, D, ALIGNED>(a, in, d0, rot && a.freqs != nullptr, turn, y);
-    if (out != nullptr) *reinterpret_cast<uint4*>(out) = pack8<T>(y);
   }
 }
 
-template <typename T, int D, bool ALIGNED, int STEPS>
+template <typename T, int D, bool ALIGNED>
 __global__ void __launch_bounds__(PC_THREADS) append_rows_kernel(const AppendArgs a) {
   pdl_wait_prior_grid();
   pdl_launch_dependents();
-  append_rows<T, D, ALIGNED, STEPS, false>(a, static_cast<long long>(blockIdx.x) * PC_WARPS + (threadIdx.x >> 5));
+  append_rows<T, D, ALIGNED, false>(a, static_cast<long long>(blockIdx.x) * PC_WARPS + (threadIdx.x >> 5));
 }
 
 // One unit: the new rows of K (which == 0) or V of one head in one page, by `GROUPS` groups of D / 8 lanes (group index
 // `group`), at most ROWS rows per group. BLOCK: the groups span the CTA, else one warp.
 template <typename T, int D, bool ALIGNED, int ROWS, bool BLOCK>
-__device__ __forceinline__ void append_unit(const AppendArgs& a, int b, int first_row, int count, int ctx, int page_idx,
+__device__ __forceinline__ void append_unit(const AppendArgs& a, int page, int first_row, int count, int ctx, int page_idx,
                                             int head, int which, float* s_max) {
   constexpr int LPR = D / 8;
   constexpr int GROUPS = (BLOCK ? PC_THREADS : 32) / LPR;
@@ -208,8 +251,6 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, int b, int firs
   const long long p0 = static_cast<long long>(page_idx) << a.kv.page_shift;  // first position of the page
   const int lo = p0 < ctx ? static_cast<int>(ctx - p0) : 0;                   // slots [lo, hi) are new
   const int hi = static_cast<int>(min(static_cast<long long>(ps), static_cast<long long>(ctx) + count - p0));
-  const int page = find_page(a.kv, b, p0);
-  if (page < 0) return;
   const T* in = which == 0 ? reinterpret_cast<const T*>(a.k) + head * a.ks.head
                            : reinterpret_cast<const T*>(a.v) + head * a.vs.head;
   const int64_t tok_stride = which == 0 ? a.ks.tok : a.vs.tok;
@@ -241,7 +282,7 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, int b, int firs
   amax = warp_max(amax);
   if (BLOCK) {
     if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
-    __syncthreads();  // also: every thread has read the old scale
+    __syncthreads();  // also: every thread has read the old scale. s_max alternates from head to head
 #pragma unroll
     for (int w = 0; w < PC_WARPS; ++w) amax = fmaxf(amax, s_max[w]);
   }
@@ -287,7 +328,7 @@ __global__ void __launch_bounds__(PC_THREADS) append_e4m3_token_kernel(const App
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5;
   if (static_cast<int>(blockIdx.x) >= a.unit_blocks) {
-    append_rows<T, D, ALIGNED, 1, true>(a, static_cast<long long>(blockIdx.x - a.unit_blocks) * PC_WARPS + warp);
+    append_rows<T, D, ALIGNED, true>(a, static_cast<long long>(blockIdx.x - a.unit_blocks) * PC_WARPS + warp);
     return;
   }
   const long long u = static_cast<long long>(blockIdx.x) * PC_WARPS + warp;
@@ -299,22 +340,23 @@ __global__ void __launch_bounds__(PC_THREADS) append_e4m3_token_kernel(const App
     mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(ctx));
     return;
   }
-  append_unit<T, D, ALIGNED, 1, false>(a, b, b, 1, ctx, ctx >> a.kv.page_shift, r >> 1, r & 1, nullptr);
+  const int page = find_page(a.kv, b, ctx);
+  if (page >= 0) append_unit<T, D, ALIGNED, 1, false>(a, page, b, 1, ctx, ctx >> a.kv.page_shift, r >> 1, r & 1, nullptr);
 }
 
-// e4m3 pages, any number of new tokens: a CTA per (sequence, page, head, K or V), then the q rows. Units are numbered
+// e4m3 pages, any number of new tokens: a CTA per (sequence, page, block of heads, K or V), then the q rows. Pages are numbered
 // through: sequence b's start at cu[b] / page_size + 2 b, which leaves room for every page that its tokens can touch.
 template <typename T, int D, bool ALIGNED, int ROWS>
 __global__ void __launch_bounds__(PC_THREADS) append_e4m3_kernel(const AppendArgs a) {
-  __shared__ float s_max[PC_WARPS];
+  __shared__ float s_max[2][PC_WARPS];
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   if (static_cast<int>(blockIdx.x) >= a.unit_blocks) {
-    append_rows<T, D, ALIGNED, 4, true>(
+    append_rows<T, D, ALIGNED, true>(
         a, static_cast<long long>(blockIdx.x - a.unit_blocks) * PC_WARPS + (threadIdx.x >> 5));
     return;
   }
-  const int per_page = 2 * a.kv.kv_heads;
+  const int per_page = 2 * ((a.kv.kv_heads + a.unit_heads - 1) / a.unit_heads);
   const int u = blockIdx.x / per_page, r = blockIdx.x % per_page;
   const int32_t* cu = a.kv.cu;
   const int sh = a.kv.page_shift;
@@ -329,7 +371,12 @@ __global__ void __launch_bounds__(PC_THREADS) append_e4m3_kernel(const AppendArg
   }
   const int page_idx = (ctx >> sh) + u - ((first >> sh) + 2 * b);
   if (count == 0 || (static_cast<long long>(page_idx) << sh) >= static_cast<long long>(ctx) + count) return;
-  append_unit<T, D, ALIGNED, ROWS, true>(a, b, first, count, ctx, page_idx, r >> 1, r & 1, s_max);
+  const int page = find_page(a.kv, b, static_cast<long long>(page_idx) << sh);
+  if (page < 0) return;
+  const int head0 = (r >> 1) * a.unit_heads, head1 = min(a.kv.kv_heads, head0 + a.unit_heads);
+#pragma unroll 1
+  for (int head = head0; head < head1; ++head)
+    append_unit<T, D, ALIGNED, ROWS, true>(a, page, first, count, ctx, page_idx, head, r & 1, s_max[head & 1]);
 }
 
 template <typename T, int D, bool ALIGNED>
@@ -339,31 +386,36 @@ mui_status_t launch_append(cudaStream_t stream, AppendArgs a, bool e4m3, int pag
   const dim3 block(PC_THREADS);
   const long long limit = 0x7fffffff;
   auto blocks = [](long long units) { return (units + PC_WARPS - 1) / PC_WARPS; };
+  // Turns of heads per warp: one while that leaves the GPU unfilled (64 warps for each of 148 SMs), up to all heads of a token
+  // where it does not: what a warp looks up then serves 12 KiB of a 32 + 8-head token instead of 512 bytes.
+  auto choose_steps = [&](int heads) {
+    const int turns = (heads + RPS - 1) / RPS;
+    a.steps = 1;
+    while (a.steps < turns && static_cast<long long>(a.kv.total) * ((turns + a.steps - 1) / a.steps) > 148 * 64) a.steps *= 2;
+    a.head_blocks = (turns + a.steps - 1) / a.steps;
+  };
   if (!e4m3) {
-    // one step of rows per warp while that leaves the GPU unfilled, four (loads in flight, shared table row) above
-    const int heads = a.Hq + 2 * a.kv.kv_heads;
-    const long long one = static_cast<long long>(a.kv.total) * ((heads + RPS - 1) / RPS);
-    const bool wide = one > 148 * 64;
-    a.head_blocks = wide ? (heads + 4 * RPS - 1) / (4 * RPS) : (heads + RPS - 1) / RPS;
+    choose_steps(a.Hq + 2 * a.kv.kv_heads);
     const long long n = blocks(static_cast<long long>(a.kv.total) * a.head_blocks);
     MUI_REQUIRE(n <= limit, MUI_ERR_UNSUPPORTED, "too many rows");
-    if (wide)
-      MUI_CUDA_CHECK(mui_launch(append_rows_kernel<T, D, ALIGNED, 4>, dim3((unsigned)n), block, 0, stream, pdl, a));
-    else
-      MUI_CUDA_CHECK(mui_launch(append_rows_kernel<T, D, ALIGNED, 1>, dim3((unsigned)n), block, 0, stream, pdl, a));
+    MUI_CUDA_CHECK(mui_launch(append_rows_kernel<T, D, ALIGNED>, dim3((unsigned)n), block, 0, stream, pdl, a));
     return MUI_OK;
   }
+  choose_steps(a.Hq);
+  if (a.Hq == 0) a.head_blocks = 1;
+  const long long q_blocks = a.Hq == 0 ? 0 : blocks(static_cast<long long>(a.kv.total) * a.head_blocks);
   if (a.kv.cu == nullptr) {
-    a.head_blocks = (a.Hq + RPS - 1) / RPS;
     a.unit_blocks = static_cast<int>(blocks(static_cast<long long>(a.kv.batch) * 2 * a.kv.kv_heads));
-    const long long n = a.unit_blocks + blocks(static_cast<long long>(a.kv.total) * a.head_blocks);
+    const long long n = a.unit_blocks + q_blocks;
     MUI_REQUIRE(n <= limit, MUI_ERR_UNSUPPORTED, "too many rows");
     MUI_CUDA_CHECK(mui_launch(append_e4m3_token_kernel<T, D, ALIGNED>, dim3((unsigned)n), block, 0, stream, pdl, a));
     return MUI_OK;
   }
-  a.head_blocks = (a.Hq + 4 * RPS - 1) / (4 * RPS);
-  const long long units = static_cast<long long>(a.kv.total / page_size + 2 * a.kv.batch) * 2 * a.kv.kv_heads;
-  const long long n = units + blocks(static_cast<long long>(a.kv.total) * a.head_blocks);
+  const long long pages = a.kv.total / page_size + 2ll * a.kv.batch;
+  a.unit_heads = 1;  // as for the rows: eight CTAs for each SM
+  while (a.unit_heads < a.kv.kv_heads && pages * 2 * (a.kv.kv_heads / a.unit_heads) > 148 * 8) a.unit_heads *= 2;
+  const long long units = pages * 2 * ((a.kv.kv_heads + a.unit_heads - 1) / a.unit_heads);
+  const long long n = units + q_blocks;
   MUI_REQUIRE(n <= limit, MUI_ERR_UNSUPPORTED, "too many rows");
   a.unit_blocks = static_cast<int>(units);
   constexpr int GROUPS = PC_THREADS / (D / 8);  // 16 rows at a time for head dim 128, 32 for 64
@@ -416,6 +468,8 @@ extern "C" mui_status_t mui_paged_kv_append(void* stream, mui_dtype_t dtype, con
   a.interleaved = interleaved != 0;
   const bool aligned = (num_q_heads == 0 || row_aligned(q, q_strides)) && row_aligned(k, k_strides) &&
                        row_aligned(v, v_strides) && (a.interleaved || (a.rotary & 15) == 0);
+  const int whole = a.interleaved ? 8 : 16;  // rotary_dim of which a lane's eight elements are all rotated or none, and paired alike
+  a.freqs_vec = freqs != nullptr && (reinterpret_cast<uintptr_t>(freqs) & 15) == 0 && a.rotary % whole == 0;
   const bool e4m3 = cache->format == MUI_KV_E4M3;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int ps = cache->page_size;
