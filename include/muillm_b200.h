@@ -467,7 +467,7 @@ MUI_API mui_status_t mui_embedding_forward(void* stream, mui_dtype_t dtype, int 
  * b; context_lens[b] is the number of tokens that sequence b had in the cache BEFORE the new tokens of the call. The
  * new tokens of all sequences are packed: sequence b owns rows cu_tokens[b] .. cu_tokens[b + 1] - 1 of q, k, v and of
  * the output (cu_tokens[0] == 0), row i of them standing at cache position context_lens[b] + i; cu_tokens == NULL means
- * one new token per sequence. Rows from cu_tokens[batch] on (padding) are neither read nor written. The same description
+ * one new token per sequence. Rows from cu_tokens[batch] on (padding) have no effect and are not written. The same description
  * serves the append and the attention of one layer; everything it points to lives on the device and may change between
  * replays of a captured graph.
  *

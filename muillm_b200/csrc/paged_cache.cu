@@ -94,43 +94,68 @@ __device__ __forceinline__ void load_turn(const AppendArgs& a, long long pos, in
   }
 }
 
-// The lane's eight elements of a row as fp32, rotated when `turn`. ALIGNED: rows are 16-byte aligned and, in the half
-// layout, rotary / 2 is a multiple of eight. Whole warp (shuffles); lanes of rows that do not exist pass row = nullptr.
-template <typename T, int D, bool ALIGNED>
-__device__ __forceinline__ void load_row8(const AppendArgs& a, const T* row, int d0, bool turn, const Turn& t,
-                                          float (&y)[8]) {
-  float x[8], p[8];
+// The lane's eight elements of a row as they are in memory, and, when rows are not ALIGNED, their partners in the rotation.
+// ALIGNED: rows are 16-byte aligned and, in the half layout, rotary / 2 is a multiple of eight: the partners are another lane's
+// eight elements (half) or neighbours (interleaved).
+struct RawRow {
+  uint4 x, p;
+};
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ RawRow load_row(const AppendArgs& a, const T* row, int d0) {  // row == nullptr: zeros
+  RawRow r;
+  r.x = r.p = make_uint4(0, 0, 0, 0);
+  if (row == nullptr) return r;
   if (ALIGNED) {
-    const uint4 raw = row ? ld_act16(row + d0) : make_uint4(0, 0, 0, 0);
-    unpack8<T>(raw, x);
-    if (a.interleaved) {
+    r.x = ld_act16(row + d0);
+    return r;
+  }
+  const unsigned short* e16 = reinterpret_cast<const unsigned short*>(row);
+  const int half = a.rotary >> 1;
+  uint32_t x[8], p[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = x[i ^ 1];
-    } else {
-      const int step = a.rotary >> 4;  // lanes from an element to its partner
-      const int l = d0 >> 3;
-      const int other = (threadIdx.x & 31) + (l < step ? step : -step);
-      const int src = l < 2 * step ? other : (threadIdx.x & 31);
-      uint4 q;
-      q.x = __shfl_sync(MUI_FULL_MASK, raw.x, src);
-      q.y = __shfl_sync(MUI_FULL_MASK, raw.y, src);
-      q.z = __shfl_sync(MUI_FULL_MASK, raw.z, src);
-      q.w = __shfl_sync(MUI_FULL_MASK, raw.w, src);
-      unpack8<T>(q, p);
-    }
+  for (int i = 0; i < 8; ++i) {
+    const int d = d0 + i;
+    int o = d;
+    if (d < a.rotary) o = a.interleaved ? (d ^ 1) : (d < half ? d + half : d - half);
+    x[i] = __ldcg(e16 + d);
+    p[i] = __ldcg(e16 + o);
+  }
+  r.x = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+  r.p = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
+  return r;
+}
+// The eight elements in fp32, rotated when `turn` (the same for the whole warp, which exchanges elements).
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void turn_row(const AppendArgs& a, const RawRow& r, int d0, bool turn, const Turn& t, float (&y)[8]) {
+  float x[8], p[8];
+  unpack8<T>(r.x, x);
+  if (!turn) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
+    return;
+  }
+  if (!ALIGNED) {
+    unpack8<T>(r.p, p);
+  } else if (a.interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = x[i ^ 1];
   } else {
-    const int half = a.rotary >> 1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = d0 + i;
-      int o = d;
-      if (d < a.rotary) o = a.interleaved ? (d ^ 1) : (d < half ? d + half : d - half);
-      x[i] = row ? ld_act_f32<T>(row + d) : 0.f;
-      p[i] = row ? ld_act_f32<T>(row + o) : 0.f;
-    }
+    const int step = a.rotary >> 4, l = d0 >> 3, lane = threadIdx.x & 31;  // lanes from an element to its partner
+    const int src = l < step ? lane + step : (l < 2 * step ? lane - step : lane);
+    uint4 q;
+    q.x = __shfl_sync(MUI_FULL_MASK, r.x.x, src);
+    q.y = __shfl_sync(MUI_FULL_MASK, r.x.y, src);
+    q.z = __shfl_sync(MUI_FULL_MASK, r.x.z, src);
+    q.w = __shfl_sync(MUI_FULL_MASK, r.x.w, src);
+    unpack8<T>(q, p);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = (turn && d0 + i < a.rotary) ? fmaf(x[i], t.c[i], p[i] * t.s[i]) : x[i];
+  for (int i = 0; i < 8; ++i) y[i] = fmaf(x[i], t.c[i], p[i] * t.s[i]);
+  if (d0 + 8 > a.rotary) {  // elements that pass through, infinities and all
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (d0 + i >= a.rotary) y[i] = x[i];
+  }
 }
 
 // sequence, place and rotary position of new token t; false for a token behind the last sequence. Whole warp.
@@ -174,20 +199,36 @@ __device__ __forceinline__ int find_page(const PagedView& kv, int b, long long p
 }
 
 // Rows of token t and a block of the heads of the concatenation q | k | v (q only with QONLY): a warp looks the token up and
-// loads its (cos, sin) row once for all of them, and has four turns of rows in flight.
-template <typename T, int D, bool ALIGNED, bool QONLY>
+// loads its (cos, sin) row once for all of them. The rows come TURNS turns at a time, requested before the token is looked up
+// and then before the turns in front of them are stored (the compiler must keep loads and stores in order).
+template <typename T, int D, bool ALIGNED, bool QONLY, int TURNS>
 __device__ __forceinline__ void append_rows(const AppendArgs& a, long long unit) {
   constexpr int LPR = D / 8, RPS = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int t = static_cast<int>(unit / a.head_blocks);
-  const int block0 = static_cast<int>(unit % a.head_blocks) * (a.steps * RPS);
+  const int h_begin = static_cast<int>(unit % a.head_blocks) * (a.steps * RPS);
+  const int h_end = min(QONLY ? a.Hq : a.Hq + 2 * a.kv.kv_heads, h_begin + a.steps * RPS);
   const int d0 = (lane % LPR) * 8;
   if (t >= a.kv.total) return;
+  RawRow raw[TURNS];
+  auto request = [&](int h0) {
+#pragma unroll
+    for (int st = 0; st < TURNS; ++st) {
+      const int h = h0 + st * RPS + lane / LPR, hk = h - a.Hq, hv = hk - a.kv.kv_heads;
+      const T* in = nullptr;
+      if (h < h_end) {
+        if (QONLY || hk < 0) in = reinterpret_cast<const T*>(a.q) + t * a.qs.tok + h * a.qs.head;
+        else if (hv < 0) in = reinterpret_cast<const T*>(a.k) + t * a.ks.tok + hk * a.ks.head;
+        else in = reinterpret_cast<const T*>(a.v) + t * a.vs.tok + hv * a.vs.head;
+      }
+      raw[st] = load_row<T, ALIGNED>(a, in, d0);
+    }
+  };
+  request(h_begin);
   int b, ctx, i;
   if (!find_token(a, t, b, ctx, i)) return;
   long long pos;
   if (!find_position(a, t, ctx, i, pos)) return;
-  const int heads = QONLY ? a.Hq : a.Hq + 2 * a.kv.kv_heads;
   T* krow = nullptr;
   T* vrow = nullptr;
   if (!QONLY) {
@@ -200,49 +241,51 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, long long unit)
       vrow = reinterpret_cast<T*>(a.kv.v_pages) + off;
     }
   }
+  T* qrow = reinterpret_cast<T*>(a.q_out) + static_cast<size_t>(t) * a.Hq * D + d0;
   Turn turn;
   load_turn(a, pos, d0, turn);
-  const int block_end = min(heads, block0 + a.steps * RPS);
 #pragma unroll 1
-  for (int h0 = block0; h0 < block_end; h0 += 4 * RPS) {
+  for (int h0 = h_begin; h0 < h_end; h0 += TURNS * RPS) {
+    uint4 w[TURNS];
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      if (h0 + st * RPS >= block_end) break;  // whole warps
-      int h = h0 + st * RPS + lane / LPR;
-      const T* in = nullptr;
-      T* out = nullptr;
-      bool rot = true;
-      if (h < a.Hq) {
-        in = reinterpret_cast<const T*>(a.q) + t * a.qs.tok + h * a.qs.head;
-        out = reinterpret_cast<T*>(a.q_out) + (static_cast<size_t>(t) * a.Hq + h) * D + d0;
-      } else if (h < heads) {
-        h -= a.Hq;
-        rot = h < a.kv.kv_heads;
-        if (!rot) h -= a.kv.kv_heads;
-        in = rot ? reinterpret_cast<const T*>(a.k) + t * a.ks.tok + h * a.ks.head
-                 : reinterpret_cast<const T*>(a.v) + t * a.vs.tok + h * a.vs.head;
-        out = rot ? krow : vrow;
-        if (out != nullptr) out += (static_cast<size_t>(h) << a.kv.page_shift) * D;
+    for (int st = 0; st < TURNS; ++st) {
+      const int h = h0 + st * RPS + lane / LPR;
+      const bool rot = a.freqs != nullptr && (QONLY || h < a.Hq + a.kv.kv_heads);
+      w[st] = raw[st].x;
+      if (__any_sync(MUI_FULL_MASK, rot)) {
+        float y[8];
+        turn_row<T, ALIGNED>(a, raw[st], d0, true, turn, y);
+        if (rot) w[st] = pack8<T>(y);
       }
-      float y[8];
-      load_row8<T, D, ALIGNED>(a, in, d0, rot && a.freqs != nullptr, turn, y);
-      if (out != nullptr) *reinterpret_cast<uint4*>(out) = pack8<T>(y);
+    }
+    if (h0 + TURNS * RPS < h_end) request(h0 + TURNS * RPS);
+#pragma unroll
+    for (int st = 0; st < TURNS; ++st) {
+      const int h = h0 + st * RPS + lane / LPR, hk = h - a.Hq, hv = hk - a.kv.kv_heads;
+      if (h >= h_end) continue;
+      T* out = qrow + h * D;
+      if (!QONLY && hk >= 0) {
+        out = hv < 0 ? krow : vrow;
+        if (out == nullptr) continue;
+        out += (static_cast<size_t>(hv < 0 ? hk : hv) << a.kv.page_shift) * D;
+      }
+      *reinterpret_cast<uint4*>(out) = w[st];
     }
   }
 }
 
-template <typename T, int D, bool ALIGNED>
+template <typename T, int D, bool ALIGNED, int TURNS>
 __global__ void __launch_bounds__(PC_THREADS) append_rows_kernel(const AppendArgs a) {
   pdl_wait_prior_grid();
   pdl_launch_dependents();
-  append_rows<T, D, ALIGNED, false>(a, static_cast<long long>(blockIdx.x) * PC_WARPS + (threadIdx.x >> 5));
+  append_rows<T, D, ALIGNED, false, TURNS>(a, static_cast<long long>(blockIdx.x) * PC_WARPS + (threadIdx.x >> 5));
 }
 
-// One unit: the new rows of K (which == 0) or V of one head in one page, by `GROUPS` groups of D / 8 lanes (group index
-// `group`), at most ROWS rows per group. BLOCK: the groups span the CTA, else one warp.
+// Units: the new rows of K (which == 0) or V of the heads [head, head_end) in one page, by `GROUPS` groups of D / 8 lanes, at
+// most ROWS rows per group. BLOCK: the groups span the CTA (s_max: two sets of one float per warp, used in turn), else one warp.
 template <typename T, int D, bool ALIGNED, int ROWS, bool BLOCK>
-__device__ __forceinline__ void append_unit(const AppendArgs& a, int page, int first_row, int count, int ctx, int page_idx,
-                                            int head, int which, float* s_max) {
+__device__ __forceinline__ void append_units(const AppendArgs& a, int page, int first_row, int count, int ctx, int page_idx,
+                                             int head, int head_end, int which, float (*s_max)[PC_WARPS]) {
   constexpr int LPR = D / 8;
   constexpr int GROUPS = (BLOCK ? PC_THREADS : 32) / LPR;
   const int tid = BLOCK ? threadIdx.x : (threadIdx.x & 31);
@@ -251,73 +294,93 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, int page, int f
   const long long p0 = static_cast<long long>(page_idx) << a.kv.page_shift;  // first position of the page
   const int lo = p0 < ctx ? static_cast<int>(ctx - p0) : 0;                   // slots [lo, hi) are new
   const int hi = static_cast<int>(min(static_cast<long long>(ps), static_cast<long long>(ctx) + count - p0));
-  const T* in = which == 0 ? reinterpret_cast<const T*>(a.k) + head * a.ks.head
-                           : reinterpret_cast<const T*>(a.v) + head * a.vs.head;
-  const int64_t tok_stride = which == 0 ? a.ks.tok : a.vs.tok;
-  float* scale_p = (which == 0 ? a.kv.k_scales : a.kv.v_scales) + static_cast<size_t>(page) * a.kv.kv_heads + head;
-  uint8_t* out = reinterpret_cast<uint8_t*>(which == 0 ? a.kv.k_pages : a.kv.v_pages) +
-                 ((static_cast<size_t>(page) * a.kv.kv_heads + head) << a.kv.page_shift) * D + d0;
-  const float old_scale = lo > 0 ? __ldcg(scale_p) : 0.f;
+  const mui_strides2_t st = which == 0 ? a.ks : a.vs;
+  const T* in = reinterpret_cast<const T*>(which == 0 ? a.k : a.v);
+  const bool rot = which == 0 && a.freqs != nullptr;
 
-  float y[ROWS][8];
   bool have[ROWS];
-  float amax = 0.f;
+  long long pos[ROWS];
+  const T* src[ROWS];
 #pragma unroll
   for (int r = 0; r < ROWS; ++r) {
     const int slot = lo + r * GROUPS + group;
     const int i = static_cast<int>(p0 - ctx) + slot;  // place among the sequence's new tokens
     have[r] = slot < hi;
-    long long pos = 0;
-    if (have[r]) have[r] = find_position(a, first_row + i, ctx, i, pos);
-    Turn turn;
-    const bool rot = which == 0 && a.freqs != nullptr;
-    if (rot) load_turn(a, have[r] ? pos : 0, d0, turn);
-    load_row8<T, D, ALIGNED>(a, have[r] ? in + (first_row + i) * tok_stride : nullptr, d0, rot, turn, y[r]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float m = fabsf(y[r][e]);
-      if (m <= 3.402823466e38f) amax = fmaxf(amax, m);  // false for infinities and NaN
-    }
+    pos[r] = 0;
+    if (have[r]) have[r] = find_position(a, first_row + i, ctx, i, pos[r]);
+    if (!have[r]) pos[r] = 0;
+    src[r] = in + (first_row + i) * st.tok;
   }
-  amax = warp_max(amax);
-  if (BLOCK) {
-    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
-    __syncthreads();  // also: every thread has read the old scale. s_max alternates from head to head
+  RawRow raw[ROWS];
+  float old_scale = 0.f;
+  auto request = [&](int h) {
 #pragma unroll
-    for (int w = 0; w < PC_WARPS; ++w) amax = fmaxf(amax, s_max[w]);
-  }
-  float scale = exp2_int(e4m3_scale_exp(amax));
-  float inv = exp2_int(-e4m3_scale_exp(amax));
-  if (lo > 0 && !(old_scale < scale)) {
-    scale = old_scale;
-    inv = 1.f / old_scale;
-  } else if (lo > 0) {
-    // the page's earlier rows move to the larger scale
-    const float ratio = old_scale * inv;
-    for (int slot = group; slot < lo; slot += GROUPS) {
-      uint2* p = reinterpret_cast<uint2*>(out + static_cast<size_t>(slot) * D);
-      const uint2 w = __ldcg(p);
-      uint32_t n[2];
+    for (int r = 0; r < ROWS; ++r) raw[r] = load_row<T, ALIGNED>(a, have[r] ? src[r] + h * st.head : nullptr, d0);
+    float* p = (which == 0 ? a.kv.k_scales : a.kv.v_scales) + static_cast<size_t>(page) * a.kv.kv_heads + h;
+    old_scale = lo > 0 ? __ldcg(p) : 0.f;
+  };
+  request(head);
+#pragma unroll 1
+  for (; head < head_end; ++head) {
+    float* scale_p = (which == 0 ? a.kv.k_scales : a.kv.v_scales) + static_cast<size_t>(page) * a.kv.kv_heads + head;
+    uint8_t* out = reinterpret_cast<uint8_t*>(which == 0 ? a.kv.k_pages : a.kv.v_pages) +
+                   ((static_cast<size_t>(page) * a.kv.kv_heads + head) << a.kv.page_shift) * D + d0;
+    const float was = old_scale;
+    float y[ROWS][8];
+    float amax = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t u = h == 0 ? w.x : w.y;
-        const float2 f0 = Elt<__half>::unpack2(e4m3_to_half2(static_cast<uint16_t>(u)));
-        const float2 f1 = Elt<__half>::unpack2(e4m3_to_half2(static_cast<uint16_t>(u >> 16)));
-        n[h] = e4m3_pack2(f0.x * ratio, f0.y * ratio) | (e4m3_pack2(f1.x * ratio, f1.y * ratio) << 16);
+    for (int r = 0; r < ROWS; ++r) {
+      Turn turn;
+      if (rot) load_turn(a, pos[r], d0, turn);
+      turn_row<T, ALIGNED>(a, raw[r], d0, rot, turn, y[r]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float m = fabsf(y[r][e]);
+        if (m <= 3.402823466e38f) amax = fmaxf(amax, m);  // false for infinities and NaN
       }
-      *p = make_uint2(n[0], n[1]);
     }
-  }
-  if (!BLOCK) __syncwarp();
-  if (tid == 0) *scale_p = scale;
+    if (head + 1 < head_end) request(head + 1);  // in flight while this head is stored
+    amax = warp_max(amax);
+    if (BLOCK) {
+      float* m = s_max[head & 1];
+      if ((threadIdx.x & 31) == 0) m[threadIdx.x >> 5] = amax;
+      __syncthreads();  // also: every thread has the old scale
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    if (!have[r]) continue;
-    const int slot = lo + r * GROUPS + group;
-    uint2 w;
-    w.x = e4m3_pack2(y[r][0] * inv, y[r][1] * inv) | (e4m3_pack2(y[r][2] * inv, y[r][3] * inv) << 16);
-    w.y = e4m3_pack2(y[r][4] * inv, y[r][5] * inv) | (e4m3_pack2(y[r][6] * inv, y[r][7] * inv) << 16);
-    *reinterpret_cast<uint2*>(out + static_cast<size_t>(slot) * D) = w;
+      for (int w = 0; w < PC_WARPS; ++w) amax = fmaxf(amax, m[w]);
+    }
+    float scale = exp2_int(e4m3_scale_exp(amax));
+    float inv = exp2_int(-e4m3_scale_exp(amax));
+    if (lo > 0 && !(was < scale)) {
+      scale = was;
+      inv = 1.f / was;
+    } else if (lo > 0) {
+      // the page's earlier rows move to the larger scale
+      const float ratio = was * inv;
+      for (int slot = group; slot < lo; slot += GROUPS) {
+        uint2* p = reinterpret_cast<uint2*>(out + static_cast<size_t>(slot) * D);
+        const uint2 w = __ldcg(p);
+        uint32_t n[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t u = h == 0 ? w.x : w.y;
+          const float2 f0 = Elt<__half>::unpack2(e4m3_to_half2(static_cast<uint16_t>(u)));
+          const float2 f1 = Elt<__half>::unpack2(e4m3_to_half2(static_cast<uint16_t>(u >> 16)));
+          n[h] = e4m3_pack2(f0.x * ratio, f0.y * ratio) | (e4m3_pack2(f1.x * ratio, f1.y * ratio) << 16);
+        }
+        *p = make_uint2(n[0], n[1]);
+      }
+    }
+    if (!BLOCK) __syncwarp();
+    if (tid == 0) *scale_p = scale;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (!have[r]) continue;
+      const int slot = lo + r * GROUPS + group;
+      uint2 w;
+      w.x = e4m3_pack2(y[r][0] * inv, y[r][1] * inv) | (e4m3_pack2(y[r][2] * inv, y[r][3] * inv) << 16);
+      w.y = e4m3_pack2(y[r][4] * inv, y[r][5] * inv) | (e4m3_pack2(y[r][6] * inv, y[r][7] * inv) << 16);
+      *reinterpret_cast<uint2*>(out + static_cast<size_t>(slot) * D) = w;
+    }
   }
 }
 
@@ -328,7 +391,7 @@ __global__ void __launch_bounds__(PC_THREADS) append_e4m3_token_kernel(const App
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5;
   if (static_cast<int>(blockIdx.x) >= a.unit_blocks) {
-    append_rows<T, D, ALIGNED, true>(a, static_cast<long long>(blockIdx.x - a.unit_blocks) * PC_WARPS + warp);
+    append_rows<T, D, ALIGNED, true, 1>(a, static_cast<long long>(blockIdx.x - a.unit_blocks) * PC_WARPS + warp);
     return;
   }
   const long long u = static_cast<long long>(blockIdx.x) * PC_WARPS + warp;
@@ -341,7 +404,8 @@ __global__ void __launch_bounds__(PC_THREADS) append_e4m3_token_kernel(const App
     return;
   }
   const int page = find_page(a.kv, b, ctx);
-  if (page >= 0) append_unit<T, D, ALIGNED, 1, false>(a, page, b, 1, ctx, ctx >> a.kv.page_shift, r >> 1, r & 1, nullptr);
+  if (page >= 0) 
+    append_units<T, D, ALIGNED, 1, false>(a, page, b, 1, ctx, ctx >> a.kv.page_shift, r >> 1, (r >> 1) + 1, r & 1, nullptr);
 }
 
 // e4m3 pages, any number of new tokens: a CTA per (sequence, page, block of heads, K or V), then the q rows. Pages are numbered
@@ -352,7 +416,7 @@ __global__ void __launch_bounds__(PC_THREADS) append_e4m3_kernel(const AppendArg
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   if (static_cast<int>(blockIdx.x) >= a.unit_blocks) {
-    append_rows<T, D, ALIGNED, true>(
+    append_rows<T, D, ALIGNED, true, 4>(
         a, static_cast<long long>(blockIdx.x - a.unit_blocks) * PC_WARPS + (threadIdx.x >> 5));
     return;
   }
@@ -373,10 +437,9 @@ __global__ void __launch_bounds__(PC_THREADS) append_e4m3_kernel(const AppendArg
   if (count == 0 || (static_cast<long long>(page_idx) << sh) >= static_cast<long long>(ctx) + count) return;
   const int page = find_page(a.kv, b, static_cast<long long>(page_idx) << sh);
   if (page < 0) return;
-  const int head0 = (r >> 1) * a.unit_heads, head1 = min(a.kv.kv_heads, head0 + a.unit_heads);
-#pragma unroll 1
-  for (int head = head0; head < head1; ++head)
-    append_unit<T, D, ALIGNED, ROWS, true>(a, page, first, count, ctx, page_idx, head, r & 1, s_max[head & 1]);
+  const int head = (r >> 1) * a.unit_heads;
+  append_units<T, D, ALIGNED, ROWS, true>(a, page, first, count, ctx, page_idx, head, min(a.kv.kv_heads, head + a.unit_heads), r & 1,
+                                          s_max);
 }
 
 template <typename T, int D, bool ALIGNED>
@@ -398,7 +461,10 @@ mui_status_t launch_append(cudaStream_t stream, AppendArgs a, bool e4m3, int pag
     choose_steps(a.Hq + 2 * a.kv.kv_heads);
     const long long n = blocks(static_cast<long long>(a.kv.total) * a.head_blocks);
     MUI_REQUIRE(n <= limit, MUI_ERR_UNSUPPORTED, "too many rows");
-    MUI_CUDA_CHECK(mui_launch(append_rows_kernel<T, D, ALIGNED>, dim3((unsigned)n), block, 0, stream, pdl, a));
+    if (a.steps == 1)
+      MUI_CUDA_CHECK(mui_launch(append_rows_kernel<T, D, ALIGNED, 1>, dim3((unsigned)n), block, 0, stream, pdl, a));
+    else
+      MUI_CUDA_CHECK(mui_launch(append_rows_kernel<T, D, ALIGNED, 4>, dim3((unsigned)n), block, 0, stream, pdl, a));
     return MUI_OK;
   }
   choose_steps(a.Hq);
