@@ -275,7 +275,7 @@ __device__ __forceinline__ void append_rows(const AppendArgs& a, long long unit)
 }
 
 template <typename T, int D, bool ALIGNED, int TURNS>
-__global__ void __launch_bounds__(PC_THREADS) append_rows_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(PC_THREADS, TURNS == 1 ? 4 : 3) append_rows_kernel(const AppendArgs a) {
   pdl_wait_prior_grid();
   pdl_launch_dependents();
   append_rows<T, D, ALIGNED, false, TURNS>(a, static_cast<long long>(blockIdx.x) * PC_WARPS + (threadIdx.x >> 5));
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(PC_THREADS) append_e4m3_token_kernel(const App
 // e4m3 pages, any number of new tokens: a CTA per (sequence, page, block of heads, K or V), then the q rows. Pages are numbered
 // through: sequence b's start at cu[b] / page_size + 2 b, which leaves room for every page that its tokens can touch.
 template <typename T, int D, bool ALIGNED, int ROWS>
-__global__ void __launch_bounds__(PC_THREADS) append_e4m3_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(PC_THREADS, ROWS <= 2 ? 3 : 2) append_e4m3_kernel(const AppendArgs a) {
   __shared__ float s_max[2][PC_WARPS];
   pdl_wait_prior_grid();
   pdl_launch_dependents();
