@@ -322,6 +322,33 @@ def test_attention_scales_and_peaks(dtype, e4m3):
     _check_attention(c, q.to(dtype), scale=0.02)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("ctx,new,Hq,Hkv,D,page", [
+    ([5000], [40], 8, 2, 128, 64),                      # a short prompt behind a long context: the span is split and joined
+    ([3000, 4100], [33, 9], 4, 1, 64, 16),              # the same, two sequences
+    ([300, 40, 900, 7], [1, 90, 2, 1], 8, 2, 128, 16),  # single tokens and prompts in one call: both kernels
+    ([20, 0, 129], [300, 128, 1], 16, 1, 64, 128),
+    ([1], [1023], 2, 1, 128, 32),                       # rows of two whole tiles but one
+])
+def test_attention_prompts_split_and_mixed(e4m3, ctx, new, Hq, Hkv, D, page):
+    for dtype in (F16, BF16):
+        c = _filled(ctx, new, Hkv, D, page, dtype, e4m3, seed=24, spread=0.5)
+        q = torch.randn(sum(new), Hq, D, generator=_gen(25)).to(dtype)
+        _check_attention(c, q)
+        _check_attention(c, q, window=700, sinks=5)
+
+
+@pytest.mark.parametrize("new", [1, 60])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
+def test_attention_scales_of_any_sign(new, scale):
+    """A scale of 0 (the mean over the visible rows), a negative one, and one that lets a single row win."""
+    for e4m3 in (False, True):
+        c = _filled([170, 3], [new, new], 2, 64, 16, F16, e4m3, seed=26, spread=0.2)
+        q = torch.randn(2 * new, 4, 64, generator=_gen(27)).to(F16)
+        _check_attention(c, q, scale=scale)
+        _check_attention(c, torch.zeros_like(q), scale=scale, window=20, sinks=2)
+
+
 @pytest.mark.parametrize("hint", [1, 64, 600, 100000])
 def test_attention_context_hint_does_not_matter(hint):
     c = _filled([900, 10, 0], [1, 1, 1], 2, 128, 16, F16, False, seed=17)
@@ -449,6 +476,45 @@ def test_sample_ties_and_constant_rows(dtype):
         _check_sample(x.to(dtype), u, top_k=torch.tensor([1, 7, 20000, 49999], dtype=torch.int32))
         _check_sample(x.to(dtype), u, top_p=torch.tensor([0.1, 0.37, 0.9, 0.61]),
                       top_k=torch.tensor([0, 30000, 0, 12345], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_sample_many_candidates(dtype, rows):
+    """Flat rows: more kept tokens than are collected in one place, for each kind of cut and all together."""
+    g = _gen(35 + rows)
+    V = 60000
+    logits = torch.randn(rows, V, generator=g).to(dtype)
+    u = torch.rand(rows, generator=g)
+    t = 1.0 + torch.rand(rows, generator=g)
+    k = torch.randint(12200, 50000, (rows,), generator=g).to(torch.int32)
+    p = 0.6 + 0.39 * torch.rand(rows, generator=g)
+    m = 0.01 + 0.02 * torch.rand(rows, generator=g)
+    _check_sample(logits, u, t)
+    _check_sample(logits, u, t, top_k=k)
+    _check_sample(logits, u, t, top_p=p)
+    _check_sample(logits, u, t, min_p=m)
+    _check_sample(logits, u, t, top_k=k, top_p=p)
+    _check_sample(logits, u, t, top_p=p, min_p=m)
+    _check_sample(logits, u, t, top_k=k, top_p=p, min_p=m)
+    # so hot that one bin holds thousands
+    _check_sample(logits, u, 60 * t, top_k=k, top_p=p)
+    _check_sample(logits, u, 400 * t, top_p=p)
+
+
+def test_sample_masked_logits():
+    """Tokens that a grammar forbids carry the type's lowest value or -infinity."""
+    g = _gen(36)
+    x = 3 * torch.randn(6, 5000, generator=g)
+    allowed = torch.rand(6, 5000, generator=g) < 0.01
+    u = torch.rand(6, generator=g)
+    for dtype in (F16, BF16, torch.float32):
+        for low in (torch.finfo(dtype).min, -math.inf):
+            y = torch.where(allowed, x, torch.tensor(low)).to(dtype)
+            for kw in ({}, dict(top_k=torch.full((6,), 200, dtype=torch.int32)), dict(top_p=torch.full((6,), 0.99)),
+                       dict(min_p=torch.full((6,), 1e-6))):
+                tokens = _check_sample(y, u, **kw)
+                assert allowed[torch.arange(6), tokens.cpu()].all()
 
 
 def test_sample_special_values():
