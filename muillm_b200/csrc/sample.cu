@@ -13,7 +13,7 @@
 //   2. with top-k or top-p, a histogram of z in 2048 equal bins down to the smallest z that still has weight. Counts give the
 //      bin that holds the top_k-th token exactly; counts times the bin centre's weight tell the bin in which top_p ends,
 //      nearly always. Not needed where min-p alone leaves few tokens;
-//   3. all tokens up to that bin (or above min-p's cut) are collected in rank 0's shared memory if they are at most 12288, with
+//   3. all tokens up to that bin (or above min-p's cut) are collected in rank 0's shared memory if they are at most 16384, with
 //      the weight of the whole row where top-p asks for it. Rank 0 sums them by bins of z, sorts the bins in which top-k and
 //      top-p end, sums the kept ones by parts of the index range and sorts the part that holds the drawn point.
 // More tokens than that (a wide nucleus, a temperature without cuts):
@@ -41,8 +41,8 @@ constexpr int SM_THREADS = 512;
 constexpr int SM_WARPS = SM_THREADS / 32;
 constexpr int SM_CHUNK = 256;    // tokens of one warp step: eight consecutive ones per lane
 constexpr int SM_BINS = 2048;
-constexpr int SM_LIST = 12288;   // tokens collected at most
-constexpr int SM_SMALL = 4096;   // tokens of one bin at most
+constexpr int SM_LIST = 16384;   // tokens collected at most
+constexpr int SM_SMALL = 2048;   // tokens of one bin at most
 constexpr int SM_MAX_VOCAB = 1 << 22;  // a part of an index range in SM_BINS parts fits the small list
 constexpr int SM_RUNS = SM_THREADS;  // runs of chunks whose kept weight a CTA holds
 constexpr int SM_MAX_CLUSTER = 8;
@@ -92,11 +92,6 @@ __device__ __forceinline__ uint32_t peer_addr(const void* local, unsigned rank) 
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
   return r;
 }
-__device__ __forceinline__ uint32_t peer_u32(const void* local, unsigned rank) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_addr(local, rank)) : "memory");
-  return v;
-}
 __device__ __forceinline__ void store_peer_u64(u64* local, unsigned rank, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(peer_addr(local, rank)), "l"(v) : "memory");
 }
@@ -116,12 +111,11 @@ struct Shared {
   float warp_f32[SM_WARPS];
   uint32_t warp_u32[SM_WARPS];
   uint32_t list_n[2];
-  uint32_t T, T_idx;
-  // rank 0's findings, read by its peers
-  struct {
-    uint32_t verdict, before_k, collect;
+  // rank 0's findings, and their copy in every CTA
+  struct Say {
+    uint32_t verdict, before_k, collect, small_bins, T, T_idx;
     int bin_k, bin_p;
-  } say;
+  } say, said;
   float est_total;
   // a bin that rank 0 looks for, with what lies in front of it
   int bin;
@@ -129,6 +123,20 @@ struct Shared {
   u64 bin_mass;
   int hit;
 };
+
+// Rank 0 hands its findings to every CTA of the cluster (all of them call this).
+__device__ __forceinline__ void tell(Shared& s, int cluster, unsigned rank) {
+  constexpr int WORDS = sizeof(Shared::Say) / 4;
+  if (rank == 0) {
+    __syncthreads();
+    const int to = threadIdx.x / WORDS, word = threadIdx.x % WORDS;
+    if (to < cluster)
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(peer_addr(reinterpret_cast<uint32_t*>(&s.said) + word, to)),
+                   "r"(reinterpret_cast<const uint32_t*>(&s.say)[word])
+                   : "memory");
+  }
+  cluster_sync(cluster);
+}
 
 // Eight tokens as they sit in memory: 16 bytes, or twice 16 bytes of fp32. A lane's eight tokens of a chunk are consecutive
 // 16-bit ones, or four and another four half a chunk on, so that a warp reads whole lines: token e is i + e + gap<T>(e).
@@ -572,7 +580,36 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
 
   // Rank 0 turns a complete list of the tokens in front (n of them, `total` the weight of the row for top-p without top-k) into
   // the drawn token. cut_p: the list ends where top-p was expected to end; false is returned when it does not.
+  // a few tokens: sorted whole, by rank and then by index
+  auto finish_few = [&](int n, u64 total, bool cut_p) {
+    sort_list(s.list, n);
+    const u64 all = weigh_list<32>(s, s.list, s.small_w, n, w);
+    auto before = [&](int i) { return i < n ? s.small_w[i] : all; };
+    int keep = use_k ? min(n, k_raw) : n;
+    if (use_p) {
+      const double target = static_cast<double>(top_p) * static_cast<double>(use_k ? before(keep) : total);
+      if (cut_p && static_cast<double>(all) < target) return false;
+      keep = max(1, leading(keep, [&](int i) { return static_cast<double>(before(i)) < target; }));
+    }
+    keep = leading(keep, [&](int i) { return before(i + 1) - before(i) >= w_min; });
+    const u64 mass = before(keep);
+    const double want = u * static_cast<double>(mass);
+    for (int i = tid; i < keep; i += SM_THREADS) s.small[i] = s.list[i] << 32 | s.list[i] >> 32;  // ~index, key
+    __syncthreads();
+    sort_list(s.small, keep);
+    weigh_list<0>(s, s.small, s.small_w, keep, w);
+    for (int i = tid; i < keep; i += SM_THREADS) {
+      // the first token at which the running weight exceeds the point
+      const u64 from = s.small_w[i], to = i + 1 < keep ? s.small_w[i + 1] : mass;
+      if (static_cast<double>(to) > want && static_cast<double>(from) <= want) {
+        a.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.small[i] >> 32));
+        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(to - from) / static_cast<double>(mass)));
+      }
+    }
+    return true;
+  };
   auto finish = [&](int n, u64 total, bool cut_p) {
+    if (n <= SM_THREADS) return finish_few(n, total, cut_p);
     constexpr int PER = SM_BINS / SM_THREADS;
     uint32_t cn[PER], cb = 0;
     u64 mn[PER], mb = 0, all = 0;
@@ -733,8 +770,8 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     }
     return true;
   };
-  // Collects the tokens that in(x) names in rank 0's list. v[0]: the weight of the whole row if asked for, v[1]: their number
-  // (over SM_LIST: the list is incomplete).
+  // Collects the tokens that in(x) names in rank 0's list. v[0]: the weight of the whole row if asked for, v[1]: their number if
+  // asked for (over SM_LIST: the list is incomplete).
   const uint32_t count_at[2] = {peer_addr(&s.list_n[0], 0), peer_addr(&s.list_n[1], 0)};
   const uint32_t list_at[2] = {peer_addr(s.list, 0), peer_addr(s.small, 0)};
   auto put = [&](int which, float x, int i, uint32_t room) {
@@ -744,7 +781,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list_at[which] + at * 8), "l"(rank_entry(x, i)) : "memory");
   };
   u64 v[3];
-  auto collect = [&](auto in, bool weigh) {
+  auto collect = [&](auto in, bool weigh, bool count) {
     v[0] = v[1] = v[2] = 0;
     row.each([&](int i, float(&x)[8]) {
       if (weigh) {
@@ -761,13 +798,15 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
           ++v[1];
         }
     });
-    cluster_sum3(s, C, rank, turn, v);  // its barrier also publishes the list
+    // a barrier of the cluster either way: it publishes the list
+    if (weigh || count) cluster_sum3(s, C, rank, turn, v);
+    else cluster_sync(C);
   };
 
   uint32_t T_key = 0, T_idx = 0;  // nothing to cut: every key that has weight is above 0
   bool bisect = false;
   if (min_p > 0.f && !use_k) {
-    collect([&](float x) { return x >= x_min; }, use_p);
+    collect([&](float x) { return x >= x_min; }, use_p, true);
     if (v[1] <= SM_LIST) {
       if (rank == 0) finish(static_cast<int>(v[1]), v[0], false);
       return;
@@ -797,6 +836,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
       if (tid == 0) {
         s.say.bin_k = s.say.bin_p = SM_BINS;
         s.say.before_k = 0;
+        s.say.small_bins = 1;
       }
       uint32_t n[PER], nc = 0, n_all;
       float m[PER], mc = 0.f, all;
@@ -807,6 +847,10 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
         nc += n[h];
         mc += m[h];
       }
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < PER; ++h)
+        if (n[h] > SM_SMALL) s.say.small_bins = 0;
       const uint32_t nb = block_scan(nc, s.warp_u32, n_all);
       const float mb = block_scan(mc, s.warp_f32, all);
       if (use_k) {
@@ -856,26 +900,28 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
       __syncthreads();
       if (tid == 0) s.say.bin_p = bin_p;
     }
-    cluster_sync(C);
-    const int bin_k = static_cast<int>(peer_u32(&s.say.bin_k, 0));
-    int bin_p = static_cast<int>(peer_u32(&s.say.bin_p, 0));
-    const uint32_t before_k = peer_u32(&s.say.before_k, 0);
-    if (peer_u32(&s.say.collect, 0)) {
+    tell(s, C, rank);
+    const int bin_k = s.said.bin_k;
+    int bin_p = s.said.bin_p;
+    const uint32_t before_k = s.said.before_k;
+    if (s.said.collect) {
       // 3. the tokens in front
       const int last = use_k ? bin_k : min(bin_p + 1, SM_BINS);
-      collect([&](float x) { return w.bin(x) < SM_BINS && w.bin(x) <= last; }, use_p && !use_k);
+      collect([&](float x) { return w.bin(x) < SM_BINS && w.bin(x) <= last; }, use_p && !use_k, false);
+      // with top-k the list is complete for sure: only rank 0 goes on
+      const bool sure = use_k && s.said.small_bins;
+      if (sure && rank != 0) return;
       if (rank == 0) {
         const bool ok = finish(static_cast<int>(s.list_n[0]), v[0], use_p && !use_k && last < SM_BINS);
+        if (sure) return;
         __syncthreads();
         if (tid == 0) {
           s.say.verdict = ok ? SM_FOUND : SM_UP;
           s.list_n[0] = 0;
         }
       }
-      cluster_sync(C);
-      const bool ok = peer_u32(&s.say.verdict, 0) == SM_FOUND;
-      if (C > 1) cluster_sync(C);  // the verdict has been read
-      if (ok) return;
+      tell(s, C, rank);
+      if (s.said.verdict == SM_FOUND) return;
     }
     bisect = use_p || bin_k < SM_BINS;  // a top_p next to 1 may end in no bin
     for (int attempt = 0; attempt < 4 && bin_p < SM_BINS; ++attempt) {
@@ -945,8 +991,8 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
             if (next < 0 || next > bin_k || next >= SM_BINS) say = SM_BISECT;
           }
           if (tid == 0) {
-            s.T = static_cast<uint32_t>(last >> 32);
-            s.T_idx = ~static_cast<uint32_t>(last);
+            s.say.T = static_cast<uint32_t>(last >> 32);
+            s.say.T_idx = ~static_cast<uint32_t>(last);
           }
         }
         __syncthreads();
@@ -956,12 +1002,12 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
         }
         if (tid < 2) s.list_n[tid] = 0;
       }
-      cluster_sync(C);
-      const uint32_t verdict = peer_u32(&s.say.verdict, 0);
-      bin_p = static_cast<int>(peer_u32(&s.say.bin_p, 0));
-      T_key = peer_u32(&s.T, 0);
-      T_idx = peer_u32(&s.T_idx, 0);
-      cluster_sync(C);  // rank 0's findings have been read
+      tell(s, C, rank);
+      const uint32_t verdict = s.said.verdict;
+      bin_p = s.said.bin_p;
+      T_key = s.said.T;
+      T_idx = s.said.T_idx;
+      cluster_sync(C);  // the findings have been read before rank 0 has others
       bisect = verdict != SM_FOUND;
       if (verdict == SM_FOUND || verdict == SM_BISECT) break;
     }
