@@ -12,7 +12,8 @@
 //   1. the largest logit (from HBM; the later passes find the row in L2);
 //   2. with top-k or top-p, a histogram of z in 2048 equal bins down to the smallest z that still has weight. Counts give the
 //      bin that holds the top_k-th token exactly; counts times the bin centre's weight tell the bin in which top_p ends,
-//      nearly always. Not needed where min-p alone leaves few tokens;
+//      nearly always. Not needed where min-p alone leaves few tokens, nor for a top_k of at most the number of threads: there
+//      the threads' own largest logits, known from 1, are counted instead of all, and give a bin that is far enough down;
 //   3. all tokens up to that bin (or above min-p's cut) are collected in rank 0's shared memory if they are at most 16384, with
 //      the weight of the whole row where top-p asks for it. Rank 0 sums them by bins of z, sorts the bins in which top-k and
 //      top-p end, sums the kept ones by parts of the index range and sorts the part that holds the drawn point.
@@ -495,6 +496,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   for (int i = tid; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0;
   if (tid < 2) s.list_n[tid] = 0;
   u64 best = 0;
+  float m = -INFINITY;  // the thread's own
   if (greedy) {
     row.each([&](int i, float(&x)[8]) {
 #pragma unroll
@@ -505,7 +507,6 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
       }
     });
   } else {
-    float m = -INFINITY;
     int c = row.c0 + warp;
     for (; c + 7 * SM_WARPS < row.c1; c += 8 * SM_WARPS) {  // eight chunks of loads in flight, 128 KiB per CTA of fp32
       Raw q[8];
@@ -813,6 +814,58 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     }
     if (tid == 0) s.list_n[0] = 0;  // a barrier follows before the next token is put there
   }
+  // bins of all CTAs summed in rank 0's
+  auto join_bins = [&]() {
+    if (rank != 0) {
+      __syncthreads();
+      for (int i = tid; i < SM_BINS; i += SM_THREADS)
+        if (const uint32_t n = s.bins[i])
+          asm volatile("red.shared::cluster.add.u32 [%0], %1;" ::"r"(peer_addr(&s.bins[i], 0)), "r"(n) : "memory");
+    }
+    cluster_sync(C);
+  };
+  if (use_k && k_raw <= C * SM_THREADS) {
+    // The largest logits of k threads are k tokens: whatever the bin of the k-th of them, the top-k lie in the bins up to it.
+    if (row.inf) m = m == INFINITY ? 0.f : -INFINITY;
+    const int mine = w.bin(m);
+    if (mine < SM_BINS) atomicAdd(&s.bins[mine], 1u);
+    join_bins();
+    if (rank == 0) {
+      constexpr int PER = SM_BINS / SM_THREADS;
+      const uint32_t k = static_cast<uint32_t>(k_raw);
+      uint32_t n[PER], at = 0, all;
+#pragma unroll
+      for (int h = 0; h < PER; ++h) {
+        n[h] = s.bins[PER * tid + h];
+        at += n[h];
+      }
+      if (tid == 0) s.say.bin_k = SM_BINS;
+      at = block_scan(at, s.warp_u32, all);
+#pragma unroll
+      for (int h = 0; h < PER; ++h) {
+        if (at < k && at + n[h] >= k) s.say.bin_k = PER * tid + h;  // one thread at most
+        at += n[h];
+      }
+    }
+    tell(s, C, rank);
+    const int last = s.said.bin_k;
+    collect([&](float x) { return w.bin(x) <= min(last, SM_BINS - 1); }, false, true);
+    if (v[1] <= SM_LIST) {
+      // SM_THREADS tokens or fewer are always brought to an end
+      if (rank != 0 && v[1] <= SM_THREADS) return;
+      if (rank == 0) {
+        const bool ok = finish(static_cast<int>(v[1]), 0, false);
+        if (v[1] <= SM_THREADS) return;
+        __syncthreads();
+        if (tid == 0) s.say.verdict = ok ? SM_FOUND : SM_UP;
+      }
+      tell(s, C, rank);
+      if (s.said.verdict == SM_FOUND) return;
+    }
+    for (int i = tid; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0;
+    if (tid == 0) s.list_n[0] = 0;
+    cluster_sync(C);
+  }
   if (use_k || use_p) {
     // 2. histogram
     row.each([&](int, float(&x)[8]) {
@@ -822,13 +875,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
         if (b < SM_BINS) atomicAdd(&s.bins[b], 1u);
       }
     });
-    if (rank != 0) {
-      __syncthreads();
-      for (int i = tid; i < SM_BINS; i += SM_THREADS)
-        if (const uint32_t n = s.bins[i])
-          asm volatile("red.shared::cluster.add.u32 [%0], %1;" ::"r"(peer_addr(&s.bins[i], 0)), "r"(n) : "memory");
-    }
-    cluster_sync(C);
+    join_bins();
     constexpr int PER = SM_BINS / SM_THREADS;
     const uint32_t k = static_cast<uint32_t>(k_raw);
     if (rank == 0) {
