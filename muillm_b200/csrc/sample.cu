@@ -45,6 +45,7 @@ constexpr int SM_BINS = 2048;
 constexpr int SM_LIST = 16384;   // tokens collected at most
 constexpr int SM_SMALL = 2048;   // tokens of one bin at most
 constexpr int SM_MAX_VOCAB = 1 << 22;  // a part of an index range in SM_BINS parts fits the small list
+constexpr int SM_FEW = 256;      // tokens that are compared pair by pair
 constexpr int SM_RUNS = SM_THREADS;  // runs of chunks whose kept weight a CTA holds
 constexpr int SM_MAX_CLUSTER = 8;
 // what rank 0 finds in the collected tokens: the threshold, that top-p ends further up or down the ranking, or too many tokens
@@ -581,36 +582,49 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
 
   // Rank 0 turns a complete list of the tokens in front (n of them, `total` the weight of the row for top-p without top-k) into
   // the drawn token. cut_p: the list ends where top-p was expected to end; false is returned when it does not.
-  // a few tokens: sorted whole, by rank and then by index
+  // Few tokens, one per thread: the tokens in front of each, by rank and then by index, are found by looking at all of them.
   auto finish_few = [&](int n, u64 total, bool cut_p) {
-    sort_list(s.list, n);
-    const u64 all = weigh_list<32>(s, s.list, s.small_w, n, w);
-    auto before = [&](int i) { return i < n ? s.small_w[i] : all; };
-    int keep = use_k ? min(n, k_raw) : n;
-    if (use_p) {
-      const double target = static_cast<double>(top_p) * static_cast<double>(use_k ? before(keep) : total);
-      if (cut_p && static_cast<double>(all) < target) return false;
-      keep = max(1, leading(keep, [&](int i) { return static_cast<double>(before(i)) < target; }));
-    }
-    keep = leading(keep, [&](int i) { return before(i + 1) - before(i) >= w_min; });
-    const u64 mass = before(keep);
-    const double want = u * static_cast<double>(mass);
-    for (int i = tid; i < keep; i += SM_THREADS) s.small[i] = s.list[i] << 32 | s.list[i] >> 32;  // ~index, key
+    const u64 mine = tid < n ? s.list[tid] : 0;
+    const u64 q = w(tid < n ? key_logit(static_cast<uint32_t>(mine >> 32)) : 0.f, tid < n);
+    if (tid < n) s.small_w[tid] = q;
     __syncthreads();
-    sort_list(s.small, keep);
-    weigh_list<0>(s, s.small, s.small_w, keep, w);
-    for (int i = tid; i < keep; i += SM_THREADS) {
-      // the first token at which the running weight exceeds the point
-      const u64 from = s.small_w[i], to = i + 1 < keep ? s.small_w[i + 1] : mass;
-      if (static_cast<double>(to) > want && static_cast<double>(from) <= want) {
-        a.tokens[r] = static_cast<int64_t>(~static_cast<uint32_t>(s.small[i] >> 32));
-        if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(to - from) / static_cast<double>(mass)));
+    int place = 0;
+    u64 front = 0;
+    if (tid < n)
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const bool before = s.list[j] > mine;
+        place += before;
+        front += before ? s.small_w[j] : 0ull;
       }
+    bool keep = tid < n && (!use_k || place < k_raw);
+    u64 within;
+    if (use_p) {
+      block_scan(keep ? q : 0ull, s.warp_u64, within);
+      const double target = static_cast<double>(top_p) * static_cast<double>(use_k ? within : total);
+      if (cut_p && static_cast<double>(within) < target) return false;
+      keep = keep && (place == 0 || static_cast<double>(front) < target);
+    }
+    keep = keep && q >= w_min;
+    __syncthreads();
+    if (tid < n) s.small_w[tid] = keep ? q : 0ull;
+    u64 mass;
+    block_scan(keep ? q : 0ull, s.warp_u64, mass);  // and a barrier
+    if (!keep) return true;
+    front = 0;
+    const uint32_t index = ~static_cast<uint32_t>(mine);
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) front += ~static_cast<uint32_t>(s.list[j]) < index ? s.small_w[j] : 0ull;
+    // the first token at which the running weight exceeds the point
+    const double want = u * static_cast<double>(mass);
+    if (static_cast<double>(front + q) > want && static_cast<double>(front) <= want) {
+      a.tokens[r] = static_cast<int64_t>(index);
+      if (a.logprobs) a.logprobs[r] = static_cast<float>(log(static_cast<double>(q) / static_cast<double>(mass)));
     }
     return true;
   };
   auto finish = [&](int n, u64 total, bool cut_p) {
-    if (n <= SM_THREADS) return finish_few(n, total, cut_p);
+    if (n <= SM_FEW) return finish_few(n, total, cut_p);
     constexpr int PER = SM_BINS / SM_THREADS;
     uint32_t cn[PER], cb = 0;
     u64 mn[PER], mb = 0, all = 0;
@@ -851,11 +865,11 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     const int last = s.said.bin_k;
     collect([&](float x) { return w.bin(x) <= min(last, SM_BINS - 1); }, false, true);
     if (v[1] <= SM_LIST) {
-      // SM_THREADS tokens or fewer are always brought to an end
-      if (rank != 0 && v[1] <= SM_THREADS) return;
+      // few tokens are always brought to an end
+      if (rank != 0 && v[1] <= SM_FEW) return;
       if (rank == 0) {
         const bool ok = finish(static_cast<int>(v[1]), 0, false);
-        if (v[1] <= SM_THREADS) return;
+        if (v[1] <= SM_FEW) return;
         __syncthreads();
         if (tid == 0) s.say.verdict = ok ? SM_FOUND : SM_UP;
       }
