@@ -189,6 +189,15 @@ __device__ __forceinline__ uint4 lds16(uint32_t addr) {
   return v;
 }
 
+// Which elements of a word are infinite or NaN, all bits of each set. A V row that only some rows of a tile see must not reach
+// the others as 0 * NaN: such elements are taken out of V and added, as they are, to the rows that see them.
+template <typename T, bool KV8>
+__device__ __forceinline__ uint32_t not_finite(uint32_t x) {
+  if (KV8) return __vcmpeq4(x & 0x7f7f7f7fu, 0x7f7f7f7fu);  // e4m3 has NaN only
+  constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  return __vcmpeq2(x & E, E);
+}
+
 // eight consecutive elements of a q row (zeros for a row that does not exist); vec: rows are 16-byte aligned
 template <typename T>
 __device__ __forceinline__ uint4 load_q8(const T* p, int vec) {
@@ -468,11 +477,13 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
       __syncwarp();
       issue(grp + 2, 0);
 
+      unsigned shut = 0;  // tiles that some new tokens see and others do not
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int tb = meta[u].tb;
         const float ks = KV8 ? meta[u].ks : 1.f;
         const bool open = tb >= 0 && tb + PA_TILE - 1 <= ctx && (tb >= lo_max || tb + PA_TILE <= a.sinks);
+        if (!open && tb >= 0 && count > 1) shut |= 1u << u;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -572,6 +583,52 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
               v[r][4 * c + 1] = w.y;
               v[r][4 * c + 2] = w.z;
               v[r][4 * c + 3] = w.w;
+            }
+          }
+        }
+        if (shut >> u & 1) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int w = 0; w < I::VW; ++w) any |= not_finite<M, KV8>(v[r][w]);
+          if (__any_sync(MUI_FULL_MASK, any != 0)) {  // rare
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+#pragma unroll 1
+              for (int src = 0; src < 4; ++src) {  // the lanes that hold the same dims of the tile's other rows
+                const int j = meta[u].tb + 2 * src + (r & 1) + (r >> 1) * 8;
+                bool see[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) see[n][i] = j <= hi[n][i] && (j >= lo[n][i] || j < a.sinks);
+#pragma unroll
+                for (int w = 0; w < I::VW; ++w) {
+                  const uint32_t x = __shfl_sync(MUI_FULL_MASK, v[r][w] & not_finite<M, KV8>(v[r][w]), (lane & ~3) | src);
+                  constexpr int PAIRS = KV8 ? 2 : 1;
+#pragma unroll
+                  for (int h = 0; h < PAIRS; ++h) {
+                    float2 add;
+                    if (KV8) {
+                      add.x = x >> (16 * h) & 0xffu ? __int_as_float(0x7fffffff) : 0.f;
+                      add.y = x >> (16 * h + 8) & 0xffu ? __int_as_float(0x7fffffff) : 0.f;
+                    } else {
+                      add = Elt<M>::unpack2(x);
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                      for (int i = 0; i < 2; ++i)
+                        if (see[n][i]) {
+                          o[w * PAIRS + h][n][i] += add.x;
+                          o[w * PAIRS + h][n][2 + i] += add.y;
+                        }
+                  }
+                }
+              }
+#pragma unroll
+              for (int w = 0; w < I::VW; ++w) v[r][w] &= ~not_finite<M, KV8>(v[r][w]);
             }
           }
         }
@@ -906,6 +963,99 @@ __device__ __forceinline__ bool prompt_tile(const PaArgs& a, int x, PromptTile& 
   return true;
 }
 
+// The rows of a CTA again, a thread per row on the fp32 pipes, where one of them came out infinite or NaN: the tensor cores
+// multiply V rows that a row does not see by 0, and 0 * NaN must not reach it. Here only what a row sees is added. About twenty
+// times slower. q is still in shared memory; the ring is idle. (Inlined: as a function of its own it made every call 4 % slower.)
+template <typename T, bool KV8, int D>
+__device__ __forceinline__ void prompt_again(const PaArgs& a, uint32_t q_tiles, const float* q_back) {
+  using M = typename std::conditional<KV8, __half, T>::type;
+  const int kvh = blockIdx.x % a.kv.kv_heads, split = blockIdx.y, row = threadIdx.x;
+  PromptTile t;
+  if (!prompt_tile(a, static_cast<int>((gridDim.x - 1 - blockIdx.x) / a.kv.kv_heads), t)) return;
+  const int rr = t.r0 + row;
+  const bool mine = rr < t.R;
+  const int pos = mine ? t.ctx + rr / a.G : -1, lo = a.window > 0 ? pos - a.window + 1 : 0;
+  const uint32_t ring = q_tiles + PT_ROWS * D * 2;  // K, then V: 16 rows of fp32 each
+  const uint32_t q_row = q_tiles + row / PT_GROUP * (PT_GROUP * D * 2) + row % PT_GROUP * 128;
+  const float sc = KV8 ? a.scale_log2 * q_back[row] : fmaxf(a.scale_log2, 1e-37f);
+  auto ldf4 = [](uint32_t at) {
+    const uint4 w = lds16(at);
+    return make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+  };
+  float m = -INFINITY, l = 0.f, o[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) o[d] = 0.f;
+  const int i_begin = split * t.per * PT_SUB, i_end = min(t.sp.n, i_begin + t.per * PT_SUB);
+#pragma unroll 1
+  for (int i = i_begin; i < i_end; ++i) {
+    const int b0 = span_tile(t.sp, i) * PA_TILE;
+    const int page = __ldcg(a.kv.block_table + static_cast<size_t>(t.b) * a.kv.table_stride + (b0 >> a.kv.page_shift));
+    if (page < 0 || page >= a.kv.num_pages) continue;  // recorded before
+    const size_t head = static_cast<size_t>(page) * a.kv.kv_heads + kvh;
+    const size_t first = ((head << a.kv.page_shift) + (b0 & ((1 << a.kv.page_shift) - 1))) * D;
+    const float ks = KV8 ? __ldcg(a.kv.k_scales + head) : 1.f, vs = KV8 ? __ldcg(a.kv.v_scales + head) : 1.f;
+    asm volatile("bar.sync 1, %0;" ::"n"(PT_ROWS) : "memory");
+    for (int e = row; e < 2 * PA_TILE * D; e += PT_ROWS) {
+      const size_t at = first + e % (PA_TILE * D);
+      const void* pages = e < PA_TILE * D ? a.kv.k_pages : a.kv.v_pages;
+      float x;
+      if (KV8)
+        x = Elt<__half>::unpack2(e4m3_to_half2(reinterpret_cast<const unsigned char*>(pages)[at])).x;
+      else
+        x = Elt<T>::to_f32(reinterpret_cast<const T*>(pages)[at]);
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(ring + e * 4), "f"(x) : "memory");
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(PT_ROWS) : "memory");
+#pragma unroll 1
+    for (int r = 0; r < PA_TILE; ++r) {
+      const int j = b0 + r;
+      if (j > pos || j >= t.sp.kv_len || (j < lo && j >= a.sinks)) continue;
+      float s = 0.f;
+#pragma unroll 1
+      for (int ch = 0; ch < D / 8; ++ch) {
+        const uint4 w = lds16(q_row + (ch >> 3) * (PT_GROUP * 128) + (((ch & 7) ^ (row & 7)) << 4));
+        float q[8];
+        unpack8<M>(w, q);
+        const float4 k0 = ldf4(ring + (r * D + ch * 8) * 4), k1 = ldf4(ring + (r * D + ch * 8) * 4 + 16);
+        s = fmaf(q[0], k0.x, fmaf(q[1], k0.y, fmaf(q[2], k0.z, fmaf(q[3], k0.w, s))));
+        s = fmaf(q[4], k1.x, fmaf(q[5], k1.y, fmaf(q[6], k1.z, fmaf(q[7], k1.w, s))));
+      }
+      s *= KV8 ? fmaxf(sc * ks, 1e-37f) : sc;
+      if (s > m) {
+        const float f = m == -INFINITY ? 0.f : ex2(m - s);
+        m = s;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < D; ++d) o[d] *= f;
+      }
+      const float p = ex2(s - (m == -INFINITY ? 0.f : m));
+      l += p;
+#pragma unroll
+      for (int d = 0; d < D; d += 4) {
+        const float4 v = ldf4(ring + ((PA_TILE + r) * D + d) * 4);
+        o[d] = fmaf(p * vs, v.x, o[d]);
+        o[d + 1] = fmaf(p * vs, v.y, o[d + 1]);
+        o[d + 2] = fmaf(p * vs, v.z, o[d + 2]);
+        o[d + 3] = fmaf(p * vs, v.w, o[d + 3]);
+      }
+    }
+  }
+  if (!mine) return;
+  const size_t out_row = static_cast<size_t>(t.first + rr / a.G) * a.Hq + kvh * a.G + rr % a.G;
+  if (t.active == 1) {
+    const float norm = l != 0.f ? 1.f / l : 0.f;
+    T* out = reinterpret_cast<T*>(a.out) + out_row * D;
+#pragma unroll
+    for (int d = 0; d < D; ++d) out[d] = Elt<T>::from_f32(o[d] * norm);
+  } else {
+    float* part = a.partials + (out_row * a.splits + split) * (D + 2);
+    part[0] = m;
+    part[1] = l;
+#pragma unroll
+    for (int d = 0; d < D; ++d) part[2 + d] = o[d];
+  }
+}
+
 template <typename T, bool KV8, int D>
 __global__ void __launch_bounds__(PT_THREADS, 1)
     paged_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PaArgs a) {
@@ -918,7 +1068,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   __shared__ uint64_t kv_full[PT_SLOTS], kv_empty[PT_SLOTS], s_full[2], p_half[2], p_full[2], pv_done[2];
   __shared__ float q_back[PT_ROWS];
   __shared__ uint32_t tmem_s;
-  __shared__ int abort_s;
+  __shared__ int abort_s, redo_s;
   const uint32_t tiles = (smem_u32(pt_raw) + 1023u) & ~1023u;  // Q0, Q1, then the ring
   const uint32_t ring = tiles + 2 * QT;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -948,7 +1098,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       mbar_init(&p_full[g], PT_GROUP);
       mbar_init(&pv_done[g], 1);
     }
-    abort_s = 0;
+    abort_s = redo_s = 0;
     mbar_fence_init();
   }
   if (warp == PT_MMA_WARP) {
@@ -1432,6 +1582,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           part[0] = ref;
           part[1] = l;
         }
+        float2 check[4] = {};  // NaN when any element is infinite or NaN
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
@@ -1444,6 +1595,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
           if (!mine) continue;
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] *= norm;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            check[e / 2 & 3] = fma2(make_float2(o[e], o[e + 1]), make_float2(0.f, 0.f), check[e / 2 & 3]);
           if (direct) {
             uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + out_row * D + c * 32);
 #pragma unroll
@@ -1456,11 +1610,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
               *reinterpret_cast<float2*>(part + 2 + c * 32 + 2 * e) = make_float2(o[2 * e], o[2 * e + 1]);
           }
         }
+        check[0] = add2(add2(check[0], check[1]), add2(check[2], check[3]));
+        if (check[0].x + check[0].y != 0.f) redo_s = 1;
       }
     }
   }
   tc_before();
   __syncthreads();
+  if (redo_s && tid < PT_ROWS) prompt_again<T, KV8, D>(a, tiles, q_back);
   if (warp == PT_MMA_WARP) {
     tc_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");

@@ -103,8 +103,9 @@ def visible(c, n, window, sinks):
     return see
 
 
-def attention(q, k_pages, v_pages, k_scales, v_scales, table, ctx, new, window=0, sinks=0, scale=None):
-    """(out fp64 [total, Hq, D], sum of p |v| of the same shape). Rows that nobody sees may hold anything."""
+def attention(q, k_pages, v_pages, k_scales, v_scales, table, ctx, new, window=0, sinks=0, scale=None, row_by_row=False):
+    """(out fp64 [total, Hq, D], sum of p |v| of the same shape). Rows that nobody sees may hold anything. What a token does
+    not see has weight 0, or, row_by_row, is left out of its sums, so that infinities there do not matter either."""
     total, Hq, D = q.shape
     Hkv, ps = k_pages.shape[1:3]
     G = Hq // Hkv
@@ -129,6 +130,12 @@ def attention(q, k_pages, v_pages, k_scales, v_scales, table, ctx, new, window=0
             a = torch.einsum("tgd,ld->gtl", q[at: at + n, h * G: (h + 1) * G].double(), kk[:, h]) * scale
             a = a.masked_fill(~see[:, rows][None], -math.inf)
             w = torch.softmax(a, dim=-1)
+            if row_by_row:
+                for t in range(n):
+                    seen = see[t, rows]
+                    for res, val in ((out, vv[:, h]), (mag, vv[:, h].abs())):
+                        res[at + t, h * G: (h + 1) * G] = torch.einsum("gl,ld->gd", w[:, t, seen], val[seen])
+                continue
             out[at: at + n, h * G: (h + 1) * G] = torch.einsum("gtl,ld->tgd", w, vv[:, h])
             mag[at: at + n, h * G: (h + 1) * G] = torch.einsum("gtl,ld->tgd", w, vv[:, h].abs())
         at += n

@@ -338,6 +338,44 @@ def test_attention_prompts_split_and_mixed(e4m3, ctx, new, Hq, Hkv, D, page):
         _check_attention(c, q, window=700, sinks=5)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("ctx,new,Hq,Hkv,D,page", [
+    ([40, 0], [3, 8], 8, 2, 128, 16),                   # few new tokens
+    ([1000], [5], 20, 4, 64, 64),
+    ([2000], [30], 1, 1, 64, 16),                       # thirty-two rows; split over CTAs
+    ([70, 0, 500], [90, 300, 40], 4, 2, 128, 16),       # prompts
+    ([3000], [40], 8, 1, 64, 64),                       # a split prompt
+    ([130], [270], 2, 2, 128, 128),
+])
+def test_attention_hidden_infinities(e4m3, ctx, new, Hq, Hkv, D, page):
+    """Infinities and NaN in K and V of rows that only some of the new tokens see: the others are as without them, and what
+    the formula makes infinite or NaN is so."""
+    for dtype, (window, sinks) in itertools.product((F16, BF16), ((0, 0), (21, 2))):
+        c = _filled(ctx, new, Hkv, D, page, dtype, e4m3, seed=41, spread=0.3, poison=False)
+        for b, (a, n) in enumerate(zip(ctx, new)):
+            # late rows, and one that a window drops half-way through the new tokens
+            for i, j in enumerate({a + n - 1, a + n // 2, max(0, a + n // 2 - 21), max(0, a + 1 - 21)}):
+                pg, slot = int(c.table[b, j // page]), j % page
+                for pool, d in ((c.pools[1], 3 + 5 * i), (c.pools[1], D - 2 - i), (c.pools[0], 0)):
+                    if pool is c.pools[0] and j != a + n - 1:
+                        continue
+                    value = (math.nan, math.inf, -math.inf, math.nan)[i]
+                    if e4m3:
+                        pool.view(torch.uint8)[pg, 0, slot, d] = 0xFF if i & 1 else 0x7F
+                    else:
+                        pool[pg, 0, slot, d] = value
+        q = torch.randn(sum(new), Hq, D, generator=_gen(42)).to(dtype)
+        d = c.cuda()
+        want, mag = oracle.attention(q, *c.oracle_args(), c.table, c.ctx, c.new, window, sinks, row_by_row=True)
+        got = ops.paged_attention(q.cuda(), max_new_tokens=max(new), window=window, sinks=sinks, **d).double().cpu()
+        fine = torch.isfinite(want)
+        assert 0.5 < fine.double().mean() < 1
+        assert torch.equal(torch.isfinite(got), fine)
+        prompt = max(new) * (Hq // Hkv) > 32
+        tol = _attention_tolerance(dtype, e4m3, prompt, want, mag)
+        _within(got.masked_fill(~fine, 0), want.masked_fill(~fine, 0), tol.masked_fill(~fine, 1))
+
+
 @pytest.mark.parametrize("new", [1, 60])
 @pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
 def test_attention_scales_of_any_sign(new, scale):
