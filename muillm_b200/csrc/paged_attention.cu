@@ -99,6 +99,11 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 // CTA streams the same number of bytes whatever the lengths are. A run that covers a triple whole writes its output; the
 // others leave partial results, at most two per CTA (the triple that the run starts in and the one it ends in), which
 // paged_merge_kernel joins in order.
+// Measured (device time with the merge; 32 q and 8 KV heads of 128, copy bandwidth 6560 GB/s): 24 sequences of 150 to 6500
+// tokens, bf16, 61 us = 5.2 TB/s; 32 sequences of 413 to 8111, e4m3, 63 us = 4.5 TB/s; one sequence of 131000, 64 q heads,
+// e4m3, 57 us = 4.7 TB/s; 16 long ones with a window of 4096 and 4 sinks, 40 q heads, 52 us = 5.0 TB/s; one sequence of 300 tokens
+// 12.4 us. About 8 us of a launch go to the chain before the first and after the last item (lengths, block table, q, merge);
+// in between e4m3 is bound by its instructions: a conversion for each pair of elements, and byte permutes for V.
 struct Run {
   int seq, first, count, ctx;  // sequence at the run's first place
   long long begin;             // place at which that sequence begins
@@ -839,6 +844,12 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
 // above it: then O is rescaled in tensor memory, which is rare after the first tiles; P stays below 2^8 and the sums are right in
 // any case. P is rounded once to the type of the tensor-core operands (half a step is 2^-9 of it for bf16, 2^-12 for fp16).
 // Bound: exp2 (16 a cycle and SM) and the MMAs need about 2050 cycles a step each.
+// Measured (32 q and 8 KV heads of 128, device time; tensor cores 1651 TFLOP/s): one prompt of 8192 tokens, bf16 pages, 555 us =
+// 990 TFLOP/s; three chunks of 1023 to 2049 tokens behind up to 2100, 223 us = 774 TFLOP/s (the last round of CTAs is not full);
+// e4m3 pages 357 us (the three warps that convert K and V). A step takes 2.0 us, 1.6 of it MMA time: a group's softmax ends
+// a little late for the other group's products. A part of the exponentials as polynomials on the fp32 pipes was slower (a
+// quarter of them 231, half of them 239 us): their instructions come out of the same issue slots. So were tiles ordered by
+// length over all sequences (269 us: the search costs each CTA more than it saves).
 constexpr int PT_ROWS = 256, PT_GROUP = 128, PT_KEYS = 128;
 constexpr int PT_SUB = PT_KEYS / PA_TILE;          // 16-row tiles of a step
 constexpr int PT_SLOTS = 4;                        // ring of K and V tiles
