@@ -229,6 +229,12 @@ struct Row {
   }
 };
 
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Weights of one row. table: lane j of every warp holds 2^(j / 32).
 struct Weigh {
   float top, floor, bin_scale;  // floor: at and below it a weight rounds to 0
@@ -267,6 +273,10 @@ struct Weigh {
       p[e] *= __shfl_sync(MUI_FULL_MASK, table, k);
       p[e] = __hiloint2double(__double2hiint(p[e]) + ((k >> 5) + frac_bits) * (1 << 20), __double2loint(p[e]));
     }
+  }
+  // 2^S exp(z) in fp32: off by less than 2^-14 of itself (z up to 46 with three roundings of 2^-24, and ex2's own error)
+  __device__ __forceinline__ float rough(float x) const {
+    return ex2((fmaxf(x, floor) - top) * static_cast<float>(scale * (1.0 / 32.0)) + static_cast<float>(frac_bits));
   }
   // values below 2^51 added to 2^52 leave their rounded sum in the mantissa
   static __device__ __forceinline__ u64 bits(double v) {
@@ -626,7 +636,8 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     }
     return true;
   };
-  auto finish = [&](int n, u64 total, bool cut_p) {
+  // Inlined in every place: as a function it takes all of the state through memory (one row of fp16 logits 12 -> 20 us).
+  auto finish = [&](int n, u64 total, bool cut_p) __attribute__((always_inline)) {
     if (n <= SM_FEW) return finish_few(n, total, cut_p);
     constexpr int PER = SM_BINS / SM_THREADS;
     uint32_t cn[PER], cb = 0;
@@ -715,7 +726,15 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     };
 
     u64 edge = 0;  // entries from here on are kept
-    if (use_k || use_p) {
+    bool cut = use_k || use_p;
+    if (!use_k && !cut_p && use_p) {  // less weight than top-p asks for: all are kept
+      u64 sum = 0;
+      tokens([&](u64, u64 q) { sum += q; });
+      block_scan(sum, s.warp_u64, all);
+      __syncthreads();
+      cut = !(static_cast<double>(all) < static_cast<double>(top_p) * static_cast<double>(total));
+    }
+    if (cut) {
       clear();
       tokens([&](u64 e, u64 q) {
         const int b = bin_of(e);
@@ -799,34 +818,76 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
       asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list_at[which] + at * 8), "l"(rank_entry(x, i)) : "memory");
   };
   u64 v[3];
-  auto collect = [&](auto in, bool weigh, bool count) {
+  enum { NO_WEIGHT, ROUGH, EXACT };
+  auto collect = [&](auto in, int weigh, bool count) {
     v[0] = v[1] = v[2] = 0;
+    float rough = 0.f;
     row.each([&](int i, float(&x)[8]) {
-      if (weigh) {
+      if (weigh == ROUGH) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += w.rough(x[e]);
+        rough += sum;
+      } else if (weigh == EXACT) {
         double p[8], sum = 4503599627370496.0;  // 2^52
         w.values(x, p);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum += p[e];
         v[0] += Weigh::bits(sum);
       }
+      // places in the list are taken once for the warp
+      unsigned mine = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (in(x[e])) {
-          put(0, x[e], i + e + gap<T>(e), SM_LIST);
-          ++v[1];
-        }
+      for (int e = 0; e < 8; ++e) mine |= in(x[e]) ? 1u << e : 0u;
+      if (__any_sync(MUI_FULL_MASK, mine != 0)) {
+        const uint32_t upto = warp_scan(static_cast<uint32_t>(__popc(mine)));
+        uint32_t at = 0;
+        if ((tid & 31) == 31)
+          asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(count_at[0]), "r"(upto) : "memory");
+        at = __shfl_sync(MUI_FULL_MASK, at, 31) + upto - __popc(mine);
+        v[1] += __popc(mine);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (mine >> e & 1) {
+            if (at < SM_LIST)
+              asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(list_at[0] + at * 8), "l"(rank_entry(x[e], i + e + gap<T>(e)))
+                           : "memory");
+            ++at;
+          }
+      }
     });
+    if (weigh == ROUGH) v[0] = static_cast<u64>(rough);
     // a barrier of the cluster either way: it publishes the list
-    if (weigh || count) cluster_sum3(s, C, rank, turn, v);
+    if (weigh != NO_WEIGHT || count) cluster_sum3(s, C, rank, turn, v);
     else cluster_sync(C);
   };
 
   uint32_t T_key = 0, T_idx = 0;  // nothing to cut: every key that has weight is above 0
   bool bisect = false;
   if (min_p > 0.f && !use_k) {
-    collect([&](float x) { return x >= x_min; }, use_p, true);
+    // Where the collected tokens are certain to end before top-p does, a rough weight of the row is enough: it is off by less
+    // than 2^-14, and as much again for the fp32 sums of a thread (at most 2^22 / 4096 + 8 additions). Less 2^-10 it is a bound.
+    collect([&](float x) { return x >= x_min; }, use_p ? ROUGH : NO_WEIGHT, true);
     if (v[1] <= SM_LIST) {
-      if (rank == 0) finish(static_cast<int>(v[1]), v[0], false);
+      const int n = static_cast<int>(v[1]);
+      if (use_p) {
+        if (rank == 0) {
+          const u64 least = v[0] - (v[0] >> 10);
+          u64 sum = 0, listed;
+#pragma unroll 1
+          for (int base = 0; base < n; base += SM_THREADS) {
+            const int i = base + tid;
+            sum += w(i < n ? key_logit(static_cast<uint32_t>(s.list[i] >> 32)) : 0.f, i < n);
+          }
+          block_scan(sum, s.warp_u64, listed);
+          const bool sure = static_cast<double>(listed) < static_cast<double>(top_p) * static_cast<double>(least);
+          v[0] = least;
+          if (tid == 0) s.say.verdict = sure ? SM_FOUND : SM_BISECT;
+        }
+        tell(s, C, rank);
+        if (s.said.verdict != SM_FOUND) collect([](float) { return false; }, EXACT, false);
+      }
+      if (rank == 0) finish(n, v[0], false);
       return;
     }
     if (tid == 0) s.list_n[0] = 0;  // a barrier follows before the next token is put there
@@ -866,7 +927,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     }
     tell(s, C, rank);
     const int last = s.said.bin_k;
-    collect([&](float x) { return w.bin(x) <= min(last, SM_BINS - 1); }, false, true);
+    collect([&](float x) { return w.bin(x) <= min(last, SM_BINS - 1); }, NO_WEIGHT, true);
     if (v[1] <= SM_LIST) {
       // few tokens are always brought to an end
       if (rank != 0 && v[1] <= SM_FEW) return;
@@ -971,7 +1032,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     if (s.said.collect) {
       // 3. the tokens in front
       const int last = use_k ? bin_k : min(bin_p + 1, SM_BINS);
-      collect([&](float x) { return w.bin(x) < SM_BINS && w.bin(x) <= last; }, use_p && !use_k, false);
+      collect([&](float x) { return w.bin(x) < SM_BINS && w.bin(x) <= last; }, use_p && !use_k ? EXACT : NO_WEIGHT, false);
       // with top-k the list is complete for sure: only rank 0 goes on
       const bool sure = use_k && s.said.small_bins;
       if (sure && rank != 0) return;
