@@ -15,7 +15,8 @@
 //      nearly always. Not needed where min-p alone leaves few tokens, nor for a top_k of at most the number of threads: there
 //      the threads' own largest logits, known from 1, are counted instead of all, and give a bin that is far enough down;
 //   3. all tokens up to that bin (or above min-p's cut) are collected in rank 0's shared memory if they are at most 16384, with
-//      the weight of the whole row where top-p asks for it. Rank 0 sums them by bins of z, sorts the bins in which top-k and
+//      the weight of the whole row where top-p asks for it (with min-p first roughly, in fp32: mostly the list is certain to
+//      end before top-p does). Rank 0 sums them by bins of z, sorts the bins in which top-k and
 //      top-p end, sums the kept ones by parts of the index range and sorts the part that holds the drawn point.
 // More tokens than that (a wide nucleus, a temperature without cuts):
 //   3'. exact sums of the weight above and between the boundary bins, whose own tokens are collected and sorted to give T and
@@ -27,8 +28,9 @@
 // Bound: rows * vocab * size bytes for large batches, then eleven fp64 operations a weight (fp64 runs at half the fp32 rate);
 // for few rows the chain of passes and cluster barriers.
 // Measured (device time): one row of 128256 fp16 logits, top-k 50 and top-p 0.9, 12 us (floor 0.04 us: five dependent steps of
-// about 2 us); 128 rows of 202048 fp32 logits, top-p 0.95 and min-p 0.02, 113 us (floor 15.8 us; 49 us are the weights of every
-// token in fp64, which top-p alone makes necessary); 32 rows of 128256 with top-k 50, 26 us; one row with top-p alone, 42 us.
+// about 2 us); 128 rows of 202048 fp32 logits, top-p 0.95 and min-p 0.02, 91 us (floor 15.8 us; 60 us for most rows, the one with
+// the longest list sets the time; with the row's weight in fp64 instead of roughly, 113 us); 32 rows of 128256 with top-k 50 and
+// top-p, 16 us; one row with top-p alone, 36 us; 64 rows with top-p alone whose nucleus is wide, 112 us.
 #include "common.cuh"
 
 #include <atomic>
@@ -53,6 +55,7 @@ constexpr int SM_RUNS = SM_THREADS;  // runs of chunks whose kept weight a CTA h
 constexpr int SM_MAX_CLUSTER = 8;
 // what rank 0 finds in the collected tokens: the threshold, that top-p ends further up or down the ranking, or too many tokens
 enum : uint32_t { SM_FOUND, SM_UP, SM_DOWN, SM_BISECT };
+constexpr u64 SM_ENDLESS = ~0ull;  // a row's weight so large that top-p keeps all that was collected
 
 struct SampleArgs {
   const void* logits;
@@ -727,7 +730,9 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
 
     u64 edge = 0;  // entries from here on are kept
     bool cut = use_k || use_p;
-    if (!use_k && !cut_p && use_p) {  // less weight than top-p asks for: all are kept
+    if (!use_k && use_p && total == SM_ENDLESS) {
+      cut = false;
+    } else if (!use_k && !cut_p && use_p) {  // less weight than top-p asks for: all are kept
       u64 sum = 0;
       tokens([&](u64, u64 q) { sum += q; });
       block_scan(sum, s.warp_u64, all);
@@ -789,10 +794,15 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     const int part = find([&](uint32_t, uint32_t, u64 f, u64 m) {
       return static_cast<double>(f + m) > want && static_cast<double>(f) <= want;
     });
-    tokens([&](u64 e, u64 q) {
-      if (e >= edge && q >= w_min && index_of(e) >> shift == part)
-        s.small[atomicAdd(&s.small_n, 1u)] = e << 32 | e >> 32;  // ~index, key
-    });
+#pragma unroll 1
+    for (int base = 0; base < n; base += SM_THREADS) {
+      const int i = base + tid;
+      const u64 e = i < n ? s.list[i] : 0;
+      const bool here = i < n && e >= edge && index_of(e) >> shift == part;
+      if (!__any_sync(MUI_FULL_MASK, here)) continue;
+      const u64 q = w(here ? key_logit(static_cast<uint32_t>(e >> 32)) : 0.f, here);
+      if (here && q >= w_min) s.small[atomicAdd(&s.small_n, 1u)] = e << 32 | e >> 32;  // ~index, key
+    }
     __syncthreads();
     const int m = s.small_n;
     sort_list(s.small, m);
@@ -842,7 +852,9 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
       if (__any_sync(MUI_FULL_MASK, mine != 0)) {
         const uint32_t upto = warp_scan(static_cast<uint32_t>(__popc(mine)));
         uint32_t at = 0;
-        if ((tid & 31) == 31)
+        if (C == 1) {
+          if ((tid & 31) == 31) at = atomicAdd(&s.list_n[0], upto);
+        } else if ((tid & 31) == 31)
           asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(at) : "r"(count_at[0]), "r"(upto) : "memory");
         at = __shfl_sync(MUI_FULL_MASK, at, 31) + upto - __popc(mine);
         v[1] += __popc(mine);
@@ -881,7 +893,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
           }
           block_scan(sum, s.warp_u64, listed);
           const bool sure = static_cast<double>(listed) < static_cast<double>(top_p) * static_cast<double>(least);
-          v[0] = least;
+          v[0] = SM_ENDLESS;
           if (tid == 0) s.say.verdict = sure ? SM_FOUND : SM_BISECT;
         }
         tell(s, C, rank);
