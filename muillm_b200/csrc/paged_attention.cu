@@ -571,26 +571,27 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
 
       copy_wait<3>();
       __syncwarp();
+      // this lane's words of a V row
+      auto v_words = [&](int u, int row, uint32_t(&x)[I::VW]) {
+        const uint32_t at = vslot + (u * PA_TILE + row) * I::RB;
+        if (I::CPR == 4) {
+          lds_v2(at + (((g >> 1) ^ I::swizzle(row)) << 4) + (g & 1) * 8, x[0], x[1]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < I::VW / 4; ++c) {
+            const uint4 w = lds16(at + (((c * 8 + g) ^ I::swizzle(row)) << 4));
+            x[4 * c] = w.x;
+            x[4 * c + 1] = w.y;
+            x[4 * c + 2] = w.z;
+            x[4 * c + 3] = w.w;
+          }
+        }
+      };
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         uint32_t v[4][I::VW];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int slot = 2 * tq + (r & 1) + (r >> 1) * 8;
-          const uint32_t at = vslot + (u * PA_TILE + slot) * I::RB;
-          if (I::CPR == 4) {
-            lds_v2(at + (((g >> 1) ^ I::swizzle(slot)) << 4) + (g & 1) * 8, v[r][0], v[r][1]);
-          } else {
-#pragma unroll
-            for (int c = 0; c < I::VW / 4; ++c) {
-              const uint4 w = lds16(at + (((c * 8 + g) ^ I::swizzle(slot)) << 4));
-              v[r][4 * c] = w.x;
-              v[r][4 * c + 1] = w.y;
-              v[r][4 * c + 2] = w.z;
-              v[r][4 * c + 3] = w.w;
-            }
-          }
-        }
+        for (int r = 0; r < 4; ++r) v_words(u, 2 * tq + (r & 1) + (r >> 1) * 8, v[r]);
         if (shut >> u & 1) {
           uint32_t any = 0;
 #pragma unroll
@@ -598,43 +599,39 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
 #pragma unroll
             for (int w = 0; w < I::VW; ++w) any |= not_finite<M, KV8>(v[r][w]);
           if (__any_sync(MUI_FULL_MASK, any != 0)) {  // rare
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
 #pragma unroll 1
-              for (int src = 0; src < 4; ++src) {  // the lanes that hold the same dims of the tile's other rows
-                const int j = meta[u].tb + 2 * src + (r & 1) + (r >> 1) * 8;
-                bool see[NT][2];
+            for (int row = 0; row < PA_TILE; ++row) {
+              const int j = meta[u].tb + row;
+              uint32_t x[I::VW];
+              v_words(u, row, x);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+              for (int w = 0; w < I::VW; ++w) {
+                x[w] &= not_finite<M, KV8>(x[w]);
+                constexpr int PAIRS = KV8 ? 2 : 1;
 #pragma unroll
-                  for (int i = 0; i < 2; ++i) see[n][i] = j <= hi[n][i] && (j >= lo[n][i] || j < a.sinks);
-#pragma unroll
-                for (int w = 0; w < I::VW; ++w) {
-                  const uint32_t x = __shfl_sync(MUI_FULL_MASK, v[r][w] & not_finite<M, KV8>(v[r][w]), (lane & ~3) | src);
-                  constexpr int PAIRS = KV8 ? 2 : 1;
-#pragma unroll
-                  for (int h = 0; h < PAIRS; ++h) {
-                    float2 add;
-                    if (KV8) {
-                      add.x = x >> (16 * h) & 0xffu ? __int_as_float(0x7fffffff) : 0.f;
-                      add.y = x >> (16 * h + 8) & 0xffu ? __int_as_float(0x7fffffff) : 0.f;
-                    } else {
-                      add = Elt<M>::unpack2(x);
-                    }
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                      for (int i = 0; i < 2; ++i)
-                        if (see[n][i]) {
-                          o[w * PAIRS + h][n][i] += add.x;
-                          o[w * PAIRS + h][n][2 + i] += add.y;
-                        }
+                for (int h = 0; h < PAIRS; ++h) {
+                  float2 add;
+                  if (KV8) {
+                    add.x = x[w] >> (16 * h) & 0xffu ? __int_as_float(0x7fffffff) : 0.f;
+                    add.y = x[w] >> (16 * h + 8) & 0xffu ? __int_as_float(0x7fffffff) : 0.f;
+                  } else {
+                    add = Elt<M>::unpack2(x[w]);
                   }
+#pragma unroll
+                  for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                      if (j <= hi[n][i] && (j >= lo[n][i] || j < a.sinks)) {
+                        o[w * PAIRS + h][n][i] += add.x;
+                        o[w * PAIRS + h][n][2 + i] += add.y;
+                      }
                 }
               }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
               for (int w = 0; w < I::VW; ++w) v[r][w] &= ~not_finite<M, KV8>(v[r][w]);
-            }
           }
         }
 #pragma unroll

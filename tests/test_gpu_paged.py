@@ -750,3 +750,39 @@ def test_two_streams_at_once():
     for i in range(2):
         for x in got[i]:
             assert torch.equal(x, want[i])
+
+
+@pytest.mark.parametrize("rows", [2, 200])
+def test_sample_top_p_around_the_end_of_min_p(rows):
+    """Top-p that ends before, at and behind the end of min-p's tokens: a few of them, some hundred, some thousand."""
+    vocab = 20000
+    g = _gen(51)
+    logits, top_p, min_p = [], [], []
+    for spread in (0.5, 1.0, 2.0, 4.0):
+        x = spread * torch.randn(vocab, generator=g)
+        w = torch.softmax(x.double(), 0)
+        m = 0.05
+        part = float(w[w >= m * w.max()].sum())
+        for p in (0.2 * part, 0.99 * part, part * (1 - 1e-5), part * (1 + 1e-5), part * 1.0005, part * 1.002, 0.5 * (1 + part)):
+            logits.append(x)
+            top_p.append(min(p, 0.99999))
+            min_p.append(m)
+    n = len(logits)
+    x = torch.stack(logits)
+    pick = torch.arange(rows) % n
+    u = torch.rand(rows, generator=g)
+    p, m = torch.tensor(top_p)[pick], torch.tensor(min_p)[pick]
+    if rows == 2:
+        for first in range(0, n, 2):
+            sub = slice(first, first + 2)
+            _check_rows(x[sub], u, torch.tensor(top_p)[sub], torch.tensor(min_p)[sub])
+    else:
+        _check_rows(x[pick], u, p, m)
+
+
+def _check_rows(x, u, top_p, min_p):
+    tokens, logprobs = ops.sample_tokens(x.cuda(), u.cuda(), top_p=top_p.cuda(), min_p=min_p.cuda())
+    for i in range(x.shape[0]):
+        want, share, _ = oracle.sample(x[i], float(u[i]), top_p=float(top_p[i]), min_p=float(min_p[i]))
+        assert int(tokens[i]) == want
+        assert abs(float(logprobs[i]) - share) < 1e-5
