@@ -100,7 +100,7 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 // others leave partial results, at most two per CTA (the triple that the run starts in and the one it ends in), which
 // paged_merge_kernel joins in order.
 // Measured (device time with the merge; 32 q and 8 KV heads of 128, copy bandwidth 6560 GB/s): 24 sequences of 150 to 6500
-// tokens, bf16, 61 us = 5.2 TB/s; 32 sequences of 413 to 8111, e4m3, 63 us = 4.5 TB/s; one sequence of 131000, 64 q heads,
+// tokens, bf16, 61 us = 5.2 TB/s; 32 sequences of 413 to 8111, e4m3, 62 us = 4.6 TB/s; one sequence of 131000, 64 q heads,
 // e4m3, 57 us = 4.7 TB/s; 16 long ones with a window of 4096 and 4 sinks, 40 q heads, 52 us = 5.0 TB/s; one sequence of 300 tokens
 // 12.4 us. About 8 us of a launch go to the chain before the first and after the last item (lengths, block table, q, merge);
 // in between e4m3 is bound by its instructions: a conversion for each pair of elements, and byte permutes for V.
