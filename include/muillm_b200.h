@@ -509,7 +509,7 @@ MUI_API mui_status_t mui_paged_kv_append(void* stream, mui_dtype_t dtype, const 
 /* out[t, h, :] = softmax_j( q[t, h, :] . K[j, h / G, :] * scale ) V over the cache rows j of the token's sequence (G =
  * num_q_heads / kv_heads, at most 32): a token at cache position p sees j <= p, its own row (appended before) included, and
  * with window > 0 of those only j > p - window or j < sinks. out is contiguous [total_tokens, num_q_heads, head_dim].
- * max_new_tokens bounds the new tokens of every sequence. max_context (> 0) is a hint for the work split, the longest
+ * max_new_tokens bounds the new tokens of every sequence (1 where cu_tokens is NULL, whatever is given). max_context (> 0) is a hint for the work split, the longest
  * sequence expected (any value gives right results). What a token does not see does not reach its result, infinities and
  * NaN included (prompts that have any in V take about twenty times longer). Softmax statistics, sums and outputs are held in fp32 and rounded once. workspace:
  * mui_paged_attention_workspace_bytes() bytes of scratch for the same sizes, 16-byte aligned, any contents; it may be

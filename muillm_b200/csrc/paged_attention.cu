@@ -934,25 +934,20 @@ __device__ __forceinline__ uint32_t f16_idesc(int is_bf16, int n, int b_mn) {
          static_cast<uint32_t>(b_mn) << 16 | static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(128 >> 4) << 24;
 }
 
-// Which rows a CTA owns and what they see. false: nothing to do.
+// Which rows a CTA owns and what they see. false: nothing to do. The prompt kernel runs with cu_tokens only: without them a
+// sequence has one new token, at most 32 rows.
 struct PromptTile {
   int b, first, count, ctx, r0, R;
   Span sp;
   int steps, per, active;  // steps of 128 cache rows; steps per split; splits that have any
 };
 __device__ __forceinline__ bool prompt_tile(const PaArgs& a, int x, PromptTile& t) {
-  int tile;
-  if (a.kv.cu != nullptr) {
-    // tiles are numbered through: sequence b's start at floor(cu[b] * G / 256) + b
-    const int32_t* cu = a.kv.cu;
-    auto start = [&](int k) { return static_cast<int>(static_cast<long long>(__ldcg(cu + k)) * a.G / PT_ROWS) + k; };
-    t.b = warp_count_le(a.kv.batch, x, [&](int k) { return start(k + 1); });
-    if (t.b >= a.kv.batch) return false;
-    tile = x - start(t.b);
-  } else {
-    t.b = x;  // one new token: at most 32 rows
-    tile = 0;
-  }
+  // tiles are numbered through: sequence b's start at floor(cu[b] * G / 256) + b
+  const int32_t* cu = a.kv.cu;
+  auto start = [&](int k) { return static_cast<int>(static_cast<long long>(__ldcg(cu + k)) * a.G / PT_ROWS) + k; };
+  t.b = warp_count_le(a.kv.batch, x, [&](int k) { return start(k + 1); });
+  if (t.b >= a.kv.batch) return false;
+  const int tile = x - start(t.b);
   paged_new_tokens(a.kv, t.b, t.first, t.count);
   t.ctx = __ldcg(a.kv.context_lens + t.b);
   t.r0 = tile * PT_ROWS;
@@ -1641,15 +1636,14 @@ __global__ void __launch_bounds__(PA_THREADS) paged_prompt_merge_kernel(const Pa
   const int tok = static_cast<int>(row / a.Hq), head = static_cast<int>(row % a.Hq);
   int active = 0;
   if (tok < a.kv.total) {
-    int b = tok;
     const int32_t* cu = a.kv.cu;
-    if (cu != nullptr) b = warp_count_le(a.kv.batch, tok, [&](int k) { return __ldcg(cu + 1 + k); });
+    const int b = warp_count_le(a.kv.batch, tok, [&](int k) { return __ldcg(cu + 1 + k); });
     if (b < a.kv.batch) {
       int first, count;
       paged_new_tokens(a.kv, b, first, count);
       const int x = ((tok - first) * a.G + head % a.G) / PT_ROWS;
       PromptTile t;
-      const int start = cu != nullptr ? static_cast<int>(static_cast<long long>(__ldcg(cu + b)) * a.G / PT_ROWS) + b : b;
+      const int start = static_cast<int>(static_cast<long long>(__ldcg(cu + b)) * a.G / PT_ROWS) + b;
       if (prompt_tile(a, start + x, t)) active = t.active;
     }
   }
@@ -1806,11 +1800,14 @@ size_t mui_paged_attention_workspace_bytes(int total_tokens, int batch, int num_
       max_context <= 0)
     return 0;
   const MuiDeviceInfo* di = mui_current_device_info();
-  PaPlan p;
-  if (num_q_heads < kv_heads || !di ||
-      !pa_plan(*di, total_tokens, batch, num_q_heads, kv_heads, head_dim, max_new_tokens, max_context, window, sinks, p))
-    return 0;
-  return p.bytes;
+  if (num_q_heads < kv_heads || !di) return 0;
+  auto bytes = [&](int max_new) {
+    PaPlan p;
+    return pa_plan(*di, total_tokens, batch, num_q_heads, kv_heads, head_dim, max_new, max_context, window, sinks, p) ? p.bytes
+                                                                                                                       : 0;
+  };
+  // as many tokens as sequences may stand for a call without cu_tokens, which counts max_new_tokens as 1
+  return std::max(bytes(max_new_tokens), total_tokens == batch ? bytes(1) : 0);
 }
 
 mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_paged_kv_t* cache, int num_q_heads,
@@ -1826,6 +1823,7 @@ mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const mui_page
   MUI_REQUIRE(max_new_tokens >= 1 && max_context >= 1 && window >= 0 && sinks >= 0, MUI_ERR_INVALID_ARG,
               "bad max_new_tokens=%d max_context=%d window=%d sinks=%d", max_new_tokens, max_context, window, sinks);
   if (cache->batch == 0 || cache->total_tokens == 0) return MUI_OK;
+  if (cache->cu_tokens == nullptr) max_new_tokens = 1;  // a looser bound would launch the prompt kernel, which reads cu_tokens
   MUI_REQUIRE(q && out, MUI_ERR_INVALID_ARG, "q and out must be non-null");
   MUI_REQUIRE((reinterpret_cast<uintptr_t>(out) & 15) == 0, MUI_ERR_INVALID_ARG, "out must be 16-byte aligned");
   const MuiDeviceInfo* di = mui_current_device_info();

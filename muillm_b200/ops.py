@@ -673,8 +673,8 @@ def paged_attention(q, k_pages, v_pages, block_table, context_lens, cu_tokens=No
                     v_scales=None, scale=None, window=0, sinks=0, max_context=None, out=None, flags=0):
     """Causal attention of the new tokens' queries over a paged cache that already holds their own rows (paged_kv_append
     of the same description). q [total, Hq, head_dim] (a view with innermost stride 1), the cache tensors, context_lens
-    and cu_tokens as in paged_kv_append; max_new_tokens bounds the new tokens of every sequence (default: 1 without
-    cu_tokens, else total). window > 0 limits a token at position p to the rows j > p - window and the first `sinks`
+    and cu_tokens as in paged_kv_append; max_new_tokens bounds the new tokens of every sequence (default: total;
+    without cu_tokens it counts as 1). window > 0 limits a token at position p to the rows j > p - window and the first `sinks`
     rows. max_context is the longest sequence expected, a hint for the number of CTAs (default: the block table's reach).
     Returns [total, Hq, head_dim]. mui_paged_attention in the C ABI."""
     device, dtype = _device_of(q, "q"), q.dtype

@@ -1,0 +1,44 @@
+"""Calls of the paged-cache and sampling operators at the ends of what their documentation allows."""
+import ctypes
+
+import pytest
+import torch
+
+from muillm_b200 import capi, ops
+from oracle import paged_oracle as oracle
+from test_gpu_paged import F16, _attention_tolerance, _filled, _gen, _i32, _within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("batch,G,max_new", [(64, 4, 16), (40, 8, 4096), (1, 8, 64), (3, 32, 2)])
+def test_attention_loose_bound_on_new_tokens(batch, G, max_new, e4m3):
+    """One token per sequence, without cu_tokens, and a max_new_tokens that is not reached. Behind the lengths, in the same
+    buffer, there are words that are no lengths."""
+    ctx = [(37 * b) % 120 for b in range(batch)]
+    c = _filled(ctx, [1] * batch, 1, 64, 16, F16, e4m3, seed=71, spread=0.3)
+    q = torch.randn(batch, G, 64, generator=_gen(72)).to(F16)
+    d = c.cuda()
+    d["context_lens"] = _i32(ctx + [-9] * 400)[:batch]
+    want, mag = oracle.attention(q, *c.oracle_args(), c.table, c.ctx, c.new)
+    got = ops.paged_attention(q.cuda(), max_new_tokens=max_new, **d)
+    _within(got, want, _attention_tolerance(F16, e4m3, False, want, mag))
+    assert capi.device_status(clear=False) == 0
+    assert torch.equal(got, ops.paged_attention(q.cuda(), **d))
+    # the scratch that the C call asks for is the scratch that it is content with
+    kv = capi.PagedKV(capi.MUI_KV_E4M3 if e4m3 else capi.MUI_KV_16BIT, c.num_pages, 16, 1, 64, batch, c.table.shape[1], batch,
+                      d["k_pages"].data_ptr(), d["v_pages"].data_ptr(),
+                      d["k_scales"].data_ptr() if e4m3 else None, d["v_scales"].data_ptr() if e4m3 else None,
+                      d["block_table"].data_ptr(), d["context_lens"].data_ptr(), None)
+    for max_context in (1, 3000, 2 ** 31 - 1):
+        n = capi.lib().mui_paged_attention_workspace_bytes(batch, batch, G, 1, 64, max_new, max_context, 0, 0)
+        ws = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
+        qq, out = q.cuda(), torch.full_like(q, 7.0, device="cuda")
+        capi.check(capi.lib().mui_paged_attention(
+            torch.cuda.current_stream().cuda_stream, capi.MUI_F16, ctypes.byref(kv), G, max_new, max_context, 0, 0, 0.125,
+            qq.data_ptr(), capi.Strides2(G * 64, 64), out.data_ptr(), ws.data_ptr() if n else None, n, 0))
+        _within(out, want, _attention_tolerance(F16, e4m3, False, want, mag))
