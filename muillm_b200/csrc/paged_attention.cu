@@ -36,6 +36,11 @@ struct PaArgs {
   float scale_log2;
 };
 
+// Length before the new tokens; 32-bit positions end at 2^31 - 1, so that no sum of a position passes 32 bits.
+__device__ __forceinline__ int context_of(const PaArgs& a, int b, int count) {
+  return min(__ldcg(a.kv.context_lens + b), 0x7fffffff - count);
+}
+
 // The cache rows that a sequence's new tokens see: tiles [0, n_sink) and [first, first + n - n_sink)
 struct Span {
   int kv_len, lo_min, n_sink, first, n;
@@ -46,7 +51,8 @@ __device__ __forceinline__ Span visible_span(const PaArgs& a, int ctx, int count
   s.kv_len = static_cast<int>(min(room, static_cast<long long>(ctx) + count));
   s.lo_min = a.window > 0 ? max(0, ctx - a.window + 1) : 0;
   s.first = s.lo_min / PA_TILE;
-  s.n_sink = min((min(a.sinks, s.lo_min) + PA_TILE - 1) / PA_TILE, s.first);
+  // kv_len: a position behind the block table may have more sinks than the table has rows
+  s.n_sink = min((min(min(a.sinks, s.lo_min), s.kv_len) + PA_TILE - 1) / PA_TILE, s.first);
   s.n = s.n_sink + max(0, (s.kv_len + PA_TILE - 1) / PA_TILE - s.first);
   return s;
 }
@@ -112,7 +118,7 @@ struct Run {
 // Length of a sequence's triples in places: `lead` places for their beginning, then one for each tile; 0: nothing to do
 __device__ __forceinline__ int seq_places(const PaArgs& a, int b, Run& r) {
   paged_new_tokens(a.kv, b, r.first, r.count);
-  r.ctx = __ldcg(a.kv.context_lens + b);
+  r.ctx = context_of(a, b, r.count);
   r.seq = b;
   if (r.count == 0 || r.ctx < 0 || r.count > a.max_new) return 0;
   if (a.mixed && r.count * a.G > PA_MAX_DECODE_ROWS) return 0;  // the prompt kernel's
@@ -949,7 +955,7 @@ __device__ __forceinline__ bool prompt_tile(const PaArgs& a, int x, PromptTile& 
   if (t.b >= a.kv.batch) return false;
   const int tile = x - start(t.b);
   paged_new_tokens(a.kv, t.b, t.first, t.count);
-  t.ctx = __ldcg(a.kv.context_lens + t.b);
+  t.ctx = context_of(a, t.b, t.count);
   t.r0 = tile * PT_ROWS;
   t.R = t.count * a.G;
   if (tile < 0 || t.r0 >= t.R) return false;

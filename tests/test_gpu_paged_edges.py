@@ -42,3 +42,25 @@ def test_attention_loose_bound_on_new_tokens(batch, G, max_new, e4m3):
             torch.cuda.current_stream().cuda_stream, capi.MUI_F16, ctypes.byref(kv), G, max_new, max_context, 0, 0, 0.125,
             qq.data_ptr(), capi.Strides2(G * 64, 64), out.data_ptr(), ws.data_ptr() if n else None, n, 0))
         _within(out, want, _attention_tolerance(F16, e4m3, False, want, mag))
+
+
+@pytest.mark.parametrize("ctx", [33, 500, 2 ** 31 - 3])
+@pytest.mark.parametrize("sinks", [40, 300, 2 ** 31 - 1])
+@pytest.mark.parametrize("new", [1, 50])
+def test_attention_sinks_beyond_the_table(new, sinks, ctx):
+    """More sink tokens than the block table has rows for, and a position behind it: the table is not read further than it
+    reaches."""
+    c = _filled([32], [0], 1, 64, 16, F16, False, seed=75, spread=0.3)
+    d = c.cuda()
+    table = torch.full((4, 2), 2 ** 30, dtype=torch.int32)  # behind the sequence's own row there are no pages
+    table[0] = c.table[0, :2]
+    d["block_table"] = table.cuda()[:1]
+    d["context_lens"] = _i32([ctx])
+    d["cu_tokens"] = _i32([0, new])
+    q = torch.randn(new, 2, 64, generator=_gen(76)).to(F16)
+    got = ops.paged_attention(q.cuda(), max_new_tokens=new, window=4, sinks=sinks, **d)
+    assert capi.device_status(clear=True) >> 24 == 5  # a length, not a bad page
+    k, v = (torch.cat([p[int(i), 0].double() for i in c.table[0, :2]]) for p in c.pools)
+    for h in range(2):
+        w = torch.softmax(q[:, h].double() @ k.T * 64 ** -0.5, 1)
+        _within(got[:, h], w @ v, _attention_tolerance(F16, False, new * 2 > 32, w @ v, w @ v.abs()))
