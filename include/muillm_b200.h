@@ -479,7 +479,8 @@ MUI_API mui_status_t mui_embedding_forward(void* stream, mui_dtype_t dtype, int 
  *
  * Two sequences may share full pages; the page that a sequence appends to must be its own. A block-table entry outside
  * [0, num_pages), a position beyond the table or beyond the rotary table, or more new tokens than max_new_tokens are
- * recorded in the device status word and skipped (nothing is read or written out of bounds). No counterpart in the
+ * recorded in the device status word and skipped (nothing is read or written out of bounds). cu_tokens must not decrease;
+ * where they do, tokens may land in other rows of the sequences' own pages from context_lens[b] on, and nowhere else. No counterpart in the
  * reference, whose caches are static, dynamic or sliding tensors (muillm/modules/kvcache/cache_utils.py:206-270). */
 typedef enum { MUI_KV_16BIT = 0, MUI_KV_E4M3 = 1 } mui_kv_format_t;
 typedef struct mui_strides2 { int64_t tok, head; } mui_strides2_t; /* in elements; innermost stride 1 */

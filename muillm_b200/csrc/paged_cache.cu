@@ -439,7 +439,8 @@ __global__ void __launch_bounds__(PC_THREADS, ROWS <= 2 ? 3 : 2) append_e4m3_ker
     return;
   }
   const int page_idx = (ctx >> sh) + u - ((first >> sh) + 2 * b);
-  if (count == 0 || (static_cast<long long>(page_idx) << sh) >= static_cast<long long>(ctx) + count) return;
+  // never in front of the first new row's page, which cu_tokens that decrease would otherwise bring about
+  if (count == 0 || page_idx < (ctx >> sh) || (static_cast<long long>(page_idx) << sh) >= static_cast<long long>(ctx) + count) return;
   const int page = find_page(a.kv, b, static_cast<long long>(page_idx) << sh);
   if (page < 0) return;
   const int head = (r >> 1) * a.unit_heads;

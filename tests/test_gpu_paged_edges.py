@@ -6,9 +6,34 @@ import torch
 
 from muillm_b200 import capi, ops
 from oracle import paged_oracle as oracle
-from test_gpu_paged import F16, _attention_tolerance, _filled, _gen, _i32, _within
+from test_gpu_paged import E4M3, F16, _attention_tolerance, _filled, _gen, _i32, _within
 
 pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cu", [[0, -40, 3], [-40, -20, 3], [3, 0, 3], [0, 90, 3]])
+def test_append_new_token_counts_that_make_no_sense(cu):
+    """cu_tokens that decrease or are negative: nothing outside the sequences' own pages is written."""
+    ctx, ps = [40, 24], 16
+    for e4m3 in (False, True):
+        dt = E4M3 if e4m3 else F16
+        kp = torch.ones(12, 1, ps, 64, dtype=F16, device="cuda").to(dt)
+        vp = kp.clone()
+        extra = {}
+        if e4m3:
+            extra = {n: torch.zeros(12, 1, device="cuda") for n in ("k_scales", "v_scales")}
+        table = _i32([[4, 5, 6, 7], [8, 9, 10, 11]])
+        x = torch.ones(3, 1, 64, dtype=F16, device="cuda")
+        before = kp.view(torch.uint8).clone()
+        ops.paged_kv_append(kp, vp, table, _i32(ctx), None, x, x, cu_tokens=_i32(cu), **extra)
+        for pool in (kp, vp):
+            assert torch.equal(pool.view(torch.uint8)[:4], before[:4])
+            # the rows in front of the new ones, but for those in the page that the first new one falls into
+            assert torch.equal(pool.view(torch.uint8)[[4, 5, 8]], before[[4, 5, 8]])
+        capi.device_status(clear=True)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
