@@ -95,6 +95,14 @@ __device__ __forceinline__ void cluster_sync(int cluster) {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// A peer's shared memory may be touched only once the peer runs: every thread says so first, and waits for the others' word
+// before its CTA's first access, which costs nothing where there is work in between.
+__device__ __forceinline__ void cluster_started(int cluster) {
+  if (cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_started(int cluster) {
+  if (cluster > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t peer_addr(const void* local, unsigned rank) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
@@ -491,6 +499,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   const unsigned rank = C > 1 ? cta_rank() : 0;
   const int r = blockIdx.x / C;
   int turn = 0;
+  cluster_started(C);
   pdl_wait_prior_grid();
   pdl_launch_dependents();
 
@@ -552,6 +561,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   }
   if (lane == 0) s.warp_u64[warp] = best;
   __syncthreads();
+  cluster_wait_started(C);
   if (warp == 0) {
     best = lane < SM_WARPS ? s.warp_u64[lane] : 0ull;
 #pragma unroll

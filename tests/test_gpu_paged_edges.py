@@ -12,6 +12,29 @@ pytestmark = pytest.mark.gpu
 
 
 # ---------------------------------------------------------------------------------------------------------------------
+# sampling
+# ---------------------------------------------------------------------------------------------------------------------
+def test_sample_clusters_beside_other_work():
+    """Rows shared by a cluster of CTAs, launched while another stream fills the GPU: every launch gives the same tokens."""
+    g = _gen(63)
+    x = (2.5 * torch.randn(3, 40000, generator=g)).cuda()
+    u = torch.rand(3, generator=g).cuda()
+    p = torch.full((3,), 0.9, device="cuda")
+    want = ops.sample_tokens(x, u, top_p=p)
+    other = torch.cuda.Stream()
+    a = torch.randn(2048, 2048, device="cuda")
+    other.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(30):
+        with torch.cuda.stream(other):
+            a = a * 1.0001
+        got.append(ops.sample_tokens(x, u, top_p=p))
+    torch.cuda.synchronize()
+    for tokens, logprobs in got:
+        assert torch.equal(tokens, want[0]) and torch.equal(logprobs, want[1])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
 # append
 # ---------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("cu", [[0, -40, 3], [-40, -20, 3], [3, 0, 3], [0, 90, 3]])
