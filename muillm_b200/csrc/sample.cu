@@ -892,6 +892,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     collect([&](float x) { return x >= x_min; }, use_p ? ROUGH : NO_WEIGHT, true);
     if (v[1] <= SM_LIST) {
       const int n = static_cast<int>(v[1]);
+      bool cuts = use_p;  // top-p may end within the list
       if (use_p) {
         if (rank == 0) {
           const u64 least = v[0] - (v[0] >> 10);
@@ -907,10 +908,21 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
           if (tid == 0) s.say.verdict = sure ? SM_FOUND : SM_BISECT;
         }
         tell(s, C, rank);
-        if (s.said.verdict != SM_FOUND) collect([](float) { return false; }, EXACT, false);
+        cuts = s.said.verdict != SM_FOUND;
+        if (cuts) collect([](float) { return false; }, EXACT, false);
       }
-      if (rank == 0) finish(n, v[0], false);
-      return;
+      // a list that is not cut, or of few tokens, is always brought to an end
+      const bool ends = !cuts || n <= SM_FEW;
+      if (ends && rank != 0) return;
+      if (rank == 0) {
+        const bool ok = finish(n, v[0], false);
+        if (ends) return;
+        __syncthreads();
+        if (tid == 0) s.say.verdict = ok ? SM_FOUND : SM_UP;
+      }
+      tell(s, C, rank);
+      if (s.said.verdict == SM_FOUND) return;
+      // top-p ends in a bin of more tokens than are sorted
     }
     if (tid == 0) s.list_n[0] = 0;  // a barrier follows before the next token is put there
   }

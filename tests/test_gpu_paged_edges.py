@@ -6,7 +6,7 @@ import torch
 
 from muillm_b200 import capi, ops
 from oracle import paged_oracle as oracle
-from test_gpu_paged import E4M3, F16, _attention_tolerance, _filled, _gen, _i32, _within
+from test_gpu_paged import BF16, E4M3, F16, _attention_tolerance, _filled, _gen, _i32, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -14,6 +14,43 @@ pytestmark = pytest.mark.gpu
 # ---------------------------------------------------------------------------------------------------------------------
 # sampling
 # ---------------------------------------------------------------------------------------------------------------------
+def _check_written(logits, u, **kw):
+    """Tokens and log shares into buffers that hold something else before the call."""
+    rows, vocab = logits.shape
+    code = {F16: capi.MUI_F16, BF16: capi.MUI_BF16, torch.float32: capi.MUI_COMM_F32}[logits.dtype]
+    x, dev = logits.cuda(), {n: t.cuda() for n, t in kw.items()}
+    tokens = torch.full((rows,), -7, dtype=torch.int64, device="cuda")
+    logprobs = torch.full((rows,), 7.0, device="cuda")
+    uu = u.cuda()
+
+    def ptr(n):
+        return dev[n].data_ptr() if n in dev else None
+
+    capi.check(capi.lib().mui_sample_tokens(
+        torch.cuda.current_stream().cuda_stream, code, rows, vocab, x.data_ptr(), x.stride(0), ptr("temperature"),
+        ptr("top_k"), ptr("top_p"), ptr("min_p"), uu.data_ptr(), tokens.data_ptr(), logprobs.data_ptr(), 0))
+    for r in range(rows):
+        one = {n: t[r].item() for n, t in kw.items()}
+        want, lp, _ = oracle.sample(logits[r], u[r].item(), **one)
+        assert int(tokens[r]) == want, (r, int(tokens[r]), want, one)
+        got = float(logprobs[r])
+        assert got == lp or abs(got - lp) <= 1e-6 * max(1.0, abs(lp)), (r, got, lp)  # fp32 rounding of the logarithm
+
+
+@pytest.mark.parametrize("rows", [2, 100])
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_sample_min_p_and_top_p_within_thousands_of_alike_logits(dtype, rows):
+    """Top-p ends among thousands of tokens of about the same logit, all of which min-p keeps."""
+    g = _gen(61)
+    vocab = 9000
+    ties = torch.where(torch.rand(rows, vocab, generator=g) < 0.4, 0.0, -3.0)
+    hot = torch.randn(rows, vocab, generator=g)
+    u = torch.rand(rows, generator=g)
+    top_p = 0.1 + 0.5 * torch.rand(rows, generator=g)
+    _check_written(ties.to(dtype), u, top_p=top_p, min_p=torch.full((rows,), 0.5))
+    _check_written(hot.to(dtype), u, top_p=top_p, min_p=torch.full((rows,), 0.5), temperature=torch.full((rows,), 40.0))
+
+
 def test_sample_clusters_beside_other_work():
     """Rows shared by a cluster of CTAs, launched while another stream fills the GPU: every launch gives the same tokens."""
     g = _gen(63)
