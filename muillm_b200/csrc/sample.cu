@@ -597,7 +597,8 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   w.floor = fmaxf(fminf(w.top - z_range * t, key_logit(best_key - 1)), -3.402823466e38f);
   w.scale = 46.166241308446828 / static_cast<double>(t);  // 32 / ln 2
   w.table = exp2(static_cast<double>(lane) / 32.0);
-  w.bin_scale = static_cast<float>(SM_BINS) / z_range / t;
+  // finite, so that the largest logit is in bin 0: next to logits of 0 the smallest temperatures only make the bins wider
+  w.bin_scale = fminf(static_cast<float>(SM_BINS) / z_range / t, 3.402823466e38f);
   const u64 one = 1ull << a.frac_bits;
   // min-p in the integers of the weights (the largest token has weight 1 and always stays), and a logit safely below its cut
   const float min_w = fminf(min_p, 1.f);

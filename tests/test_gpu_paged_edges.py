@@ -1,5 +1,6 @@
 """Calls of the paged-cache and sampling operators at the ends of what their documentation allows."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -49,6 +50,33 @@ def test_sample_min_p_and_top_p_within_thousands_of_alike_logits(dtype, rows):
     top_p = 0.1 + 0.5 * torch.rand(rows, generator=g)
     _check_written(ties.to(dtype), u, top_p=top_p, min_p=torch.full((rows,), 0.5))
     _check_written(hot.to(dtype), u, top_p=top_p, min_p=torch.full((rows,), 0.5), temperature=torch.full((rows,), 40.0))
+
+
+@pytest.mark.parametrize("which", ["none", "k", "p", "kp", "m", "pm", "kpm"])
+def test_sample_smallest_temperatures_at_logits_of_zero(which):
+    """Temperatures next to the smallest normal number in rows whose largest logit is 0 or +infinity: the steps between
+    logits next to 0 are not smaller than those temperatures, so several tokens have weight."""
+    g = _gen(62)
+    near = -torch.rand(4, 3001, generator=g) * 4e-37
+    far = -torch.rand(4, 3001, generator=g)
+    far[:, 77] = 0.0
+    near[:, 1234] = 0.0
+    inf = far.clone()
+    inf[:, [5, 900]] = math.inf
+    u = torch.tensor([0.0, 0.3, 0.6, 0.95])
+    kw = {}
+    if "k" in which:
+        kw["top_k"] = torch.tensor([1, 40, 700, 3000], dtype=torch.int32)
+    if "p" in which:
+        kw["top_p"] = torch.tensor([0.9, 0.5, 0.97, 0.3])
+    if "m" in which:
+        kw["min_p"] = torch.tensor([0.01, 0.2, 1e-4, 0.05])
+    for t in (1.2e-38, 1e-37, 1.6e-37, 1e-36):
+        for x in (near, far, inf):
+            _check_written(x, u, temperature=torch.full((4,), t), **kw)
+    for t in (1e-38, 1e-45):  # below the smallest normal number: as that one, which these rows cannot tell
+        for x in (far, inf):
+            _check_written(x, u, temperature=torch.full((4,), t), **kw)
 
 
 def test_sample_clusters_beside_other_work():
