@@ -479,7 +479,9 @@ MUI_API mui_status_t mui_embedding_forward(void* stream, mui_dtype_t dtype, int 
  *
  * Two sequences may share full pages; the page that a sequence appends to must be its own. A block-table entry outside
  * [0, num_pages), a position beyond the table or beyond the rotary table, or more new tokens than max_new_tokens are
- * recorded in the device status word and skipped (nothing is read or written out of bounds). cu_tokens must not decrease;
+ * recorded in the device status word and skipped (nothing is read or written out of bounds): tokens behind the table's reach
+ * attend to what the table holds, with result 0 where that is nothing, and sequences of a negative length or of too many new
+ * tokens get no result. cu_tokens must not decrease;
  * where they do, tokens may land in other rows of the sequences' own pages from context_lens[b] on, and nowhere else. No counterpart in the
  * reference, whose caches are static, dynamic or sliding tensors (muillm/modules/kvcache/cache_utils.py:206-270). */
 typedef enum { MUI_KV_16BIT = 0, MUI_KV_E4M3 = 1 } mui_kv_format_t;

@@ -261,8 +261,16 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
     Run r;
     const long long n = static_cast<long long>(seq_places(a, s, r)) * pairs;
     // sequences that cannot be served have no places: say so
-    if (blockIdx.x == 0 && n == 0 && r.count > 0 && (r.ctx < 0 || r.count > a.max_new))
-      mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(r.ctx < 0 ? r.ctx : r.count));
+    if (blockIdx.x == 0 && n == 0 && r.count > 0) {
+      if (r.ctx < 0 || r.count > a.max_new) {
+        mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(r.ctx < 0 ? r.ctx : r.count));
+      } else if (!a.mixed || r.count * a.G <= PA_MAX_DECODE_ROWS) {
+        // a window behind the block table's reach: nothing to see
+        mui_dev_set_status(MUI_DEV_BAD_LENGTH, static_cast<unsigned>(r.ctx));
+        uint4* row = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + static_cast<size_t>(r.first) * a.Hq * D);
+        for (int e = 0; e < r.count * a.Hq * (D / 8); ++e) row[e] = make_uint4(0, 0, 0, 0);
+      }
+    }
     if (place >= begin && place < begin + n) {
       r.begin = begin;
       s_run = r;

@@ -157,6 +157,43 @@ def test_attention_loose_bound_on_new_tokens(batch, G, max_new, e4m3):
         _within(out, want, _attention_tolerance(F16, e4m3, False, want, mag))
 
 
+BEYOND = [
+    # new tokens of the sequence that lies beyond its table, window, sinks
+    (1, 10, 0), (3, 10, 0), (50, 10, 0), (1, 0, 0), (50, 0, 0), (1, 10, 5), (50, 10, 5),
+]
+
+
+@pytest.mark.parametrize("ctx", [32, 500, 2 ** 31 - 3])
+@pytest.mark.parametrize("new,window,sinks", BEYOND)
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_attention_beyond_the_table(new, window, sinks, ctx, e4m3):
+    """Positions behind the block table's reach are recorded; their tokens see what the table holds, 0 where that is
+    nothing. The other sequences of the call are served."""
+    c = _filled([20, 9], [12, 1], 2, 64, 16, F16, e4m3, seed=73, spread=0.3)
+    d = c.cuda()
+    d["block_table"] = d["block_table"][:, :2].contiguous()
+    d["context_lens"] = _i32([ctx, 9])
+    d["cu_tokens"] = _i32([0, new, new + 1])
+    q = torch.randn(new + 1, 4, 64, generator=_gen(74)).to(F16)
+    out = torch.full((new + 1, 4, 64), 7.0, dtype=F16, device="cuda")
+    ops.paged_attention(q.cuda(), max_new_tokens=new, window=window, sinks=sinks, out=out, **d)
+    assert capi.device_status(clear=True) >> 24 == 5
+    # what a token at ctx + i sees of the 32 rows that there are
+    far = [min(ctx, 10 ** 6) + i for i in range(new)]
+    rows = torch.arange(32)
+    see = torch.stack([(rows <= p) & ((rows > p - window) | (rows < sinks) if window else rows >= 0) for p in far])
+    pk, pv, sk, sv = c.oracle_args()
+    for h in range(4):
+        k, v = (torch.cat([p[int(c.table[0, i]), h // 2].float().double() * (1.0 if s is None else float(s[int(c.table[0, i]), h // 2]))
+                           for i in range(2)]) for p, s in ((pk, sk), (pv, sv)))
+        a = (q[:new, h].double() @ k.T * 64 ** -0.5).masked_fill(~see, -math.inf)
+        w = torch.softmax(a, 1).nan_to_num(0.0)
+        want, mag = w @ v, w @ v.abs()
+        _within(out[:new, h], want, _attention_tolerance(F16, e4m3, new * 2 > 32, want, mag))
+    want, mag = oracle.attention(q[new:], pk, pv, sk, sv, c.table[1:], [9], [1], window, sinks)
+    _within(out[new:], want, _attention_tolerance(F16, e4m3, False, want, mag))
+
+
 @pytest.mark.parametrize("ctx", [33, 500, 2 ** 31 - 3])
 @pytest.mark.parametrize("sinks", [40, 300, 2 ** 31 - 1])
 @pytest.mark.parametrize("new", [1, 50])
