@@ -224,7 +224,7 @@ __device__ __forceinline__ uint4 load_q8(const T* p, int vec) {
 
 struct TileMeta {
   int tb;        // first cache row, -1: nothing to see
-  float ks, vs;  // page scales (e4m3)
+  float ks, lv;  // e4m3: K scale of the page, logarithm of its V scale
 };
 
 // 4 warps; row = new token * G + head in the group; NT blocks of eight rows per CTA
@@ -235,6 +235,11 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
   // row that brings its largest element near 1, and the probabilities
   using M = typename std::conditional<KV8, __half, T>::type;
   constexpr bool SPLIT_P = std::is_same<M, __nv_bfloat16>::value;  // probabilities as bf16 value + bf16 rest
+  // Probabilities in fp16 are taken times 2^LIFT, the largest one next to the end of fp16's range, so that they have all eleven
+  // bits down to 2^-29 of it (at 2^-14, without, half a million rows of little weight lose theirs together). Over e4m3 pages what is
+  // rounded is the probability times V's scale, against the row's own largest such product. The references m (of the sum) and mo (of
+  // the output, e4m3) stand LIFT below those maxima.
+  constexpr float LIFT = std::is_same<M, __half>::value ? 15.f : 0.f;
   constexpr int U = I::U, KB = I::KB, KS = I::KS, MT = D / 16;
   extern __shared__ __align__(128) unsigned char pa_smem[];        // [warp][PA_RING][PA_ITEM]; the join reuses it
   __shared__ float sm_m[PA_WARPS][NT * 8], sm_l[PA_WARPS][NT * 8];
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
     const int my_groups = groups > warp ? (groups - warp + PA_WARPS - 1) / PA_WARPS : 0;
     // The next 32 are begun half a batch ahead: pages first, their scales once the pages are there.
     int my_page = -1, my_tb = -1, next_page = -1, next_tb = -1;
-    float my_ks = 0.f, my_vs = 0.f, next_ks = 0.f, next_vs = 0.f;
+    float my_ks = 0.f, my_lv = 0.f, next_ks = 0.f, next_vs = 0.f;
     auto ask_pages = [&](int grp) {
       const int i = i_begin + ((grp + lane / U) * PA_WARPS + warp) * U + lane % U;
       next_page = next_tb = -1;
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
             my_page = next_page;
             my_tb = next_tb;
             my_ks = next_ks;
-            my_vs = next_vs;
+            if (KV8) my_lv = log2f(next_vs);
           }
           if (phase == 16) ask_pages(grp + 16 / U);
           if (phase == 24) ask_scales();
@@ -345,7 +350,7 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
             TileMeta& t = sm_meta[warp][grp & 1][lane % U];
             t.tb = my_tb;
             t.ks = my_ks;
-            t.vs = my_vs;
+            t.lv = my_lv;
           }
         }
         const unsigned char* base = reinterpret_cast<const unsigned char*>(which == 0 ? a.kv.k_pages : a.kv.v_pages);
@@ -448,10 +453,10 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
     }
     const int lo_max = a.window > 0 ? ctx + count - a.window : 0;  // first row the last new token's window holds
 
-    float m[NT][2], l[NT][2], o[MT][NT][4], vref = 0.f;
+    float m[NT][2], mo[NT][2], l[NT][2], o[MT][NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      m[n][0] = m[n][1] = -INFINITY;
+      m[n][0] = m[n][1] = mo[n][0] = mo[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < MT; ++j) o[j][n][0] = o[j][n][1] = o[j][n][2] = o[j][n][3] = 0.f;
@@ -515,33 +520,40 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
             }
           }
       }
-      float turn = 1.f;  // e4m3: change of the reference scale of the output
-      if (KV8) {
-        float v = vref;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (meta[u].tb >= 0) v = fmaxf(v, meta[u].vs);
-        if (v > vref) {
-          turn = vref / v;
-          vref = v;
-        }
-      }
-      bool moved = turn != 1.f;
-      float corr[NT][2];
+      bool moved = false;
+      float corr[NT][2];  // of the output
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float mx = -INFINITY;
+          float mx = -INFINITY, mv = -INFINITY;
 #pragma unroll
-          for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(s[u][n][i], s[u][n][2 + i]));
-          mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, 16));
-          const float mn = fmaxf(m[n][i], mx);
+          for (int u = 0; u < U; ++u) {
+            const float t = fmaxf(s[u][n][i], s[u][n][2 + i]);
+            mx = fmaxf(mx, t);
+            if (KV8) mv = fmaxf(mv, t + meta[u].lv);
+          }
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(MUI_FULL_MASK, mx, x));
+            if (KV8) mv = fmaxf(mv, __shfl_xor_sync(MUI_FULL_MASK, mv, x));
+          }
+          const float mn = fmaxf(m[n][i], mx - LIFT);
           const float use = mn == -INFINITY ? 0.f : mn;
           corr[n][i] = ex2(m[n][i] - use);
-          moved |= mn != m[n][i];
+          l[n][i] *= corr[n][i];
+          float f[U];
+          if (KV8) {
+            const float vn = fmaxf(mo[n][i], mv - LIFT);
+            const float use_v = vn == -INFINITY ? 0.f : vn;
+            corr[n][i] = ex2(mo[n][i] - use_v);
+            moved |= vn != mo[n][i];
+            mo[n][i] = vn;
+#pragma unroll
+            for (int u = 0; u < U; ++u) f[u] = ex2(fminf(use - use_v + meta[u].lv, 120.f));  // finite: 0 stays 0
+          } else {
+            moved |= mn != m[n][i];
+          }
           m[n][i] = mn;
           float sum = 0.f;
 #pragma unroll
@@ -549,31 +561,32 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
             s[u][n][i] = ex2(s[u][n][i] - use);
             s[u][n][2 + i] = ex2(s[u][n][2 + i] - use);
             sum += s[u][n][i] + s[u][n][2 + i];
+            if (KV8) {
+              s[u][n][i] *= f[u];
+              s[u][n][2 + i] *= f[u];
+            }
           }
-          l[n][i] = l[n][i] * corr[n][i] + sum;
+          l[n][i] += sum;
         }
       if (__any_sync(MUI_FULL_MASK, moved)) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float c0 = corr[n][0] * turn, c1 = corr[n][1] * turn;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
-            o[j][n][0] *= c0;
-            o[j][n][1] *= c1;
-            o[j][n][2] *= c0;
-            o[j][n][3] *= c1;
+            o[j][n][0] *= corr[n][0];
+            o[j][n][1] *= corr[n][1];
+            o[j][n][2] *= corr[n][0];
+            o[j][n][3] *= corr[n][1];
           }
-        }
       }
       uint32_t pb[U][NT][2], pr[U][NT][2];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float f = KV8 ? (meta[u].tb >= 0 && vref > 0.f ? meta[u].vs / vref : 0.f) : 1.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float p0 = KV8 ? s[u][n][2 * h] * f : s[u][n][2 * h], p1 = KV8 ? s[u][n][2 * h + 1] * f : s[u][n][2 * h + 1];
+            const float p0 = s[u][n][2 * h], p1 = s[u][n][2 * h + 1];
             const uint32_t x = Elt<M>::pack2(p0, p1);
             pb[u][n][h] = movmatrix(x);
             if (SPLIT_P) {
@@ -690,10 +703,11 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
         v += __shfl_xor_sync(MUI_FULL_MASK, v, 16);
         const int r = n * 8 + 2 * tq + i;
         if (g == 0) {
-          sm_m[warp][r] = m[n][i];
-          sm_l[warp][r] = v;
+          sm_m[warp][r] = m[n][i] + LIFT;
+          sm_l[warp][r] = v * exp2_int(-static_cast<int>(LIFT));
         }
-        const float f = KV8 ? vref : 1.f;
+        // o relative to the row's maximum, like the sum
+        const float f = !KV8 ? exp2_int(-static_cast<int>(LIFT)) : mo[n][i] == -INFINITY ? 0.f : ex2(mo[n][i] - m[n][i] - LIFT);
         float* row = sm_o + (warp * NT * 8 + r) * D;
 #pragma unroll
         for (int j = 0; j < MT; ++j) {

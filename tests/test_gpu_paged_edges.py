@@ -214,3 +214,60 @@ def test_attention_sinks_beyond_the_table(new, sinks, ctx):
     for h in range(2):
         w = torch.softmax(q[:, h].double() @ k.T * 64 ** -0.5, 1)
         _within(got[:, h], w @ v, _attention_tolerance(F16, False, new * 2 > 32, w @ v, w @ v.abs()))
+
+
+def _low_rows(n, new, dtype, e4m3, low_scale, D=64, page=64):
+    """One sequence of n rows and one KV head. Rows 0, 32, ... 224 win: their V is 1 in element 0, and 0 elsewhere. All other
+    rows have 128.5 * 2^-24 of the winners' probability, half-way between two fp16 numbers, and V in the other elements;
+    on e4m3 pages the V scale is low_scale for the pages behind row 256. Returns (arguments, q, want)."""
+    g = _gen(81)
+    pages = -(-n // page)
+    k, v = torch.zeros(pages * page, D), 0.5 + torch.rand(pages * page, D, generator=g)
+    v[:, 0] = 0.0
+    win = torch.arange(0, 256, 32)
+    k[win, 0] = 11.0
+    v[win] = 0.0
+    v[win, 0] = 1.0
+    k, v = (x.reshape(pages, 1, page, D).to(E4M3 if e4m3 else dtype) for x in (k, v))
+    scale = math.log(2.0 ** 24 / 128.5) / 11.0
+    args = dict(k_pages=k.cuda(), v_pages=v.cuda(), block_table=torch.arange(pages, dtype=torch.int32)[None].cuda(),
+                context_lens=_i32([n - new]), scale=scale, max_new_tokens=new, max_context=1)
+    v = v.float().double()
+    if e4m3:
+        sv = torch.where(torch.arange(pages) * page < 256, 1.0, low_scale)[:, None].clone()
+        args.update(k_scales=torch.ones(pages, 1, device="cuda"), v_scales=sv.cuda())
+        v = v * sv.double()[:, :, None, None]
+    if new > 1:
+        args["cu_tokens"] = _i32([0, new])
+    q = torch.zeros(new, 2, D)
+    q[..., 0] = 1.0
+    a = k.float().double().reshape(-1, D)[:, 0] * float(torch.tensor(scale, dtype=torch.float32))
+    v = v.reshape(-1, D)
+    return args, q.to(dtype), lambda t: torch.softmax(a[: n - new + 1 + t], 0) @ v[: n - new + 1 + t]
+
+
+LOW_ROWS = pytest.mark.parametrize("dtype,e4m3,low_scale", [
+    (F16, False, None), (BF16, False, None), (F16, True, 1.0), (BF16, True, 2.0 ** -9), (F16, True, 3.0 * 2.0 ** -8),
+    (F16, True, 2.0 ** 9)])
+
+
+def _check_low_rows(n, new, dtype, e4m3, low_scale, **kw):
+    """The running sums are fp32: of the output, an addition for every 16 rows, which the tensor cores may cut off (2^-23 of the
+    sum); of the weights, at most as many, rounded (2^-24). One CTA takes all rows: four warps a quarter each (up to 32
+    rows of queries), or one accumulator."""
+    args, q, want_of = _low_rows(n, new, dtype, e4m3, low_scale, **kw)
+    got = ops.paged_attention(q.cuda(), **args)
+    prompt = 2 * new > 32
+    steps = n / 16 / (1 if prompt else 4)
+    for t in {0, new - 1}:
+        want = want_of(t)[None].expand(2, -1)
+        _within(got[t], want, _attention_tolerance(dtype, e4m3, prompt, want, want) + want * steps * (2.0 ** -23 + 2.0 ** -24))
+
+
+@LOW_ROWS
+def test_attention_many_rows_of_little_weight(dtype, e4m3, low_scale):
+    """Thousands of rows of 2^-17 of the largest probability each, which have elements of V to themselves."""
+    _check_low_rows(400000, 1, dtype, e4m3, low_scale)
+    _check_low_rows(200000, 16, dtype, e4m3, low_scale, D=128, page=32)
+    _check_low_rows(20000, 1, dtype, e4m3, low_scale)
+    _check_low_rows(20000, 16, dtype, e4m3, low_scale, D=128, page=32)
