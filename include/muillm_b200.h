@@ -515,8 +515,9 @@ MUI_API mui_status_t mui_paged_kv_append(void* stream, mui_dtype_t dtype, const 
  * max_new_tokens bounds the new tokens of every sequence (1 where cu_tokens is NULL, whatever is given). max_context (> 0) is a hint for the work split, the longest
  * sequence expected (any value gives right results). What a token does not see does not reach its result, infinities and
  * NaN included (prompts that have any in V take about twenty times longer). Softmax statistics, sums and outputs are held in fp32 and rounded once;
- * with up to 32 queries a KV head and sequence the probabilities enter the second product as bf16 and a bf16 rest (bf16 pages) or as
- * fp16, over e4m3 pages times V's scale, with eleven bits down to 2^-29 of the row's largest. workspace:
+ * the probabilities enter the second product in 16 bits: with bf16 pages as bf16, up to 32 queries a KV head and sequence (new
+ * tokens times heads) with a bf16 rest; else as fp16, over e4m3 pages times V's scale, with eleven bits down to 2^-29 (more than 32
+ * queries: 2^-21) of the row's largest. workspace:
  * mui_paged_attention_workspace_bytes() bytes of scratch for the same sizes, 16-byte aligned, any contents; it may be
  * used by one call at a time. */
 MUI_API size_t mui_paged_attention_workspace_bytes(int total_tokens, int batch, int num_q_heads, int kv_heads,

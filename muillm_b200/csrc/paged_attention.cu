@@ -867,7 +867,8 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
 //
 // The reference of a row's exponents is its running maximum, but moves only when the maximum is more than 8 (a factor 256)
 // above it: then O is rescaled in tensor memory, which is rare after the first tiles; P stays below 2^8 and the sums are right in
-// any case. P is rounded once to the type of the tensor-core operands (half a step is 2^-9 of it for bf16, 2^-12 for fp16).
+// any case. P is rounded once to the type of the tensor-core operands (half a step is 2^-9 of it for bf16, 2^-12 for fp16: there P is
+// taken times 2^7, so that it has all its bits down to 2^-21 of the reference).
 // Bound: exp2 (16 a cycle and SM) and the MMAs need about 2050 cycles a step each.
 // Measured (32 q and 8 KV heads of 128, device time; tensor cores 1651 TFLOP/s): one prompt of 8192 tokens, bf16 pages, 555 us =
 // 990 TFLOP/s; three chunks of 1023 to 2049 tokens behind up to 2100, 223 us = 774 TFLOP/s (the last round of CTAs is not full);
@@ -1095,6 +1096,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
   constexpr int KT = PT_KEYS * D * 2;                  // bytes of a K or V tile
   constexpr int BLOCK = PT_KEYS * 128;                 // bytes of one 64-element block of a tile (Q, K or V)
   constexpr uint32_t TM_S = 0, TM_O = 2 * PT_KEYS;     // tensor-memory columns
+  constexpr float PT_LIFT = std::is_same<M, __half>::value ? 7.f : 0.f;  // with the slack 2^15 at most, of fp16's 2^16
   extern __shared__ unsigned char pt_raw[];
   __shared__ uint64_t kv_full[PT_SLOTS], kv_empty[PT_SLOTS], s_full[2], p_half[2], p_full[2], pv_done[2];
   __shared__ float q_back[PT_ROWS];
@@ -1444,7 +1446,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       const int hi_all = t.ctx + (t.r0 + g * PT_GROUP) / a.G;
       const int lo_all = a.window > 0 ? t.ctx + last_row / a.G - a.window + 1 : 0;
       const float sc = KV8 ? a.scale_log2 * q_back[g * PT_GROUP + row] : fmaxf(a.scale_log2, 1e-37f);
-      float ref = -INFINITY, l = 0.f, vref = 0.f;
+      // references of the sum and, over e4m3 pages, of the output: there what is rounded is the probability times V's scale, against
+      // the row's own largest such product
+      float ref = -INFINITY, vref = -INFINITY, l = 0.f;
       int page, tb, next_page, next_tb;
       float ks = 0.f, vs = 0.f;
       auto scales = [&](int p, float& k, float& v) {
@@ -1469,7 +1473,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
         tc_after();
         // factor of the scores of 16 columns; above 0, since -infinity stands for what a row does not see
         auto factor_of = [&](int sub) { return KV8 ? fmaxf(sc * __shfl_sync(MUI_FULL_MASK, ks, sub), 1e-37f) : sc; };
-        float mx = -INFINITY;
+        const float lv = KV8 ? log2f(vs) : 0.f;
+        float mx = -INFINITY, mv = -INFINITY;
+        auto see_top = [&](int sub, float x) {  // the largest score of 16 columns
+          mx = fmaxf(mx, x);
+          if (KV8) mv = fmaxf(mv, x + __shfl_sync(MUI_FULL_MASK, lv, sub));
+        };
         if (open) {
           uint32_t s0[32], s1[32];
           auto top = [&](int c, const uint32_t(&s)[32]) {
@@ -1481,7 +1490,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 m0 = fmaxf(m0, __uint_as_float(s[16 * h + e]));
                 m1 = fmaxf(m1, __uint_as_float(s[16 * h + e + 1]));
               }
-              mx = fmaxf(mx, fmaxf(m0, m1) * factor_of(2 * c + h));
+              see_top(2 * c + h, fmaxf(m0, m1) * factor_of(2 * c + h));
             }
           };
           tmem_ask32(ts, s0);
@@ -1518,25 +1527,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
                 top = fmaxf(top, x);
                 w[e] = __float_as_uint(x);
               }
-              mx = fmaxf(mx, top * f);
+              see_top(2 * c + h, top * f);
               tmem_store16(ts + c * 32 + 16 * h, w);
             }
           }
           tmem_store_wait();
         }
-        float turn = 1.f;  // e4m3: change of the output's reference scale
-        if (KV8) {
-          const float v = fmaxf(vref, warp_max(lane < PT_SUB ? vs : 0.f));
-          if (v > vref) {
-            turn = vref / v;
-            vref = v;
-          }
-        }
-        float factor = turn;
+        float factor = 1.f;  // of the output so far
         if (mx > ref + PT_SLACK || ref == -INFINITY) {
-          factor *= ref == -INFINITY ? 0.f : ex2(ref - mx);
-          l *= ref == -INFINITY ? 0.f : ex2(ref - mx);
+          factor = ref == -INFINITY ? 0.f : ex2(ref - mx);
+          l *= factor;
           ref = mx;
+        }
+        if (KV8) {
+          factor = 1.f;
+          if (mv > vref + PT_SLACK || vref == -INFINITY) {
+            factor = vref == -INFINITY ? 0.f : ex2(vref - mv);
+            vref = mv;
+          }
         }
         if (j > 0 && __any_sync(MUI_FULL_MASK, factor != 1.f)) {
           ok = __all_sync(MUI_FULL_MASK, wait(&pv_done[g], j - 1, 0x310 + g));
@@ -1556,7 +1564,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
             }
           }
         }
-        const float use = ref == -INFINITY ? 0.f : -ref;
+        const float ref0 = ref == -INFINITY ? 0.f : ref, use = PT_LIFT - ref0;
+        const float turn = KV8 ? ref0 - (vref == -INFINITY ? 0.f : vref) : 0.f;
         {
           uint32_t s0[32], s1[32];
           float2 sum = make_float2(0.f, 0.f);
@@ -1565,7 +1574,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float f = factor_of(2 * c + h);
-              const float pf = KV8 ? (vref > 0.f ? __shfl_sync(MUI_FULL_MASK, vs, 2 * c + h) / vref : 0.f) : 1.f;
+              // finite: 0 stays 0
+              const float pf = KV8 ? ex2(fminf(turn + __shfl_sync(MUI_FULL_MASK, lv, 2 * c + h), 120.f)) : 1.f;
 #pragma unroll
               for (int e = 0; e < 16; e += 2) {
                 float2 p = fma2(make_float2(__uint_as_float(s[16 * h + e]), __uint_as_float(s[16 * h + e + 1])),
@@ -1606,7 +1616,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1)
       tc_after();
       if (ok) {
         const bool direct = t.active == 1;
-        const float norm = (direct ? (l != 0.f ? 1.f / l : 0.f) : 1.f) * (KV8 ? vref : 1.f);
+        l *= exp2_int(-static_cast<int>(PT_LIFT));
+        const float back = !KV8 ? exp2_int(-static_cast<int>(PT_LIFT)) : vref == -INFINITY ? 0.f : ex2(vref - ref - PT_LIFT);
+        const float norm = direct ? (l != 0.f ? back / l : 0.f) : back;
         const size_t out_row = static_cast<size_t>(t.first + rr / a.G) * a.Hq + kvh * a.G + rr % a.G;
         float* part = a.partials + (out_row * a.splits + split) * (D + 2);
         if (mine && !direct) {

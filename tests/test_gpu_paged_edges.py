@@ -271,3 +271,10 @@ def test_attention_many_rows_of_little_weight(dtype, e4m3, low_scale):
     _check_low_rows(200000, 16, dtype, e4m3, low_scale, D=128, page=32)
     _check_low_rows(20000, 1, dtype, e4m3, low_scale)
     _check_low_rows(20000, 16, dtype, e4m3, low_scale, D=128, page=32)
+
+
+@LOW_ROWS
+def test_attention_prompts_many_rows_of_little_weight(dtype, e4m3, low_scale):
+    """The same for prompts."""
+    _check_low_rows(20000, 40, dtype, e4m3, low_scale)
+    _check_low_rows(9000, 70, dtype, e4m3, low_scale, D=128, page=128)
