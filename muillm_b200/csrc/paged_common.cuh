@@ -63,18 +63,21 @@ inline mui_status_t paged_check(mui_dtype_t dtype, const mui_paged_kv_t* c) {
 }
 
 // How many of the `batch` non-decreasing values value(0), value(1), ... are <= x: with value(i) = the first unit of
-// sequence i + 1 that is the sequence of unit x. Whole warp, one load per lane and 32 sequences.
+// sequence i + 1 that is the sequence of unit x. Whole warp: the range is cut into 32 blocks whose last values the lanes look at,
+// until a block has one value: one step for 32 sequences, two for 1024, four for 65535 (one after the other, 4096 sequences cost
+// each token 128 round trips). Values that are not in order give a number within the range.
 template <typename F>
 __device__ __forceinline__ int warp_count_le(int batch, int x, F value) {
   const int lane = threadIdx.x & 31;
-  int n = 0;
-  for (int base = 0; base < batch; base += 32) {
-    const int i = base + lane;
-    const unsigned m = __ballot_sync(MUI_FULL_MASK, i < batch && value(i) <= x);
-    n += __popc(m);
-    if (m != MUI_FULL_MASK) break;
+  int lo = 0, n = batch;  // the answer is in [lo, lo + n]
+  while (n > 0) {
+    const int step = (n + 31) / 32, i = lane * step + step - 1;
+    const unsigned m = __ballot_sync(MUI_FULL_MASK, i < n && value(lo + i) <= x);
+    const int whole = m == MUI_FULL_MASK ? 32 : __ffs(~m) - 1;  // blocks of which all values are <= x
+    lo += whole * step;
+    n = min(step - 1, n - whole * step);
   }
-  return n;
+  return lo;
 }
 
 // new tokens of sequence b as [first row, count], clamped to the rows that exist

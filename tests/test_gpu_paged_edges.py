@@ -7,7 +7,7 @@ import torch
 
 from muillm_b200 import capi, ops
 from oracle import paged_oracle as oracle
-from test_gpu_paged import BF16, E4M3, F16, _attention_tolerance, _filled, _gen, _i32, _within
+from test_gpu_paged import BF16, E4M3, F16, Cache, _attention_tolerance, _check_append, _filled, _gen, _i32, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -278,3 +278,25 @@ def test_attention_prompts_many_rows_of_little_weight(dtype, e4m3, low_scale):
     """The same for prompts."""
     _check_low_rows(20000, 40, dtype, e4m3, low_scale)
     _check_low_rows(9000, 70, dtype, e4m3, low_scale, D=128, page=128)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("batch", [1, 129, 1500])
+def test_large_batches(batch, e4m3):
+    """Append and attention for many sequences of few or no new tokens: each token finds its sequence, each result its row."""
+    g = _gen(91)
+    new = torch.randint(0, 4, (batch,), generator=g).tolist()
+    new[-1] = 40
+    for counts in (new, [1] * batch):
+        ctx = torch.randint(0, 30, (batch,), generator=g).tolist()
+        c = Cache(ctx, counts, 1, 64, 16, F16, e4m3, seed=92, spread=0.3)
+        k, v = (torch.randn(sum(counts), 1, 64, generator=g).to(F16) for _ in range(2))
+        q = torch.randn(sum(counts), 2, 64, generator=g).to(F16)
+        d, _ = _check_append(c, q, k, v, oracle.rotary_table(80, 64), False)
+        for max_new in {max(counts), 40 if max(counts) > 1 else 1}:
+            got = ops.paged_attention(q.cuda(), max_new_tokens=max_new, **d)
+            c.pools = [d[n].cpu() for n in ("k_pages", "v_pages")]
+            if e4m3:
+                c.scales = [d[n].cpu() for n in ("k_scales", "v_scales")]
+            want, mag = oracle.attention(q, *c.oracle_args(), c.table, c.ctx, c.new)
+            _within(got, want, _attention_tolerance(F16, e4m3, max_new > 16, want, mag))
