@@ -31,6 +31,7 @@ struct PaArgs {
   mui_strides2_t qs;
   void* out;
   float* partials;  // [ctas, 2, rows per block, D + 2]: maximum, sum, unnormalised output
+  long long* begins;  // [batch + 1] first place of each sequence and their number; nullptr: the merge works them out
   int Hq, G, ctas, row_blocks, splits, mixed, lead, max_new, window, sinks, q_vec;
   uint32_t q_flip;  // sign bits turned over in q
   float scale_log2;
@@ -279,6 +280,10 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
     if (place >= begin && place < begin + n) {
       r.begin = begin;
       s_run = r;
+    }
+    if (blockIdx.x == 0 && a.begins != nullptr) {
+      a.begins[s] = begin;
+      if (s == a.kv.batch - 1) a.begins[s + 1] = total;
     }
     begin += n;
   }
@@ -761,7 +766,9 @@ __global__ void __launch_bounds__(PA_THREADS, NT == 1 ? 3 : 2) paged_decode_kern
 }
 
 // Joins the partial results of the triples that several CTAs shared. A CTA per (triple, row): its warps take the partial
-// results in turn and are joined in shared memory, always in the same order.
+// results in turn and are joined in shared memory, always in the same order. Where a sequence's places begin it works out from the
+// lengths when they are one per thread, which is done while the attention kernel still runs; of larger batches (each CTA would read
+// all of it) the attention kernel's first CTA leaves a table.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a) {
   __shared__ long long s_warp[PA_WARPS];
@@ -781,17 +788,20 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
     pdl_wait_prior_grid();
     return;
   }
-  const int per_thread = (a.kv.batch + PA_THREADS - 1) / PA_THREADS;
-  long long begin;
-  const long long total = scan_sequences(a, per_thread, begin, s_warp);
-  if (b / per_thread == static_cast<int>(threadIdx.x)) {
-    for (int i = threadIdx.x * per_thread; i < b; ++i) begin += static_cast<long long>(seq_places(a, i)) * pairs;
-    s_begin = begin;
-  }
-  __syncthreads();
   const int places = seq_places(a, b);
+  long long begin, total;
+  if (a.begins == nullptr) {
+    total = scan_sequences(a, 1, begin, s_warp);
+    if (b == static_cast<int>(threadIdx.x)) s_begin = begin;
+    __syncthreads();
+    begin = s_begin;
+  } else {
+    pdl_wait_prior_grid();
+    total = __ldcg(a.begins + a.kv.batch);
+    begin = __ldcg(a.begins + b);
+  }
   const long long len = run_length(total, a.ctas);
-  const long long at = s_begin + static_cast<long long>(pair) * places;
+  const long long at = begin + static_cast<long long>(pair) * places;
   // the runs of the first and of the last tile; the first one left slot 1 (the triple begins in it), the others slot 0
   const int c0 = static_cast<int>((at + a.lead) / len), c1 = static_cast<int>((at + places - 1) / len);
   pdl_wait_prior_grid();
@@ -1726,7 +1736,7 @@ struct PaPlan {
   bool decode, prompt;
   int block, row_blocks, ctas;  // decode: rows per block (8, else blocks of 16)
   int tiles, splits;            // prompt
-  size_t decode_bytes, bytes;
+  size_t begins_at, decode_bytes, bytes;  // begins_at: offset of the table of first places, 0: none
 };
 bool pa_plan(const MuiDeviceInfo& di, int total, int batch, int Hq, int kv_heads, int D, int max_new, int max_context,
              int window, int sinks, PaPlan& p) {
@@ -1749,6 +1759,10 @@ bool pa_plan(const MuiDeviceInfo& di, int total, int batch, int Hq, int kv_heads
     const long long most = static_cast<long long>(di.sm_count) * (p.block == 8 ? 3 : 2);
     p.ctas = static_cast<int>(std::max<long long>(1, std::min(most, (tiles + PA_MIN_TILES - 1) / PA_MIN_TILES)));
     if (p.ctas > 1) p.decode_bytes = (static_cast<size_t>(p.ctas) * 2 * p.block * (D + 2) * sizeof(float) + 255) / 256 * 256;
+    if (p.ctas > 1 && batch > PA_THREADS) {
+      p.begins_at = p.decode_bytes;
+      p.decode_bytes += ((static_cast<size_t>(batch) + 1) * sizeof(long long) + 255) / 256 * 256;
+    }
   }
   p.bytes = p.decode_bytes;
   if (p.prompt) {
@@ -1820,6 +1834,7 @@ template <typename T, bool KV8, int D>
 mui_status_t launch_attention(cudaStream_t stream, PaArgs a, const PaPlan& p, void* workspace, int pdl, int device) {
   if (p.decode) {
     a.partials = reinterpret_cast<float*>(workspace);
+    if (p.begins_at) a.begins = reinterpret_cast<long long*>(reinterpret_cast<char*>(workspace) + p.begins_at);
     const mui_status_t s = p.block == 8 ? launch_decode<T, KV8, D, 1>(stream, a, pdl, device)
                                         : launch_decode<T, KV8, D, 2>(stream, a, pdl, device);
     if (s != MUI_OK) return s;
