@@ -99,6 +99,21 @@ def test_sample_clusters_beside_other_work():
         assert torch.equal(tokens, want[0]) and torch.equal(logprobs, want[1])
 
 
+@pytest.mark.parametrize("kw", [{}, dict(top_k=50, top_p=0.9), dict(top_p=0.95), dict(top_p=0.9, min_p=0.02), dict(min_p=1e-4),
+                                dict(top_k=3000)])
+def test_sample_rows_do_not_depend_on_the_batch(kw):
+    """A row draws the same token, with the same log share to the last bit, alone (by eight CTAs) and among many (by one)."""
+    g = _gen(64)
+    for spread in (0.2, 2.5):
+        x = (spread * torch.randn(100, 40000, generator=g)).cuda()
+        u = torch.rand(100, generator=g).cuda()
+        one = {n: torch.full((100,), v, dtype=torch.int32 if n == "top_k" else torch.float32, device="cuda") for n, v in kw.items()}
+        tokens, logprobs = ops.sample_tokens(x, u, **one)
+        for r in range(0, 100, 9):
+            t, lp = ops.sample_tokens(x[r:r + 1], u[r:r + 1], **{n: v[r:r + 1] for n, v in one.items()})
+            assert int(t) == int(tokens[r]) and float(lp) == float(logprobs[r])
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # append
 # ---------------------------------------------------------------------------------------------------------------------
