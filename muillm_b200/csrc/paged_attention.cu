@@ -159,7 +159,8 @@ __device__ __forceinline__ long long scan_sequences(const PaArgs& a, int per_thr
   return all;
 }
 __device__ __forceinline__ long long run_length(long long total, int ctas) {
-  return max(static_cast<long long>(PA_MIN_TILES), (total + ctas - 1) / ctas);  // more than `lead`
+  // may be less than `lead`: a run that lies within one then has nothing to do, and the triple's first tile belongs to a later run
+  return max(static_cast<long long>(PA_MIN_TILES), (total + ctas - 1) / ctas);
 }
 
 // K and V pass through shared memory in items of 4 KiB, a ring of four per warp (K, V, K, V), copied asynchronously: three

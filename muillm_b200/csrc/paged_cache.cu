@@ -449,18 +449,18 @@ __global__ void __launch_bounds__(PC_THREADS, ROWS <= 2 ? 3 : 2) append_e4m3_ker
 }
 
 template <typename T, int D, bool ALIGNED>
-mui_status_t launch_append(cudaStream_t stream, AppendArgs a, bool e4m3, int page_size, unsigned flags) {
+mui_status_t launch_append(cudaStream_t stream, AppendArgs a, bool e4m3, int page_size, int sms, unsigned flags) {
   constexpr int RPS = 32 / (D / 8);
   const int pdl = (flags & MUI_FLAG_PDL) ? 1 : 0;
   const dim3 block(PC_THREADS);
   const long long limit = 0x7fffffff;
   auto blocks = [](long long units) { return (units + PC_WARPS - 1) / PC_WARPS; };
-  // Turns of heads per warp: one while that leaves the GPU unfilled (64 warps for each of 148 SMs), up to all heads of a token
+  // Turns of heads per warp: one while that leaves the GPU unfilled (64 warps for each SM), up to all heads of a token
   // where it does not: what a warp looks up then serves 12 KiB of a 32 + 8-head token instead of 512 bytes.
   auto choose_steps = [&](int heads) {
     const int turns = (heads + RPS - 1) / RPS;
     a.steps = 1;
-    while (a.steps < turns && static_cast<long long>(a.kv.total) * ((turns + a.steps - 1) / a.steps) > 148 * 64) a.steps *= 2;
+    while (a.steps < turns && static_cast<long long>(a.kv.total) * ((turns + a.steps - 1) / a.steps) > sms * 64ll) a.steps *= 2;
     a.head_blocks = (turns + a.steps - 1) / a.steps;
   };
   if (!e4m3) {
@@ -485,7 +485,7 @@ mui_status_t launch_append(cudaStream_t stream, AppendArgs a, bool e4m3, int pag
   }
   const long long pages = a.kv.total / page_size + 2ll * a.kv.batch;
   a.unit_heads = 1;  // as for the rows: eight CTAs for each SM
-  while (a.unit_heads < a.kv.kv_heads && pages * 2 * (a.kv.kv_heads / a.unit_heads) > 148 * 8) a.unit_heads *= 2;
+  while (a.unit_heads < a.kv.kv_heads && pages * 2 * (a.kv.kv_heads / a.unit_heads) > sms * 8ll) a.unit_heads *= 2;
   const long long units = pages * 2 * ((a.kv.kv_heads + a.unit_heads - 1) / a.unit_heads);
   const long long n = units + q_blocks;
   MUI_REQUIRE(n <= limit, MUI_ERR_UNSUPPORTED, "too many rows");
@@ -523,6 +523,8 @@ extern "C" mui_status_t mui_paged_kv_append(void* stream, mui_dtype_t dtype, con
   if (cache->batch == 0 || cache->total_tokens == 0) return MUI_OK;
   MUI_REQUIRE(k && v && (num_q_heads == 0 || (q && q_out)), MUI_ERR_INVALID_ARG, "q, k, v and q_out must be non-null");
   MUI_REQUIRE((reinterpret_cast<uintptr_t>(q_out) & 15) == 0, MUI_ERR_INVALID_ARG, "q_out must be 16-byte aligned");
+  const MuiDeviceInfo* di = mui_current_device_info();
+  if (!di) return MUI_ERR_CUDA;
   AppendArgs a = {};
   a.kv = paged_view(*cache);
   a.q = q;
@@ -544,9 +546,9 @@ extern "C" mui_status_t mui_paged_kv_append(void* stream, mui_dtype_t dtype, con
   a.freqs_vec = freqs != nullptr && (reinterpret_cast<uintptr_t>(freqs) & 15) == 0 && a.rotary % whole == 0;
   const bool e4m3 = cache->format == MUI_KV_E4M3;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int ps = cache->page_size;
+  const int ps = cache->page_size, sms = di->sm_count;
 #define PC_GO(T, D) \
-  (aligned ? launch_append<T, D, true>(st, a, e4m3, ps, flags) : launch_append<T, D, false>(st, a, e4m3, ps, flags))
+  (aligned ? launch_append<T, D, true>(st, a, e4m3, ps, sms, flags) : launch_append<T, D, false>(st, a, e4m3, ps, sms, flags))
   if (dtype == MUI_F16) return cache->head_dim == 128 ? PC_GO(__half, 128) : PC_GO(__half, 64);
   return cache->head_dim == 128 ? PC_GO(__nv_bfloat16, 128) : PC_GO(__nv_bfloat16, 64);
 #undef PC_GO
