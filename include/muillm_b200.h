@@ -536,8 +536,8 @@ MUI_API mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const 
  * token at least), and of those the ones with w >= min(min_p, 1). The drawn token is the first one, in index order, at which the
  * running weight of the kept ones exceeds uniform * their weight. temperature, top_k, top_p, min_p and uniforms ([rows];
  * fp32, top_k int32) live on the device; NULL means 1, off, off, off; top_k <= 0, top_p >= 1 and min_p <= 0 are off too;
- * a temperature that is not above 0 takes the largest logit (lowest index), one below 2^-126 counts as 2^-126. Logits of -infinity or NaN are never drawn
- * (a row of nothing else gives token 0). logprobs (may be NULL): log of the drawn token's share of the kept weight.
+ * a temperature that is not above 0 takes the largest logit (lowest index), one below 2^-126 or above 10^29 counts as that. Logits
+ * of -infinity or NaN are never drawn (a row of nothing else gives token 0). logprobs (may be NULL): log of the drawn token's share of the kept weight.
  * Weights are evaluated in fp64 and summed in integers, so a result depends neither on the order of summation nor on
  * the launch. The reference samples through Hugging Face's logits processors (examples/llama3_8b.py:51-58). */
 MUI_API mui_status_t mui_sample_tokens(void* stream, int dtype, int rows, int vocab, const void* logits,

@@ -208,12 +208,16 @@ struct Row {
   const T* p;
   int V, c0, c1;  // this CTA's chunks
   bool vec;
-  bool inf;       // the largest logit is +infinity: 0 stands for it then, and -infinity for every other one
+  // The largest logit is +infinity or the lowest finite number, so that nothing finite is below it: 0 stands for it then, and
+  // -infinity for everything else. (Below the lowest number there would be no place for logits without weight.)
+  bool alone;
+  float peak;  // that logit
+  __device__ __forceinline__ float stand_in(float x) const { return x == peak ? 0.f : -INFINITY; }
   __device__ __forceinline__ void unpack(const Raw& r, float (&x)[8]) const {
     unpack_raw<T>(r, x);
-    if (inf) {
+    if (alone) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = x[e] == INFINITY ? 0.f : -INFINITY;
+      for (int e = 0; e < 8; ++e) x[e] = stand_in(x[e]);
     }
   }
   // f(first token of the lane, its eight logits) for every chunk of this CTA; warps take chunks in turn, the next four in
@@ -507,7 +511,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   row.p = reinterpret_cast<const T*>(a.logits) + r * a.stride;
   row.V = a.V;
   row.vec = (reinterpret_cast<uintptr_t>(row.p) & 15) == 0;
-  row.inf = false;
+  row.alone = false;
   const int chunks = (a.V + SM_CHUNK - 1) / SM_CHUNK, per_cta = (chunks + C - 1) / C;
   row.c0 = min(chunks, static_cast<int>(rank) * per_cta);
   row.c1 = min(chunks, row.c0 + per_cta);
@@ -584,16 +588,18 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
     }
     return;
   }
-  if (w.top == INFINITY) {
-    row.inf = true;
+  if (w.top == INFINITY || w.top == -3.402823466e38f) {
+    row.alone = true;
+    row.peak = w.top;
     w.top = 0.f;
   }
   const uint32_t best_key = logit_key(w.top);
   w.frac_bits = a.frac_bits;
   // z below -(S + 2) ln 2 has a weight under a quarter of the last bit. A temperature so small that the next smaller logit
-  // lies beyond that, or so large that all logits are alike, is brought to where this is just the case.
+  // lies beyond that, or so large that all logits are alike, is brought to where this is just the case. (10^29: the range, 3.5 * 10^30,
+  // is below the distance of the largest fp32 numbers, so that the floor stays above the lowest one.)
   const float z_range = (a.frac_bits + 2) * 0.693147181f;
-  t = fminf(fmaxf(fmaxf(t, (w.top - key_logit(best_key - 1)) / z_range), 1.17549435e-38f), 1e30f);
+  t = fmaxf(fmaxf(fminf(t, 1e29f), (w.top - key_logit(best_key - 1)) / z_range), 1.17549435e-38f);
   w.floor = fmaxf(fminf(w.top - z_range * t, key_logit(best_key - 1)), -3.402823466e38f);
   w.scale = 46.166241308446828 / static_cast<double>(t);  // 32 / ln 2
   w.table = exp2(static_cast<double>(lane) / 32.0);
@@ -939,7 +945,7 @@ __global__ void __launch_bounds__(SM_THREADS, 1) sample_kernel(const SampleArgs 
   };
   if (use_k && k_raw <= C * SM_THREADS) {
     // The largest logits of k threads are k tokens: whatever the bin of the k-th of them, the top-k lie in the bins up to it.
-    if (row.inf) m = m == INFINITY ? 0.f : -INFINITY;
+    if (row.alone) m = row.stand_in(m);
     const int mine = w.bin(m);
     if (mine < SM_BINS) atomicAdd(&s.bins[mine], 1u);
     join_bins();

@@ -79,6 +79,34 @@ def test_sample_smallest_temperatures_at_logits_of_zero(which):
             _check_written(x, u, temperature=torch.full((4,), t), **kw)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16, torch.float32])
+@pytest.mark.parametrize("temperature", [1.0, 0.3, 3e38])
+def test_sample_rows_of_lowest_values(dtype, temperature):
+    """Rows whose tokens all carry the type's lowest value, or that and next to nothing more: what lies behind the row's end
+    has no part in them, nor do -infinity and NaN."""
+    g = _gen(65)
+    low = torch.finfo(dtype).min
+    for vocab in (3, 219, 9001):
+        x = torch.full((6, vocab), low)
+        x[1, 1:] = -math.inf
+        x[2, ::2] = math.nan
+        x[3, torch.rand(vocab, generator=g) < 0.3] = -math.inf
+        x[4, ::3] = low * (1 - 3 * torch.finfo(dtype).eps)  # the next larger numbers
+        x[5, 0] = -1.0
+        u = torch.rand(6, generator=g)
+        one = dict(temperature=torch.full((6,), temperature))
+        for kw in ({}, dict(top_p=torch.full((6,), 0.5558)), dict(top_k=torch.full((6,), 50, dtype=torch.int32)),
+                   dict(top_p=torch.full((6,), 0.9), min_p=torch.full((6,), 0.05)),
+                   dict(top_p=torch.full((6,), 0.3), top_k=torch.full((6,), 100, dtype=torch.int32))):
+            y = x.to(dtype)
+            if temperature > 1e30:
+                # counts as 10^29, which these rows can tell only where logits of that size differ
+                y = y[[0, 1, 2, 3]]
+                _check_written(y, u[:4], **{n: t[:4] for n, t in {**one, **kw}.items()})
+            else:
+                _check_written(y, u, **one, **kw)
+
+
 def test_sample_clusters_beside_other_work():
     """Rows shared by a cluster of CTAs, launched while another stream fills the GPU: every launch gives the same tokens."""
     g = _gen(63)
