@@ -512,9 +512,10 @@ MUI_API mui_status_t mui_paged_kv_append(void* stream, mui_dtype_t dtype, const 
 /* out[t, h, :] = softmax_j( q[t, h, :] . K[j, h / G, :] * scale ) V over the cache rows j of the token's sequence (G =
  * num_q_heads / kv_heads, at most 32): a token at cache position p sees j <= p, its own row (appended before) included, and
  * with window > 0 of those only j > p - window or j < sinks. out is contiguous [total_tokens, num_q_heads, head_dim].
- * max_new_tokens bounds the new tokens of every sequence (1 where cu_tokens is NULL, whatever is given). max_context (> 0) is a hint for the work split, the longest
- * sequence expected (any value gives right results). What a token does not see does not reach its result, infinities and
- * NaN included (prompts that have any in V take about twenty times longer). Softmax statistics, sums and outputs are held in fp32 and rounded once;
+ * max_new_tokens bounds the new tokens of every sequence (1 where cu_tokens is NULL, whatever is given). max_context (> 0) is a
+ * hint for the work split, the longest sequence expected (any value gives right results). What a token does not see does not reach
+ * its result, infinities and NaN included (prompts that have any in V take about twenty times longer). Softmax statistics, sums and
+ * outputs are held in fp32 and rounded once;
  * the probabilities enter the second product in 16 bits: with bf16 pages as bf16, up to 32 queries a KV head and sequence (new
  * tokens times heads) with a bf16 rest; else as fp16, over e4m3 pages times V's scale, with eleven bits down to 2^-29 (more than 32
  * queries: 2^-21) of the row's largest. workspace:
@@ -538,8 +539,9 @@ MUI_API mui_status_t mui_paged_attention(void* stream, mui_dtype_t dtype, const 
  * fp32, top_k int32) live on the device; NULL means 1, off, off, off; top_k <= 0, top_p >= 1 and min_p <= 0 are off too;
  * a temperature that is not above 0 takes the largest logit (lowest index), one below 2^-126 or above 10^29 counts as that. Logits
  * of -infinity or NaN are never drawn (a row of nothing else gives token 0). logprobs (may be NULL): log of the drawn token's share of the kept weight.
- * Weights are evaluated in fp64 and summed in integers, so a result depends neither on the order of summation nor on
- * the launch. The reference samples through Hugging Face's logits processors (examples/llama3_8b.py:51-58). */
+ * Weights are evaluated in fp64 and summed in integers, as multiples of 2^-S of the largest (S = min(48, 62 - ceil(log2(vocab)))), so
+ * a result depends neither on the order of summation nor on the launch; the ends of top-p and min-p and the drawn point are right to
+ * about sqrt(vocab) * 2^-S, and a token of less than half such a unit is never drawn. The reference samples through Hugging Face's logits processors (examples/llama3_8b.py:51-58). */
 MUI_API mui_status_t mui_sample_tokens(void* stream, int dtype, int rows, int vocab, const void* logits,
                                        int64_t row_stride, const float* temperature, const int32_t* top_k,
                                        const float* top_p, const float* min_p, const float* uniforms, int64_t* tokens,

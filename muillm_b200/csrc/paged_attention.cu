@@ -107,9 +107,9 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 // others leave partial results, at most two per CTA (the triple that the run starts in and the one it ends in), which
 // paged_merge_kernel joins in order.
 // Measured (device time with the merge; 32 q and 8 KV heads of 128, copy bandwidth 6560 GB/s): 24 sequences of 150 to 6500
-// tokens, bf16, 61 us = 5.2 TB/s; 32 sequences of 413 to 8111, e4m3, 62 us = 4.6 TB/s; one sequence of 131000, 64 q heads,
-// e4m3, 57 us = 4.7 TB/s; 16 long ones with a window of 4096 and 4 sinks, 40 q heads, 52 us = 5.0 TB/s; one sequence of 300 tokens
-// 12.4 us. About 8 us of a launch go to the chain before the first and after the last item (lengths, block table, q, merge);
+// tokens, bf16, 62 us = 5.1 TB/s; 32 sequences of 413 to 8111, e4m3, 62 us = 4.6 TB/s; one sequence of 131000, 64 q heads,
+// e4m3, 57 us = 4.7 TB/s; 16 long ones with a window of 4096 and 4 sinks, 40 q heads, 53 us = 5.0 TB/s; one sequence of 300 tokens
+// 13.2 us; 200 of 300 to 2500, e4m3, 135 us. About 8 us of a launch go to the chain before the first and after the last item (lengths, block table, q, merge);
 // in between e4m3 is bound by its instructions: a conversion for each pair of elements, and byte permutes for V.
 struct Run {
   int seq, first, count, ctx;  // sequence at the run's first place
@@ -881,9 +881,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_merge_kernel(const PaArgs a)
 // any case. P is rounded once to the type of the tensor-core operands (half a step is 2^-9 of it for bf16, 2^-12 for fp16: there P is
 // taken times 2^7, so that it has all its bits down to 2^-21 of the reference).
 // Bound: exp2 (16 a cycle and SM) and the MMAs need about 2050 cycles a step each.
-// Measured (32 q and 8 KV heads of 128, device time; tensor cores 1651 TFLOP/s): one prompt of 8192 tokens, bf16 pages, 555 us =
-// 990 TFLOP/s; three chunks of 1023 to 2049 tokens behind up to 2100, 223 us = 774 TFLOP/s (the last round of CTAs is not full);
-// e4m3 pages 357 us (the three warps that convert K and V). A step takes 2.0 us, 1.6 of it MMA time: a group's softmax ends
+// Measured (32 q and 8 KV heads of 128, device time; tensor cores 1651 TFLOP/s): one prompt of 8192 tokens, bf16 pages, 600 us =
+// 920 TFLOP/s; three chunks of 1023 to 2049 tokens behind up to 2100, 222 us = 778 TFLOP/s (the steps alone are
+// 147 us; the last round of CTAs is not full, and each of four CTAs in a row on an SM begins and ends with nothing beside it); e4m3
+// pages 356 us (the three warps that convert K and V). A step takes 2.0 us, 1.6 of it MMA time: a group's softmax ends
 // a little late for the other group's products. A part of the exponentials as polynomials on the fp32 pipes was slower (a
 // quarter of them 231, half of them 239 us): their instructions come out of the same issue slots. So were tiles ordered by
 // length over all sequences (269 us: the search costs each CTA more than it saves).

@@ -12,10 +12,10 @@
 //    the new rows are rounded. No atomics, and K and V are units of their own. The q rows of an e4m3 call are rows as above, in
 //    further CTAs of the same launch.
 // Measured (device time; 32 q and 8 KV heads of 128, copy bandwidth 6560 GB/s): one token 2.6 us and 64 tokens into e4m3 pages
-// 3.0 us, both the launch and the round trips; 9 prompts of 700 to 2500 tokens, 16-bit pages, 81 us = 4.6 TB/s, bound by the
-// instructions of the rotation and its addresses (about 2 a byte moved; more rows in flight and packed arithmetic did not help);
-// 3 prompts of 1021 to 2801 tokens, e4m3 pages of 32, 40 q heads, 41 us = 3.9 TB/s, bound by the two steps of a unit: all of
-// its rows have to be there before the first one can be rounded.
+// 3.0 us, both the launch and the round trips; 9 prompts of 700 to 2500 tokens, 16-bit pages, 82 us = 4.6 TB/s: loads, rotation and
+// stores of a warp alternate, at 24 warps an SM neither memory (47 %) nor the issue slots (60 %) are full (more rows in flight and packed
+// arithmetic did not help); 3 prompts of 1021 to 2801 tokens, e4m3 pages of 32, 40 q heads, 42 us = 3.9 TB/s, the same: three
+// quarters of the bytes are q rows, which are handled as with 16-bit pages.
 // Eight consecutive elements of a row sit in one lane (16 bytes). In the half layout the partner of an element is
 // rotary_dim / 2 elements away: in another lane, fetched with a shuffle, when that distance is a multiple of eight.
 #include "paged_common.cuh"

@@ -28,9 +28,10 @@
 // Bound: rows * vocab * size bytes for large batches, then eleven fp64 operations a weight (fp64 runs at half the fp32 rate);
 // for few rows the chain of passes and cluster barriers.
 // Measured (device time): one row of 128256 fp16 logits, top-k 50 and top-p 0.9, 12 us (floor 0.04 us: five dependent steps of
-// about 2 us); 128 rows of 202048 fp32 logits, top-p 0.95 and min-p 0.02, 91 us (floor 15.8 us; 60 us for most rows, the one with
-// the longest list sets the time; with the row's weight in fp64 instead of roughly, 113 us); 32 rows of 128256 with top-k 50 and
-// top-p, 16 us; one row with top-p alone, 36 us; 64 rows with top-p alone whose nucleus is wide, 112 us.
+// about 2 us); 128 rows of 202048 fp32 logits, top-p 0.95 and min-p 0.02, 90 us (floor 15.8 us; 60 us for most rows, the one with
+// the longest list sets the time; with the row's weight in fp64 instead of roughly, 113 us). Of 128256 fp16 logits: 32 rows with top-k 50
+// and top-p 0.9, 16 us, 96 rows 25 us; one row with top-p 0.9 alone, 35 us, 64 rows with 0.95, 104 us; 64 rows without cuts, 28 us; the
+// largest logit of one row, 4.9 us.
 #include "common.cuh"
 
 #include <atomic>
